@@ -8,7 +8,7 @@ NAME=$1; SRC=$2; shift 2
 CS=$ROOT/multimodalspectraltransformer_amd/csrc
 mkdir -p $ROOT/tools/exp
 BASE=$(basename $SRC .hip)
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC "$@" -c $CS/$BASE.hip -o $ROOT/tools/exp/$BASE.$NAME.o
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Xclang -target-feature -Xclang -packed-fp32-ops "$@" -c $CS/$BASE.hip -o $ROOT/tools/exp/$BASE.$NAME.o
 OBJS=""
 for o in $CS/_build/*.o; do
   if [ "$(basename $o .o)" = "$BASE" ]; then OBJS="$OBJS $ROOT/tools/exp/$BASE.$NAME.o"; else OBJS="$OBJS $o"; fi

@@ -9,7 +9,7 @@ mkdir -p $ROOT/tools/exp
 if [ "$1" = build ]; then
   OBJS=""
   for f in ffn ffn_wgrad attn gemm; do
-    /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -DMMST_WG_LOG -c $CS/$f.hip -o $ROOT/tools/exp/$f.wglog.o
+    /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Xclang -target-feature -Xclang -packed-fp32-ops -DMMST_WG_LOG -c $CS/$f.hip -o $ROOT/tools/exp/$f.wglog.o
   done
   for o in $CS/_build/*.o; do
     b=$(basename $o .o)
