@@ -29,6 +29,7 @@
  */
 #ifndef MMST_H
 #define MMST_H
+#include <stddef.h>
 #include <stdint.h>
 
 #ifdef __cplusplus
@@ -403,6 +404,40 @@ int mmst_transpose_bf16(const void* src, void* dst, int n, const uint32_t* offse
 typedef struct { const void* src; void* dst; int rows, cols, ld, transpose; } mmst_frag_desc;
 #define MMST_FRAG_MAX 32   /* descriptors per launch; longer lists take several launches */
 int mmst_fragment_bf16(int n, const mmst_frag_desc* descs, void* stream);
+
+/* ---- row operators of any width: dropout and layer norm ----
+ * What the width-128 launches above fuse into their epilogues, for rows of any width, in fp32, bf16 or fp16 (dtype; sums
+ * and statistics always fp32).  Row r of a tensor starts ld* elements behind row r - 1, ld* >= cols; any alignment of an
+ * element is served, 16-byte aligned rows of a multiple of 8 columns fastest.  An output may be the same tensor as an
+ * input of the same call (same pointer, same stride), other overlaps are not allowed.
+ *
+ * The dropout mask is Philox4x32-10 of (seed, offset, element), see csrc/philox.h: element i = r * cols + c of the tensor
+ * read row by row, whatever its strides and type, and the same in mmst_dropout, mmst_layer_norm and mmst_layer_norm_bwd.
+ * A caller gives every use of a (seed, offset) pair to one tensor only, for instance a run's seed and a running count of
+ * the dropout sites.  p is rounded to a multiple of 1 / 65536 and what is kept is scaled by 1 / (1 - that); p = 1 drops
+ * everything.  Dropped elements are 0 also where the input is infinite or NaN. */
+enum mmst_dtype { MMST_F32 = 0, MMST_BF16 = 1, MMST_F16 = 2 };
+#define MMST_LN_MAX_COLS 16384
+
+/* y = dropout(x); on the gradient of y it is its own backward pass.  rows or cols 0: nothing to do. */
+int mmst_dropout(const void* x, long ldx, void* y, long ldy, int dtype, long rows, long cols, double p, uint64_t seed,
+                 uint64_t offset, void* stream);
+/* z = residual + dropout(x) (residual may be NULL), y = (z - mean) rstd gamma + beta with the row's mean and
+ * rstd = 1 / sqrt(variance + eps) of the unrounded z.  gamma / beta fp32 [cols] or NULL (1 / 0).  z (optional): z in the
+ * tensors' type, needed by the backward pass unless it is x; stats (optional): (mean, rstd) [rows][2]. */
+int mmst_layer_norm(const void* x, long ldx, const void* residual, long ldr, const float* gamma, const float* beta, void* y,
+                    long ldy, void* z, long ldz, float* stats, int dtype, long rows, int cols, float eps, double p,
+                    uint64_t seed, uint64_t offset, void* stream);
+/* From dy, z, stats, gamma and (p, seed, offset) as in the forward call: dz = the gradient at z, which is also the
+ * residual's, plus dz_in (optional: what reaches z by another path); dx = dz through the dropout mask (unused where p
+ * rounds to 0: the gradient at x is dz then); dgamma / dbeta (optional, fp32 [cols]): overwritten, or added to where
+ * accumulate != 0.  They are summed in a fixed order, so equal calls give equal bits; ws holds the workgroups' partial
+ * sums (mmst_layer_norm_bwd_ws says how many bytes; may be NULL where neither is asked for). */
+int mmst_layer_norm_bwd(const void* dy, long lddy, const void* z, long ldz, const float* stats, const float* gamma,
+                        const void* dz_in, long lddz_in, void* dz, long lddz, void* dx, long lddx, float* dgamma,
+                        float* dbeta, int accumulate, int dtype, long rows, int cols, double p, uint64_t seed,
+                        uint64_t offset, void* ws, size_t ws_bytes, void* stream);
+int mmst_layer_norm_bwd_ws(long rows, int cols, size_t* bytes);
 
 /* ---- CLIP contrastive head on the encoder half (utils_MMT/models_CLIP_v15_4.py), all fp32 ---- */
 
