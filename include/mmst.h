@@ -439,6 +439,43 @@ int mmst_layer_norm_bwd(const void* dy, long lddy, const void* z, long ldz, cons
                         uint64_t offset, void* ws, size_t ws_bytes, void* stream);
 int mmst_layer_norm_bwd_ws(long rows, int cols, size_t* bytes);
 
+/* ---- linear layer with softmax cross entropy over a large vocabulary, without the logits in memory ----
+ * logits = h w^T + bias (bf16 operands, fp32 accumulation), loss[n] = logsumexp(logits[n]) - logits[n][target[n]]: what
+ * the fc_out GEMM and mmst_ce_loss do for at most 64 words, for any vocabulary.  grad != 0 also computes, for
+ * sum_n grad_scale dloss[n] loss[n], the gradients dh, dw and dbias.
+ *   - rows whose target is ignore_index do not count: loss, lse and dh 0, nothing in dw, whatever h holds there, and no
+ *     work in the products.  A target that is no word and not ignore_index gives loss and lse NaN and no gradient.
+ *   - masked words: bias may be -infinity or the lowest float.  A row whose every logit is -infinity has lse -infinity,
+ *     loss +infinity and no gradient.
+ *   - h, w, dh, dw rows 16-byte aligned; D a multiple of 8.  dw [V][D] and dbias [V] (both without a stride) in bf16,
+ *     overwritten, or with grad_f32 in fp32, added to (as the other parameter gradients of this library).  All sums run in
+ *     a fixed order: equal calls give equal bits.
+ *   - the gradient works through the rows in pieces; the workspace holds the logits' gradient of one piece in bf16
+ *     (rows_per_piece x V, rounded up to multiples of 256; 0: as many rows as 4 GiB hold) and its gathered rows, with
+ *     bf16 gradients of more than one piece also their fp32 sums.  mmst_linear_ce_ws says how many bytes (its pointers may
+ *     be unset except dbias, which only has to say whether there is one); it has to be 256-byte aligned. */
+#define MMST_LINEAR_CE_MAX_ROWS (1 << 24)
+#define MMST_LINEAR_CE_MAX_VOCAB (1 << 22)
+#define MMST_LINEAR_CE_MAX_DIM 32768
+#define MMST_LINEAR_CE_MAX_LD (1 << 20)
+typedef struct {
+  const void* h; long ldh;             /* [N][D] bf16 */
+  const void* w; long ldw;             /* [V][D] bf16 */
+  const float* bias;                   /* [V] or NULL */
+  const int64_t* target;               /* [N] */
+  int64_t ignore_index;
+  int N, D, V;
+  int rows_per_piece;                  /* gradient only, 0: default */
+  float* loss; float* lse;             /* out [N]; lse may be NULL */
+  const float* dloss; float grad_scale; /* gradient only: [N] weights of the losses, or NULL (1) */
+  int grad_f32;
+  void* dh; long lddh; void* dw; void* dbias;   /* dbias may be NULL */
+  void* ws; size_t ws_bytes;
+} mmst_linear_ce_args;
+int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream);
+int mmst_linear_ce_ws(const mmst_linear_ce_args* args, int grad, size_t* bytes);
+int mmst_sizeof_linear_ce_args(void);
+
 /* ---- CLIP contrastive head on the encoder half (utils_MMT/models_CLIP_v15_4.py), all fp32 ---- */
 
 /* C[M][N] = alpha * sum_k A(i,k) B(k,j) + beta * C + bias[j], with A(i,k) = A[i*sai + k*sak] and

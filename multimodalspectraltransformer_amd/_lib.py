@@ -95,7 +95,8 @@ def lib():
                 _lib.mmst_sizeof_ffn_wgrad_batch() != C.sizeof(FfnWgradBatch) or \
                 _lib.mmst_sizeof_dec_stack_step() != C.sizeof(DecStackStep) or \
                 _lib.mmst_sizeof_step_plan() != C.sizeof(StepPlan) or \
-                _lib.mmst_sizeof_step_args() != C.sizeof(StepArgs):
+                _lib.mmst_sizeof_step_args() != C.sizeof(StepArgs) or \
+                _lib.mmst_sizeof_linear_ce_args() != C.sizeof(LinearCeArgs):
             raise MMSTError("struct layout mismatch between _lib.py and libmmst.so")
     return _lib
 
@@ -243,6 +244,14 @@ class StepArgs(C.Structure):
                  ("adam_step", C.c_int)] +
                 [(n, C.c_float) for n in ("lr", "beta1", "beta2", "eps", "weight_decay", "grad_scale")] +
                 [("on_segment", SEGMENT_CALLBACK), ("user", C.c_void_p)])
+
+
+class LinearCeArgs(C.Structure):
+    _fields_ = [("h", C.c_void_p), ("ldh", C.c_long), ("w", C.c_void_p), ("ldw", C.c_long), ("bias", C.c_void_p),
+                ("target", C.c_void_p), ("ignore_index", C.c_int64), ("N", C.c_int), ("D", C.c_int), ("V", C.c_int),
+                ("rows_per_piece", C.c_int), ("loss", C.c_void_p), ("lse", C.c_void_p), ("dloss", C.c_void_p),
+                ("grad_scale", C.c_float), ("grad_f32", C.c_int), ("dh", C.c_void_p), ("lddh", C.c_long),
+                ("dw", C.c_void_p), ("dbias", C.c_void_p), ("ws", C.c_void_p), ("ws_bytes", C.c_size_t)]
 
 
 class BeamState(C.Structure):

@@ -1,0 +1,712 @@
+// Linear layer with softmax cross entropy over a large vocabulary, loss and gradients, without the logits in memory.
+//
+//   l[n][v] = sum_d h[n][d] w[v][d] + bias[v]          lse[n] = log sum_v exp l[n][v]       loss[n] = lse[n] - l[n][t_n]
+//   g[n][v] = dloss[n] (exp(l[n][v] - lse[n]) - [v == t_n])        dh = g w        dw = g^T h        dbias = sum_n g
+//
+// All of it is matrix products over tiles of 256 x 256 (or 128 x 128 where those are too few) on
+// v_mfma_f32_16x16x32_bf16 with fp32 accumulation; a softmax never leaves the tile that made its logits:
+//   stats  a tile of logits becomes (max, sum exp) per row: 8 bytes per row and tile of the vocabulary
+//   rows   a row's pairs are joined into lse and the loss
+//   grad   the tile of logits once more, now as g in bf16
+//   dh, dw products with g, whose operands lie along the wrong axis and are read through transposing LDS reads
+// The gradient goes in pieces of the ROWS: a piece's g [rows][V] is the only large buffer.  Rows that do not count
+// (ignore_index) are left out at the start: the others are numbered through on the device and gathered, so a padded batch
+// costs what its tokens cost, and what padding holds (NaN, infinities) reaches nothing.
+#include "../../include/mmst.h"
+#include "common.h"
+
+namespace {
+
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef LDS_AS unsigned char lds_byte;
+typedef __attribute__((address_space(3))) void* lptr_t;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int VT = 256;   // g is padded to whole tiles of the vocabulary, its rows to whole tiles as well
+
+enum { LOGIT_STATS = 0, LOGIT_GRAD = 1, DH = 2, DW = 3 };
+
+struct CeGemm {
+  const bf16* P; const bf16* Q;      // operands; the token / vocabulary side of the output's rows, and its columns
+  long ldp, ldq;
+  int Pn, Qn, K;                     // extents; K for DH is the vocabulary
+  const int* count;                  // device: rows that count; the piece holds clamp(count - row0, 0, rows_max) of them
+  int row0, rows_max;                // (count == NULL: rows_max rows)
+  int ptiles, qtiles, ksplit;
+  // logits
+  const float* bias; const int64_t* target; const int* index;
+  float2* part; float* tlogit;       // per (tile column, row): max, sum of exp; the target's logit
+  const float* lse; const float* weight; bf16* g; long ldg; float* dbias_part;
+  // products
+  void* out; long ldo; int out_f32; int accumulate;   // out_f32: fp32, else bf16; accumulate: added to
+  const float* acc_in; float* slab;
+};
+
+__device__ __forceinline__ int piece_rows(const CeGemm& a) {
+  if (!a.count) return a.rows_max;
+  const int left = *a.count - a.row0;
+  return left < 0 ? 0 : left < a.rows_max ? left : a.rows_max;
+}
+
+__device__ __forceinline__ int key_p(int r) { return r & 7; }
+__device__ __forceinline__ int key_q(int r) { return (r & 3) | (((r >> 3) & 1) << 2); }
+
+// One operand's tile in LDS: B rows (or columns) x 64 of the contraction.
+//   rows along the contraction (T == false): B rows of 128 bytes, the eight 16-byte pieces of a row exchanged by its key
+//   columns along the contraction (T == true): 64 rows of 2 B bytes, their 32-byte pieces exchanged by the row's key
+// The exchange makes the fragment reads of 16 rows hit all banks; it is applied to the SOURCE address, since the LDS-DMA
+// writes lane i's 16 bytes at i * 16.  What lies outside the operand reads as zero (the buffer's bounds check; the tail of
+// the contraction by an offset past every bound).
+template <bool T, bool QSIDE, int B, int NTHR> struct Operand {
+  static constexpr int NI = B * 8 / NTHR;   // DMA instructions per thread and step
+  static constexpr int BYTES = B * 128;
+  static constexpr uint32_t OUT = 0xFFFFFFF0u;
+  uint32_t off[NI];
+  const bf16* base;
+  long ld;
+  int K, wide;   // wide: columns of the operand right of the tile's first (T)
+  long rows;     // rows of the operand below the tile's first (!T)
+
+  __device__ __forceinline__ void init(const bf16* p, long ld_, int first, int n, int K_, int tid) {
+    ld = ld_;
+    K = K_;
+    base = T ? p + first : p + (long)first * ld_;
+    rows = wide = n - first;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int slot = i * NTHR + tid;
+      if constexpr (!T) {
+        const int r = slot >> 3, c = (slot & 7) ^ (QSIDE ? key_q(r) : key_p(r));
+        off[i] = (uint32_t)(r * (int)ld_ * 2 + c * 16);
+      } else {
+        const int r = slot / (B / 8), c16 = slot % (B / 8);
+        off[i] = (uint32_t)(r * (int)ld_ * 2 + ((((c16 >> 1) ^ key_q(r)) << 1) | (c16 & 1)) * 16);
+      }
+    }
+  }
+  __device__ __forceinline__ void issue(lds_byte* img, int k0, int tid, int wave) const {
+    const bf16* p;
+    long bytes;
+    if constexpr (!T) {
+      p = base + k0;
+      bytes = ((rows - 1) * ld + ((K + 7) & ~7) - k0) * 2;   // whole 16-byte pieces: g's rows are padded
+    } else {
+      p = base + (long)k0 * ld;
+      bytes = ((long)(K - k0 - 1) * ld + ((wide + 7) & ~7)) * 2;
+    }
+    bytes = bytes < 0 ? 0 : bytes > 0x7FFFFFFF ? 0x7FFFFFFF : bytes;
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)bytes, 0x00020000);
+    const bool tail = !T && K - k0 < 64;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      uint32_t o = off[i];
+      if (tail) {
+        const int slot = i * NTHR + tid, r = slot >> 3, c = (slot & 7) ^ (QSIDE ? key_q(r) : key_p(r));
+        if (c * 8 >= K - k0) o = OUT;
+      }
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lptr_t)(img + i * NTHR * 16 + wave * 1024), 16, (int)o, 0, 0, 0);
+    }
+  }
+  // fragment of 16 rows at r0 for the 32 contraction steps ks: lane (i = lane & 15, j = lane >> 4) gets row i, steps 8 j ..
+  // 8 j + 7.  QSIDE: the 16 rows are 8 (i >> 2) + 4 half + (i & 3) of the 32 at r0, so that two fragments leave eight
+  // consecutive columns of the result in a lane.
+  __device__ __forceinline__ static bf16x8 frag(const lds_byte* img, int r0, int half, int ks, int lane) {
+    if constexpr (!T) {
+      const int i = lane & 15;
+      const int r = QSIDE ? r0 + 8 * (i >> 2) + 4 * half + (i & 3) : r0 + i;
+      const int c = (ks * 4 + (lane >> 4)) ^ (QSIDE ? key_q(r) : key_p(r));
+      return *reinterpret_cast<const LDS_AS bf16x8*>(img + r * 128 + c * 16);
+    } else {
+      const int k = ks * 32 + 8 * (lane >> 4) + ((lane & 15) >> 2);
+      const int col = QSIDE ? r0 + 8 * (lane & 3) + 4 * half : r0 + 4 * (lane & 3);
+      const lds_byte* p = img + k * (B * 2) + (((col >> 4) ^ key_q(k)) << 5) + (col & 15) * 2;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s16x4*)p);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s16x4*)(p + 4 * (B * 2)));   // (same key)
+      return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  }
+};
+
+template <int MODE, int BP, int BQ, int WP, int WQ>
+struct CeTile {
+  static constexpr int NW = WP * WQ, NTHR = NW * 64, MT = BP / WP / 16, NT = BQ / WQ / 16;
+  static constexpr bool TP = MODE == DW, TQ = MODE == DH || MODE == DW;
+  using OpP = Operand<TP, false, BP, NTHR>;
+  using OpQ = Operand<TQ, true, BQ, NTHR>;
+  static constexpr int STAGE = OpP::BYTES + OpQ::BYTES, SMEM = 2 * STAGE;
+
+  // one step of 64: the next step's operands are requested into `wr`, the products of `rd` are made.  The two never
+  // overlap, and saying so is what keeps the compiler from waiting for the DMA before every LDS read.
+  static __device__ __forceinline__ void step(f32x4 (&acc)[MT][NT], const OpP& p, const OpQ& q, lds_byte* __restrict__ wr,
+                                              const lds_byte* __restrict__ rd, bool more, int k1, int tid, int wave,
+                                              int pw0, int qw0, int lane) {
+    if (more) {
+      p.issue(wr, k1, tid, wave);
+      q.issue(wr + OpP::BYTES, k1, tid, wave);
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      bf16x8 pf[MT], qf[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) qf[nt] = OpQ::frag(rd + OpP::BYTES, qw0 + (nt >> 1) * 32, nt & 1, ks, lane);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) pf[mt] = OpP::frag(rd, pw0 + mt * 16, 0, ks, lane);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          acc[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf[nt], pf[mt], acc[mt][nt], 0, 0, 0);
+    }
+  }
+};
+
+template <int MODE, int BP, int BQ, int WP, int WQ>
+__global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_gemm_kernel(const CeGemm a) {
+  using Tile = CeTile<MODE, BP, BQ, WP, WQ>;
+  constexpr int MT = Tile::MT, NT = Tile::NT, NTHR = Tile::NTHR;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[Tile::SMEM];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // consecutive tiles to one XCD (workgroups go round the eight of them), in groups of eight rows of tiles: what runs at
+  // the same time there shares its operands in that XCD's L2
+  int id, ks_id = 0;
+  {
+    const int n = gridDim.x, q8 = n >> 3, r8 = n & 7, x = blockIdx.x & 7;
+    id = (x < r8 ? x * (q8 + 1) : r8 * (q8 + 1) + (x - r8) * q8) + ((int)blockIdx.x >> 3);
+  }
+  const int per = a.ptiles * a.qtiles;
+  if (MODE == DH) { ks_id = id / per; id -= ks_id * per; }
+  const int group = 8 * a.qtiles, gi = id / group, gp = a.ptiles - gi * 8 < 8 ? a.ptiles - gi * 8 : 8;
+  const int in = id - gi * group;
+  const int pt = gi * 8 + in % gp, qt = in / gp;
+  const int rows = piece_rows(a);
+  const int p0 = pt * BP, q0 = qt * BQ;
+  int K = a.K, kbeg = 0;
+  int Pn = a.Pn;
+  if (MODE == DW) K = rows;
+  else Pn = rows;
+  if (MODE != DW && p0 >= rows) return;   // (uniform: before any barrier)
+  int nsteps = (K + 63) >> 6;
+  if (MODE == DH && a.ksplit > 1) {
+    const int s0 = (int)((long)nsteps * ks_id / a.ksplit), s1 = (int)((long)nsteps * (ks_id + 1) / a.ksplit);
+    kbeg = s0 << 6;
+    nsteps = s1 - s0;
+  }
+  const int pw0 = (wave / WQ) * (BP / WP), qw0 = (wave % WQ) * (BQ / WQ);
+  typename Tile::OpP op;
+  typename Tile::OpQ oq;
+  op.init(a.P, a.ldp, p0, Pn, K, tid);
+  oq.init(a.Q, a.ldq, q0, a.Qn, K, tid);
+
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  lds_byte* const lds = (lds_byte*)smem;
+  if (nsteps > 0) {
+    op.issue(lds, kbeg, tid, wave);
+    oq.issue(lds + Tile::OpP::BYTES, kbeg, tid, wave);
+  }
+  for (int s = 0; s < nsteps; ++s) {
+    // this wave's share of step s has landed; behind the barrier everybody's has, and nobody reads the other stage
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    Tile::step(acc, op, oq, lds + ((s + 1) & 1) * Tile::STAGE, lds + (s & 1) * Tile::STAGE, s + 1 < nsteps,
+               kbeg + (s + 1) * 64, tid, wave, pw0, qw0, lane);
+  }
+
+  const int i16 = lane & 15, j4 = lane >> 4;
+  if constexpr (MODE == LOGIT_STATS || MODE == LOGIT_GRAD) {
+    // logits: row i16 of each 16, columns 32 tp + 8 j4 + e
+    if (a.bias) {
+#pragma unroll
+      for (int tp = 0; tp < NT / 2; ++tp)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int v = q0 + qw0 + tp * 32 + 8 * j4 + e;
+          const float b = v < a.Qn ? a.bias[v] : 0.f;
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) acc[mt][2 * tp + (e >> 2)][e & 3] += b;
+        }
+    }
+  }
+  if constexpr (MODE == LOGIT_STATS) {
+    float* red = reinterpret_cast<float*>(smem);   // [WQ][BP]
+    float mx[MT], sum[MT];
+    const bool edge = q0 + BQ > a.Qn;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const int m = p0 + pw0 + mt * 16 + i16;
+      if (edge) {   // columns past the vocabulary
+#pragma unroll
+        for (int tp = 0; tp < NT / 2; ++tp)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (q0 + qw0 + tp * 32 + 8 * j4 + e >= a.Qn) acc[mt][2 * tp + (e >> 2)][e & 3] = -INFINITY;
+      }
+      if (m < rows) {   // the target's logit, by the one lane that holds it
+        const int n = a.index ? a.index[m] : m;
+        const int64_t t = a.target[n] - (q0 + qw0 + 8 * j4);
+        if (t >= 0 && t < BQ / WQ && (t & 31) < 8) {
+          float x = 0.f;
+#pragma unroll
+          for (int tp = 0; tp < NT / 2; ++tp)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (t == tp * 32 + e) x = acc[mt][2 * tp + (e >> 2)][e & 3];
+          a.tlogit[m] = x;
+        }
+      }
+      float v = acc[mt][0][0];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v = fmaxf(v, acc[mt][nt][e]);
+      mx[mt] = xor32_max(xor16_max(v));
+    }
+    __syncthreads();   // every wave is done with the operands
+    if (j4 == 0)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) red[(wave % WQ) * BP + pw0 + mt * 16 + i16] = mx[mt];
+    __syncthreads();
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      float v = mx[mt];
+#pragma unroll
+      for (int w = 0; w < WQ; ++w) v = fmaxf(v, red[w * BP + pw0 + mt * 16 + i16]);
+      mx[mt] = v;
+      const float at = v == -INFINITY ? 0.f : v;   // a tile whose every logit is masked: exp(-inf - 0), not of NaN
+      float s = 0.f;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f((acc[mt][nt][e] - at) * LOG2E);
+      sum[mt] = xor32_sum(xor16_sum(s));
+    }
+    __syncthreads();
+    if (j4 == 0)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) red[(wave % WQ) * BP + pw0 + mt * 16 + i16] = sum[mt];
+    __syncthreads();
+    if (wave % WQ == 0 && j4 == 0)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        const int r = pw0 + mt * 16 + i16;
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < WQ; ++w) s += red[w * BP + r];
+        if (p0 + r < rows) a.part[(size_t)qt * a.rows_max + p0 + r] = make_float2(mx[mt], s);
+      }
+  }
+  if constexpr (MODE == LOGIT_GRAD) {
+    // the whole tile is written, zeros where no word is: the products read whole 16-byte pieces of a row
+    float col[NT / 2][8];
+#pragma unroll
+    for (int tp = 0; tp < NT / 2; ++tp)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) col[tp][e] = 0.f;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const int m = p0 + pw0 + mt * 16 + i16;
+      float lse = 0.f, wt = 0.f;
+      int64_t t = -1;
+      bool ok = m < rows;
+      if (ok) {
+        lse = a.lse[m];
+        wt = a.weight[m];
+        t = a.target[a.index[m]] - (q0 + qw0 + 8 * j4);
+        ok = lse != -INFINITY;   // a row whose every logit is masked has no gradient
+      }
+#pragma unroll
+      for (int tp = 0; tp < NT / 2; ++tp) {
+        bf16x8 o;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int v = q0 + qw0 + tp * 32 + 8 * j4 + e;
+          float x = __builtin_amdgcn_exp2f((acc[mt][2 * tp + (e >> 2)][e & 3] - lse) * LOG2E);
+          x = (x - (t == tp * 32 + e ? 1.f : 0.f)) * wt;
+          x = ok && v < a.Qn ? x : 0.f;
+          col[tp][e] += x;
+          o[e] = (bf16)x;
+        }
+        *reinterpret_cast<bf16x8*>(a.g + (size_t)m * a.ldg + q0 + qw0 + tp * 32 + 8 * j4) = o;
+      }
+    }
+    if (a.dbias_part) {
+      float* red = reinterpret_cast<float*>(smem);   // [WP][BQ]
+      __syncthreads();
+#pragma unroll
+      for (int tp = 0; tp < NT / 2; ++tp)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float s = row16_sum(col[tp][e]);
+          if (i16 == 0) red[(wave / WQ) * BQ + qw0 + tp * 32 + 8 * j4 + e] = s;
+        }
+      __syncthreads();
+      for (int c = tid; c < BQ; c += NTHR) {
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < WP; ++w) s += red[w * BQ + c];
+        a.dbias_part[(size_t)pt * a.ldg + q0 + c] = s;
+      }
+    }
+  }
+  if constexpr (MODE == DH || MODE == DW) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const int m = p0 + pw0 + mt * 16 + i16;
+      if (m >= Pn) continue;
+#pragma unroll
+      for (int tp = 0; tp < NT / 2; ++tp) {
+        const int c = q0 + qw0 + tp * 32 + 8 * j4;
+        if (c >= a.Qn) continue;   // (Qn is a multiple of 8)
+        f32x4 lo = acc[mt][2 * tp], hi = acc[mt][2 * tp + 1];
+        if (MODE == DH && a.slab) {
+          float* d = a.slab + ((size_t)ks_id * a.rows_max + m) * a.Qn + c;
+          *reinterpret_cast<f32x4*>(d) = lo;
+          *reinterpret_cast<f32x4*>(d + 4) = hi;
+          continue;
+        }
+        const size_t row = MODE == DH ? (size_t)a.index[m] : (size_t)m;
+        if (MODE == DW && a.acc_in) {
+          const float* s = a.acc_in + row * a.Qn + c;
+          lo += *reinterpret_cast<const f32x4*>(s);
+          hi += *reinterpret_cast<const f32x4*>(s + 4);
+        }
+        if (MODE == DW && a.out_f32) {
+          float* d = (float*)a.out + row * a.ldo + c;
+          *reinterpret_cast<f32x4*>(d) = lo;
+          *reinterpret_cast<f32x4*>(d + 4) = hi;
+        } else {
+          bf16x8 o;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { o[e] = (bf16)lo[e]; o[4 + e] = (bf16)hi[e]; }
+          *reinterpret_cast<bf16x8*>((bf16*)a.out + row * a.ldo + c) = o;
+        }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------- rows
+// The rows that count, numbered through in their order (one workgroup: 16 waves look at 1024 targets at a time), and the
+// losses of those that do not: 0 where the target is ignore_index, NaN where it is no word (and no gradient).
+__global__ __launch_bounds__(1024) void ce_index_kernel(const int64_t* target, int64_t ignore, int N, int V, int* index,
+                                                        int* count, float* loss, float* lse) {
+  __shared__ int waves[16];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int done = 0;
+  for (int base = 0; base < N; base += 1024) {
+    const int n = base + (int)threadIdx.x;
+    int64_t t = ignore;
+    if (n < N) t = target[n];
+    const bool word = t >= 0 && t < V, keep = n < N && t != ignore && word;
+    if (n < N && !keep) {
+      const float x = t == ignore ? 0.f : __builtin_nanf("");
+      loss[n] = x;
+      if (lse) lse[n] = x;
+    }
+    const unsigned long long b = __ballot(keep);
+    __syncthreads();
+    if (lane == 0) waves[w] = __popcll(b);
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int c = waves[i];
+      before += i < w ? c : 0;
+      all += c;
+    }
+    if (keep) index[done + before + __popcll(b & ((1ull << lane) - 1))] = n;
+    done += all;
+  }
+  if (threadIdx.x == 0) *count = done;
+}
+
+// A piece's rows, one after another (16 bytes per lane), and their weights
+__global__ __launch_bounds__(256) void ce_gather_kernel(const bf16* h, long ldh, int D8, const int* index, const int* count,
+                                                        int row0, int rows_max, const float* dloss, float scale, bf16* out,
+                                                        float* weight) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  const int r = (int)(i / D8), c = (int)(i - (long)r * D8);
+  int rows = *count - row0;
+  rows = rows < rows_max ? rows : rows_max;
+  if (r >= rows) return;
+  const int n = index[row0 + r];
+  if (c == 0) weight[r] = scale * (dloss ? dloss[n] : 1.f);
+  reinterpret_cast<uint4*>(out)[(long)r * D8 + c] = reinterpret_cast<const uint4*>(h + (long)n * ldh)[c];
+}
+
+// A row's pairs (max, sum) of all tiles of the vocabulary -> lse and loss: 16 rows per workgroup, 16 lanes each
+__global__ __launch_bounds__(256) void ce_rows_kernel(const float2* part, int tiles, int ld, const int* count, int row0,
+                                                      int rows_max, const int* index, const int64_t* target, int64_t ignore,
+                                                      int V, const float* tlogit, float* lse_c, float* loss, float* lse) {
+  __shared__ float rm[16][16], rs[16][16];
+  int rows = rows_max;
+  if (count) {
+    rows = *count - row0;
+    rows = rows < rows_max ? rows : rows_max;
+  }
+  const int i = threadIdx.x & 15, j = threadIdx.x >> 4, r = blockIdx.x * 16 + i;
+  if ((int)blockIdx.x * 16 >= rows) return;
+  float m = -INFINITY, s = 0.f;
+  if (r < rows)
+    for (int q = j; q < tiles; q += 16) {
+      const float2 p = part[(size_t)q * ld + r];
+      const float top = fmaxf(m, p.x), at = top == -INFINITY ? 0.f : top;
+      s = s * __builtin_amdgcn_exp2f((m - at) * LOG2E) + p.y * __builtin_amdgcn_exp2f((p.x - at) * LOG2E);
+      m = top;
+    }
+  rm[j][i] = m;
+  rs[j][i] = s;
+  __syncthreads();
+  if (j != 0 || r >= rows) return;
+  float top = m;
+#pragma unroll
+  for (int k = 1; k < 16; ++k) top = fmaxf(top, rm[k][i]);
+  const float at = top == -INFINITY ? 0.f : top;
+  float all = 0.f;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) all += rs[k][i] * __builtin_amdgcn_exp2f((rm[k][i] - at) * LOG2E);
+  float l = at + logf(all);   // all == 0: -inf, every logit of the row is masked
+  if (lse_c) lse_c[r] = l;
+  const int n = index ? index[row0 + r] : r;
+  float x;
+  const int64_t t = target[n];
+  if (!index && (t == ignore || t < 0 || t >= V)) x = l = t == ignore ? 0.f : __builtin_nanf("");
+  else x = l == -INFINITY ? INFINITY : l - tlogit[r];
+  loss[n] = x;
+  if (lse) lse[n] = l;
+}
+
+// dh of a piece from the slabs of its split contraction
+__global__ __launch_bounds__(256) void ce_slabs_kernel(const float* slab, int n, int rows_max, const int* index,
+                                                       const int* count, int row0, int D4, bf16* dh, long lddh) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  const int r = (int)(i / D4), c = (int)(i - (long)r * D4) * 4;
+  int rows = *count - row0;
+  rows = rows < rows_max ? rows : rows_max;
+  if (r >= rows) return;
+  const size_t stride = (size_t)rows_max * D4 * 4;
+  const float* p = slab + (size_t)r * D4 * 4 + c;
+  f32x4 s = *reinterpret_cast<const f32x4*>(p);
+  for (int k = 1; k < n; ++k) s += *reinterpret_cast<const f32x4*>(p + k * stride);
+  bf16x4 o;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = (bf16)s[e];
+  *reinterpret_cast<bf16x4*>(dh + (long)index[row0 + r] * lddh + c) = o;
+}
+
+// dh of the rows that do not count
+__global__ __launch_bounds__(256) void ce_zero_rows_kernel(const int64_t* target, int64_t ignore, int N, int V, int D8,
+                                                           bf16* dh, long lddh) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  const int n = (int)(i / D8), c = (int)(i - (long)n * D8);
+  if (n >= N) return;
+  const int64_t t = target[n];
+  if (t != ignore && t >= 0 && t < V) return;
+  reinterpret_cast<uint4*>(dh + (long)n * lddh)[c] = make_uint4(0, 0, 0, 0);
+}
+
+// dbias from the column sums of a piece's tiles, in order: acc_in (earlier pieces, or the caller's sum) + theirs
+__global__ __launch_bounds__(256) void ce_dbias_kernel(const float* part, long ld, int BP, const int* count, int row0,
+                                                       int rows_max, int V, const float* acc_in, void* out, int out_f32) {
+  const int v = blockIdx.x * 256 + threadIdx.x;
+  if (v >= V) return;
+  int rows = *count - row0;
+  rows = rows < 0 ? 0 : rows < rows_max ? rows : rows_max;
+  float s = 0.f;
+  for (int t = 0; t < (rows + BP - 1) / BP; ++t) s += part[(size_t)t * ld + v];
+  if (acc_in) s += acc_in[v];
+  if (out_f32) ((float*)out)[v] = s;
+  else ((bf16*)out)[v] = (bf16)s;
+}
+
+// ---------------------------------------------------------------------------------------------------- host
+struct CePlan {
+  long rows;          // per piece, a multiple of 256
+  int pieces, ksplit;
+  bool big;           // 256 x 256 tiles for the logits and dw
+  bool big_dh, big_dw;
+  long Vp;
+  size_t index, tlogit, lse, weight, part, hc, g, slab, dwacc, dbpart, dbacc, total;
+};
+
+constexpr size_t PIECE_BYTES = (size_t)4 << 30;   // g of a piece, unless the caller says how many rows
+
+bool sizes_ok(const mmst_linear_ce_args* a) {
+  return a && a->N >= 0 && a->N <= MMST_LINEAR_CE_MAX_ROWS && a->V >= 1 && a->V <= MMST_LINEAR_CE_MAX_VOCAB && a->D >= 8 &&
+         a->D % 8 == 0 && a->D <= MMST_LINEAR_CE_MAX_DIM && a->rows_per_piece >= 0 &&
+         (((long)a->N + 127) / 128) * (((long)a->V + 127) / 128) < 0x7FFFFFFFL;   // tiles of one launch
+}
+
+bool args_ok(const mmst_linear_ce_args* a, bool grad) {
+  if (!sizes_ok(a)) return false;
+  auto rows_ok = [&](const void* p, long ld, long n) {
+    return p && (uintptr_t)p % 16 == 0 && ld % 8 == 0 && (n <= 1 || ld >= a->D) && ld <= MMST_LINEAR_CE_MAX_LD;
+  };
+  if (!rows_ok(a->w, a->ldw, a->V)) return false;
+  if (a->N > 0 && (!rows_ok(a->h, a->ldh, a->N) || !a->target || !a->loss)) return false;
+  if (!grad) return true;
+  return (a->N == 0 || rows_ok(a->dh, a->lddh, a->N)) && a->dw && (uintptr_t)a->dw % 16 == 0;
+}
+
+size_t align(size_t x) { return (x + 255) & ~(size_t)255; }
+
+CePlan plan(const mmst_linear_ce_args* a, bool grad) {
+  CePlan p = {};
+  p.Vp = ((long)a->V + VT - 1) / VT * VT;
+  const long all = ((long)a->N + 255) / 256 * 256;
+  p.rows = all ? all : 256;
+  if (grad) {
+    long fit = a->rows_per_piece ? ((long)a->rows_per_piece + 255) / 256 * 256 : (long)(PIECE_BYTES / (p.Vp * 2)) / 256 * 256;
+    if (fit < 256) fit = 256;
+    if (p.rows > fit) p.rows = fit;
+  }
+  p.pieces = grad && all ? (int)((all + p.rows - 1) / p.rows) : 1;
+  auto tiles = [](long n, long m, int b) { return ((n + b - 1) / b) * ((m + b - 1) / b); };
+  p.big = tiles(p.rows, a->V, 256) >= 256;
+  p.big_dh = a->D > 128;
+  p.big_dw = a->D > 128 && tiles(a->V, a->D, 256) >= 256;
+  p.ksplit = 1;
+  if (grad) {
+    const long t = tiles(p.rows, a->D, p.big_dh ? 256 : 128), steps = p.Vp / 64;
+    long s = 256 / (t < 256 ? t : 256);
+    if (s > steps / 8) s = steps / 8;
+    p.ksplit = (int)(s < 1 ? 1 : s > 32 ? 32 : s);
+  }
+  size_t at = 256;   // [0]: count
+  auto take = [&](size_t n) { const size_t o = at; at += align(n); return o; };
+  const long qt = (a->V + (p.big ? 256 : 128) - 1) / (p.big ? 256 : 128);
+  p.tlogit = take(p.rows * 4);
+  p.part = take((size_t)qt * p.rows * 8);
+  if (grad) {
+    p.index = take((size_t)(all + 256) * 4);
+    p.lse = take(p.rows * 4);
+    p.weight = take(p.rows * 4);
+    p.hc = take((size_t)p.rows * a->D * 2);
+    p.g = take((size_t)p.rows * p.Vp * 2);
+    if (p.ksplit > 1) p.slab = take((size_t)p.ksplit * p.rows * a->D * 4);
+    if (p.pieces > 1 && !a->grad_f32) p.dwacc = take((size_t)a->V * a->D * 4);
+    if (a->dbias) {
+      p.dbpart = take((size_t)(p.rows / 128) * p.Vp * 4);
+      if (p.pieces > 1 && !a->grad_f32) p.dbacc = take((size_t)a->V * 4);
+    }
+  }
+  p.total = at;
+  return p;
+}
+
+template <int MODE> void launch(CeGemm& g, bool big, long prows, long qcols, hipStream_t st) {
+  const int b = big ? 256 : 128;
+  g.ptiles = (int)((prows + b - 1) / b);
+  g.qtiles = (int)((qcols + b - 1) / b);
+  const unsigned grid = (unsigned)(g.ptiles * g.qtiles * g.ksplit);
+  if (big) hipLaunchKernelGGL((ce_gemm_kernel<MODE, 256, 256, 2, 4>), dim3(grid), dim3(512), 0, st, g);
+  else hipLaunchKernelGGL((ce_gemm_kernel<MODE, 128, 128, 2, 2>), dim3(grid), dim3(256), 0, st, g);
+}
+
+}  // namespace
+
+extern "C" {
+
+int mmst_linear_ce_ws(const mmst_linear_ce_args* args, int grad, size_t* bytes) {
+  if (!bytes || !sizes_ok(args)) return MMST_ERR_ARG;
+  *bytes = plan(args, grad != 0).total;
+  return MMST_OK;
+}
+
+int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
+  if (!args_ok(args, grad != 0)) return MMST_ERR_ARG;
+  const mmst_linear_ce_args& A = *args;
+  const CePlan p = plan(args, grad != 0);
+  if (A.N == 0 && !grad) return MMST_OK;
+  if (!A.ws || (uintptr_t)A.ws % 256 || A.ws_bytes < p.total) return MMST_ERR_ARG;
+  hipStream_t st = (hipStream_t)stream;
+  char* ws = (char*)A.ws;
+  int* count = (int*)ws;
+  int* index = (int*)(ws + p.index);
+  const bf16* w = (const bf16*)A.w;
+  const int D = A.D, V = A.V, N = A.N, D8 = D / 8;
+
+  CeGemm logit = {};
+  logit.Q = w; logit.ldq = A.ldw; logit.Qn = V; logit.K = D; logit.ksplit = 1;
+  logit.bias = A.bias; logit.target = A.target;
+  logit.part = (float2*)(ws + p.part); logit.tlogit = (float*)(ws + p.tlogit);
+  logit.rows_max = (int)p.rows;
+  if (!grad) {
+    logit.P = (const bf16*)A.h; logit.ldp = A.ldh; logit.rows_max = N; logit.Pn = N;
+    launch<LOGIT_STATS>(logit, p.big, N, V, st);
+    MMST_CHECK_LAUNCH();
+    hipLaunchKernelGGL(ce_rows_kernel, dim3((N + 15) / 16), dim3(256), 0, st, logit.part, logit.qtiles, N, nullptr, 0, N,
+                       nullptr, A.target, A.ignore_index, V, logit.tlogit, nullptr, A.loss, A.lse);
+    MMST_CHECK_LAUNCH();
+    return MMST_OK;
+  }
+
+  hipLaunchKernelGGL(ce_index_kernel, dim3(1), dim3(1024), 0, st, A.target, A.ignore_index, N, V, index, count, A.loss, A.lse);
+  MMST_CHECK_LAUNCH();
+  if (N > 0) {
+    hipLaunchKernelGGL(ce_zero_rows_kernel, dim3((unsigned)(((long)N * D8 + 255) / 256)), dim3(256), 0, st, A.target,
+                       A.ignore_index, N, V, D8, (bf16*)A.dh, A.lddh);
+    MMST_CHECK_LAUNCH();
+  }
+  bf16* hc = (bf16*)(ws + p.hc);
+  bf16* gbuf = (bf16*)(ws + p.g);
+  float* lse_c = (float*)(ws + p.lse);
+  float* weight = (float*)(ws + p.weight);
+  const int BPg = p.big ? 256 : 128;
+  for (int i = 0; i < p.pieces; ++i) {
+    const int row0 = (int)(i * p.rows);
+    const int rows_max = (int)p.rows;
+    hipLaunchKernelGGL(ce_gather_kernel, dim3((unsigned)((p.rows * D8 + 255) / 256)), dim3(256), 0, st, (const bf16*)A.h, A.ldh,
+                       D8, index, count, row0, rows_max, A.dloss, A.grad_scale, hc, weight);
+    MMST_CHECK_LAUNCH();
+    logit.P = hc; logit.ldp = D; logit.Pn = rows_max; logit.count = count; logit.row0 = row0; logit.index = index + row0;
+    launch<LOGIT_STATS>(logit, p.big, p.rows, V, st);
+    MMST_CHECK_LAUNCH();
+    hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)(p.rows / 16)), dim3(256), 0, st, logit.part, logit.qtiles, rows_max, count,
+                       row0, rows_max, index, A.target, A.ignore_index, V, logit.tlogit, lse_c, A.loss, A.lse);
+    MMST_CHECK_LAUNCH();
+    CeGemm gr = logit;
+    gr.lse = lse_c; gr.weight = weight; gr.g = gbuf; gr.ldg = p.Vp;
+    gr.dbias_part = A.dbias ? (float*)(ws + p.dbpart) : nullptr;
+    launch<LOGIT_GRAD>(gr, p.big, p.rows, p.Vp, st);
+    MMST_CHECK_LAUNCH();
+
+    CeGemm dh = {};
+    dh.P = gbuf; dh.ldp = p.Vp; dh.Pn = rows_max; dh.Q = w; dh.ldq = A.ldw; dh.Qn = D; dh.K = V;
+    dh.count = count; dh.row0 = row0; dh.rows_max = rows_max; dh.index = index + row0; dh.ksplit = p.ksplit;
+    dh.out = A.dh; dh.ldo = A.lddh; dh.slab = p.ksplit > 1 ? (float*)(ws + p.slab) : nullptr;
+    launch<DH>(dh, p.big_dh, p.rows, D, st);
+    MMST_CHECK_LAUNCH();
+    if (p.ksplit > 1) {
+      hipLaunchKernelGGL(ce_slabs_kernel, dim3((unsigned)((p.rows * (D / 4) + 255) / 256)), dim3(256), 0, st,
+                         (const float*)dh.slab, p.ksplit, rows_max, index, count, row0, D / 4, (bf16*)A.dh, A.lddh);
+      MMST_CHECK_LAUNCH();
+    }
+
+    // dw and dbias: in fp32 added to what is there; in bf16 written once, behind sums in fp32 where there are more pieces
+    const bool last = i + 1 == p.pieces;
+    CeGemm dw = {};
+    dw.P = gbuf; dw.ldp = p.Vp; dw.Pn = V; dw.Q = hc; dw.ldq = D; dw.Qn = D;
+    dw.count = count; dw.row0 = row0; dw.rows_max = rows_max; dw.ksplit = 1;
+    float* acc = (float*)(ws + p.dwacc);
+    dw.ldo = D;
+    if (A.grad_f32) { dw.out = A.dw; dw.out_f32 = 1; dw.acc_in = (const float*)A.dw; }
+    else { dw.out = last ? A.dw : (void*)acc; dw.out_f32 = last ? 0 : 1; dw.acc_in = i > 0 ? acc : nullptr; }
+    launch<DW>(dw, p.big_dw, V, D, st);
+    MMST_CHECK_LAUNCH();
+    if (A.dbias) {
+      float* bacc = (float*)(ws + p.dbacc);
+      const float* from = A.grad_f32 ? (const float*)A.dbias : i > 0 ? bacc : nullptr;
+      void* to = A.grad_f32 || last ? A.dbias : (void*)bacc;
+      hipLaunchKernelGGL(ce_dbias_kernel, dim3((V + 255) / 256), dim3(256), 0, st, (const float*)(ws + p.dbpart), p.Vp, BPg, count,
+                         row0, rows_max, V, from, to, A.grad_f32 || !last ? 1 : 0);
+      MMST_CHECK_LAUNCH();
+    }
+  }
+  return MMST_OK;
+}
+
+int mmst_sizeof_linear_ce_args(void) { return (int)sizeof(mmst_linear_ce_args); }
+
+}  // extern "C"

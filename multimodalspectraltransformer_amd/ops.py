@@ -122,6 +122,8 @@ _SIGNATURES = {
     "mmst_layer_norm_bwd": [_P, _LONG, _P, _LONG, _P, _P, _P, _LONG, _P, _LONG, _P, _LONG, _P, _P, _I, _I, _LONG, _I, _D,
                             _U64, _U64, _P, _SIZE, _P],
     "mmst_layer_norm_bwd_ws": [_LONG, _I, _P],
+    "mmst_linear_ce": [_P, _I, _P],
+    "mmst_linear_ce_ws": [_P, _I, _P],
 }
 _functions = {}
 
@@ -276,3 +278,81 @@ def layer_norm_bwd(dy, z, stats, gamma=None, dz_in=None, p=0.0, seed=0, offset=0
           dz.data_ptr(), cols, dx.data_ptr(), cols, dgp, dbp, int(accumulate), _DTYPES[dtype], rows, cols, p, seed, offset,
           ws.data_ptr(), nbytes.value)
     return dz, dx, dgamma, dbeta
+
+
+# ---------------------------------------------------------------------------------------------
+# linear layer + softmax cross entropy over a large vocabulary (mmst_linear_ce)
+# ---------------------------------------------------------------------------------------------
+def _linear_ce_args(h, w, target, bias, ignore_index, what):
+    for t, name in ((h, "h"), (w, "w")):
+        _check(isinstance(t, torch.Tensor) and t.is_cuda, f"{what}: {name} on the GPU expected (there is no CPU path)")
+        _check(t.dtype == torch.bfloat16 and t.dim() == 2, f"{what}: {name} as a bf16 matrix expected, got {t.dtype} {tuple(t.shape)}")
+    device, (n, d), v = h.device, h.shape, w.shape[0]
+    _check(w.device == device and w.shape[1] == d, f"{what}: h {tuple(h.shape)} and w {tuple(w.shape)} do not fit")
+    _check(v >= 1 and d >= 8 and d % 8 == 0, f"{what}: a vocabulary and a width that is a multiple of 8 expected, got {v} and {d}")
+    _check(target.dtype == torch.int64 and target.device == device and target.shape == (n,),
+           f"{what}: target as int64 [{n}] on {device} expected, got {target.dtype} {tuple(target.shape)} on {target.device}")
+    a = L.LinearCeArgs()
+    keep = []   # copies of inputs whose layout the kernels do not read
+    for t, name in ((h, "h"), (w, "w")):
+        if t.stride(1) != 1 or t.stride(0) % 8 or (t.shape[0] > 1 and t.stride(0) < d) or t.data_ptr() % 16:
+            t = torch.empty_like(t, memory_format=torch.contiguous_format).copy_(t)
+            keep.append(t)
+        setattr(a, name, t.data_ptr())
+        setattr(a, "ld" + name, t.stride(0) if t.shape[0] > 1 else d)
+    if not target.is_contiguous():
+        target = target.contiguous()
+        keep.append(target)
+    a.target = target.data_ptr()
+    a.bias = _vector(bias, v, device, f"{what}: bias")
+    a.ignore_index = ignore_index
+    a.N, a.D, a.V = n, d, v
+    return a, keep
+
+
+def _linear_ce_call(a, grad, device):
+    nbytes = C.c_size_t()
+    _check(_function("mmst_linear_ce_ws")(C.byref(a), grad, C.byref(nbytes)) == 0,
+           f"linear_ce: sizes outside the limits: {a.N} rows, {a.V} words, width {a.D}")
+    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=device)
+    a.ws, a.ws_bytes = ws.data_ptr(), nbytes.value
+    _call("mmst_linear_ce", device, C.byref(a), grad)
+
+
+def linear_ce(h, w, target, bias=None, ignore_index=-100):
+    """(loss, lse), both fp32 [N]: softmax cross entropy of the logits h w^T + bias against target, and the rows' log sum
+    exp, without the logits in memory.  h [N, D], w [V, D] bf16, target int64 [N], bias fp32 [V] or None; D a multiple of 8.
+    Rows whose target is ignore_index have loss and lse 0; a target that is no word gives NaN."""
+    a, keep = _linear_ce_args(h, w, target, bias, ignore_index, "linear_ce")
+    loss, lse = torch.empty(2, a.N, dtype=torch.float32, device=h.device).unbind(0)
+    a.loss, a.lse = loss.data_ptr(), lse.data_ptr()
+    _linear_ce_call(a, 0, h.device)
+    return loss, lse
+
+
+def linear_ce_grad(h, w, target, bias=None, dloss=None, grad_scale=1.0, ignore_index=-100, dw=None, dbias=None,
+                   rows_per_piece=0):
+    """(loss, lse, dh, dw, dbias): linear_ce() and the gradients of sum(grad_scale * dloss * loss) (dloss fp32 [N], None:
+    ones).  dh is bf16; dw and dbias are bf16 as well, or, where fp32 tensors are given, added to those.  dbias is None
+    without a bias.  rows_per_piece bounds the workspace: that many rows' gradient of the logits, in bf16, at a time."""
+    a, keep = _linear_ce_args(h, w, target, bias, ignore_index, "linear_ce_grad")
+    device, n, d, v = h.device, a.N, a.D, a.V
+    _check(rows_per_piece >= 0, "linear_ce_grad: rows_per_piece must not be negative")
+    loss, lse = torch.empty(2, n, dtype=torch.float32, device=device).unbind(0)
+    dh = torch.empty(n, d, dtype=torch.bfloat16, device=device)
+    a.loss, a.lse, a.dh, a.lddh = loss.data_ptr(), lse.data_ptr(), dh.data_ptr(), d
+    a.dloss = _vector(dloss, n, device, "linear_ce_grad: dloss")
+    a.grad_scale, a.rows_per_piece = grad_scale, rows_per_piece
+    if dw is None:
+        _check(dbias is None, "linear_ce_grad: dbias to be added to comes with dw")
+        dw = torch.empty(v, d, dtype=torch.bfloat16, device=device)
+        dbias = None if bias is None else torch.empty(v, dtype=torch.bfloat16, device=device)
+    else:
+        _check(dw.dtype == torch.float32 and dw.device == device and dw.shape == (v, d) and dw.is_contiguous() and dw.data_ptr() % 16 == 0,
+               f"linear_ce_grad: dw as contiguous fp32 [{v}, {d}] on {device} expected")
+        _check((dbias is None) == (bias is None), "linear_ce_grad: dbias comes with bias")
+        _vector(dbias, v, device, "linear_ce_grad: dbias")
+        a.grad_f32 = 1
+    a.dw, a.dbias = dw.data_ptr(), None if dbias is None else dbias.data_ptr()
+    _linear_ce_call(a, 1, device)
+    return loss, lse, dh, dw, dbias
