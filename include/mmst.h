@@ -437,7 +437,7 @@ int mmst_layer_norm_bwd(const void* dy, long lddy, const void* z, long ldz, cons
                         const void* dz_in, long lddz_in, void* dz, long lddz, void* dx, long lddx, float* dgamma,
                         float* dbeta, int accumulate, int dtype, long rows, int cols, double p, uint64_t seed,
                         uint64_t offset, void* ws, size_t ws_bytes, void* stream);
-int mmst_layer_norm_bwd_ws(long rows, int cols, size_t* bytes);
+int mmst_layer_norm_bwd_ws(int dtype, long rows, int cols, size_t* bytes);
 
 /* ---- linear layer with softmax cross entropy over a large vocabulary, without the logits in memory ----
  * logits = h w^T + bias (bf16 operands, fp32 accumulation), loss[n] = logsumexp(logits[n]) - logits[n][target[n]]: what

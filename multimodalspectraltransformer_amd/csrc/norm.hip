@@ -8,8 +8,8 @@
 //
 // All of it is bound by HBM: every tensor is read or written once and a row stays in registers between the statistics and
 // the output.  TPR lanes own a row (16 lanes for 128 columns up to a workgroup of 1024 for 16384), NV groups of eight
-// columns each, so that a lane's accesses are 16 bytes wide; rows that are not made of aligned groups of eight (odd
-// widths, odd strides, unaligned pointers) take the same kernels with one element per lane and access.
+// columns each, so that a lane's accesses are 16 bytes wide, whatever their alignment; only the last group of a row whose
+// width is no multiple of eight goes by elements.
 #include "../../include/mmst.h"
 #include "philox.h"
 
@@ -18,11 +18,15 @@ namespace {
 typedef _Float16 f16;
 template <typename T> struct Vec8 { T v[8]; } __attribute__((aligned(16)));
 
+// Eight elements as 16-byte accesses at any alignment of an element: the hardware takes them (a wave's 1 KiB touches one
+// more cache line then), so rows of odd widths and strides need no form of their own.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <int A> struct __attribute__((packed, aligned(A))) Packed16 { u32x4 v; };
 template <typename T> __device__ __forceinline__ void load_vec(Vec8<T>& d, const T* p) {
   constexpr int N = sizeof(Vec8<T>) / 16;
-  uint4 u[N];
+  u32x4 u[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) u[i] = reinterpret_cast<const uint4*>(p)[i];
+  for (int i = 0; i < N; ++i) u[i] = reinterpret_cast<const Packed16<sizeof(T)>*>(p)[i].v;
   __builtin_memcpy(&d, u, sizeof d);
 }
 template <typename T> __device__ __forceinline__ void store_vec(T* p, const float (&v)[8]) {
@@ -30,10 +34,10 @@ template <typename T> __device__ __forceinline__ void store_vec(T* p, const floa
 #pragma unroll
   for (int e = 0; e < 8; ++e) d.v[e] = (T)v[e];
   constexpr int N = sizeof(Vec8<T>) / 16;
-  uint4 u[N];
+  u32x4 u[N];
   __builtin_memcpy(u, &d, sizeof d);
 #pragma unroll
-  for (int i = 0; i < N; ++i) reinterpret_cast<uint4*>(p)[i] = u[i];
+  for (int i = 0; i < N; ++i) reinterpret_cast<Packed16<sizeof(T)>*>(p)[i].v = u[i];
 }
 
 // ---------------------------------------------------------------------------------------------------- dropout
@@ -43,7 +47,7 @@ struct DropArgs {
   DropKey key;
 };
 
-// blocks of eight elements that lie inside one row and can be read as vectors; FLAT: rows follow one another
+// blocks of eight elements that lie inside one row; FLAT: rows follow one another
 template <typename T, bool FLAT, int U>
 __global__ __launch_bounds__(256) void dropout_vec_kernel(const DropArgs a) {
   const uint64_t nb = a.n >> 3, per_row = a.cols >> 3;
@@ -86,7 +90,8 @@ __global__ __launch_bounds__(256) void dropout_vec_kernel(const DropArgs a) {
   }
 }
 
-// any strides and alignment: a wave owns 512 consecutive elements, a lane one element per access
+// rows of an odd width that do not follow one another, so that a block may lie in two or more: a wave owns 512 consecutive
+// elements, a lane one element per access
 template <typename T>
 __global__ __launch_bounds__(256) void dropout_elem_kernel(const DropArgs a) {
   __shared__ uint4 slots[4][65];
@@ -117,10 +122,10 @@ __global__ __launch_bounds__(256) void dropout_elem_kernel(const DropArgs a) {
     if (first + j * 64 + lane < a.n) ((T*)a.y)[oy[j]] = (T)v[j];
 }
 
-template <typename T> int launch_dropout(const DropArgs& a, bool vec, hipStream_t st) {
+template <typename T> int launch_dropout(const DropArgs& a, hipStream_t st) {
   const bool flat = a.ldx == a.cols && a.ldy == a.cols;
   constexpr int U = sizeof(T) == 4 ? 1 : 2;
-  if (vec && (flat || a.cols % 8 == 0)) {
+  if (flat || a.cols % 8 == 0) {
     const uint64_t grid = (a.n / 8 + 256 * U - 1) / (256 * U);
     if (grid > 0x7FFFFFFFu) return MMST_ERR_ARG;
     if (flat) hipLaunchKernelGGL((dropout_vec_kernel<T, true, U>), dim3(grid ? (unsigned)grid : 1u), dim3(256), 0, st, a);
@@ -167,97 +172,85 @@ template <int TPR, int BLK> __device__ __forceinline__ float row_sum(float v, fl
   }
 }
 
-// column of element e of group q of lane t: groups of eight consecutive columns, or one column per lane of a wave
-template <bool VEC, int TPR> __device__ __forceinline__ int ln_col(int q, int e, int t) {
-  constexpr int G = TPR < 64 ? TPR : 64;
-  if constexpr (VEC) return (q * TPR + t) * 8 + e;
-  else return (q * TPR + (t / G) * G) * 8 + e * G + t % G;
-}
-
-template <typename T, bool VEC, int TPR, int NV>
+// Group q of lane t of a row: columns (q * TPR + t) * 8 .. + 7.  ODD: cols is no multiple of eight, so one lane's last
+// group is cut off.
+template <typename T, bool ODD, int TPR, int NV>
 __device__ __forceinline__ void ln_load(Vec8<T> (&d)[NV], const T* row, int cols, int t, bool ok) {
 #pragma unroll
   for (int q = 0; q < NV; ++q) {
-    if constexpr (VEC) {
-      const int c = (q * TPR + t) * 8;
-      if (ok && c < cols) load_vec(d[q], row + c);
-      else
-#pragma unroll
-        for (int e = 0; e < 8; ++e) d[q].v[e] = (T)0.f;
+    const int c = (q * TPR + t) * 8;
+    if (ok && c + (ODD ? 7 : 0) < cols) {
+      load_vec(d[q], row + c);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int c = ln_col<false, TPR>(q, e, t);
-        d[q].v[e] = ok && c < cols ? row[c] : (T)0.f;
-      }
+      for (int e = 0; e < 8; ++e) d[q].v[e] = (T)0.f;
+      if (ODD && ok && c < cols)
+#pragma unroll
+        for (int e = 0; e < 7; ++e)
+          if (c + e < cols) d[q].v[e] = row[c + e];
     }
   }
 }
-template <typename T, bool VEC, int TPR>
+template <typename T, bool ODD, int TPR>
 __device__ __forceinline__ void ln_store(T* row, const float (&v)[8], int cols, int q, int t) {
-  if constexpr (VEC) {
-    const int c = (q * TPR + t) * 8;
-    if (c < cols) store_vec(row + c, v);
-  } else {
+  const int c = (q * TPR + t) * 8;
+  if (c + (ODD ? 7 : 0) < cols) {
+    store_vec(row + c, v);
+  } else if (ODD && c < cols) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int c = ln_col<false, TPR>(q, e, t);
-      if (c < cols) row[c] = (T)v[e];
-    }
+    for (int e = 0; e < 7; ++e)
+      if (c + e < cols) row[c + e] = (T)v[e];
   }
 }
-template <bool VEC, int TPR>
+template <bool ODD, int TPR>
 __device__ __forceinline__ void ln_vec_f32(float (&v)[8], const float* p, float none, int cols, int q, int t) {
-  if constexpr (VEC) {
-    const int c = (q * TPR + t) * 8;
-    if (p && c < cols) {
-      const f32x4 a = *reinterpret_cast<const f32x4*>(p + c), b = *reinterpret_cast<const f32x4*>(p + c + 4);
+  const int c = (q * TPR + t) * 8;
+  if (p && c + (ODD ? 7 : 0) < cols) {
+    Vec8<float> d;
+    load_vec(d, p + c);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
-      return;
-    }
+    for (int e = 0; e < 8; ++e) v[e] = d.v[e];
+  } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = none;
-  } else {
+    if (ODD && p && c < cols)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int c = ln_col<false, TPR>(q, e, t);
-      v[e] = p && c < cols ? p[c] : none;
-    }
+      for (int e = 0; e < 7; ++e)
+        if (c + e < cols) v[e] = p[c + e];
   }
 }
 // dropout of group q of row r, whose elements are r * cols + column of the tensor read row by row
-template <bool VEC, int TPR>
+template <bool ODD, int TPR>
 __device__ __forceinline__ void ln_drop(float (&v)[8], const DropKey& k, long r, int cols, int q, int t, uint4* slots) {
-  if constexpr (VEC) {
+  if constexpr (!ODD) {
     drop_block(v, philox_block((uint64_t)r * (uint64_t)(cols >> 3) + (uint64_t)(q * TPR + t), k), k);
   } else {
     constexpr int G = TPR < 64 ? TPR : 64;
-    drop_elements<G>(v, (uint64_t)r * cols + (uint64_t)((q * TPR + (t / G) * G) * 8), k,
-                     slots + (threadIdx.x / G) * (G + 1), t % G);
+    drop_straddling<G>(v, (uint64_t)r * cols + (uint64_t)((q * TPR + (t / G) * G) * 8), k,
+                       slots + (threadIdx.x / G) * (G + 1), t % G);
   }
 }
 
-template <typename T, bool VEC, int TPR, int NV, int BLK>
+template <typename T, bool ODD, int TPR, int NV, int BLK>
 __global__ __launch_bounds__(BLK) void ln_fwd_kernel(const LnArgs a) {
   constexpr int RPB = BLK / TPR, G = TPR < 64 ? TPR : 64;
   __shared__ float red[2][BLK / 64];
-  __shared__ uint4 slots[VEC ? 1 : (BLK / G) * (G + 1)];
+  __shared__ uint4 slots[!ODD ? 1 : (BLK / G) * (G + 1)];
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, cols = a.cols;
   int turn = 0;
   for (long base = (long)blockIdx.x * RPB; base < a.rows; base += (long)gridDim.x * RPB) {
     const long r = base + sub;
     const bool ok = r < a.rows;
     Vec8<T> x[NV], rs[NV];
-    ln_load<T, VEC, TPR, NV>(x, (const T*)a.x + r * a.ldx, cols, t, ok);
-    if (a.res) ln_load<T, VEC, TPR, NV>(rs, (const T*)a.res + r * a.ldr, cols, t, ok);
+    ln_load<T, ODD, TPR, NV>(x, (const T*)a.x + r * a.ldx, cols, t, ok);
+    if (a.res) ln_load<T, ODD, TPR, NV>(rs, (const T*)a.res + r * a.ldr, cols, t, ok);
     float z[NV][8];
     float s = 0.f;
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) z[q][e] = (float)x[q].v[e];
-      if (a.key.thr) ln_drop<VEC, TPR>(z[q], a.key, r, cols, q, t, slots);
+      if (a.key.thr) ln_drop<ODD, TPR>(z[q], a.key, r, cols, q, t, slots);
       if (a.res)
 #pragma unroll
         for (int e = 0; e < 8; ++e) z[q][e] += (float)rs[q].v[e];
@@ -270,31 +263,31 @@ __global__ __launch_bounds__(BLK) void ln_fwd_kernel(const LnArgs a) {
     for (int q = 0; q < NV; ++q)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float d = ln_col<VEC, TPR>(q, e, t) < cols ? z[q][e] - mean : 0.f;
+        const float d = (q * TPR + t) * 8 + (ODD ? e : 0) < cols ? z[q][e] - mean : 0.f;
         vs += d * d;
       }
     const float rstd = 1.0f / sqrtf(row_sum<TPR, BLK>(vs, red, turn) / (float)cols + a.eps);
     if (ok) {
 #pragma unroll
       for (int q = 0; q < NV; ++q) {
-        if (a.z) ln_store<T, VEC, TPR>((T*)a.z + r * a.ldz, z[q], cols, q, t);
+        if (a.z) ln_store<T, ODD, TPR>((T*)a.z + r * a.ldz, z[q], cols, q, t);
         float g[8], b[8], y[8];
-        ln_vec_f32<VEC, TPR>(g, a.gamma, 1.f, cols, q, t);
-        ln_vec_f32<VEC, TPR>(b, a.beta, 0.f, cols, q, t);
+        ln_vec_f32<ODD, TPR>(g, a.gamma, 1.f, cols, q, t);
+        ln_vec_f32<ODD, TPR>(b, a.beta, 0.f, cols, q, t);
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = (z[q][e] - mean) * rstd * g[e] + b[e];
-        ln_store<T, VEC, TPR>((T*)a.y + r * a.ldy, y, cols, q, t);
+        ln_store<T, ODD, TPR>((T*)a.y + r * a.ldy, y, cols, q, t);
       }
       if (t == 0 && a.stats) { a.stats[2 * r] = mean; a.stats[2 * r + 1] = rstd; }
     }
   }
 }
 
-template <typename T, bool VEC, int TPR, int NV, int BLK>
+template <typename T, bool ODD, int TPR, int NV, int BLK>
 __global__ __launch_bounds__(BLK) void ln_bwd_kernel(const LnArgs a) {
   constexpr int RPB = BLK / TPR, G = TPR < 64 ? TPR : 64, CAP = TPR * NV * 8;
   __shared__ float red[2][BLK / 64];
-  __shared__ uint4 slots[VEC ? 1 : (BLK / G) * (G + 1)];
+  __shared__ uint4 slots[!ODD ? 1 : (BLK / G) * (G + 1)];
   __shared__ float sums[RPB > 1 ? RPB * CAP : 1];
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, cols = a.cols;
   int turn = 0;
@@ -307,16 +300,16 @@ __global__ __launch_bounds__(BLK) void ln_bwd_kernel(const LnArgs a) {
     const long r = base + sub;
     const bool ok = r < a.rows;
     Vec8<T> dy[NV], zv[NV], add[NV];
-    ln_load<T, VEC, TPR, NV>(dy, (const T*)a.x + r * a.ldx, cols, t, ok);
-    ln_load<T, VEC, TPR, NV>(zv, (const T*)a.zin + r * a.ldzin, cols, t, ok);
-    if (a.res) ln_load<T, VEC, TPR, NV>(add, (const T*)a.res + r * a.ldr, cols, t, ok);
+    ln_load<T, ODD, TPR, NV>(dy, (const T*)a.x + r * a.ldx, cols, t, ok);
+    ln_load<T, ODD, TPR, NV>(zv, (const T*)a.zin + r * a.ldzin, cols, t, ok);
+    if (a.res) ln_load<T, ODD, TPR, NV>(add, (const T*)a.res + r * a.ldr, cols, t, ok);
     const float mean = ok ? a.stats[2 * r] : 0.f, rstd = ok ? a.stats[2 * r + 1] : 0.f;
     float xh[NV][8], qv[NV][8];
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
       float g[8];
-      ln_vec_f32<VEC, TPR>(g, a.gamma, 1.f, cols, q, t);
+      ln_vec_f32<ODD, TPR>(g, a.gamma, 1.f, cols, q, t);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float d = (float)dy[q].v[e];   // zero past the last column and row, so every sum is
@@ -338,10 +331,10 @@ __global__ __launch_bounds__(BLK) void ln_bwd_kernel(const LnArgs a) {
       if (a.res)
 #pragma unroll
         for (int e = 0; e < 8; ++e) dz[e] += (float)add[q].v[e];
-      if (ok) ln_store<T, VEC, TPR>((T*)a.y + r * a.ldy, dz, cols, q, t);
+      if (ok) ln_store<T, ODD, TPR>((T*)a.y + r * a.ldy, dz, cols, q, t);
       if (a.key.thr) {   // (every lane: the lanes of a row share the generator's words)
-        ln_drop<VEC, TPR>(dz, a.key, r, cols, q, t, slots);
-        if (ok) ln_store<T, VEC, TPR>((T*)a.z + r * a.ldz, dz, cols, q, t);
+        ln_drop<ODD, TPR>(dz, a.key, r, cols, q, t, slots);
+        if (ok) ln_store<T, ODD, TPR>((T*)a.z + r * a.ldz, dz, cols, q, t);
       }
     }
   }
@@ -355,7 +348,7 @@ __global__ __launch_bounds__(BLK) void ln_bwd_kernel(const LnArgs a) {
       for (int q = 0; q < NV; ++q)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int c = ln_col<VEC, TPR>(q, e, t);
+          const int c = (q * TPR + t) * 8 + e;
           if (c < cols) part[w * cols + c] = w ? pb[q][e] : pg[q][e];
         }
     } else {
@@ -363,7 +356,7 @@ __global__ __launch_bounds__(BLK) void ln_bwd_kernel(const LnArgs a) {
 #pragma unroll
       for (int q = 0; q < NV; ++q)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sums[sub * CAP + ln_col<VEC, TPR>(q, e, t)] = w ? pb[q][e] : pg[q][e];
+        for (int e = 0; e < 8; ++e) sums[sub * CAP + (q * TPR + t) * 8 + e] = w ? pb[q][e] : pg[q][e];
       __syncthreads();
       for (int c = threadIdx.x; c < cols; c += BLK) {
         float s = 0.f;
@@ -375,25 +368,28 @@ __global__ __launch_bounds__(BLK) void ln_bwd_kernel(const LnArgs a) {
   }
 }
 
-// dgamma / dbeta = sum over the n workgroups' column sums, in order: 64 columns per workgroup, 16 slices of the rows
+// dgamma / dbeta = sum over the n workgroups' column sums, in order: 16 columns per workgroup, 64 slices of the rows, so
+// that the up to 1024 rows of a narrow layer norm are 16 loads deep (with 64 columns and 16 slices: 6.0 us at 1024 x 256)
 __global__ __launch_bounds__(1024) void ln_cols_kernel(const float* part, int n, int cols, float* dgamma, float* dbeta,
                                                        int accumulate) {
-  __shared__ float red[16][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const long c = (long)blockIdx.x * 64 + lane;
+  __shared__ float red[64][17];
+  const int lane = threadIdx.x & 15, w = threadIdx.x >> 4;
+  const long c = (long)blockIdx.x * 16 + lane;
   float s = 0.f;
   if (c < 2L * cols) {
 #pragma unroll 4
-    for (int i = w; i < n; i += 16) s += part[(size_t)i * 2 * cols + c];
+    for (int i = w; i < n; i += 64) s += part[(size_t)i * 2 * cols + c];
   }
   red[w][lane] = s;
   __syncthreads();
-  if (w == 0 && c < 2L * cols) {
-    s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s += red[i][lane];
-    float* out = c < cols ? (dgamma ? dgamma + c : nullptr) : (dbeta ? dbeta + (c - cols) : nullptr);
-    if (out) *out = accumulate ? *out + s : s;
+  if (w < 16) {   // transposed: 16 lanes per column, four slices each
+    s = red[4 * lane][w] + red[4 * lane + 1][w] + red[4 * lane + 2][w] + red[4 * lane + 3][w];
+    s = row16_sum(s);
+    const long k = (long)blockIdx.x * 16 + w;
+    if (lane == 0 && k < 2L * cols) {
+      float* out = k < cols ? (dgamma ? dgamma + k : nullptr) : (dbeta ? dbeta + (k - cols) : nullptr);
+      if (out) *out = accumulate ? *out + s : s;
+    }
   }
 }
 
@@ -410,11 +406,15 @@ LnShape ln_fwd_shape(long rows, int cols) {
   s.grid = (int)(need < 4096 ? need : 4096);
   return s;
 }
-LnShape ln_bwd_shape(long rows, int cols) {
+// The backward pass keeps two sums per column besides the row: two accesses per lane only where the 128 registers of a
+// 1024-lane workgroup hold that (16-bit types, even widths), or where there is no wider workgroup.
+LnShape ln_bwd_shape(long rows, int cols, int dtype) {
   LnShape s;
+  const bool one = cols % 8 || dtype == MMST_F32;
   s.blk = cols <= 1024 ? 256 : 1024;
-  s.tpr = cols <= 128 ? 16 : cols <= 256 ? 32 : cols <= 1024 ? 64 : cols <= 4096 ? 256 : cols <= 8192 ? 512 : 1024;
-  s.nv = cols <= 512 ? 1 : cols <= 1024 ? 2 : cols <= 2048 ? 1 : 2;
+  s.tpr = cols <= 128 ? 16 : cols <= 256 ? 32 : cols <= 1024 ? 64 : cols <= 2048 ? 256 : cols <= 4096 ? (one ? 512 : 256)
+        : cols <= 8192 ? (one ? 1024 : 512) : 1024;
+  s.nv = (cols + s.tpr * 8 - 1) / (s.tpr * 8);
   const long need = (rows + s.blk / s.tpr - 1) / (s.blk / s.tpr), most = s.blk == 256 ? 1024 : 256;
   s.grid = (int)(need < most ? need : most);
   return s;
@@ -422,11 +422,16 @@ LnShape ln_bwd_shape(long rows, int cols) {
 
 #define LN_CASE(K, TPR, NV, BLK)                                                                     \
   if (s.tpr == TPR && s.nv == NV && s.blk == BLK) {                                                 \
-    if (vec) hipLaunchKernelGGL((K<T, true, TPR, NV, BLK>), dim3(s.grid), dim3(BLK), 0, st, a);     \
+    if (a.cols % 8) hipLaunchKernelGGL((K<T, true, TPR, NV, BLK>), dim3(s.grid), dim3(BLK), 0, st, a); \
     else hipLaunchKernelGGL((K<T, false, TPR, NV, BLK>), dim3(s.grid), dim3(BLK), 0, st, a);        \
     return;                                                                                         \
   }
-template <typename T> void launch_ln_fwd(const LnArgs& a, const LnShape& s, bool vec, hipStream_t st) {
+#define LN_WIDE(TPR)                                                                                 \
+  if (s.tpr == TPR && s.nv == 2) {                                                                  \
+    hipLaunchKernelGGL((ln_bwd_kernel<T, false, TPR, 2, 1024>), dim3(s.grid), dim3(1024), 0, st, a); \
+    return;                                                                                         \
+  }
+template <typename T> void launch_ln_fwd(const LnArgs& a, const LnShape& s, hipStream_t st) {
   LN_CASE(ln_fwd_kernel, 16, 1, 256)
   LN_CASE(ln_fwd_kernel, 32, 1, 256)
   LN_CASE(ln_fwd_kernel, 64, 1, 256)
@@ -436,22 +441,26 @@ template <typename T> void launch_ln_fwd(const LnArgs& a, const LnShape& s, bool
   LN_CASE(ln_fwd_kernel, 256, 4, 256)
   LN_CASE(ln_fwd_kernel, 1024, 2, 1024)
 }
-template <typename T> void launch_ln_bwd(const LnArgs& a, const LnShape& s, bool vec, hipStream_t st) {
+template <typename T> void launch_ln_bwd(const LnArgs& a, const LnShape& s, hipStream_t st) {
   LN_CASE(ln_bwd_kernel, 16, 1, 256)
   LN_CASE(ln_bwd_kernel, 32, 1, 256)
   LN_CASE(ln_bwd_kernel, 64, 1, 256)
   LN_CASE(ln_bwd_kernel, 64, 2, 256)
   LN_CASE(ln_bwd_kernel, 256, 1, 1024)
-  LN_CASE(ln_bwd_kernel, 256, 2, 1024)
-  LN_CASE(ln_bwd_kernel, 512, 2, 1024)
   LN_CASE(ln_bwd_kernel, 1024, 2, 1024)
+  if constexpr (sizeof(T) == 2)
+    if (a.cols % 8 == 0) {
+      LN_WIDE(256)
+      LN_WIDE(512)
+    }
+  LN_CASE(ln_bwd_kernel, 512, 1, 1024)
+  LN_CASE(ln_bwd_kernel, 1024, 1, 1024)
 }
 #undef LN_CASE
+#undef LN_WIDE
 
 bool drop_ok(double p) { return p >= 0.0 && p <= 1.0; }   // (false for NaN)
-size_t type_size(int dtype) { return dtype == MMST_F32 ? 4 : dtype == MMST_BF16 || dtype == MMST_F16 ? 2 : 0; }
-// a tensor whose rows can be read as aligned groups of eight elements
-bool vec_ok(const void* p, long ld, size_t size) { return !p || ((uintptr_t)p % 16 == 0 && (ld * size) % 16 == 0); }
+bool type_ok(int dtype) { return dtype == MMST_F32 || dtype == MMST_BF16 || dtype == MMST_F16; }
 bool ld_ok(const void* p, long ld, long cols, long rows) { return !p || rows <= 1 || ld >= cols; }
 
 }  // namespace
@@ -460,43 +469,38 @@ extern "C" {
 
 int mmst_dropout(const void* x, long ldx, void* y, long ldy, int dtype, long rows, long cols, double p, uint64_t seed,
                  uint64_t offset, void* stream) {
-  const size_t size = type_size(dtype);
-  if (!size || rows < 0 || cols < 0 || !drop_ok(p)) return MMST_ERR_ARG;
+  if (!type_ok(dtype) || rows < 0 || cols < 0 || !drop_ok(p)) return MMST_ERR_ARG;
   if (rows == 0 || cols == 0) return MMST_OK;
   if (!x || !y || !ld_ok(x, ldx, cols, rows) || !ld_ok(y, ldy, cols, rows)) return MMST_ERR_ARG;
   if (rows > (long)(0x7FFFFFFFFFFFL / cols)) return MMST_ERR_ARG;
   if (rows == 1) ldx = ldy = cols;
   DropArgs a{x, y, (uint64_t)rows * (uint64_t)cols, (uint64_t)cols, (uint64_t)ldx, (uint64_t)ldy, drop_key(p, seed, offset)};
-  const bool vec = vec_ok(x, ldx, ldx == cols && ldy == cols ? 16 : size) && vec_ok(y, ldy, ldx == cols && ldy == cols ? 16 : size);
-  if (dtype == MMST_F32) return launch_dropout<float>(a, vec, (hipStream_t)stream);
-  if (dtype == MMST_BF16) return launch_dropout<bf16>(a, vec, (hipStream_t)stream);
-  return launch_dropout<f16>(a, vec, (hipStream_t)stream);
+  if (dtype == MMST_F32) return launch_dropout<float>(a, (hipStream_t)stream);
+  if (dtype == MMST_BF16) return launch_dropout<bf16>(a, (hipStream_t)stream);
+  return launch_dropout<f16>(a, (hipStream_t)stream);
 }
 
 int mmst_layer_norm(const void* x, long ldx, const void* residual, long ldr, const float* gamma, const float* beta, void* y,
                     long ldy, void* z, long ldz, float* stats, int dtype, long rows, int cols, float eps, double p,
                     uint64_t seed, uint64_t offset, void* stream) {
-  const size_t size = type_size(dtype);
-  if (!size || rows < 0 || cols < 1 || cols > MMST_LN_MAX_COLS || !drop_ok(p) || !(eps >= 0.f)) return MMST_ERR_ARG;
+  if (!type_ok(dtype) || rows < 0 || cols < 1 || cols > MMST_LN_MAX_COLS || !drop_ok(p) || !(eps >= 0.f)) return MMST_ERR_ARG;
   if (rows == 0) return MMST_OK;
   if (!x || !y || !ld_ok(x, ldx, cols, rows) || !ld_ok(residual, ldr, cols, rows) || !ld_ok(y, ldy, cols, rows) ||
       !ld_ok(z, ldz, cols, rows) || rows > 0x7FFFFFFFFFFFL / cols)
     return MMST_ERR_ARG;
   LnArgs a{x, residual, nullptr, gamma, beta, y, z, stats, nullptr, rows, cols, ldx, ldr, 0, ldy, ldz,
            eps, 1.0f / (float)cols, drop_key(p, seed, offset)};
-  const bool vec = cols % 8 == 0 && vec_ok(x, ldx, size) && vec_ok(residual, ldr, size) && vec_ok(y, ldy, size) &&
-                   vec_ok(z, ldz, size) && vec_ok(gamma, 0, 4) && vec_ok(beta, 0, 4);
   const LnShape s = ln_fwd_shape(rows, cols);
-  if (dtype == MMST_F32) launch_ln_fwd<float>(a, s, vec, (hipStream_t)stream);
-  else if (dtype == MMST_BF16) launch_ln_fwd<bf16>(a, s, vec, (hipStream_t)stream);
-  else launch_ln_fwd<f16>(a, s, vec, (hipStream_t)stream);
+  if (dtype == MMST_F32) launch_ln_fwd<float>(a, s, (hipStream_t)stream);
+  else if (dtype == MMST_BF16) launch_ln_fwd<bf16>(a, s, (hipStream_t)stream);
+  else launch_ln_fwd<f16>(a, s, (hipStream_t)stream);
   MMST_CHECK_LAUNCH();
   return MMST_OK;
 }
 
-int mmst_layer_norm_bwd_ws(long rows, int cols, size_t* bytes) {
-  if (!bytes || rows < 0 || cols < 1 || cols > MMST_LN_MAX_COLS) return MMST_ERR_ARG;
-  *bytes = (size_t)ln_bwd_shape(rows, cols).grid * 2 * cols * sizeof(float);
+int mmst_layer_norm_bwd_ws(int dtype, long rows, int cols, size_t* bytes) {
+  if (!bytes || !type_ok(dtype) || rows < 0 || cols < 1 || cols > MMST_LN_MAX_COLS) return MMST_ERR_ARG;
+  *bytes = (size_t)ln_bwd_shape(rows, cols, dtype).grid * 2 * cols * sizeof(float);
   return MMST_OK;
 }
 
@@ -504,9 +508,8 @@ int mmst_layer_norm_bwd(const void* dy, long lddy, const void* z, long ldz, cons
                         const void* dz_in, long lddz_in, void* dz, long lddz, void* dx, long lddx, float* dgamma,
                         float* dbeta, int accumulate, int dtype, long rows, int cols, double p, uint64_t seed,
                         uint64_t offset, void* ws, size_t ws_bytes, void* stream) {
-  const size_t size = type_size(dtype);
-  if (!size || rows < 0 || cols < 1 || cols > MMST_LN_MAX_COLS || !drop_ok(p)) return MMST_ERR_ARG;
-  const LnShape s = ln_bwd_shape(rows, cols);
+  if (!type_ok(dtype) || rows < 0 || cols < 1 || cols > MMST_LN_MAX_COLS || !drop_ok(p)) return MMST_ERR_ARG;
+  const LnShape s = ln_bwd_shape(rows, cols, dtype);
   const bool sums = dgamma || dbeta;
   if (sums && ws_bytes < (size_t)s.grid * 2 * cols * sizeof(float)) return MMST_ERR_ARG;
   if (rows > 0) {
@@ -517,15 +520,13 @@ int mmst_layer_norm_bwd(const void* dy, long lddy, const void* z, long ldz, cons
       return MMST_ERR_ARG;
     LnArgs a{dy, dz_in, z, gamma, nullptr, dz, dx, const_cast<float*>(stats), sums ? (float*)ws : nullptr, rows, cols,
              lddy, lddz_in, ldz, lddz, lddx, 0.f, 1.0f / (float)cols, key};
-    const bool vec = cols % 8 == 0 && vec_ok(dy, lddy, size) && vec_ok(z, ldz, size) && vec_ok(dz_in, lddz_in, size) &&
-                     vec_ok(dz, lddz, size) && vec_ok(key.thr ? dx : nullptr, lddx, size) && vec_ok(gamma, 0, 4);
-    if (dtype == MMST_F32) launch_ln_bwd<float>(a, s, vec, (hipStream_t)stream);
-    else if (dtype == MMST_BF16) launch_ln_bwd<bf16>(a, s, vec, (hipStream_t)stream);
-    else launch_ln_bwd<f16>(a, s, vec, (hipStream_t)stream);
+    if (dtype == MMST_F32) launch_ln_bwd<float>(a, s, (hipStream_t)stream);
+    else if (dtype == MMST_BF16) launch_ln_bwd<bf16>(a, s, (hipStream_t)stream);
+    else launch_ln_bwd<f16>(a, s, (hipStream_t)stream);
     MMST_CHECK_LAUNCH();
   }
   if (sums) {
-    hipLaunchKernelGGL(ln_cols_kernel, dim3((2 * cols + 63) / 64), dim3(1024), 0, (hipStream_t)stream, (const float*)ws,
+    hipLaunchKernelGGL(ln_cols_kernel, dim3((2 * cols + 15) / 16), dim3(1024), 0, (hipStream_t)stream, (const float*)ws,
                        rows > 0 ? s.grid : 0, cols, dgamma, dbeta, accumulate);
     MMST_CHECK_LAUNCH();
   }

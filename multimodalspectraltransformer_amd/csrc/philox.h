@@ -73,3 +73,31 @@ __device__ __forceinline__ void drop_elements(float (&v)[8], uint64_t first, con
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 }
+
+// For lanes that own eight consecutive elements first + 8 l .. + 7 where `first` need not be at a block border, so that
+// they lie in two blocks: G lanes, each makes one block (lane 0 also the one behind the last), the words change lanes
+// through `slot` (G + 1 blocks of LDS that only these lanes of one wave use).
+typedef uint32_t __attribute__((may_alias)) u32_alias;
+template <int G>
+__device__ __forceinline__ void drop_straddling(float (&v)[8], uint64_t first, const DropKey& d, uint4* slot, int l) {
+  const uint64_t block0 = first >> 3;
+  const int mis = (int)(first & 7);
+  uint4 w = philox_block(block0 + l, d);
+  if (__ballot(mis != 0)) {   // (of any row of the wave)
+    __builtin_amdgcn_wave_barrier();
+    slot[l] = w;
+    if (l == 0) slot[G] = philox_block(block0 + G, d);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const u32_alias* p = reinterpret_cast<const u32_alias*>(slot) + l * 4 + (mis >> 1);
+    const int odd = (mis & 1) * 16;
+    const uint32_t u[5] = {p[0], p[1], p[2], p[3], p[4]};
+    w.x = (uint32_t)((((uint64_t)u[1] << 32) | u[0]) >> odd);
+    w.y = (uint32_t)((((uint64_t)u[2] << 32) | u[1]) >> odd);
+    w.z = (uint32_t)((((uint64_t)u[3] << 32) | u[2]) >> odd);
+    w.w = (uint32_t)((((uint64_t)u[4] << 32) | u[3]) >> odd);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+  drop_block(v, w, d);
+}

@@ -85,10 +85,10 @@ def test_layer_norm_bwd_refusals(kw):
 
 def test_workspace_query():
     n = C.c_size_t()
-    assert _rc("mmst_layer_norm_bwd_ws", 1000, 128, C.byref(n)) == 0 and n.value >= 2 * 128 * 4
-    assert _rc("mmst_layer_norm_bwd_ws", 0, 128, C.byref(n)) == 0
-    assert _rc("mmst_layer_norm_bwd_ws", 10, 0, C.byref(n)) == -1
-    assert _rc("mmst_layer_norm_bwd_ws", 10, 128, None) == -1
+    assert _rc("mmst_layer_norm_bwd_ws", 1, 1000, 128, C.byref(n)) == 0 and n.value >= 2 * 128 * 4
+    assert _rc("mmst_layer_norm_bwd_ws", 1, 0, 128, C.byref(n)) == 0
+    assert _rc("mmst_layer_norm_bwd_ws", 1, 10, 0, C.byref(n)) == -1
+    assert _rc("mmst_layer_norm_bwd_ws", 1, 10, 128, None) == -1
 
 
 def test_wrappers_refuse_cpu_tensors_and_bad_arguments():
