@@ -47,24 +47,30 @@ __device__ __forceinline__ int piece_rows(const CeGemm& a) {
   return left < 0 ? 0 : left < a.rows_max ? left : a.rows_max;
 }
 
-__device__ __forceinline__ int key_p(int r) { return r & 7; }
-__device__ __forceinline__ int key_q(int r) { return (r & 3) | (((r >> 3) & 1) << 2); }
-
-// One operand's tile in LDS: B rows (or columns) x 64 of the contraction.
-//   rows along the contraction (T == false): B rows of 128 bytes, the eight 16-byte pieces of a row exchanged by its key
-//   columns along the contraction (T == true): 64 rows of 2 B bytes, their 32-byte pieces exchanged by the row's key
+// One operand's tile in LDS: B rows (or columns) x BK of the contraction.
+//   rows along the contraction (T == false): B rows of 2 BK bytes, the 16-byte pieces of a row exchanged by its key
+//   columns along the contraction (T == true): BK rows of 2 B bytes, their 32-byte pieces exchanged by the row's key
 // The exchange makes the fragment reads of 16 rows hit all banks; it is applied to the SOURCE address, since the LDS-DMA
 // writes lane i's 16 bytes at i * 16.  What lies outside the operand reads as zero (the buffer's bounds check; the tail of
 // the contraction by an offset past every bound).
-template <bool T, bool QSIDE, int B, int NTHR> struct Operand {
-  static constexpr int NI = B * 8 / NTHR;   // DMA instructions per thread and step
-  static constexpr int BYTES = B * 128;
+template <bool T, bool QSIDE, int B, int NTHR, int BK> struct Operand {
+  static constexpr int PIECES = B * BK / 8, NI = PIECES / NTHR;   // 16-byte pieces; DMA instructions per thread and step
+  static constexpr int BYTES = B * BK * 2, ROW = BK / 8;          // pieces per row (!T)
   static constexpr uint32_t OUT = 0xFFFFFFF0u;
+  static_assert(PIECES % NTHR == 0 && (BK == 32 || BK == 64), "tile shape");
   uint32_t off[NI];
   const bf16* base;
   long ld;
   int K, wide;   // wide: columns of the operand right of the tile's first (T)
   long rows;     // rows of the operand below the tile's first (!T)
+
+  // a fragment reads 16 rows: r0 + i (P), r0 + 8 (i >> 2) + 4 half + (i & 3) (Q); 64 banks of 4 bytes
+  static __device__ __forceinline__ int key(int r) {
+    if constexpr (T) return (r & 3) | (((r >> 3) & 1) << 2);
+    else if constexpr (BK == 64) return QSIDE ? (r & 3) | (((r >> 3) & 1) << 2) : r & 7;
+    else return QSIDE ? (r >> 3) & 3 : (r >> 2) & 3;
+  }
+  static __device__ __forceinline__ int piece(int slot) { const int r = slot / ROW; return (slot % ROW) ^ key(r); }   // (!T)
 
   __device__ __forceinline__ void init(const bf16* p, long ld_, int first, int n, int K_, int tid) {
     ld = ld_;
@@ -75,15 +81,15 @@ template <bool T, bool QSIDE, int B, int NTHR> struct Operand {
     for (int i = 0; i < NI; ++i) {
       const int slot = i * NTHR + tid;
       if constexpr (!T) {
-        const int r = slot >> 3, c = (slot & 7) ^ (QSIDE ? key_q(r) : key_p(r));
-        off[i] = (uint32_t)(r * (int)ld_ * 2 + c * 16);
+        off[i] = (uint32_t)((slot / ROW) * (int)ld_ * 2 + piece(slot) * 16);
       } else {
         const int r = slot / (B / 8), c16 = slot % (B / 8);
-        off[i] = (uint32_t)(r * (int)ld_ * 2 + ((((c16 >> 1) ^ key_q(r)) << 1) | (c16 & 1)) * 16);
+        off[i] = (uint32_t)(r * (int)ld_ * 2 + ((((c16 >> 1) ^ key(r)) << 1) | (c16 & 1)) * 16);
       }
     }
   }
-  __device__ __forceinline__ void issue(lds_byte* img, int k0, int tid, int wave) const {
+  // DMA instructions lo .. hi - 1 of step k0
+  template <int LO, int HI> __device__ __forceinline__ void issue(lds_byte* img, int k0, int tid, int wave) const {
     const bf16* p;
     long bytes;
     if constexpr (!T) {
@@ -95,30 +101,26 @@ template <bool T, bool QSIDE, int B, int NTHR> struct Operand {
     }
     bytes = bytes < 0 ? 0 : bytes > 0x7FFFFFFF ? 0x7FFFFFFF : bytes;
     const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)bytes, 0x00020000);
-    const bool tail = !T && K - k0 < 64;
+    const bool tail = !T && K - k0 < BK;   // of the contraction (uniform)
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
+    for (int i = LO; i < HI; ++i) {
       uint32_t o = off[i];
-      if (tail) {
-        const int slot = i * NTHR + tid, r = slot >> 3, c = (slot & 7) ^ (QSIDE ? key_q(r) : key_p(r));
-        if (c * 8 >= K - k0) o = OUT;
-      }
+      if (tail) o = piece(i * NTHR + tid) * 8 >= K - k0 ? OUT : o;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lptr_t)(img + i * NTHR * 16 + wave * 1024), 16, (int)o, 0, 0, 0);
     }
   }
   // fragment of 16 rows at r0 for the 32 contraction steps ks: lane (i = lane & 15, j = lane >> 4) gets row i, steps 8 j ..
-  // 8 j + 7.  QSIDE: the 16 rows are 8 (i >> 2) + 4 half + (i & 3) of the 32 at r0, so that two fragments leave eight
-  // consecutive columns of the result in a lane.
+  // 8 j + 7.  QSIDE: two fragments (half 0, 1) leave eight consecutive columns of the result in a lane.
   __device__ __forceinline__ static bf16x8 frag(const lds_byte* img, int r0, int half, int ks, int lane) {
     if constexpr (!T) {
       const int i = lane & 15;
       const int r = QSIDE ? r0 + 8 * (i >> 2) + 4 * half + (i & 3) : r0 + i;
-      const int c = (ks * 4 + (lane >> 4)) ^ (QSIDE ? key_q(r) : key_p(r));
-      return *reinterpret_cast<const LDS_AS bf16x8*>(img + r * 128 + c * 16);
+      const int c = (ks * 4 + (lane >> 4)) ^ key(r);
+      return *reinterpret_cast<const LDS_AS bf16x8*>(img + r * (BK * 2) + c * 16);
     } else {
       const int k = ks * 32 + 8 * (lane >> 4) + ((lane & 15) >> 2);
       const int col = QSIDE ? r0 + 8 * (lane & 3) + 4 * half : r0 + 4 * (lane & 3);
-      const lds_byte* p = img + k * (B * 2) + (((col >> 4) ^ key_q(k)) << 5) + (col & 15) * 2;
+      const lds_byte* p = img + k * (B * 2) + (((col >> 4) ^ key(k)) << 5) + (col & 15) * 2;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s16x4*)p);
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s16x4*)(p + 4 * (B * 2)));   // (same key)
       return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -130,31 +132,150 @@ template <int MODE, int BP, int BQ, int WP, int WQ>
 struct CeTile {
   static constexpr int NW = WP * WQ, NTHR = NW * 64, MT = BP / WP / 16, NT = BQ / WQ / 16;
   static constexpr bool TP = MODE == DW, TQ = MODE == DH || MODE == DW;
-  using OpP = Operand<TP, false, BP, NTHR>;
-  using OpQ = Operand<TQ, true, BQ, NTHR>;
-  static constexpr int STAGE = OpP::BYTES + OpQ::BYTES, SMEM = 2 * STAGE;
+  static constexpr int BK = 64, NS = 2;   // a step of the contraction; stages
+  using OpP = Operand<TP, false, BP, NTHR, BK>;
+  using OpQ = Operand<TQ, true, BQ, NTHR, BK>;
+  static constexpr int STAGE = OpP::BYTES + OpQ::BYTES, SMEM = NS * STAGE;
 
-  // one step of 64: the next step's operands are requested into `wr`, the products of `rd` are made.  The two never
+  struct Frags { bf16x8 p[MT], q[NT]; };
+  static __device__ __forceinline__ void read(Frags& f, const lds_byte* rd, int ks, int pw0, int qw0, int lane) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) f.q[nt] = OpQ::frag(rd + OpP::BYTES, qw0 + (nt >> 1) * 32, nt & 1, ks, lane);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) f.p[mt] = OpP::frag(rd, pw0 + mt * 16, 0, ks, lane);
+  }
+  static __device__ __forceinline__ void products(f32x4 (&acc)[MT][NT], const Frags& f) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        acc[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.q[nt], f.p[mt], acc[mt][nt], 0, 0, 0);
+  }
+  // DMA instructions LO .. HI - 1 of the step's PER: the P operand's, then the Q operand's
+  static constexpr int PER = OpP::NI + OpQ::NI;
+  template <int LO, int HI>
+  static __device__ __forceinline__ void issue(const OpP& p, const OpQ& q, lds_byte* wr, int k, int tid, int wave) {
+    if constexpr (LO < OpP::NI) p.template issue<LO, (HI < OpP::NI ? HI : OpP::NI)>(wr, k, tid, wave);
+    if constexpr (HI > OpP::NI) q.template issue<(LO > OpP::NI ? LO - OpP::NI : 0), HI - OpP::NI>(wr + OpP::BYTES, k, tid, wave);
+  }
+
+  // One step: the next step's operands are requested into `wr`, the products of `rd` are made.  The two never
   // overlap, and saying so is what keeps the compiler from waiting for the DMA before every LDS read.
   static __device__ __forceinline__ void step(f32x4 (&acc)[MT][NT], const OpP& p, const OpQ& q, lds_byte* __restrict__ wr,
                                               const lds_byte* __restrict__ rd, bool more, int k1, int tid, int wave,
                                               int pw0, int qw0, int lane) {
-    if (more) {
-      p.issue(wr, k1, tid, wave);
-      q.issue(wr + OpP::BYTES, k1, tid, wave);
+    if (more) issue<0, PER>(p, q, wr, k1, tid, wave);
+#pragma unroll
+    for (int ks = 0; ks < BK / 32; ++ks) {
+      Frags f;
+      read(f, rd, ks, pw0, qw0, lane);
+      products(acc, f);
     }
+  }
+
+  // Eight waves in two halves, one of each on every SIMD: while one half reads the fragments of 32 contraction steps, the
+  // other multiplies, and a barrier changes the roles.  Phases of step s, each ended by a barrier of the whole workgroup:
+  //              4 s                4 s + 1        4 s + 2       4 s + 3
+  //   first      read 0             multiply 0     read 1        multiply 1
+  //   second     multiply 1 (s-1)   read 0         multiply 0    read 1
+  // The stage of step s - 1 is free at phase 4 s; the DMA of step s + 1 goes there in phases 4 s and 4 s + 1, half of it
+  // each, behind the reads or between the products: issued in one go it would hold up whichever comes after it, since the
+  // address unit takes 18 cycles for each of the 64 instructions.
+  static __device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
+  static __device__ __forceinline__ void barrier() { asm volatile("s_barrier" ::: "memory"); fence(); }
+  static __device__ __forceinline__ void reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+  static __device__ __forceinline__ void dma_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+  template <int MT0, int MT1> static __device__ __forceinline__ void some(f32x4 (&acc)[MT][NT], const Frags& f) {
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      bf16x8 pf[MT], qf[NT];
+    for (int mt = MT0; mt < MT1; ++mt)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) qf[nt] = OpQ::frag(rd + OpP::BYTES, qw0 + (nt >> 1) * 32, nt & 1, ks, lane);
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) pf[mt] = OpP::frag(rd, pw0 + mt * 16, 0, ks, lane);
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          acc[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf[nt], pf[mt], acc[mt][nt], 0, 0, 0);
+      for (int nt = 0; nt < NT; ++nt)
+        acc[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.q[nt], f.p[mt], acc[mt][nt], 0, 0, 0);
+    fence();
+  }
+  static __device__ __forceinline__ void multiply(f32x4 (&acc)[MT][NT], const Frags& f) {
+    __builtin_amdgcn_s_setprio(1);
+    some<0, MT>(acc, f);
+    __builtin_amdgcn_s_setprio(0);
+  }
+  // the products with DMA instructions LO .. LO + PER / 2 - 1 between them
+  template <int LO> static __device__ __forceinline__ void multiply_issue(f32x4 (&acc)[MT][NT], const Frags& f, const OpP& p,
+                                                                          const OpQ& q, lds_byte* wr, int k, int tid, int wave) {
+    static_assert(MT == 8 && PER == 8, "eight by eight");
+    __builtin_amdgcn_s_setprio(1);
+    some<0, 1>(acc, f);
+    issue<LO, LO + 1>(p, q, wr, k, tid, wave);
+    some<1, 3>(acc, f);
+    issue<LO + 1, LO + 2>(p, q, wr, k, tid, wave);
+    some<3, 5>(acc, f);
+    issue<LO + 2, LO + 3>(p, q, wr, k, tid, wave);
+    some<5, 7>(acc, f);
+    issue<LO + 3, LO + 4>(p, q, wr, k, tid, wave);
+    some<7, 8>(acc, f);
+    __builtin_amdgcn_s_setprio(0);
+  }
+  static __device__ __forceinline__ void step_first(f32x4 (&acc)[MT][NT], const OpP& p, const OpQ& q, lds_byte* __restrict__ wr,
+                                                    const lds_byte* __restrict__ rd, int k1, int tid, int wave, int pw0,
+                                                    int qw0, int lane) {
+    Frags f;
+    read(f, rd, 0, pw0, qw0, lane);
+    fence();
+    issue<0, PER / 2>(p, q, wr, k1, tid, wave);
+    reads_done();
+    barrier();
+    multiply_issue<PER / 2>(acc, f, p, q, wr, k1, tid, wave);
+    barrier();
+    read(f, rd, 1, pw0, qw0, lane);
+    reads_done();
+    barrier();
+    multiply(acc, f);
+    dma_done();
+    barrier();
+  }
+  static __device__ __forceinline__ void step_second(f32x4 (&acc)[MT][NT], Frags& f, const OpP& p, const OpQ& q,
+                                                     lds_byte* __restrict__ wr, const lds_byte* __restrict__ rd, int k1,
+                                                     int tid, int wave, int pw0, int qw0, int lane) {
+    multiply_issue<0>(acc, f, p, q, wr, k1, tid, wave);
+    barrier();
+    read(f, rd, 0, pw0, qw0, lane);
+    fence();
+    issue<PER / 2, PER>(p, q, wr, k1, tid, wave);
+    reads_done();
+    barrier();
+    multiply(acc, f);
+    barrier();
+    read(f, rd, 1, pw0, qw0, lane);
+    reads_done();
+    dma_done();
+    barrier();
+  }
+  // No branch inside a step: the last one requests a step that is not there, which moves nothing but zeros (or, in a split
+  // contraction, the next part's first step) into the stage that nobody reads, and the second half starts by multiplying zeros.
+  static __device__ __forceinline__ void loop(f32x4 (&acc)[MT][NT], const OpP& p, const OpQ& q, lds_byte* lds, int kbeg,
+                                              int nsteps, int tid, int wave, int pw0, int qw0, int lane) {
+    if (nsteps <= 0) return;
+    issue<0, PER>(p, q, lds, kbeg, tid, wave);
+    if constexpr (NW != 8) {
+      for (int s = 0; s < nsteps; ++s) {
+        // this wave's share of step s has landed; behind the barrier everybody's has, and nobody reads the other stage
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        step(acc, p, q, lds + ((s + 1) & 1) * STAGE, lds + (s & 1) * STAGE, s + 1 < nsteps, kbeg + (s + 1) * BK, tid, wave,
+             pw0, qw0, lane);
+      }
+    } else {
+      dma_done();
+      barrier();
+      if (wave < 4) {
+        for (int s = 0; s < nsteps; ++s)
+          step_first(acc, p, q, lds + ((s + 1) & 1) * STAGE, lds + (s & 1) * STAGE, kbeg + (s + 1) * BK, tid, wave, pw0, qw0, lane);
+        barrier();   // the second half's last multiplication
+      } else {
+        Frags f = {};
+        for (int s = 0; s < nsteps; ++s)
+          step_second(acc, f, p, q, lds + ((s + 1) & 1) * STAGE, lds + (s & 1) * STAGE, kbeg + (s + 1) * BK, tid, wave, pw0, qw0, lane);
+        multiply(acc, f);
+        barrier();
+      }
     }
   }
 };
@@ -184,10 +305,10 @@ __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_
   if (MODE == DW) K = rows;
   else Pn = rows;
   if (MODE != DW && p0 >= rows) return;   // (uniform: before any barrier)
-  int nsteps = (K + 63) >> 6;
+  int nsteps = (K + Tile::BK - 1) / Tile::BK;
   if (MODE == DH && a.ksplit > 1) {
     const int s0 = (int)((long)nsteps * ks_id / a.ksplit), s1 = (int)((long)nsteps * (ks_id + 1) / a.ksplit);
-    kbeg = s0 << 6;
+    kbeg = s0 * Tile::BK;
     nsteps = s1 - s0;
   }
   const int pw0 = (wave / WQ) * (BP / WP), qw0 = (wave % WQ) * (BQ / WQ);
@@ -202,16 +323,7 @@ __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   lds_byte* const lds = (lds_byte*)smem;
-  if (nsteps > 0) {
-    op.issue(lds, kbeg, tid, wave);
-    oq.issue(lds + Tile::OpP::BYTES, kbeg, tid, wave);
-  }
-  for (int s = 0; s < nsteps; ++s) {
-    // this wave's share of step s has landed; behind the barrier everybody's has, and nobody reads the other stage
-    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-    Tile::step(acc, op, oq, lds + ((s + 1) & 1) * Tile::STAGE, lds + (s & 1) * Tile::STAGE, s + 1 < nsteps,
-               kbeg + (s + 1) * 64, tid, wave, pw0, qw0, lane);
-  }
+  Tile::loop(acc, op, oq, lds, kbeg, nsteps, tid, wave, pw0, qw0, lane);
 
   const int i16 = lane & 15, j4 = lane >> 4;
   if constexpr (MODE == LOGIT_STATS || MODE == LOGIT_GRAD) {
