@@ -23,6 +23,10 @@ typedef __attribute__((address_space(3))) void* lptr_t;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int VT = 256;   // g is padded to whole tiles of the vocabulary, its rows to whole tiles as well
 
+// Exponents are taken in units of log 2; a bias that masks with the lowest float would overflow there, so finite ones end at
+// -2^127 (the logits beside it are still at an infinite distance for exp).
+__device__ __forceinline__ float word_bias(float b) { return b < -0x1p127f && b > -INFINITY ? -0x1p127f : b; }
+
 enum { LOGIT_STATS = 0, LOGIT_GRAD = 1, DH = 2, DW = 3 };
 
 struct CeGemm {
@@ -72,11 +76,14 @@ template <bool T, bool QSIDE, int B, int NTHR, int BK> struct Operand {
   }
   static __device__ __forceinline__ int piece(int slot) { const int r = slot / ROW; return (slot % ROW) ^ key(r); }   // (!T)
 
+  __device__ __forceinline__ void seek(const bf16* p, int first, int n) {   // another tile of the operand
+    base = T ? p + first : p + (long)first * ld;
+    rows = wide = n - first;
+  }
   __device__ __forceinline__ void init(const bf16* p, long ld_, int first, int n, int K_, int tid) {
     ld = ld_;
     K = K_;
-    base = T ? p + first : p + (long)first * ld_;
-    rows = wide = n - first;
+    seek(p, first, n);
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int slot = i * NTHR + tid;
@@ -334,7 +341,7 @@ __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int v = q0 + qw0 + tp * 32 + 8 * j4 + e;
-          const float b = v < a.Qn ? a.bias[v] : 0.f;
+          const float b = v < a.Qn ? word_bias(a.bias[v]) : 0.f;
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) acc[mt][2 * tp + (e >> 2)][e & 3] += b;
         }
@@ -384,13 +391,13 @@ __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_
       float v = mx[mt];
 #pragma unroll
       for (int w = 0; w < WQ; ++w) v = fmaxf(v, red[w * BP + pw0 + mt * 16 + i16]);
-      mx[mt] = v;
-      const float at = v == -INFINITY ? 0.f : v;   // a tile whose every logit is masked: exp(-inf - 0), not of NaN
+      mx[mt] = v * LOG2E;
+      const float at = v == -INFINITY ? 0.f : mx[mt];   // a tile whose every logit is masked: exp(-inf - 0), not of NaN
       float s = 0.f;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f((acc[mt][nt][e] - at) * LOG2E);
+        for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mt][nt][e], LOG2E, -at));
       sum[mt] = xor32_sum(xor16_sum(s));
     }
     __syncthreads();
@@ -498,6 +505,211 @@ __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_
   }
 }
 
+// ---------------------------------------------------------------------------------------------------- logits, streamed
+// The logits of a narrow layer (few steps of the contraction per tile) or of few rows: the tiles, 128 x 128, are dealt out
+// to G workgroups in equal runs along the vocabulary, and a workgroup's run is ONE stream of steps, so that the next tile's
+// operands arrive during the last products and the softmax of this one (tile by tile, each beginning with an empty
+// pipeline: 109 instead of ... us for the stats of 3032 x 128 x 32000).  A lane keeps the running maximum and sum of its own
+// columns of a row over the whole run; lanes, waves and workgroups are joined at its end.  Two workgroups per CU: one's
+// exponentials run beside the other's products.
+struct CeStream {
+  long T; int G, qtiles;                            // tiles of all rows that count, workgroups that have any, tiles per row
+  __device__ __forceinline__ CeStream(int rows, int V, int grid) {
+    qtiles = (V + 127) / 128;
+    T = (long)((rows + 127) / 128) * qtiles;
+    G = T < grid ? (int)T : grid;
+  }
+  __device__ __forceinline__ long begin(int b) const { return T * b / G; }
+  __device__ __forceinline__ int owner(long tile) const { return (int)(((tile + 1) * G - 1) / T); }
+  // where workgroup b leaves its (max, sum) of the row tile pt, one of each half of the columns
+  static __device__ __forceinline__ size_t slot(int b, int pt, int half) { return ((size_t)(b + pt) * 2 + half) * 128; }
+};
+
+template <int MODE>
+__global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
+  using Tile = CeTile<MODE, 128, 128, 2, 2>;
+  constexpr int MT = Tile::MT, NT = Tile::NT, BK = Tile::BK;
+  static_assert(MT == 4 && NT == 4, "four by four");
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[Tile::SMEM];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rows = piece_rows(a);
+  const CeStream st(rows, a.Qn, gridDim.x);
+  // neighbours in the stream to one XCD (workgroups go round the eight of them)
+  int b;
+  {
+    const int n = gridDim.x, q8 = n >> 3, r8 = n & 7, x = blockIdx.x & 7;
+    b = (x < r8 ? x * (q8 + 1) : r8 * (q8 + 1) + (x - r8) * q8) + ((int)blockIdx.x >> 3);
+  }
+  if (b >= st.G) return;   // (uniform)
+  const long t0 = st.begin(b), t1 = st.begin(b + 1);
+  int pt = (int)(t0 / st.qtiles), qt = (int)(t0 - (long)pt * st.qtiles);
+  const int pw0 = (wave >> 1) * 64, qw0 = (wave & 1) * 64;
+  const int i16 = lane & 15, j4 = lane >> 4;
+  const int nsteps = (a.K + BK - 1) / BK;
+  typename Tile::OpP op;
+  typename Tile::OpQ oq;
+  op.init(a.P, a.ldp, pt * 128, rows, a.K, tid);
+  oq.init(a.Q, a.ldq, qt * 128, a.Qn, a.K, tid);
+  lds_byte* const lds = (lds_byte*)smem;
+  Tile::template issue<0, Tile::PER>(op, oq, lds, 0, tid, wave);
+
+  // a tile's products start from the bias: -infinity past the vocabulary, which leaves those columns out of everything
+  float start[NT / 2][8];
+  auto load_start = [&](int q) {
+#pragma unroll
+    for (int tp = 0; tp < NT / 2; ++tp)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int v = q * 128 + qw0 + tp * 32 + 8 * j4 + e;
+        start[tp][e] = v < a.Qn ? (a.bias ? word_bias(a.bias[v]) : 0.f) : -INFINITY;
+      }
+  };
+  load_start(qt);
+  float m2[MT], sum[MT], lse2[MT], wt[MT];   // running maximum in units of log 2, running sum; lse and weight (gradient)
+  int target[MT];
+  auto load_rows = [&](int p) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const int m = p * 128 + pw0 + mt * 16 + i16;
+      m2[mt] = -INFINITY;
+      sum[mt] = 0.f;
+      target[mt] = -1;
+      lse2[mt] = INFINITY;   // a row that is not there, or whose every logit is masked: no gradient
+      wt[mt] = 0.f;
+      if (m < rows) {
+        const int64_t t = a.target[a.index ? a.index[m] : m];
+        target[mt] = t >= 0 && t < a.Qn ? (int)t : -1;
+        if (MODE == LOGIT_GRAD) {
+          const float l = a.lse[m] * LOG2E;
+          if (l != -INFINITY) { lse2[mt] = l; wt[mt] = a.weight[m]; }
+        }
+      }
+    }
+  };
+  load_rows(pt);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+
+  int stage = 0;
+  for (long t = t0; t < t1; ++t) {
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[mt][nt][e] = start[nt >> 1][(nt & 1) * 4 + e];
+    const int q0 = qt * 128;
+    const bool new_rows = qt + 1 == st.qtiles;
+    const int pt1 = new_rows ? pt + 1 : pt, qt1 = new_rows ? 0 : qt + 1;
+    for (int s = 0; s < nsteps; ++s) {
+      if (s) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (a tile's first step: waited for before the last one's stores)
+      asm volatile("s_barrier" ::: "memory");
+      bool more = true;
+      int k1 = (s + 1) * BK;
+      if (s + 1 == nsteps) {
+        more = t + 1 < t1;
+        k1 = 0;
+        if (more) {
+          op.seek(a.P, pt1 * 128, rows);
+          oq.seek(a.Q, qt1 * 128, a.Qn);
+        }
+      }
+      Tile::step(acc, op, oq, lds + (stage ^ 1) * Tile::STAGE, lds + stage * Tile::STAGE, more, k1, tid, wave, pw0, qw0, lane);
+      stage ^= 1;
+    }
+    if (t + 1 < t1) load_start(qt1);
+    auto holds_target = [&](int mt) {   // the lane's column of the target's logit, or -1
+      const int rel = target[mt] - (q0 + qw0 + 8 * j4);
+      return target[mt] >= 0 && rel >= 0 && rel < 64 && (rel & 31) < 8 ? rel : -1;
+    };
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      if constexpr (MODE == LOGIT_STATS) {
+        float v = acc[mt][0][0];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v = fmaxf(v, acc[mt][nt][e]);
+        const float top = fmaxf(m2[mt], v * LOG2E), at = top == -INFINITY ? 0.f : top;   // nothing but masked words so far
+        float x = sum[mt] * __builtin_amdgcn_exp2f(m2[mt] - at);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mt][nt][e], LOG2E, -at));
+        m2[mt] = top;
+        sum[mt] = x;
+      } else {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            acc[mt][nt][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mt][nt][e], LOG2E, -lse2[mt])) * wt[mt];
+        const int rel = holds_target(mt);
+        if (rel >= 0) {
+#pragma unroll
+          for (int tp = 0; tp < NT / 2; ++tp)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (rel == tp * 32 + e) acc[mt][2 * tp + (e >> 2)][e & 3] -= wt[mt];
+        }
+      }
+    }
+    // The next step's operands have landed (they had the last products and all of the above to do so); waited for here and
+    // not in the loop, which would wait for the following stores as well.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const int m = pt * 128 + pw0 + mt * 16 + i16;
+      if constexpr (MODE == LOGIT_STATS) {
+        const int rel = holds_target(mt);
+        if (rel >= 0) {
+          float x = 0.f;
+#pragma unroll
+          for (int tp = 0; tp < NT / 2; ++tp)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (rel == tp * 32 + e) x = acc[mt][2 * tp + (e >> 2)][e & 3];
+          a.tlogit[m] = x;
+        }
+      } else if (m < rows) {
+#pragma unroll
+        for (int tp = 0; tp < NT / 2; ++tp) {
+          bf16x8 o;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] = (bf16)acc[mt][2 * tp + (e >> 2)][e & 3];
+          *reinterpret_cast<bf16x8*>(a.g + (size_t)m * a.ldg + q0 + qw0 + tp * 32 + 8 * j4) = o;
+        }
+      }
+    }
+    if constexpr (MODE == LOGIT_GRAD) {
+      if (a.dbias_part) {   // column sums of the wave's 64 rows
+        float* d = a.dbias_part + (size_t)(pt * 2 + (wave >> 1)) * a.ldg + q0 + qw0 + 8 * j4;
+#pragma unroll
+        for (int tp = 0; tp < NT / 2; ++tp)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float x = row16_sum((acc[0][2 * tp + (e >> 2)][e & 3] + acc[1][2 * tp + (e >> 2)][e & 3]) +
+                                      (acc[2][2 * tp + (e >> 2)][e & 3] + acc[3][2 * tp + (e >> 2)][e & 3]));
+            if (i16 == 0) d[tp * 32 + e] = x;
+          }
+      }
+    }
+    if (new_rows || t + 1 == t1) {
+      if constexpr (MODE == LOGIT_STATS) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          const float top = xor32_max(xor16_max(m2[mt])), at = top == -INFINITY ? 0.f : top;
+          const float x = xor32_sum(xor16_sum(sum[mt] * __builtin_amdgcn_exp2f(m2[mt] - at)));
+          if (j4 == 0) a.part[CeStream::slot(b, pt, wave & 1) + pw0 + mt * 16 + i16] = make_float2(top, x);
+        }
+      }
+      if (t + 1 < t1) load_rows(pt1);
+    }
+    pt = pt1;
+    qt = qt1;
+  }
+}
+
 // ---------------------------------------------------------------------------------------------------- rows
 // The rows that count, numbered through in their order (one workgroup: 16 waves look at 1024 targets at a time), and the
 // losses of those that do not: 0 where the target is ignore_index, NaN where it is no word (and no gradient).
@@ -547,8 +759,9 @@ __global__ __launch_bounds__(256) void ce_gather_kernel(const bf16* h, long ldh,
   reinterpret_cast<uint4*>(out)[(long)r * D8 + c] = reinterpret_cast<const uint4*>(h + (long)n * ldh)[c];
 }
 
-// A row's pairs (max, sum) of all tiles of the vocabulary -> lse and loss: 16 rows per workgroup, 16 lanes each
-__global__ __launch_bounds__(256) void ce_rows_kernel(const float2* part, int tiles, int ld, const int* count, int row0,
+// A row's pairs (maximum in units of log 2, sum) -> lse and loss: 16 rows per workgroup, 16 lanes each.  The pairs are those
+// of every tile of the vocabulary, [tile][ld], or (grid != 0) those that the workgroups of ce_stream_kernel left.
+__global__ __launch_bounds__(256) void ce_rows_kernel(const float2* part, int tiles, int ld, int grid, const int* count, int row0,
                                                       int rows_max, const int* index, const int64_t* target, int64_t ignore,
                                                       int V, const float* tlogit, float* lse_c, float* loss, float* lse) {
   __shared__ float rm[16][16], rs[16][16];
@@ -559,12 +772,21 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(const float2* part, int ti
   }
   const int i = threadIdx.x & 15, j = threadIdx.x >> 4, r = blockIdx.x * 16 + i;
   if ((int)blockIdx.x * 16 >= rows) return;
+  int first = 0, last = tiles, in = r, step = ld;
+  if (grid) {
+    const CeStream st(rows, V, grid);
+    const int pt = (int)blockIdx.x / 8;
+    first = (st.owner((long)pt * st.qtiles) + pt) * 2;
+    last = (st.owner((long)(pt + 1) * st.qtiles - 1) + pt) * 2 + 2;
+    in = r & 127;
+    step = 128;
+  }
   float m = -INFINITY, s = 0.f;
   if (r < rows)
-    for (int q = j; q < tiles; q += 16) {
-      const float2 p = part[(size_t)q * ld + r];
+    for (int q = first + j; q < last; q += 16) {
+      const float2 p = part[(size_t)q * step + in];
       const float top = fmaxf(m, p.x), at = top == -INFINITY ? 0.f : top;
-      s = s * __builtin_amdgcn_exp2f((m - at) * LOG2E) + p.y * __builtin_amdgcn_exp2f((p.x - at) * LOG2E);
+      s = s * __builtin_amdgcn_exp2f(m - at) + p.y * __builtin_amdgcn_exp2f(p.x - at);
       m = top;
     }
   rm[j][i] = m;
@@ -577,8 +799,8 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(const float2* part, int ti
   const float at = top == -INFINITY ? 0.f : top;
   float all = 0.f;
 #pragma unroll
-  for (int k = 0; k < 16; ++k) all += rs[k][i] * __builtin_amdgcn_exp2f((rm[k][i] - at) * LOG2E);
-  float l = at + logf(all);   // all == 0: -inf, every logit of the row is masked
+  for (int k = 0; k < 16; ++k) all += rs[k][i] * __builtin_amdgcn_exp2f(rm[k][i] - at);
+  float l = __builtin_fmaf(at, LN2, logf(all));   // all == 0: -inf, every logit of the row is masked
   if (lse_c) lse_c[r] = l;
   const int n = index ? index[row0 + r] : r;
   float x;
@@ -636,12 +858,16 @@ __global__ __launch_bounds__(256) void ce_dbias_kernel(const float* part, long l
 struct CePlan {
   long rows;          // per piece, a multiple of 256
   int pieces, ksplit;
-  bool big;           // 256 x 256 tiles for the logits and dw
+  bool stream, big;   // ce_stream_kernel, or 256 x 256 tiles, for the logits
   bool big_dh, big_dw;
   long Vp;
   size_t index, tlogit, lse, weight, part, hc, g, slab, dwacc, dbpart, dbacc, total;
 };
 
+constexpr int STREAM_GRID = 512;   // two workgroups per CU
+#ifndef CE_STREAM_DIM
+#define CE_STREAM_DIM 256
+#endif
 constexpr size_t PIECE_BYTES = (size_t)4 << 30;   // g of a piece, unless the caller says how many rows
 
 bool sizes_ok(const mmst_linear_ce_args* a) {
@@ -675,6 +901,7 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
   }
   p.pieces = grad && all ? (int)((all + p.rows - 1) / p.rows) : 1;
   auto tiles = [](long n, long m, int b) { return ((n + b - 1) / b) * ((m + b - 1) / b); };
+  p.stream = a->D <= CE_STREAM_DIM || tiles(p.rows, a->V, 256) < 256;
   p.big = tiles(p.rows, a->V, 256) >= 256;
   p.big_dh = a->D > 128;
   p.big_dw = a->D > 128 && tiles(a->V, a->D, 256) >= 256;
@@ -689,7 +916,7 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
   auto take = [&](size_t n) { const size_t o = at; at += align(n); return o; };
   const long qt = (a->V + (p.big ? 256 : 128) - 1) / (p.big ? 256 : 128);
   p.tlogit = take(p.rows * 4);
-  p.part = take((size_t)qt * p.rows * 8);
+  p.part = take(p.stream ? (size_t)(STREAM_GRID + p.rows / 128 + 1) * 2 * 128 * 8 : (size_t)qt * p.rows * 8);
   if (grad) {
     p.index = take((size_t)(all + 256) * 4);
     p.lse = take(p.rows * 4);
@@ -699,7 +926,7 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
     if (p.ksplit > 1) p.slab = take((size_t)p.ksplit * p.rows * a->D * 4);
     if (p.pieces > 1 && !a->grad_f32) p.dwacc = take((size_t)a->V * a->D * 4);
     if (a->dbias) {
-      p.dbpart = take((size_t)(p.rows / 128) * p.Vp * 4);
+      p.dbpart = take((size_t)(p.rows / 64) * p.Vp * 4);
       if (p.pieces > 1 && !a->grad_f32) p.dbacc = take((size_t)a->V * 4);
     }
   }
@@ -714,6 +941,11 @@ template <int MODE> void launch(CeGemm& g, bool big, long prows, long qcols, hip
   const unsigned grid = (unsigned)(g.ptiles * g.qtiles * g.ksplit);
   if (big) hipLaunchKernelGGL((ce_gemm_kernel<MODE, 256, 256, 2, 4>), dim3(grid), dim3(512), 0, st, g);
   else hipLaunchKernelGGL((ce_gemm_kernel<MODE, 128, 128, 2, 2>), dim3(grid), dim3(256), 0, st, g);
+}
+
+template <int MODE> void launch_logits(CeGemm& g, const CePlan& p, long prows, long qcols, hipStream_t st) {
+  if (p.stream) hipLaunchKernelGGL((ce_stream_kernel<MODE>), dim3(STREAM_GRID), dim3(256), 0, st, g);
+  else launch<MODE>(g, p.big, prows, qcols, st);
 }
 
 }  // namespace
@@ -746,9 +978,9 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
   logit.rows_max = (int)p.rows;
   if (!grad) {
     logit.P = (const bf16*)A.h; logit.ldp = A.ldh; logit.rows_max = N; logit.Pn = N;
-    launch<LOGIT_STATS>(logit, p.big, N, V, st);
+    launch_logits<LOGIT_STATS>(logit, p, N, V, st);
     MMST_CHECK_LAUNCH();
-    hipLaunchKernelGGL(ce_rows_kernel, dim3((N + 15) / 16), dim3(256), 0, st, logit.part, logit.qtiles, N, nullptr, 0, N,
+    hipLaunchKernelGGL(ce_rows_kernel, dim3((N + 15) / 16), dim3(256), 0, st, logit.part, logit.qtiles, N, p.stream ? STREAM_GRID : 0, nullptr, 0, N,
                        nullptr, A.target, A.ignore_index, V, logit.tlogit, nullptr, A.loss, A.lse);
     MMST_CHECK_LAUNCH();
     return MMST_OK;
@@ -765,7 +997,7 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
   bf16* gbuf = (bf16*)(ws + p.g);
   float* lse_c = (float*)(ws + p.lse);
   float* weight = (float*)(ws + p.weight);
-  const int BPg = p.big ? 256 : 128;
+  const int BPg = p.stream ? 64 : p.big ? 256 : 128;   // rows per partial sum of dbias
   for (int i = 0; i < p.pieces; ++i) {
     const int row0 = (int)(i * p.rows);
     const int rows_max = (int)p.rows;
@@ -773,15 +1005,16 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
                        D8, index, count, row0, rows_max, A.dloss, A.grad_scale, hc, weight);
     MMST_CHECK_LAUNCH();
     logit.P = hc; logit.ldp = D; logit.Pn = rows_max; logit.count = count; logit.row0 = row0; logit.index = index + row0;
-    launch<LOGIT_STATS>(logit, p.big, p.rows, V, st);
+    launch_logits<LOGIT_STATS>(logit, p, p.rows, V, st);
     MMST_CHECK_LAUNCH();
-    hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)(p.rows / 16)), dim3(256), 0, st, logit.part, logit.qtiles, rows_max, count,
+    hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)(p.rows / 16)), dim3(256), 0, st, logit.part, logit.qtiles, rows_max,
+                       p.stream ? STREAM_GRID : 0, count,
                        row0, rows_max, index, A.target, A.ignore_index, V, logit.tlogit, lse_c, A.loss, A.lse);
     MMST_CHECK_LAUNCH();
     CeGemm gr = logit;
     gr.lse = lse_c; gr.weight = weight; gr.g = gbuf; gr.ldg = p.Vp;
     gr.dbias_part = A.dbias ? (float*)(ws + p.dbpart) : nullptr;
-    launch<LOGIT_GRAD>(gr, p.big, p.rows, p.Vp, st);
+    launch_logits<LOGIT_GRAD>(gr, p, p.rows, p.Vp, st);
     MMST_CHECK_LAUNCH();
 
     CeGemm dh = {};
