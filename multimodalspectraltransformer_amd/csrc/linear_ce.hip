@@ -506,67 +506,99 @@ __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_
 }
 
 // ---------------------------------------------------------------------------------------------------- logits, streamed
-// The logits of a narrow layer (few steps of the contraction per tile) or of few rows: the tiles, 128 x 128, are dealt out
-// to G workgroups in equal runs along the vocabulary, and a workgroup's run is ONE stream of steps, so that the next tile's
-// operands arrive during the last products and the softmax of this one (tile by tile, each beginning with an empty
-// pipeline: 109 instead of ... us for the stats of 3032 x 128 x 32000).  A lane keeps the running maximum and sum of its own
-// columns of a row over the whole run; lanes, waves and workgroups are joined at its end.  Two workgroups per CU: one's
-// exponentials run beside the other's products.
+// The logits of a narrow layer (D <= 128, the width of this library's own layers): a tile has so few products that loading
+// it, its softmax and its stores are what counts.  The tiles, 128 x 128, are dealt out to G workgroups in equal runs along the
+// vocabulary; a wave keeps its 64 rows of h in registers for the run, and the words of the next tile arrive by LDS-DMA
+// while this one is multiplied and exponentiated: one barrier per tile.  A lane keeps the running maximum and sum of its
+// own columns of a row over the whole run; lanes, waves and workgroups are joined at its end.  Two workgroups per CU: one's
+// vector instructions (max, fused multiply-add, exponential and sum per logit, what bounds this kernel) run beside the
+// other's products.  (As single tiles, each beginning with an empty pipeline: 109 us for the stats of 3032 x 128 x 32000.)
+// A large vocabulary is cut into eight parts, one per XCD, so that the words that an XCD's workgroups read over and over stay
+// in its L2 (all of 32000 x 128 from everywhere: 48 us, at the rate of the memory behind the L2s).
 struct CeStream {
-  long T; int G, qtiles;                            // tiles of all rows that count, workgroups that have any, tiles per row
+  int ptiles, qtiles, parts, per_part;   // tiles of the rows that count and of the vocabulary; workgroups per part
+  int q0, qn, G;                         // this part's first tile of the vocabulary, how many, workgroups that have any
+  long T;
   __device__ __forceinline__ CeStream(int rows, int V, int grid) {
+    ptiles = (rows + 127) / 128;
     qtiles = (V + 127) / 128;
-    T = (long)((rows + 127) / 128) * qtiles;
-    G = T < grid ? (int)T : grid;
+    parts = qtiles >= 64 ? 8 : 1;
+    per_part = grid / parts;
+  }
+  __device__ __forceinline__ void part(int x) {
+    q0 = qtiles * x / parts;
+    qn = qtiles * (x + 1) / parts - q0;
+    T = (long)ptiles * qn;
+    G = T < per_part ? (int)T : per_part;
   }
   __device__ __forceinline__ long begin(int b) const { return T * b / G; }
   __device__ __forceinline__ int owner(long tile) const { return (int)(((tile + 1) * G - 1) / T); }
-  // where workgroup b leaves its (max, sum) of the row tile pt, one of each half of the columns
-  static __device__ __forceinline__ size_t slot(int b, int pt, int half) { return ((size_t)(b + pt) * 2 + half) * 128; }
+  // where workgroup b of part x leaves its (max, sum) of the row tile pt, one of each half of the columns
+  __device__ __forceinline__ size_t slot(int x, int b, int pt, int half) const {
+    return (((size_t)x * (per_part + ptiles) + b + pt) * 2 + half) * 128;
+  }
 };
 
 template <int MODE>
 __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
-  using Tile = CeTile<MODE, 128, 128, 2, 2>;
-  constexpr int MT = Tile::MT, NT = Tile::NT, BK = Tile::BK;
-  static_assert(MT == 4 && NT == 4, "four by four");
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[Tile::SMEM];
+  constexpr int MT = 4, NT = 4, KS = 4;   // 64 x 64 per wave, 128 of the contraction
+  using OpQ = Operand<false, true, 128, 256, 64>;
+  constexpr int STAGE = 2 * OpQ::BYTES;   // the two halves of the contraction
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * STAGE];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rows = piece_rows(a);
-  const CeStream st(rows, a.Qn, gridDim.x);
-  // neighbours in the stream to one XCD (workgroups go round the eight of them)
-  int b;
-  {
-    const int n = gridDim.x, q8 = n >> 3, r8 = n & 7, x = blockIdx.x & 7;
-    b = (x < r8 ? x * (q8 + 1) : r8 * (q8 + 1) + (x - r8) * q8) + ((int)blockIdx.x >> 3);
-  }
+  CeStream st(rows, a.Qn, gridDim.x);
+  // workgroups go round the eight XCDs: one part each, or neighbours in the stream to one XCD
+  const int xcd = blockIdx.x & 7, vocab_part = st.parts == 8 ? xcd : 0;
+  const int b = st.parts == 8 ? (int)blockIdx.x >> 3 : xcd * ((int)gridDim.x >> 3) + ((int)blockIdx.x >> 3);
+  st.part(vocab_part);
   if (b >= st.G) return;   // (uniform)
-  const long t0 = st.begin(b), t1 = st.begin(b + 1);
-  int pt = (int)(t0 / st.qtiles), qt = (int)(t0 - (long)pt * st.qtiles);
+  const long t0 = st.begin(b);
+  const int ntiles = (int)(st.begin(b + 1) - t0), qend = st.q0 + st.qn;
+  int pt = (int)(t0 / st.qn), qt = st.q0 + (int)(t0 - (long)pt * st.qn);
   const int pw0 = (wave >> 1) * 64, qw0 = (wave & 1) * 64;
   const int i16 = lane & 15, j4 = lane >> 4;
-  const int nsteps = (a.K + BK - 1) / BK;
-  typename Tile::OpP op;
-  typename Tile::OpQ oq;
-  op.init(a.P, a.ldp, pt * 128, rows, a.K, tid);
+  const bool two = a.K > 64;
+  OpQ oq;
   oq.init(a.Q, a.ldq, qt * 128, a.Qn, a.K, tid);
   lds_byte* const lds = (lds_byte*)smem;
-  Tile::template issue<0, Tile::PER>(op, oq, lds, 0, tid, wave);
-
-  // a tile's products start from the bias: -infinity past the vocabulary, which leaves those columns out of everything
-  float start[NT / 2][8];
-  auto load_start = [&](int q) {
-#pragma unroll
-    for (int tp = 0; tp < NT / 2; ++tp)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int v = q * 128 + qw0 + tp * 32 + 8 * j4 + e;
-        start[tp][e] = v < a.Qn ? (a.bias ? word_bias(a.bias[v]) : 0.f) : -INFINITY;
-      }
+  auto issue = [&](lds_byte* wr) {
+    oq.template issue<0, OpQ::NI>(wr, 0, tid, wave);
+    if (two) oq.template issue<0, OpQ::NI>(wr + OpQ::BYTES, 64, tid, wave);
   };
-  load_start(qt);
+  issue(lds);
+
+  // The bias of the lane's columns, requested a tile ahead: loads without a branch each, and nothing is done with their values
+  // before that tile begins (a compare behind each load costs 16 memory latencies per tile: 71 us instead of 48).
+  float raw[NT / 2][8];
+  auto load_bias = [&](int q) {
+    const int c = q * 128 + qw0 + 8 * j4;
+    if (!a.bias) {
+#pragma unroll
+      for (int tp = 0; tp < NT / 2; ++tp)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) raw[tp][e] = 0.f;
+    } else if (q * 128 + 128 <= a.Qn) {
+#pragma unroll
+      for (int tp = 0; tp < NT / 2; ++tp) {
+        struct __attribute__((packed, aligned(4))) F4 { f32x4 v; };
+        const f32x4 lo = reinterpret_cast<const F4*>(a.bias + c + tp * 32)->v, hi = reinterpret_cast<const F4*>(a.bias + c + tp * 32 + 4)->v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { raw[tp][e] = lo[e]; raw[tp][4 + e] = hi[e]; }
+      }
+    } else {
+#pragma unroll
+      for (int tp = 0; tp < NT / 2; ++tp)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int v = c + tp * 32 + e;
+          raw[tp][e] = a.bias[v < a.Qn ? v : a.Qn - 1];
+        }
+    }
+  };
   float m2[MT], sum[MT], lse2[MT], wt[MT];   // running maximum in units of log 2, running sum; lse and weight (gradient)
   int target[MT];
+  bf16x8 pf[MT][KS];
   auto load_rows = [&](int p) {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -576,6 +608,12 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
       target[mt] = -1;
       lse2[mt] = INFINITY;   // a row that is not there, or whose every logit is masked: no gradient
       wt[mt] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        pf[mt][ks] = bf16x8{};
+        const int k = ks * 32 + 8 * j4;
+        if (m < rows && k < a.K) pf[mt][ks] = *reinterpret_cast<const bf16x8*>(a.P + (long)m * a.ldp + k);
+      }
       if (m < rows) {
         const int64_t t = a.target[a.index ? a.index[m] : m];
         target[mt] = t >= 0 && t < a.Qn ? (int)t : -1;
@@ -585,42 +623,81 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
         }
       }
     }
+    // A use of all of it, here: the compiler waits for a loaded value where it is first used, and in the loop that would be
+    // a wait for everything requested since, once per tile.
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      asm volatile("" : "+v"(target[mt]), "+v"(lse2[mt]), "+v"(wt[mt]));
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(pf[mt][ks]));
+    }
+  };
+  auto bias_arrived = [&]() {   // (the same)
+#pragma unroll
+    for (int tp = 0; tp < NT / 2; ++tp)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(raw[tp][e]));
   };
   load_rows(pt);
+  load_bias(qt);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  bias_arrived();
 
-  int stage = 0;
-  for (long t = t0; t < t1; ++t) {
-    f32x4 acc[MT][NT];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[mt][nt][e] = start[nt >> 1][(nt & 1) * 4 + e];
+  for (int t = 0; t < ntiles; ++t) {
     const int q0 = qt * 128;
-    const bool new_rows = qt + 1 == st.qtiles;
-    const int pt1 = new_rows ? pt + 1 : pt, qt1 = new_rows ? 0 : qt + 1;
-    for (int s = 0; s < nsteps; ++s) {
-      if (s) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (a tile's first step: waited for before the last one's stores)
-      asm volatile("s_barrier" ::: "memory");
-      bool more = true;
-      int k1 = (s + 1) * BK;
-      if (s + 1 == nsteps) {
-        more = t + 1 < t1;
-        k1 = 0;
-        if (more) {
-          op.seek(a.P, pt1 * 128, rows);
-          oq.seek(a.Q, qt1 * 128, a.Qn);
-        }
-      }
-      Tile::step(acc, op, oq, lds + (stage ^ 1) * Tile::STAGE, lds + stage * Tile::STAGE, more, k1, tid, wave, pw0, qw0, lane);
-      stage ^= 1;
+    const bool new_rows = qt + 1 == qend, more = t + 1 < ntiles;
+    const int pt1 = new_rows ? pt + 1 : pt, qt1 = new_rows ? st.q0 : qt + 1;
+    // The products start from the bias: -infinity past the vocabulary, which leaves those columns out of everything.  The
+    // lowest float is rare enough to look for first (eight instructions instead of 48).
+    f32x4 start[NT];
+    if (a.bias) {
+      float low = raw[0][0];
+#pragma unroll
+      for (int tp = 0; tp < NT / 2; ++tp)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) low = fminf(low, raw[tp][e]);
+      if (__ballot(low < -0x1p127f))
+#pragma unroll
+        for (int tp = 0; tp < NT / 2; ++tp)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) raw[tp][e] = word_bias(raw[tp][e]);
     }
-    if (t + 1 < t1) load_start(qt1);
+    if (q0 + 128 > a.Qn)
+#pragma unroll
+      for (int tp = 0; tp < NT / 2; ++tp)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (q0 + qw0 + tp * 32 + 8 * j4 + e >= a.Qn) raw[tp][e] = -INFINITY;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) start[nt][e] = raw[nt >> 1][(nt & 1) * 4 + e];
+    // (this wave's share of the tile has landed, see below: behind the barrier everybody's has, and nobody reads the other stage)
+    asm volatile("s_barrier" ::: "memory");
+    f32x4 acc[MT][NT];
+    [&](lds_byte* __restrict__ wr, const lds_byte* __restrict__ rd) {
+      if (more) {
+        oq.seek(a.Q, qt1 * 128, a.Qn);
+        issue(wr);
+        load_bias(qt1);
+      }
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        if (ks >= 2 && !two) break;
+        bf16x8 qf[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          qf[nt] = OpQ::frag(rd + (ks >> 1) * OpQ::BYTES, qw0 + (nt >> 1) * 32, nt & 1, ks & 1, lane);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            acc[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf[nt], pf[mt][ks], ks ? acc[mt][nt] : start[nt], 0, 0, 0);
+      }
+    }(lds + (~t & 1) * STAGE, lds + (t & 1) * STAGE);
     auto holds_target = [&](int mt) {   // the lane's column of the target's logit, or -1
       const int rel = target[mt] - (q0 + qw0 + 8 * j4);
-      return target[mt] >= 0 && rel >= 0 && rel < 64 && (rel & 31) < 8 ? rel : -1;
+      return target[mt] >= 0 && (rel & ~39) == 0 && rel < 64 ? rel : -1;   // rel = 0..7, 32..39
     };
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -654,9 +731,17 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
         }
       }
     }
-    // The next step's operands have landed (they had the last products and all of the above to do so); waited for here and
-    // not in the loop, which would wait for the following stores as well.
+    // The next tile's words have landed (they had this tile's products and exponentials to do so, which is why those are made
+    // to be done here); waited for here and not at the barrier, which would wait for the following stores as well.
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      if constexpr (MODE == LOGIT_STATS) asm volatile("" : "+v"(sum[mt]), "+v"(m2[mt]));
+      else
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) asm volatile("" : "+v"(acc[mt][nt]));
+    }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    bias_arrived();
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       const int m = pt * 128 + pw0 + mt * 16 + i16;
@@ -682,28 +767,27 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
       }
     }
     if constexpr (MODE == LOGIT_GRAD) {
-      if (a.dbias_part) {   // column sums of the wave's 64 rows
-        float* d = a.dbias_part + (size_t)(pt * 2 + (wave >> 1)) * a.ldg + q0 + qw0 + 8 * j4;
+      if (a.dbias_part) {   // column sums of the wave's 64 rows; lane i16 of each 16 writes the i16-th of its 16 columns
+        float mine = 0.f;
 #pragma unroll
-        for (int tp = 0; tp < NT / 2; ++tp)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float x = row16_sum((acc[0][2 * tp + (e >> 2)][e & 3] + acc[1][2 * tp + (e >> 2)][e & 3]) +
-                                      (acc[2][2 * tp + (e >> 2)][e & 3] + acc[3][2 * tp + (e >> 2)][e & 3]));
-            if (i16 == 0) d[tp * 32 + e] = x;
-          }
+        for (int c = 0; c < 16; ++c) {
+          const int nt = c >> 2, e = c & 3;
+          const float x = row16_sum((acc[0][nt][e] + acc[1][nt][e]) + (acc[2][nt][e] + acc[3][nt][e]));
+          mine = i16 == c ? x : mine;
+        }
+        a.dbias_part[(size_t)(pt * 2 + (wave >> 1)) * a.ldg + q0 + qw0 + (i16 >> 3) * 32 + 8 * j4 + (i16 & 7)] = mine;
       }
     }
-    if (new_rows || t + 1 == t1) {
+    if (new_rows || !more) {
       if constexpr (MODE == LOGIT_STATS) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
           const float top = xor32_max(xor16_max(m2[mt])), at = top == -INFINITY ? 0.f : top;
           const float x = xor32_sum(xor16_sum(sum[mt] * __builtin_amdgcn_exp2f(m2[mt] - at)));
-          if (j4 == 0) a.part[CeStream::slot(b, pt, wave & 1) + pw0 + mt * 16 + i16] = make_float2(top, x);
+          if (j4 == 0) a.part[st.slot(vocab_part, b, pt, wave & 1) + pw0 + mt * 16 + i16] = make_float2(top, x);
         }
       }
-      if (t + 1 < t1) load_rows(pt1);
+      if (more) load_rows(pt1);
     }
     pt = pt1;
     qt = qt1;
@@ -772,23 +856,22 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(const float2* part, int ti
   }
   const int i = threadIdx.x & 15, j = threadIdx.x >> 4, r = blockIdx.x * 16 + i;
   if ((int)blockIdx.x * 16 >= rows) return;
-  int first = 0, last = tiles, in = r, step = ld;
-  if (grid) {
-    const CeStream st(rows, V, grid);
-    const int pt = (int)blockIdx.x / 8;
-    first = (st.owner((long)pt * st.qtiles) + pt) * 2;
-    last = (st.owner((long)(pt + 1) * st.qtiles - 1) + pt) * 2 + 2;
-    in = r & 127;
-    step = 128;
-  }
   float m = -INFINITY, s = 0.f;
-  if (r < rows)
-    for (int q = first + j; q < last; q += 16) {
-      const float2 p = part[(size_t)q * step + in];
-      const float top = fmaxf(m, p.x), at = top == -INFINITY ? 0.f : top;
-      s = s * __builtin_amdgcn_exp2f(m - at) + p.y * __builtin_amdgcn_exp2f(p.x - at);
-      m = top;
-    }
+  auto join = [&](const float2 p) {
+    const float top = fmaxf(m, p.x), at = top == -INFINITY ? 0.f : top;
+    s = s * __builtin_amdgcn_exp2f(m - at) + p.y * __builtin_amdgcn_exp2f(p.x - at);
+    m = top;
+  };
+  if (r < rows && !grid)
+    for (int q = j; q < tiles; q += 16) join(part[(size_t)q * ld + r]);
+  if (r < rows && grid) {   // lane j: part j / 2 (or j of 16 lanes the only one), half j & 1 of the columns
+    CeStream st(rows, V, grid);
+    const int pt = (int)blockIdx.x / 8, x = st.parts == 8 ? j >> 1 : 0;
+    st.part(x);
+    const int b0 = st.owner((long)pt * st.qn), b1 = st.owner((long)(pt + 1) * st.qn - 1);
+    for (int b = b0 + (st.parts == 8 ? 0 : j >> 1); b <= b1; b += st.parts == 8 ? 1 : 8)
+      join(part[st.slot(x, b, pt, j & 1) + (r & 127)]);
+  }
   rm[j][i] = m;
   rs[j][i] = s;
   __syncthreads();
@@ -848,7 +931,9 @@ __global__ __launch_bounds__(256) void ce_dbias_kernel(const float* part, long l
   int rows = *count - row0;
   rows = rows < 0 ? 0 : rows < rows_max ? rows : rows_max;
   float s = 0.f;
-  for (int t = 0; t < (rows + BP - 1) / BP; ++t) s += part[(size_t)t * ld + v];
+  const int n = (rows + BP - 1) / BP;
+#pragma unroll 8
+  for (int t = 0; t < n; ++t) s += part[(size_t)t * ld + v];
   if (acc_in) s += acc_in[v];
   if (out_f32) ((float*)out)[v] = s;
   else ((bf16*)out)[v] = (bf16)s;
@@ -865,9 +950,6 @@ struct CePlan {
 };
 
 constexpr int STREAM_GRID = 512;   // two workgroups per CU
-#ifndef CE_STREAM_DIM
-#define CE_STREAM_DIM 256
-#endif
 constexpr size_t PIECE_BYTES = (size_t)4 << 30;   // g of a piece, unless the caller says how many rows
 
 bool sizes_ok(const mmst_linear_ce_args* a) {
@@ -901,7 +983,7 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
   }
   p.pieces = grad && all ? (int)((all + p.rows - 1) / p.rows) : 1;
   auto tiles = [](long n, long m, int b) { return ((n + b - 1) / b) * ((m + b - 1) / b); };
-  p.stream = a->D <= CE_STREAM_DIM || tiles(p.rows, a->V, 256) < 256;
+  p.stream = a->D <= 128;
   p.big = tiles(p.rows, a->V, 256) >= 256;
   p.big_dh = a->D > 128;
   p.big_dw = a->D > 128 && tiles(a->V, a->D, 256) >= 256;
@@ -916,7 +998,7 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
   auto take = [&](size_t n) { const size_t o = at; at += align(n); return o; };
   const long qt = (a->V + (p.big ? 256 : 128) - 1) / (p.big ? 256 : 128);
   p.tlogit = take(p.rows * 4);
-  p.part = take(p.stream ? (size_t)(STREAM_GRID + p.rows / 128 + 1) * 2 * 128 * 8 : (size_t)qt * p.rows * 8);
+  p.part = take(p.stream ? (size_t)(STREAM_GRID + 8 * (p.rows / 128)) * 2 * 128 * 8 : (size_t)qt * p.rows * 8);
   if (grad) {
     p.index = take((size_t)(all + 256) * 4);
     p.lse = take(p.rows * 4);
