@@ -38,11 +38,13 @@ struct CeGemm {
   int ptiles, qtiles, ksplit;
   // logits
   const float* bias; const int64_t* target; const int* index;
+  const int* word;                   // the targets of the rows that count (gradient; NULL: target[row])
   float2* part; float* tlogit;       // per (tile column, row): max, sum of exp; the target's logit
-  const float* lse; const float* weight; bf16* g; long ldg; float* dbias_part;
+  const float* lse; const float* weight; bf16* g; long ldg;
   // products
   void* out; long ldo; int out_f32; int accumulate;   // out_f32: fp32, else bf16; accumulate: added to
   const float* acc_in; float* slab;
+  void* dbias; const float* dbias_in;                 // DW: sums of g over the rows, in out's type; added to dbias_in
 };
 
 __device__ __forceinline__ int piece_rows(const CeGemm& a) {
@@ -145,18 +147,34 @@ struct CeTile {
   static constexpr int STAGE = OpP::BYTES + OpQ::BYTES, SMEM = NS * STAGE;
 
   struct Frags { bf16x8 p[MT], q[NT]; };
+  // SUM (DW): also the sums of the P operand over the contraction, as one more product against ones
+  template <bool SUM> struct Acc {
+    f32x4 v[MT][NT];
+    f32x4 sum[SUM ? MT : 1];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) v[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < (SUM ? MT : 1); ++i) sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    __device__ __forceinline__ void add(const Frags& f, int mt) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) v[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.q[nt], f.p[mt], v[mt][nt], 0, 0, 0);
+      if constexpr (SUM) {
+        bf16x8 ones;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ones[e] = (bf16)1.0f;
+        sum[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, f.p[mt], sum[mt], 0, 0, 0);
+      }
+    }
+  };
   static __device__ __forceinline__ void read(Frags& f, const lds_byte* rd, int ks, int pw0, int qw0, int lane) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) f.q[nt] = OpQ::frag(rd + OpP::BYTES, qw0 + (nt >> 1) * 32, nt & 1, ks, lane);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) f.p[mt] = OpP::frag(rd, pw0 + mt * 16, 0, ks, lane);
-  }
-  static __device__ __forceinline__ void products(f32x4 (&acc)[MT][NT], const Frags& f) {
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        acc[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.q[nt], f.p[mt], acc[mt][nt], 0, 0, 0);
   }
   // DMA instructions LO .. HI - 1 of the step's PER: the P operand's, then the Q operand's
   static constexpr int PER = OpP::NI + OpQ::NI;
@@ -168,7 +186,8 @@ struct CeTile {
 
   // One step: the next step's operands are requested into `wr`, the products of `rd` are made.  The two never
   // overlap, and saying so is what keeps the compiler from waiting for the DMA before every LDS read.
-  static __device__ __forceinline__ void step(f32x4 (&acc)[MT][NT], const OpP& p, const OpQ& q, lds_byte* __restrict__ wr,
+  template <bool SUM>
+  static __device__ __forceinline__ void step(Acc<SUM>& acc, const OpP& p, const OpQ& q, lds_byte* __restrict__ wr,
                                               const lds_byte* __restrict__ rd, bool more, int k1, int tid, int wave,
                                               int pw0, int qw0, int lane) {
     if (more) issue<0, PER>(p, q, wr, k1, tid, wave);
@@ -176,7 +195,8 @@ struct CeTile {
     for (int ks = 0; ks < BK / 32; ++ks) {
       Frags f;
       read(f, rd, ks, pw0, qw0, lane);
-      products(acc, f);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) acc.add(f, mt);
     }
   }
 
@@ -192,22 +212,20 @@ struct CeTile {
   static __device__ __forceinline__ void barrier() { asm volatile("s_barrier" ::: "memory"); fence(); }
   static __device__ __forceinline__ void reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
   static __device__ __forceinline__ void dma_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-  template <int MT0, int MT1> static __device__ __forceinline__ void some(f32x4 (&acc)[MT][NT], const Frags& f) {
+  template <int MT0, int MT1, bool SUM> static __device__ __forceinline__ void some(Acc<SUM>& acc, const Frags& f) {
 #pragma unroll
-    for (int mt = MT0; mt < MT1; ++mt)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        acc[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.q[nt], f.p[mt], acc[mt][nt], 0, 0, 0);
+    for (int mt = MT0; mt < MT1; ++mt) acc.add(f, mt);
     fence();
   }
-  static __device__ __forceinline__ void multiply(f32x4 (&acc)[MT][NT], const Frags& f) {
+  template <bool SUM> static __device__ __forceinline__ void multiply(Acc<SUM>& acc, const Frags& f) {
     __builtin_amdgcn_s_setprio(1);
     some<0, MT>(acc, f);
     __builtin_amdgcn_s_setprio(0);
   }
   // the products with DMA instructions LO .. LO + PER / 2 - 1 between them
-  template <int LO> static __device__ __forceinline__ void multiply_issue(f32x4 (&acc)[MT][NT], const Frags& f, const OpP& p,
-                                                                          const OpQ& q, lds_byte* wr, int k, int tid, int wave) {
+  template <int LO, bool SUM>
+  static __device__ __forceinline__ void multiply_issue(Acc<SUM>& acc, const Frags& f, const OpP& p, const OpQ& q, lds_byte* wr,
+                                                        int k, int tid, int wave) {
     static_assert(MT == 8 && PER == 8, "eight by eight");
     __builtin_amdgcn_s_setprio(1);
     some<0, 1>(acc, f);
@@ -221,7 +239,8 @@ struct CeTile {
     some<7, 8>(acc, f);
     __builtin_amdgcn_s_setprio(0);
   }
-  static __device__ __forceinline__ void step_first(f32x4 (&acc)[MT][NT], const OpP& p, const OpQ& q, lds_byte* __restrict__ wr,
+  template <bool SUM>
+  static __device__ __forceinline__ void step_first(Acc<SUM>& acc, const OpP& p, const OpQ& q, lds_byte* __restrict__ wr,
                                                     const lds_byte* __restrict__ rd, int k1, int tid, int wave, int pw0,
                                                     int qw0, int lane) {
     Frags f;
@@ -239,7 +258,8 @@ struct CeTile {
     dma_done();
     barrier();
   }
-  static __device__ __forceinline__ void step_second(f32x4 (&acc)[MT][NT], Frags& f, const OpP& p, const OpQ& q,
+  template <bool SUM>
+  static __device__ __forceinline__ void step_second(Acc<SUM>& acc, Frags& f, const OpP& p, const OpQ& q,
                                                      lds_byte* __restrict__ wr, const lds_byte* __restrict__ rd, int k1,
                                                      int tid, int wave, int pw0, int qw0, int lane) {
     multiply_issue<0>(acc, f, p, q, wr, k1, tid, wave);
@@ -258,7 +278,8 @@ struct CeTile {
   }
   // No branch inside a step: the last one requests a step that is not there, which moves nothing but zeros (or, in a split
   // contraction, the next part's first step) into the stage that nobody reads, and the second half starts by multiplying zeros.
-  static __device__ __forceinline__ void loop(f32x4 (&acc)[MT][NT], const OpP& p, const OpQ& q, lds_byte* lds, int kbeg,
+  template <bool SUM>
+  static __device__ __forceinline__ void loop(Acc<SUM>& acc, const OpP& p, const OpQ& q, lds_byte* lds, int kbeg,
                                               int nsteps, int tid, int wave, int pw0, int qw0, int lane) {
     if (nsteps <= 0) return;
     issue<0, PER>(p, q, lds, kbeg, tid, wave);
@@ -324,13 +345,28 @@ __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_
   op.init(a.P, a.ldp, p0, Pn, K, tid);
   oq.init(a.Q, a.ldq, q0, a.Qn, K, tid);
 
-  f32x4 acc[MT][NT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   lds_byte* const lds = (lds_byte*)smem;
-  Tile::loop(acc, op, oq, lds, kbeg, nsteps, tid, wave, pw0, qw0, lane);
+  typename Tile::template Acc<false> plain;
+  f32x4 (&acc)[MT][NT] = plain.v;
+  if (MODE == DW && a.dbias && qt == 0 && wave % WQ == 0) {   // the waves that also have the sums over the rows
+    typename Tile::template Acc<MODE == DW> sums;
+    sums.clear();
+    Tile::loop(sums, op, oq, lds, kbeg, nsteps, tid, wave, pw0, qw0, lane);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const int v = p0 + pw0 + mt * 16 + (lane & 15);
+      if (lane < 16 && v < Pn) {
+        const float x = sums.sum[MODE == DW ? mt : 0][0] + (a.dbias_in ? a.dbias_in[v] : 0.f);
+        if (a.out_f32) ((float*)a.dbias)[v] = x;
+        else ((bf16*)a.dbias)[v] = (bf16)x;
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = sums.v[mt][nt];
+    }
+  } else {
+    plain.clear();
+    Tile::loop(plain, op, oq, lds, kbeg, nsteps, tid, wave, pw0, qw0, lane);
+  }
 
   const int i16 = lane & 15, j4 = lane >> 4;
   if constexpr (MODE == LOGIT_STATS || MODE == LOGIT_GRAD) {
@@ -362,8 +398,7 @@ __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_
             if (q0 + qw0 + tp * 32 + 8 * j4 + e >= a.Qn) acc[mt][2 * tp + (e >> 2)][e & 3] = -INFINITY;
       }
       if (m < rows) {   // the target's logit, by the one lane that holds it
-        const int n = a.index ? a.index[m] : m;
-        const int64_t t = a.target[n] - (q0 + qw0 + 8 * j4);
+        const int64_t t = (a.word ? (int64_t)a.word[m] : a.target[m]) - (q0 + qw0 + 8 * j4);
         if (t >= 0 && t < BQ / WQ && (t & 31) < 8) {
           float x = 0.f;
 #pragma unroll
@@ -417,11 +452,6 @@ __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_
   }
   if constexpr (MODE == LOGIT_GRAD) {
     // the whole tile is written, zeros where no word is: the products read whole 16-byte pieces of a row
-    float col[NT / 2][8];
-#pragma unroll
-    for (int tp = 0; tp < NT / 2; ++tp)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) col[tp][e] = 0.f;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       const int m = p0 + pw0 + mt * 16 + i16;
@@ -431,7 +461,7 @@ __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_
       if (ok) {
         lse = a.lse[m];
         wt = a.weight[m];
-        t = a.target[a.index[m]] - (q0 + qw0 + 8 * j4);
+        t = a.word[m] - (q0 + qw0 + 8 * j4);
         ok = lse != -INFINITY;   // a row whose every logit is masked has no gradient
       }
 #pragma unroll
@@ -443,28 +473,9 @@ __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_
           float x = __builtin_amdgcn_exp2f((acc[mt][2 * tp + (e >> 2)][e & 3] - lse) * LOG2E);
           x = (x - (t == tp * 32 + e ? 1.f : 0.f)) * wt;
           x = ok && v < a.Qn ? x : 0.f;
-          col[tp][e] += x;
           o[e] = (bf16)x;
         }
         *reinterpret_cast<bf16x8*>(a.g + (size_t)m * a.ldg + q0 + qw0 + tp * 32 + 8 * j4) = o;
-      }
-    }
-    if (a.dbias_part) {
-      float* red = reinterpret_cast<float*>(smem);   // [WP][BQ]
-      __syncthreads();
-#pragma unroll
-      for (int tp = 0; tp < NT / 2; ++tp)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float s = row16_sum(col[tp][e]);
-          if (i16 == 0) red[(wave / WQ) * BQ + qw0 + tp * 32 + 8 * j4 + e] = s;
-        }
-      __syncthreads();
-      for (int c = tid; c < BQ; c += NTHR) {
-        float s = 0.f;
-#pragma unroll
-        for (int w = 0; w < WP; ++w) s += red[w * BQ + c];
-        a.dbias_part[(size_t)pt * a.ldg + q0 + c] = s;
       }
     }
   }
@@ -518,21 +529,26 @@ __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_
 struct CeStream {
   int ptiles, qtiles, parts, per_part;   // tiles of the rows that count and of the vocabulary; workgroups per part
   int q0, qn, G;                         // this part's first tile of the vocabulary, how many, workgroups that have any
-  long T;
+  uint32_t each, extra;                  // tiles per workgroup; the first `extra` have one more
   __device__ __forceinline__ CeStream(int rows, int V, int grid) {
     ptiles = (rows + 127) / 128;
     qtiles = (V + 127) / 128;
     parts = qtiles >= 64 ? 8 : 1;
-    per_part = grid / parts;
+    per_part = parts == 8 ? grid >> 3 : grid;
   }
   __device__ __forceinline__ void part(int x) {
-    q0 = qtiles * x / parts;
-    qn = qtiles * (x + 1) / parts - q0;
-    T = (long)ptiles * qn;
-    G = T < per_part ? (int)T : per_part;
+    q0 = parts == 8 ? (qtiles * x) >> 3 : 0;
+    qn = (parts == 8 ? (qtiles * (x + 1)) >> 3 : qtiles) - q0;
+    const uint32_t T = (uint32_t)ptiles * (uint32_t)qn;   // (the host keeps the tiles of a launch below 2^31)
+    G = T < (uint32_t)per_part ? (int)T : per_part;
+    each = G ? T / (uint32_t)G : 0;
+    extra = T - each * (uint32_t)G;
   }
-  __device__ __forceinline__ long begin(int b) const { return T * b / G; }
-  __device__ __forceinline__ int owner(long tile) const { return (int)(((tile + 1) * G - 1) / T); }
+  __device__ __forceinline__ uint32_t begin(int b) const { return each * (uint32_t)b + ((uint32_t)b < extra ? (uint32_t)b : extra); }
+  __device__ __forceinline__ int owner(uint32_t tile) const {
+    const uint32_t longer = (each + 1) * extra;
+    return (int)(tile < longer ? tile / (each + 1) : extra + (tile - longer) / each);
+  }
   // where workgroup b of part x leaves its (max, sum) of the row tile pt, one of each half of the columns
   __device__ __forceinline__ size_t slot(int x, int b, int pt, int half) const {
     return (((size_t)x * (per_part + ptiles) + b + pt) * 2 + half) * 128;
@@ -544,7 +560,7 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
   constexpr int MT = 4, NT = 4, KS = 4;   // 64 x 64 per wave, 128 of the contraction
   using OpQ = Operand<false, true, 128, 256, 64>;
   constexpr int STAGE = 2 * OpQ::BYTES;   // the two halves of the contraction
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * STAGE];
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * STAGE + 1024];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rows = piece_rows(a);
   CeStream st(rows, a.Qn, gridDim.x);
@@ -553,48 +569,50 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
   const int b = st.parts == 8 ? (int)blockIdx.x >> 3 : xcd * ((int)gridDim.x >> 3) + ((int)blockIdx.x >> 3);
   st.part(vocab_part);
   if (b >= st.G) return;   // (uniform)
-  const long t0 = st.begin(b);
+  const uint32_t t0 = st.begin(b);
   const int ntiles = (int)(st.begin(b + 1) - t0), qend = st.q0 + st.qn;
-  int pt = (int)(t0 / st.qn), qt = st.q0 + (int)(t0 - (long)pt * st.qn);
+  int pt = (int)(t0 / (uint32_t)st.qn), qt = st.q0 + (int)(t0 - (uint32_t)pt * st.qn);
   const int pw0 = (wave >> 1) * 64, qw0 = (wave & 1) * 64;
   const int i16 = lane & 15, j4 = lane >> 4;
   const bool two = a.K > 64;
-  OpQ oq;
-  oq.init(a.Q, a.ldq, qt * 128, a.Qn, a.K, tid);
   lds_byte* const lds = (lds_byte*)smem;
-  auto issue = [&](lds_byte* wr) {
-    oq.template issue<0, OpQ::NI>(wr, 0, tid, wave);
-    if (two) oq.template issue<0, OpQ::NI>(wr + OpQ::BYTES, 64, tid, wave);
-  };
-  issue(lds);
-
-  // The bias of the lane's columns, requested a tile ahead: loads without a branch each, and nothing is done with their values
-  // before that tile begins (a compare behind each load costs 16 memory latencies per tile: 71 us instead of 48).
-  float raw[NT / 2][8];
-  auto load_bias = [&](int q) {
-    const int c = q * 128 + qw0 + 8 * j4;
-    if (!a.bias) {
+  // the lane's source offsets in a tile of words, both halves of the contraction (past its end: past every bound)
+  uint32_t off[2][OpQ::NI];
 #pragma unroll
-      for (int tp = 0; tp < NT / 2; ++tp)
+  for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) raw[tp][e] = 0.f;
-    } else if (q * 128 + 128 <= a.Qn) {
-#pragma unroll
-      for (int tp = 0; tp < NT / 2; ++tp) {
-        struct __attribute__((packed, aligned(4))) F4 { f32x4 v; };
-        const f32x4 lo = reinterpret_cast<const F4*>(a.bias + c + tp * 32)->v, hi = reinterpret_cast<const F4*>(a.bias + c + tp * 32 + 4)->v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) { raw[tp][e] = lo[e]; raw[tp][4 + e] = hi[e]; }
-      }
-    } else {
-#pragma unroll
-      for (int tp = 0; tp < NT / 2; ++tp)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int v = c + tp * 32 + e;
-          raw[tp][e] = a.bias[v < a.Qn ? v : a.Qn - 1];
-        }
+    for (int i = 0; i < OpQ::NI; ++i) {
+      const int slot = i * 256 + tid, c = OpQ::piece(slot) + h * 8;
+      off[h][i] = c * 8 < a.K ? (uint32_t)((slot / OpQ::ROW) * (int)a.ldq * 2 + c * 16) : OpQ::OUT;
     }
+  auto issue = [&](lds_byte* wr, int q) {
+    const int left = a.Qn - q * 128, n = left < 128 ? left : 128;
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(a.Q + (long)q * 128 * a.ldq), 0,
+                                                                          ((n - 1) * (int)a.ldq + a.K) * 2, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < OpQ::NI; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lptr_t)(wr + i * 4096 + wave * 1024), 16, (int)off[0][i], 0, 0, 0);
+    if (two)
+#pragma unroll
+      for (int i = 0; i < OpQ::NI; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lptr_t)(wr + OpQ::BYTES + i * 4096 + wave * 1024), 16, (int)off[1][i], 0, 0, 0);
+  };
+  issue(lds, qt);
+
+  // The bias of the lane's columns, requested a tile ahead, 0 past the vocabulary and without a bias; nothing is done with
+  // the values before that tile begins (a compare behind each load costs 16 memory latencies per tile: 71 us instead of 48).
+  float raw[NT / 2][8];
+  const __amdgpu_buffer_rsrc_t bias_rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)a.bias, 0, a.bias ? a.Qn * 4 : 0, 0x00020000);
+  auto load_bias = [&](int q) {
+#pragma unroll
+    for (int tp = 0; tp < NT / 2; ++tp)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        typedef int i32x4 __attribute__((ext_vector_type(4)));
+        const f32x4 v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(bias_rsrc, (qw0 + 8 * j4) * 4 + tp * 128 + h * 16, q * 512, 0));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) raw[tp][h * 4 + e] = v[e];
+      }
   };
   float m2[MT], sum[MT], lse2[MT], wt[MT];   // running maximum in units of log 2, running sum; lse and weight (gradient)
   int target[MT];
@@ -605,7 +623,7 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
       const int m = p * 128 + pw0 + mt * 16 + i16;
       m2[mt] = -INFINITY;
       sum[mt] = 0.f;
-      target[mt] = -1;
+      target[mt] = -1 << 30;
       lse2[mt] = INFINITY;   // a row that is not there, or whose every logit is masked: no gradient
       wt[mt] = 0.f;
 #pragma unroll
@@ -615,8 +633,8 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
         if (m < rows && k < a.K) pf[mt][ks] = *reinterpret_cast<const bf16x8*>(a.P + (long)m * a.ldp + k);
       }
       if (m < rows) {
-        const int64_t t = a.target[a.index ? a.index[m] : m];
-        target[mt] = t >= 0 && t < a.Qn ? (int)t : -1;
+        const int64_t t = a.word ? a.word[m] : a.target[m];
+        target[mt] = t >= 0 && t < a.Qn ? (int)t : -1 << 30;
         if (MODE == LOGIT_GRAD) {
           const float l = a.lse[m] * LOG2E;
           if (l != -INFINITY) { lse2[mt] = l; wt[mt] = a.weight[m]; }
@@ -677,8 +695,7 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
     f32x4 acc[MT][NT];
     [&](lds_byte* __restrict__ wr, const lds_byte* __restrict__ rd) {
       if (more) {
-        oq.seek(a.Q, qt1 * 128, a.Qn);
-        issue(wr);
+        issue(wr, qt1);
         load_bias(qt1);
       }
 #pragma unroll
@@ -695,10 +712,12 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
             acc[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf[nt], pf[mt][ks], ks ? acc[mt][nt] : start[nt], 0, 0, 0);
       }
     }(lds + (~t & 1) * STAGE, lds + (t & 1) * STAGE);
-    auto holds_target = [&](int mt) {   // the lane's column of the target's logit, or -1
-      const int rel = target[mt] - (q0 + qw0 + 8 * j4);
-      return target[mt] >= 0 && (rel & ~39) == 0 && rel < 64 ? rel : -1;   // rel = 0..7, 32..39
-    };
+    // the lane's column of the target's logit is 0..7 or 32..39 of the wave's; most tiles hold no row's target
+    const int base = q0 + qw0 + 8 * j4;
+    bool any = false;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) any |= ((target[mt] - base) & ~39) == 0;
+    const bool targets = __ballot(any) != 0;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       if constexpr (MODE == LOGIT_STATS) {
@@ -721,14 +740,11 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             acc[mt][nt][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mt][nt][e], LOG2E, -lse2[mt])) * wt[mt];
-        const int rel = holds_target(mt);
-        if (rel >= 0) {
+        if (targets)
 #pragma unroll
           for (int tp = 0; tp < NT / 2; ++tp)
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (rel == tp * 32 + e) acc[mt][2 * tp + (e >> 2)][e & 3] -= wt[mt];
-        }
+            for (int e = 0; e < 8; ++e) acc[mt][2 * tp + (e >> 2)][e & 3] -= target[mt] - base == tp * 32 + e ? wt[mt] : 0.f;
       }
     }
     // The next tile's words have landed (they had this tile's products and exponentials to do so, which is why those are made
@@ -746,15 +762,13 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
     for (int mt = 0; mt < MT; ++mt) {
       const int m = pt * 128 + pw0 + mt * 16 + i16;
       if constexpr (MODE == LOGIT_STATS) {
-        const int rel = holds_target(mt);
-        if (rel >= 0) {
+        if (targets) {
           float x = 0.f;
 #pragma unroll
           for (int tp = 0; tp < NT / 2; ++tp)
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (rel == tp * 32 + e) x = acc[mt][2 * tp + (e >> 2)][e & 3];
-          a.tlogit[m] = x;
+            for (int e = 0; e < 8; ++e) x = target[mt] - base == tp * 32 + e ? acc[mt][2 * tp + (e >> 2)][e & 3] : x;
+          if (((target[mt] - base) & ~39) == 0) a.tlogit[m] = x;
         }
       } else if (m < rows) {
 #pragma unroll
@@ -764,18 +778,6 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
           for (int e = 0; e < 8; ++e) o[e] = (bf16)acc[mt][2 * tp + (e >> 2)][e & 3];
           *reinterpret_cast<bf16x8*>(a.g + (size_t)m * a.ldg + q0 + qw0 + tp * 32 + 8 * j4) = o;
         }
-      }
-    }
-    if constexpr (MODE == LOGIT_GRAD) {
-      if (a.dbias_part) {   // column sums of the wave's 64 rows; lane i16 of each 16 writes the i16-th of its 16 columns
-        float mine = 0.f;
-#pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          const int nt = c >> 2, e = c & 3;
-          const float x = row16_sum((acc[0][nt][e] + acc[1][nt][e]) + (acc[2][nt][e] + acc[3][nt][e]));
-          mine = i16 == c ? x : mine;
-        }
-        a.dbias_part[(size_t)(pt * 2 + (wave >> 1)) * a.ldg + q0 + qw0 + (i16 >> 3) * 32 + 8 * j4 + (i16 & 7)] = mine;
       }
     }
     if (new_rows || !more) {
@@ -798,7 +800,7 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
 // The rows that count, numbered through in their order (one workgroup: 16 waves look at 1024 targets at a time), and the
 // losses of those that do not: 0 where the target is ignore_index, NaN where it is no word (and no gradient).
 __global__ __launch_bounds__(1024) void ce_index_kernel(const int64_t* target, int64_t ignore, int N, int V, int* index,
-                                                        int* count, float* loss, float* lse) {
+                                                        int* words, int* count, float* loss, float* lse) {
   __shared__ int waves[16];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   int done = 0;
@@ -823,7 +825,11 @@ __global__ __launch_bounds__(1024) void ce_index_kernel(const int64_t* target, i
       before += i < w ? c : 0;
       all += c;
     }
-    if (keep) index[done + before + __popcll(b & ((1ull << lane) - 1))] = n;
+    if (keep) {
+      const int at = done + before + __popcll(b & ((1ull << lane) - 1));
+      index[at] = n;
+      words[at] = (int)t;
+    }
     done += all;
   }
   if (threadIdx.x == 0) *count = done;
@@ -868,7 +874,7 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(const float2* part, int ti
     CeStream st(rows, V, grid);
     const int pt = (int)blockIdx.x / 8, x = st.parts == 8 ? j >> 1 : 0;
     st.part(x);
-    const int b0 = st.owner((long)pt * st.qn), b1 = st.owner((long)(pt + 1) * st.qn - 1);
+    const int b0 = st.owner((uint32_t)pt * st.qn), b1 = st.owner((uint32_t)(pt + 1) * st.qn - 1);
     for (int b = b0 + (st.parts == 8 ? 0 : j >> 1); b <= b1; b += st.parts == 8 ? 1 : 8)
       join(part[st.slot(x, b, pt, j & 1) + (r & 127)]);
   }
@@ -923,22 +929,6 @@ __global__ __launch_bounds__(256) void ce_zero_rows_kernel(const int64_t* target
   reinterpret_cast<uint4*>(dh + (long)n * lddh)[c] = make_uint4(0, 0, 0, 0);
 }
 
-// dbias from the column sums of a piece's tiles, in order: acc_in (earlier pieces, or the caller's sum) + theirs
-__global__ __launch_bounds__(256) void ce_dbias_kernel(const float* part, long ld, int BP, const int* count, int row0,
-                                                       int rows_max, int V, const float* acc_in, void* out, int out_f32) {
-  const int v = blockIdx.x * 256 + threadIdx.x;
-  if (v >= V) return;
-  int rows = *count - row0;
-  rows = rows < 0 ? 0 : rows < rows_max ? rows : rows_max;
-  float s = 0.f;
-  const int n = (rows + BP - 1) / BP;
-#pragma unroll 8
-  for (int t = 0; t < n; ++t) s += part[(size_t)t * ld + v];
-  if (acc_in) s += acc_in[v];
-  if (out_f32) ((float*)out)[v] = s;
-  else ((bf16*)out)[v] = (bf16)s;
-}
-
 // ---------------------------------------------------------------------------------------------------- host
 struct CePlan {
   long rows;          // per piece, a multiple of 256
@@ -946,7 +936,7 @@ struct CePlan {
   bool stream, big;   // ce_stream_kernel, or 256 x 256 tiles, for the logits
   bool big_dh, big_dw;
   long Vp;
-  size_t index, tlogit, lse, weight, part, hc, g, slab, dwacc, dbpart, dbacc, total;
+  size_t index, words, tlogit, lse, weight, part, hc, g, slab, dwacc, dbacc, total;
 };
 
 constexpr int STREAM_GRID = 512;   // two workgroups per CU
@@ -1001,16 +991,14 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
   p.part = take(p.stream ? (size_t)(STREAM_GRID + 8 * (p.rows / 128)) * 2 * 128 * 8 : (size_t)qt * p.rows * 8);
   if (grad) {
     p.index = take((size_t)(all + 256) * 4);
+    p.words = take((size_t)(all + 256) * 4);
     p.lse = take(p.rows * 4);
     p.weight = take(p.rows * 4);
     p.hc = take((size_t)p.rows * a->D * 2);
     p.g = take((size_t)p.rows * p.Vp * 2);
     if (p.ksplit > 1) p.slab = take((size_t)p.ksplit * p.rows * a->D * 4);
     if (p.pieces > 1 && !a->grad_f32) p.dwacc = take((size_t)a->V * a->D * 4);
-    if (a->dbias) {
-      p.dbpart = take((size_t)(p.rows / 64) * p.Vp * 4);
-      if (p.pieces > 1 && !a->grad_f32) p.dbacc = take((size_t)a->V * 4);
-    }
+    if (p.pieces > 1 && !a->grad_f32 && a->dbias) p.dbacc = take((size_t)a->V * 4);
   }
   p.total = at;
   return p;
@@ -1050,6 +1038,7 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
   char* ws = (char*)A.ws;
   int* count = (int*)ws;
   int* index = (int*)(ws + p.index);
+  int* words = (int*)(ws + p.words);
   const bf16* w = (const bf16*)A.w;
   const int D = A.D, V = A.V, N = A.N, D8 = D / 8;
 
@@ -1068,7 +1057,7 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
     return MMST_OK;
   }
 
-  hipLaunchKernelGGL(ce_index_kernel, dim3(1), dim3(1024), 0, st, A.target, A.ignore_index, N, V, index, count, A.loss, A.lse);
+  hipLaunchKernelGGL(ce_index_kernel, dim3(1), dim3(1024), 0, st, A.target, A.ignore_index, N, V, index, words, count, A.loss, A.lse);
   MMST_CHECK_LAUNCH();
   if (N > 0) {
     hipLaunchKernelGGL(ce_zero_rows_kernel, dim3((unsigned)(((long)N * D8 + 255) / 256)), dim3(256), 0, st, A.target,
@@ -1079,7 +1068,6 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
   bf16* gbuf = (bf16*)(ws + p.g);
   float* lse_c = (float*)(ws + p.lse);
   float* weight = (float*)(ws + p.weight);
-  const int BPg = p.stream ? 64 : p.big ? 256 : 128;   // rows per partial sum of dbias
   for (int i = 0; i < p.pieces; ++i) {
     const int row0 = (int)(i * p.rows);
     const int rows_max = (int)p.rows;
@@ -1087,6 +1075,7 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
                        D8, index, count, row0, rows_max, A.dloss, A.grad_scale, hc, weight);
     MMST_CHECK_LAUNCH();
     logit.P = hc; logit.ldp = D; logit.Pn = rows_max; logit.count = count; logit.row0 = row0; logit.index = index + row0;
+    logit.word = words + row0;
     launch_logits<LOGIT_STATS>(logit, p, p.rows, V, st);
     MMST_CHECK_LAUNCH();
     hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)(p.rows / 16)), dim3(256), 0, st, logit.part, logit.qtiles, rows_max,
@@ -1095,7 +1084,6 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
     MMST_CHECK_LAUNCH();
     CeGemm gr = logit;
     gr.lse = lse_c; gr.weight = weight; gr.g = gbuf; gr.ldg = p.Vp;
-    gr.dbias_part = A.dbias ? (float*)(ws + p.dbpart) : nullptr;
     launch_logits<LOGIT_GRAD>(gr, p, p.rows, p.Vp, st);
     MMST_CHECK_LAUNCH();
 
@@ -1118,18 +1106,16 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
     dw.count = count; dw.row0 = row0; dw.rows_max = rows_max; dw.ksplit = 1;
     float* acc = (float*)(ws + p.dwacc);
     dw.ldo = D;
-    if (A.grad_f32) { dw.out = A.dw; dw.out_f32 = 1; dw.acc_in = (const float*)A.dw; }
-    else { dw.out = last ? A.dw : (void*)acc; dw.out_f32 = last ? 0 : 1; dw.acc_in = i > 0 ? acc : nullptr; }
+    float* bacc = (float*)(ws + p.dbacc);
+    if (A.grad_f32) {
+      dw.out = A.dw; dw.out_f32 = 1; dw.acc_in = (const float*)A.dw;
+      dw.dbias = A.dbias; dw.dbias_in = (const float*)A.dbias;
+    } else {
+      dw.out = last ? A.dw : (void*)acc; dw.out_f32 = last ? 0 : 1; dw.acc_in = i > 0 ? acc : nullptr;
+      if (A.dbias) { dw.dbias = last ? A.dbias : (void*)bacc; dw.dbias_in = i > 0 ? bacc : nullptr; }
+    }
     launch<DW>(dw, p.big_dw, V, D, st);
     MMST_CHECK_LAUNCH();
-    if (A.dbias) {
-      float* bacc = (float*)(ws + p.dbacc);
-      const float* from = A.grad_f32 ? (const float*)A.dbias : i > 0 ? bacc : nullptr;
-      void* to = A.grad_f32 || last ? A.dbias : (void*)bacc;
-      hipLaunchKernelGGL(ce_dbias_kernel, dim3((V + 255) / 256), dim3(256), 0, st, (const float*)(ws + p.dbpart), p.Vp, BPg, count,
-                         row0, rows_max, V, from, to, A.grad_f32 || !last ? 1 : 0);
-      MMST_CHECK_LAUNCH();
-    }
   }
   return MMST_OK;
 }
