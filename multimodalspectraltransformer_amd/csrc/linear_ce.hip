@@ -585,67 +585,65 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
       const int slot = i * 256 + tid, c = OpQ::piece(slot) + h * 8;
       off[h][i] = c * 8 < a.K ? (uint32_t)((slot / OpQ::ROW) * (int)a.ldq * 2 + c * 16) : OpQ::OUT;
     }
-  auto issue = [&](lds_byte* wr, int q) {
+  auto words_of = [&](int q) {
     const int left = a.Qn - q * 128, n = left < 128 ? left : 128;
-    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(a.Q + (long)q * 128 * a.ldq), 0,
-                                                                          ((n - 1) * (int)a.ldq + a.K) * 2, 0x00020000);
-#pragma unroll
-    for (int i = 0; i < OpQ::NI; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lptr_t)(wr + i * 4096 + wave * 1024), 16, (int)off[0][i], 0, 0, 0);
-    if (two)
-#pragma unroll
-      for (int i = 0; i < OpQ::NI; ++i)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lptr_t)(wr + OpQ::BYTES + i * 4096 + wave * 1024), 16, (int)off[1][i], 0, 0, 0);
+    return __builtin_amdgcn_make_buffer_rsrc((void*)(a.Q + (long)q * 128 * a.ldq), 0, ((n - 1) * (int)a.ldq + a.K) * 2, 0x00020000);
   };
-  issue(lds, qt);
-
+  auto issue = [&](const __amdgpu_buffer_rsrc_t rsrc, lds_byte* wr, int h, int i) {   // instruction i of half h
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lptr_t)(wr + h * OpQ::BYTES + i * 4096 + wave * 1024), 16, (int)off[h][i], 0, 0, 0);
+  };
+  {
+    const __amdgpu_buffer_rsrc_t rsrc = words_of(qt);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < OpQ::NI; ++i) issue(rsrc, lds, h, i);
+  }
   // The bias of the lane's columns, requested a tile ahead, 0 past the vocabulary and without a bias; nothing is done with
   // the values before that tile begins (a compare behind each load costs 16 memory latencies per tile: 71 us instead of 48).
   float raw[NT / 2][8];
   const __amdgpu_buffer_rsrc_t bias_rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)a.bias, 0, a.bias ? a.Qn * 4 : 0, 0x00020000);
-  auto load_bias = [&](int q) {
+  auto load_bias = [&](int q, int i) {   // instruction i of four
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    const f32x4 v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(bias_rsrc, (qw0 + 8 * j4) * 4 + (i >> 1) * 128 + (i & 1) * 16, q * 512, 0));
 #pragma unroll
-    for (int tp = 0; tp < NT / 2; ++tp)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        typedef int i32x4 __attribute__((ext_vector_type(4)));
-        const f32x4 v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(bias_rsrc, (qw0 + 8 * j4) * 4 + tp * 128 + h * 16, q * 512, 0));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) raw[tp][h * 4 + e] = v[e];
-      }
+    for (int e = 0; e < 4; ++e) raw[i >> 1][(i & 1) * 4 + e] = v[e];
   };
   float m2[MT], sum[MT], lse2[MT], wt[MT];   // running maximum in units of log 2, running sum; lse and weight (gradient)
   int target[MT];
   bf16x8 pf[MT][KS];
-  auto load_rows = [&](int p) {
+  auto load_rows = [&](int p) {   // (no branch around a load: each would be waited for before the next)
+    const int left = rows - p * 128, n = left < 128 ? left : 128;
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(a.P + (long)p * 128 * a.ldp), 0, ((n - 1) * (int)a.ldp + a.K) * 2, 0x00020000);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      const int m = p * 128 + pw0 + mt * 16 + i16;
-      m2[mt] = -INFINITY;
-      sum[mt] = 0.f;
-      target[mt] = -1 << 30;
-      lse2[mt] = INFINITY;   // a row that is not there, or whose every logit is masked: no gradient
-      wt[mt] = 0.f;
+      const int r = pw0 + mt * 16 + i16, m = p * 128 + (r < n ? r : n - 1);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        pf[mt][ks] = bf16x8{};
         const int k = ks * 32 + 8 * j4;
-        if (m < rows && k < a.K) pf[mt][ks] = *reinterpret_cast<const bf16x8*>(a.P + (long)m * a.ldp + k);
+        pf[mt][ks] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rsrc, k < a.K ? (r * (int)a.ldp + k) * 2 : (int)OpQ::OUT, 0, 0));
       }
-      if (m < rows) {
-        const int64_t t = a.word ? a.word[m] : a.target[m];
-        target[mt] = t >= 0 && t < a.Qn ? (int)t : -1 << 30;
-        if (MODE == LOGIT_GRAD) {
-          const float l = a.lse[m] * LOG2E;
-          if (l != -INFINITY) { lse2[mt] = l; wt[mt] = a.weight[m]; }
-        }
+      target[mt] = a.word ? a.word[m] : (int)(a.target[m] >= 0 && a.target[m] < a.Qn ? a.target[m] : -1);
+      if (MODE == LOGIT_GRAD) { lse2[mt] = a.lse[m]; wt[mt] = a.weight[m]; }
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const bool there = pw0 + mt * 16 + i16 < n;
+      m2[mt] = -INFINITY;
+      sum[mt] = 0.f;
+      target[mt] = there && target[mt] >= 0 ? target[mt] : -1 << 30;
+      if (MODE == LOGIT_GRAD) {   // a row that is not there, or whose every logit is masked: no gradient
+        const bool live = there && lse2[mt] != -INFINITY;
+        lse2[mt] = live ? lse2[mt] * LOG2E : INFINITY;
+        wt[mt] = live ? wt[mt] : 0.f;
       }
     }
     // A use of all of it, here: the compiler waits for a loaded value where it is first used, and in the loop that would be
     // a wait for everything requested since, once per tile.
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      asm volatile("" : "+v"(target[mt]), "+v"(lse2[mt]), "+v"(wt[mt]));
+      asm volatile("" : "+v"(target[mt]));
+      if (MODE == LOGIT_GRAD) asm volatile("" : "+v"(lse2[mt]), "+v"(wt[mt]));
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(pf[mt][ks]));
     }
@@ -657,7 +655,8 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
       for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(raw[tp][e]));
   };
   load_rows(pt);
-  load_bias(qt);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) load_bias(qt, i);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   bias_arrived();
 
@@ -666,15 +665,18 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
     const bool new_rows = qt + 1 == qend, more = t + 1 < ntiles;
     const int pt1 = new_rows ? pt + 1 : pt, qt1 = new_rows ? st.q0 : qt + 1;
     // The products start from the bias: -infinity past the vocabulary, which leaves those columns out of everything.  The
-    // lowest float is rare enough to look for first (eight instructions instead of 48).
+    // lowest float is rare enough to look for first.
     f32x4 start[NT];
     if (a.bias) {
-      float low = raw[0][0];
+      uint32_t low = 0;   // of the bits + 2^23 only numbers below -2^127 pass 0xFF800000 (-infinity becomes 0)
 #pragma unroll
       for (int tp = 0; tp < NT / 2; ++tp)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) low = fminf(low, raw[tp][e]);
-      if (__ballot(low < -0x1p127f))
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t u = __builtin_bit_cast(uint32_t, raw[tp][e]) + 0x00800000u;
+          low = u > low ? u : low;
+        }
+      if (__ballot(low > 0xFF800000u))
 #pragma unroll
         for (int tp = 0; tp < NT / 2; ++tp)
 #pragma unroll
@@ -694,22 +696,29 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
     asm volatile("s_barrier" ::: "memory");
     f32x4 acc[MT][NT];
     [&](lds_byte* __restrict__ wr, const lds_byte* __restrict__ rd) {
-      if (more) {
-        issue(wr, qt1);
-        load_bias(qt1);
-      }
+      // The next tile's requests go between the products, since in one go they would hold those up (four waves' twelve
+      // instructions at 18 cycles each of the address unit).  A run's last tile requests itself again and nobody looks.
+      const int q1 = more ? qt1 : qt;
+      const __amdgpu_buffer_rsrc_t rsrc = words_of(q1);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        if (ks >= 2 && !two) break;
         bf16x8 qf[NT];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          qf[nt] = OpQ::frag(rd + (ks >> 1) * OpQ::BYTES, qw0 + (nt >> 1) * 32, nt & 1, ks & 1, lane);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        if (ks < 2 || two)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
-            acc[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf[nt], pf[mt][ks], ks ? acc[mt][nt] : start[nt], 0, 0, 0);
+            qf[nt] = OpQ::frag(rd + (ks >> 1) * OpQ::BYTES, qw0 + (nt >> 1) * 32, nt & 1, ks & 1, lane);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          if (ks < 2 || two)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              acc[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf[nt], pf[mt][ks], ks ? acc[mt][nt] : start[nt], 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
+          const int k = ks * MT + mt;   // 16 places
+          if (k < 8) issue(rsrc, wr, k >> 2, k & 3);
+          else if (k < 12) load_bias(q1, k - 8);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
     }(lds + (~t & 1) * STAGE, lds + (t & 1) * STAGE);
     // the lane's column of the target's logit is 0..7 or 32..39 of the wave's; most tiles hold no row's target
