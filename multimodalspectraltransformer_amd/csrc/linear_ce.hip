@@ -27,7 +27,8 @@ constexpr int VT = 256;   // g is padded to whole tiles of the vocabulary, its r
 // -2^127 (the logits beside it are still at an infinite distance for exp).
 __device__ __forceinline__ float word_bias(float b) { return b < -0x1p127f && b > -INFINITY ? -0x1p127f : b; }
 
-enum { LOGIT_STATS = 0, LOGIT_GRAD = 1, DH = 2, DW = 3 };
+enum { LOGIT_STATS = 0, LOGIT_GRAD = 1, DH = 2, DW = 3, LOGIT_EXP = 4 };
+
 
 struct CeGemm {
   const bf16* P; const bf16* Q;      // operands; the token / vocabulary side of the output's rows, and its columns
@@ -141,7 +142,7 @@ template <int MODE, int BP, int BQ, int WP, int WQ>
 struct CeTile {
   static constexpr int NW = WP * WQ, NTHR = NW * 64, MT = BP / WP / 16, NT = BQ / WQ / 16;
   static constexpr bool TP = MODE == DW, TQ = MODE == DH || MODE == DW;
-  static constexpr int BK = 64, NS = 2;   // a step of the contraction; stages
+  static constexpr int BK = 64, NS = NW == 8 && BP + BQ <= 384 ? 3 : 2;   // a step of the contraction; stages
   using OpP = Operand<TP, false, BP, NTHR, BK>;
   using OpQ = Operand<TQ, true, BQ, NTHR, BK>;
   static constexpr int STAGE = OpP::BYTES + OpQ::BYTES, SMEM = NS * STAGE;
@@ -205,39 +206,36 @@ struct CeTile {
   //              4 s                4 s + 1        4 s + 2       4 s + 3
   //   first      read 0             multiply 0     read 1        multiply 1
   //   second     multiply 1 (s-1)   read 0         multiply 0    read 1
-  // The stage of step s - 1 is free at phase 4 s; the DMA of step s + 1 goes there in phases 4 s and 4 s + 1, half of it
-  // each, behind the reads or between the products: issued in one go it would hold up whichever comes after it, since the
-  // address unit takes 18 cycles for each of the 64 instructions.
+  // The stage of step s - 1 is free at phase 4 s; the DMA of step s + NS - 1 goes there in phases 4 s and 4 s + 1, half of
+  // it each, behind the reads or between the products: issued in one go it would hold up whichever comes after it, since
+  // the address unit takes 18 cycles for each of the 64 instructions.  Step s + 1 is waited for before the last barrier of s.
   static __device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
   static __device__ __forceinline__ void barrier() { asm volatile("s_barrier" ::: "memory"); fence(); }
   static __device__ __forceinline__ void reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
-  static __device__ __forceinline__ void dma_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-  template <int MT0, int MT1, bool SUM> static __device__ __forceinline__ void some(Acc<SUM>& acc, const Frags& f) {
-#pragma unroll
-    for (int mt = MT0; mt < MT1; ++mt) acc.add(f, mt);
-    fence();
-  }
+  static __device__ __forceinline__ void dma_done() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * PER) : "memory"); }
+  static __device__ __forceinline__ void all_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
   template <bool SUM> static __device__ __forceinline__ void multiply(Acc<SUM>& acc, const Frags& f) {
     __builtin_amdgcn_s_setprio(1);
-    some<0, MT>(acc, f);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) acc.add(f, mt);
     __builtin_amdgcn_s_setprio(0);
+    fence();
   }
-  // the products with DMA instructions LO .. LO + PER / 2 - 1 between them
-  template <int LO, bool SUM>
+  // the products with DMA instructions LO .. LO + PER / 2 - 1 between them, evenly
+  template <int LO, int MT0 = 0, bool SUM>
   static __device__ __forceinline__ void multiply_issue(Acc<SUM>& acc, const Frags& f, const OpP& p, const OpQ& q, lds_byte* wr,
                                                         int k, int tid, int wave) {
-    static_assert(MT == 8 && PER == 8, "eight by eight");
-    __builtin_amdgcn_s_setprio(1);
-    some<0, 1>(acc, f);
-    issue<LO, LO + 1>(p, q, wr, k, tid, wave);
-    some<1, 3>(acc, f);
-    issue<LO + 1, LO + 2>(p, q, wr, k, tid, wave);
-    some<3, 5>(acc, f);
-    issue<LO + 2, LO + 3>(p, q, wr, k, tid, wave);
-    some<5, 7>(acc, f);
-    issue<LO + 3, LO + 4>(p, q, wr, k, tid, wave);
-    some<7, 8>(acc, f);
-    __builtin_amdgcn_s_setprio(0);
+    constexpr int N = PER / 2;
+    if constexpr (MT0 == 0) __builtin_amdgcn_s_setprio(1);
+    acc.add(f, MT0);
+    fence();
+    constexpr int lo = MT0 * N / MT, hi = (MT0 + 1) * N / MT;
+    if constexpr (hi > lo) {
+      issue<LO + lo, LO + hi>(p, q, wr, k, tid, wave);
+      fence();
+    }
+    if constexpr (MT0 + 1 < MT) multiply_issue<LO, MT0 + 1>(acc, f, p, q, wr, k, tid, wave);
+    else __builtin_amdgcn_s_setprio(0);
   }
   template <bool SUM>
   static __device__ __forceinline__ void step_first(Acc<SUM>& acc, const OpP& p, const OpQ& q, lds_byte* __restrict__ wr,
@@ -276,31 +274,47 @@ struct CeTile {
     dma_done();
     barrier();
   }
-  // No branch inside a step: the last one requests a step that is not there, which moves nothing but zeros (or, in a split
-  // contraction, the next part's first step) into the stage that nobody reads, and the second half starts by multiplying zeros.
+
+  // A tile's products: prime() requests its first NS - 1 steps (nobody may be reading a stage), ready() waits for the first,
+  // steps() makes them all.  There is no branch inside a step: the last ones request steps that are not there, which move
+  // nothing but zeros (or, in a split contraction, the next part's first steps) into stages that nobody reads, and the second
+  // half starts by multiplying zeros.  Behind steps() nobody reads a stage.
+  static __device__ __forceinline__ void prime(const OpP& p, const OpQ& q, lds_byte* lds, int kbeg, int tid, int wave) {
+    all_done();
+#pragma unroll
+    for (int s = 0; s < NS - 1; ++s) issue<0, PER>(p, q, lds + s * STAGE, kbeg + s * BK, tid, wave);
+  }
+  static __device__ __forceinline__ void ready() {
+    dma_done();
+    barrier();
+  }
   template <bool SUM>
-  static __device__ __forceinline__ void loop(Acc<SUM>& acc, const OpP& p, const OpQ& q, lds_byte* lds, int kbeg,
-                                              int nsteps, int tid, int wave, int pw0, int qw0, int lane) {
-    if (nsteps <= 0) return;
-    issue<0, PER>(p, q, lds, kbeg, tid, wave);
+  static __device__ __forceinline__ void steps(Acc<SUM>& acc, const OpP& p, const OpQ& q, lds_byte* lds, int kbeg, int nsteps,
+                                               int tid, int wave, int pw0, int qw0, int lane) {
     if constexpr (NW != 8) {
       for (int s = 0; s < nsteps; ++s) {
         // this wave's share of step s has landed; behind the barrier everybody's has, and nobody reads the other stage
-        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        if (s) asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
         step(acc, p, q, lds + ((s + 1) & 1) * STAGE, lds + (s & 1) * STAGE, s + 1 < nsteps, kbeg + (s + 1) * BK, tid, wave,
              pw0, qw0, lane);
       }
-    } else {
-      dma_done();
       barrier();
+    } else {
+      int rd = 0, wr = NS - 1;
       if (wave < 4) {
-        for (int s = 0; s < nsteps; ++s)
-          step_first(acc, p, q, lds + ((s + 1) & 1) * STAGE, lds + (s & 1) * STAGE, kbeg + (s + 1) * BK, tid, wave, pw0, qw0, lane);
+        for (int s = 0; s < nsteps; ++s) {
+          step_first(acc, p, q, lds + wr * STAGE, lds + rd * STAGE, kbeg + (s + NS - 1) * BK, tid, wave, pw0, qw0, lane);
+          wr = rd;
+          rd = rd + 1 == NS ? 0 : rd + 1;
+        }
         barrier();   // the second half's last multiplication
       } else {
         Frags f = {};
-        for (int s = 0; s < nsteps; ++s)
-          step_second(acc, f, p, q, lds + ((s + 1) & 1) * STAGE, lds + (s & 1) * STAGE, kbeg + (s + 1) * BK, tid, wave, pw0, qw0, lane);
+        for (int s = 0; s < nsteps; ++s) {
+          step_second(acc, f, p, q, lds + wr * STAGE, lds + rd * STAGE, kbeg + (s + NS - 1) * BK, tid, wave, pw0, qw0, lane);
+          wr = rd;
+          rd = rd + 1 == NS ? 0 : rd + 1;
+        }
         multiply(acc, f);
         barrier();
       }
@@ -308,32 +322,35 @@ struct CeTile {
   }
 };
 
+// consecutive tiles in groups of eight rows of tiles: what runs at the same time on one XCD shares its operands in the L2
+__device__ __forceinline__ void tile_of(int id, int ptiles, int qtiles, int& pt, int& qt) {
+  const int group = 8 * qtiles, gi = id / group, gp = ptiles - gi * 8 < 8 ? ptiles - gi * 8 : 8;
+  const int in = id - gi * group;
+  pt = gi * 8 + in % gp;
+  qt = in / gp;
+}
+
+// ---------------------------------------------------------------------------------------------------- products with g
 template <int MODE, int BP, int BQ, int WP, int WQ>
-__global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_gemm_kernel(const CeGemm a) {
+__global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_product_kernel(const CeGemm a) {
   using Tile = CeTile<MODE, BP, BQ, WP, WQ>;
-  constexpr int MT = Tile::MT, NT = Tile::NT, NTHR = Tile::NTHR;
+  constexpr int MT = Tile::MT, NT = Tile::NT;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[Tile::SMEM];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // consecutive tiles to one XCD (workgroups go round the eight of them), in groups of eight rows of tiles: what runs at
-  // the same time there shares its operands in that XCD's L2
-  int id, ks_id = 0;
+  int id, ks_id = 0;   // consecutive tiles to one XCD (workgroups go round the eight of them)
   {
     const int n = gridDim.x, q8 = n >> 3, r8 = n & 7, x = blockIdx.x & 7;
     id = (x < r8 ? x * (q8 + 1) : r8 * (q8 + 1) + (x - r8) * q8) + ((int)blockIdx.x >> 3);
   }
   const int per = a.ptiles * a.qtiles;
   if (MODE == DH) { ks_id = id / per; id -= ks_id * per; }
-  const int group = 8 * a.qtiles, gi = id / group, gp = a.ptiles - gi * 8 < 8 ? a.ptiles - gi * 8 : 8;
-  const int in = id - gi * group;
-  const int pt = gi * 8 + in % gp, qt = in / gp;
+  int pt, qt;
+  tile_of(id, a.ptiles, a.qtiles, pt, qt);
   const int rows = piece_rows(a);
   const int p0 = pt * BP, q0 = qt * BQ;
-  int K = a.K, kbeg = 0;
-  int Pn = a.Pn;
-  if (MODE == DW) K = rows;
-  else Pn = rows;
-  if (MODE != DW && p0 >= rows) return;   // (uniform: before any barrier)
-  int nsteps = (K + Tile::BK - 1) / Tile::BK;
+  const int K = MODE == DW ? rows : a.K, Pn = MODE == DW ? a.Pn : rows;
+  if (MODE == DH && p0 >= rows) return;   // (uniform: before any barrier)
+  int kbeg = 0, nsteps = (K + Tile::BK - 1) / Tile::BK;
   if (MODE == DH && a.ksplit > 1) {
     const int s0 = (int)((long)nsteps * ks_id / a.ksplit), s1 = (int)((long)nsteps * (ks_id + 1) / a.ksplit);
     kbeg = s0 * Tile::BK;
@@ -348,10 +365,14 @@ __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_
   lds_byte* const lds = (lds_byte*)smem;
   typename Tile::template Acc<false> plain;
   f32x4 (&acc)[MT][NT] = plain.v;
+  if (nsteps > 0) {
+    Tile::prime(op, oq, lds, kbeg, tid, wave);
+    Tile::ready();
+  }
   if (MODE == DW && a.dbias && qt == 0 && wave % WQ == 0) {   // the waves that also have the sums over the rows
     typename Tile::template Acc<MODE == DW> sums;
     sums.clear();
-    Tile::loop(sums, op, oq, lds, kbeg, nsteps, tid, wave, pw0, qw0, lane);
+    Tile::steps(sums, op, oq, lds, kbeg, nsteps, tid, wave, pw0, qw0, lane);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       const int v = p0 + pw0 + mt * 16 + (lane & 15);
@@ -365,154 +386,202 @@ __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_
     }
   } else {
     plain.clear();
-    Tile::loop(plain, op, oq, lds, kbeg, nsteps, tid, wave, pw0, qw0, lane);
+    Tile::steps(plain, op, oq, lds, kbeg, nsteps, tid, wave, pw0, qw0, lane);
   }
 
   const int i16 = lane & 15, j4 = lane >> 4;
-  if constexpr (MODE == LOGIT_STATS || MODE == LOGIT_GRAD) {
-    // logits: row i16 of each 16, columns 32 tp + 8 j4 + e
-    if (a.bias) {
 #pragma unroll
-      for (int tp = 0; tp < NT / 2; ++tp)
+  for (int mt = 0; mt < MT; ++mt) {
+    const int m = p0 + pw0 + mt * 16 + i16;
+    if (m >= Pn) continue;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int v = q0 + qw0 + tp * 32 + 8 * j4 + e;
-          const float b = v < a.Qn ? word_bias(a.bias[v]) : 0.f;
+    for (int tp = 0; tp < NT / 2; ++tp) {
+      const int c = q0 + qw0 + tp * 32 + 8 * j4;
+      if (c >= a.Qn) continue;   // (Qn is a multiple of 8)
+      f32x4 lo = acc[mt][2 * tp], hi = acc[mt][2 * tp + 1];
+      if (MODE == DH && a.slab) {
+        float* d = a.slab + ((size_t)ks_id * a.rows_max + m) * a.Qn + c;
+        *reinterpret_cast<f32x4*>(d) = lo;
+        *reinterpret_cast<f32x4*>(d + 4) = hi;
+        continue;
+      }
+      const size_t row = MODE == DH ? (size_t)a.index[m] : (size_t)m;
+      if (MODE == DW && a.acc_in) {
+        const float* s = a.acc_in + row * a.Qn + c;
+        lo += *reinterpret_cast<const f32x4*>(s);
+        hi += *reinterpret_cast<const f32x4*>(s + 4);
+      }
+      if (MODE == DW && a.out_f32) {
+        float* d = (float*)a.out + row * a.ldo + c;
+        *reinterpret_cast<f32x4*>(d) = lo;
+        *reinterpret_cast<f32x4*>(d + 4) = hi;
+      } else {
+        bf16x8 o;
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) acc[mt][2 * tp + (e >> 2)][e & 3] += b;
-        }
+        for (int e = 0; e < 4; ++e) { o[e] = (bf16)lo[e]; o[4 + e] = (bf16)hi[e]; }
+        *reinterpret_cast<bf16x8*>((bf16*)a.out + row * a.ldo + c) = o;
+      }
     }
   }
-  if constexpr (MODE == LOGIT_STATS) {
-    float* red = reinterpret_cast<float*>(smem);   // [WQ][BP]
-    float mx[MT], sum[MT];
-    const bool edge = q0 + BQ > a.Qn;
+}
+
+// ---------------------------------------------------------------------------------------------------- logits, tile by tile
+// One workgroup per CU walks over tiles of the logits; the first steps of the next tile's contraction are requested before
+// this tile's softmax, which a wave does for its 64 columns alone.  LOGIT_STATS: (max, sum of exponentials) per row and 64 words.  LOGIT_EXP: these, and the exponentials
+// themselves in bf16, for the gradient.
+template <int MODE, int BP, int BQ, int WP, int WQ>
+__global__ __launch_bounds__(512, 2) void ce_logits_kernel(const CeGemm a) {
+  using Tile = CeTile<MODE, BP, BQ, WP, WQ>;
+  constexpr int MT = Tile::MT, NT = Tile::NT;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[Tile::SMEM];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rows = piece_rows(a);
+  const int ptiles = (rows + BP - 1) / BP, tiles = ptiles * a.qtiles;
+  // an XCD (workgroups go round the eight of them) has a run of consecutive tiles, its workgroups take them in turn
+  const int xcd = blockIdx.x & 7, group = (int)gridDim.x >> 3, chunk = (tiles + 7) >> 3;
+  const int end = (xcd + 1) * chunk < tiles ? (xcd + 1) * chunk : tiles;
+  int id = xcd * chunk + ((int)blockIdx.x >> 3);
+  if (id >= end) return;   // (uniform)
+  const int pw0 = (wave / WQ) * (BP / WP), qw0 = (wave % WQ) * (BQ / WQ);
+  const int i16 = lane & 15, j4 = lane >> 4;
+  const int nsteps = (a.K + Tile::BK - 1) / Tile::BK;
+  lds_byte* const lds = (lds_byte*)smem;
+  const __amdgpu_buffer_rsrc_t bias_rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)a.bias, 0, a.bias ? a.Qn * 4 : 0, 0x00020000);
+
+  int pt, qt;
+  tile_of(id, ptiles, a.qtiles, pt, qt);
+  typename Tile::OpP op;
+  typename Tile::OpQ oq;
+  op.init(a.P, a.ldp, pt * BP, rows, a.K, tid);
+  oq.init(a.Q, a.ldq, qt * BQ, a.Qn, a.K, tid);
+  Tile::prime(op, oq, lds, 0, tid, wave);
+  for (;;) {
+    const int p0 = pt * BP, q0 = qt * BQ;
+    Tile::ready();
+    // bias (0 past the vocabulary and without one) and targets, there when the products are
+    float raw[NT / 2][8];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const f32x4 v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(bias_rsrc, (q0 + qw0 + 8 * j4) * 4 + (i >> 1) * 128 + (i & 1) * 16, 0, 0));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) raw[i >> 1][(i & 1) * 4 + e] = v[e];
+    }
+    int target[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      const int m = p0 + pw0 + mt * 16 + i16;
-      if (edge) {   // columns past the vocabulary
+      int m = p0 + pw0 + mt * 16 + i16;
+      m = m < rows ? m : rows - 1;
+      target[mt] = a.word ? a.word[m] : (int)(a.target[m] >= 0 && a.target[m] < a.Qn ? a.target[m] : -1 << 30);
+    }
+    typename Tile::template Acc<false> plain;
+    f32x4 (&acc)[MT][NT] = plain.v;
+    plain.clear();
+    Tile::steps(plain, op, oq, lds, 0, nsteps, tid, wave, pw0, qw0, lane);
+
+    const int next = id + group;
+    int pt1 = pt, qt1 = qt;
+    if (next < end) {
+      tile_of(next, ptiles, a.qtiles, pt1, qt1);
+      op.seek(a.P, pt1 * BP, rows);
+      oq.seek(a.Q, qt1 * BQ, a.Qn);
+      Tile::prime(op, oq, lds, 0, tid, wave);
+    }
+
+    // logits: row i16 of each 16, columns 32 tp + 8 j4 + e
+    const bool edge = q0 + BQ > a.Qn;
 #pragma unroll
-        for (int tp = 0; tp < NT / 2; ++tp)
+    for (int tp = 0; tp < NT / 2; ++tp)
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (q0 + qw0 + tp * 32 + 8 * j4 + e >= a.Qn) acc[mt][2 * tp + (e >> 2)][e & 3] = -INFINITY;
+      for (int e = 0; e < 8; ++e) {
+        float b = a.bias ? word_bias(raw[tp][e]) : 0.f;
+        if (edge && q0 + qw0 + tp * 32 + 8 * j4 + e >= a.Qn) b = -INFINITY;   // past the vocabulary
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) acc[mt][2 * tp + (e >> 2)][e & 3] += b;
       }
-      if (m < rows) {   // the target's logit, by the one lane that holds it
-        const int64_t t = (a.word ? (int64_t)a.word[m] : a.target[m]) - (q0 + qw0 + 8 * j4);
-        if (t >= 0 && t < BQ / WQ && (t & 31) < 8) {
-          float x = 0.f;
+    const int base = q0 + qw0 + 8 * j4;
+    bool any = false;
 #pragma unroll
-          for (int tp = 0; tp < NT / 2; ++tp)
+    for (int mt = 0; mt < MT; ++mt) any |= ((target[mt] - base) & ~39) == 0;   // the lane's columns are 0..7 and 32..39 of the wave's
+    const bool targets = __ballot(any) != 0;
+    float mx[MT];
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (t == tp * 32 + e) x = acc[mt][2 * tp + (e >> 2)][e & 3];
-          a.tlogit[m] = x;
-        }
-      }
+    for (int mt = 0; mt < MT; ++mt) {
       float v = acc[mt][0][0];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) v = fmaxf(v, acc[mt][nt][e]);
       mx[mt] = xor32_max(xor16_max(v));
-    }
-    __syncthreads();   // every wave is done with the operands
-    if (j4 == 0)
+      if (targets) {
+        const int m = p0 + pw0 + mt * 16 + i16;
+        float x = 0.f;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) red[(wave % WQ) * BP + pw0 + mt * 16 + i16] = mx[mt];
-    __syncthreads();
+        for (int tp = 0; tp < NT / 2; ++tp)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x = target[mt] - base == tp * 32 + e ? acc[mt][2 * tp + (e >> 2)][e & 3] : x;
+        if (((target[mt] - base) & ~39) == 0 && m < rows) a.tlogit[m] = x;
+      }
+    }
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      float v = mx[mt];
-#pragma unroll
-      for (int w = 0; w < WQ; ++w) v = fmaxf(v, red[w * BP + pw0 + mt * 16 + i16]);
-      mx[mt] = v * LOG2E;
-      const float at = v == -INFINITY ? 0.f : mx[mt];   // a tile whose every logit is masked: exp(-inf - 0), not of NaN
-      float s = 0.f;
+      const float top = mx[mt] * LOG2E, at = top == -INFINITY ? 0.f : top;   // nothing but masked words: exp(-inf - 0), not of NaN
+      float x = 0.f;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mt][nt][e], LOG2E, -at));
-      sum[mt] = xor32_sum(xor16_sum(s));
-    }
-    __syncthreads();
-    if (j4 == 0)
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) red[(wave % WQ) * BP + pw0 + mt * 16 + i16] = sum[mt];
-    __syncthreads();
-    if (wave % WQ == 0 && j4 == 0)
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const int r = pw0 + mt * 16 + i16;
-        float s = 0.f;
-#pragma unroll
-        for (int w = 0; w < WQ; ++w) s += red[w * BP + r];
-        if (p0 + r < rows) a.part[(size_t)qt * a.rows_max + p0 + r] = make_float2(mx[mt], s);
-      }
-  }
-  if constexpr (MODE == LOGIT_GRAD) {
-    // the whole tile is written, zeros where no word is: the products read whole 16-byte pieces of a row
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
+        for (int e = 0; e < 4; ++e) {
+          acc[mt][nt][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mt][nt][e], LOG2E, -at));
+          x += acc[mt][nt][e];
+        }
+      x = xor32_sum(xor16_sum(x));
       const int m = p0 + pw0 + mt * 16 + i16;
-      float lse = 0.f, wt = 0.f;
-      int64_t t = -1;
-      bool ok = m < rows;
-      if (ok) {
-        lse = a.lse[m];
-        wt = a.weight[m];
-        t = a.word[m] - (q0 + qw0 + 8 * j4);
-        ok = lse != -INFINITY;   // a row whose every logit is masked has no gradient
-      }
-#pragma unroll
-      for (int tp = 0; tp < NT / 2; ++tp) {
-        bf16x8 o;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int v = q0 + qw0 + tp * 32 + 8 * j4 + e;
-          float x = __builtin_amdgcn_exp2f((acc[mt][2 * tp + (e >> 2)][e & 3] - lse) * LOG2E);
-          x = (x - (t == tp * 32 + e ? 1.f : 0.f)) * wt;
-          x = ok && v < a.Qn ? x : 0.f;
-          o[e] = (bf16)x;
-        }
-        *reinterpret_cast<bf16x8*>(a.g + (size_t)m * a.ldg + q0 + qw0 + tp * 32 + 8 * j4) = o;
-      }
+      if (j4 == 0 && m < rows) a.part[(size_t)(qt * WQ + wave % WQ) * a.rows_max + m] = make_float2(top, x);
     }
-  }
-  if constexpr (MODE == DH || MODE == DW) {
+    if constexpr (MODE == LOGIT_EXP) {   // whole tiles: g has rows and columns for them
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const int m = p0 + pw0 + mt * 16 + i16;
-      if (m >= Pn) continue;
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int tp = 0; tp < NT / 2; ++tp) {
-        const int c = q0 + qw0 + tp * 32 + 8 * j4;
-        if (c >= a.Qn) continue;   // (Qn is a multiple of 8)
-        f32x4 lo = acc[mt][2 * tp], hi = acc[mt][2 * tp + 1];
-        if (MODE == DH && a.slab) {
-          float* d = a.slab + ((size_t)ks_id * a.rows_max + m) * a.Qn + c;
-          *reinterpret_cast<f32x4*>(d) = lo;
-          *reinterpret_cast<f32x4*>(d + 4) = hi;
-          continue;
-        }
-        const size_t row = MODE == DH ? (size_t)a.index[m] : (size_t)m;
-        if (MODE == DW && a.acc_in) {
-          const float* s = a.acc_in + row * a.Qn + c;
-          lo += *reinterpret_cast<const f32x4*>(s);
-          hi += *reinterpret_cast<const f32x4*>(s + 4);
-        }
-        if (MODE == DW && a.out_f32) {
-          float* d = (float*)a.out + row * a.ldo + c;
-          *reinterpret_cast<f32x4*>(d) = lo;
-          *reinterpret_cast<f32x4*>(d + 4) = hi;
-        } else {
+        for (int tp = 0; tp < NT / 2; ++tp) {
           bf16x8 o;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) { o[e] = (bf16)lo[e]; o[4 + e] = (bf16)hi[e]; }
-          *reinterpret_cast<bf16x8*>((bf16*)a.out + row * a.ldo + c) = o;
+          for (int e = 0; e < 8; ++e) o[e] = (bf16)acc[mt][2 * tp + (e >> 2)][e & 3];
+          *reinterpret_cast<bf16x8*>(a.g + (size_t)(p0 + pw0 + mt * 16 + i16) * a.ldg + q0 + qw0 + tp * 32 + 8 * j4) = o;
         }
-      }
     }
+    if (next >= end) return;
+    id = next;
+    pt = pt1;
+    qt = qt1;
+  }
+}
+
+// g from the exponentials of a piece, in place: a tile's times exp2(its maximum - the row's lse) and the weight, minus the
+// weight where the word is the target.  Four rows per workgroup and 2048 columns, 16 bytes per lane; bound by HBM.
+__global__ __launch_bounds__(256) void ce_scale_kernel(const CeGemm a, int tile) {
+  const int rows = piece_rows(a), across = (int)((a.ldg + 2047) / 2048), r0 = (int)(blockIdx.x / across) * 4;
+  const int c = (int)(blockIdx.x % across) * 2048 + (int)threadIdx.x * 8;
+  if (r0 >= rows || c >= a.Qn) return;
+  const int qt = c / tile;
+  bf16x8 x[4];
+  float scale[4], wt[4];
+  int hit[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = r0 + i < rows ? r0 + i : rows - 1;
+    x[i] = *reinterpret_cast<const bf16x8*>(a.g + (size_t)r * a.ldg + c);
+    const float l = a.lse[r];
+    wt[i] = a.weight[r];
+    hit[i] = a.word[r] - c;
+    // a row whose every logit is masked has no gradient
+    if (l == -INFINITY) wt[i] = 0.f;
+    scale[i] = l == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(a.part[(size_t)qt * a.rows_max + r].x - l * LOG2E) * wt[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (r0 + i >= rows) break;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[i][e] = (bf16)((float)x[i][e] * scale[i] - (hit[i] == e ? wt[i] : 0.f));
+    *reinterpret_cast<bf16x8*>(a.g + (size_t)(r0 + i) * a.ldg + c) = x[i];
   }
 }
 
@@ -859,7 +928,7 @@ __global__ __launch_bounds__(256) void ce_gather_kernel(const bf16* h, long ldh,
 }
 
 // A row's pairs (maximum in units of log 2, sum) -> lse and loss: 16 rows per workgroup, 16 lanes each.  The pairs are those
-// of every tile of the vocabulary, [tile][ld], or (grid != 0) those that the workgroups of ce_stream_kernel left.
+// of every 64 words, [.][ld], or (grid != 0) those that the workgroups of ce_stream_kernel left.
 __global__ __launch_bounds__(256) void ce_rows_kernel(const float2* part, int tiles, int ld, int grid, const int* count, int row0,
                                                       int rows_max, const int* index, const int64_t* target, int64_t ignore,
                                                       int V, const float* tlogit, float* lse_c, float* loss, float* lse) {
@@ -942,13 +1011,13 @@ __global__ __launch_bounds__(256) void ce_zero_rows_kernel(const int64_t* target
 struct CePlan {
   long rows;          // per piece, a multiple of 256
   int pieces, ksplit;
-  bool stream, big;   // ce_stream_kernel, or 256 x 256 tiles, for the logits
+  bool stream, big;   // logits: ce_stream_kernel, or tiles of 256 x 256 (otherwise 128 x 256)
   bool big_dh, big_dw;
   long Vp;
   size_t index, words, tlogit, lse, weight, part, hc, g, slab, dwacc, dbacc, total;
 };
 
-constexpr int STREAM_GRID = 512;   // two workgroups per CU
+constexpr int STREAM_GRID = 512, TILE_GRID = 256;   // two workgroups per CU, one
 constexpr size_t PIECE_BYTES = (size_t)4 << 30;   // g of a piece, unless the caller says how many rows
 
 bool sizes_ok(const mmst_linear_ce_args* a) {
@@ -983,7 +1052,9 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
   p.pieces = grad && all ? (int)((all + p.rows - 1) / p.rows) : 1;
   auto tiles = [](long n, long m, int b) { return ((n + b - 1) / b) * ((m + b - 1) / b); };
   p.stream = a->D <= 128;
-  p.big = tiles(p.rows, a->V, 256) >= 256;
+  // Tiles of 256 x 256 make the better use of a CU, 128 x 256 (15 % more per logit) leave fewer idle in the last round.
+  const long n = a->N < p.rows ? a->N : p.rows, big = tiles(n, a->V, 256), half = (n + 127) / 128 * ((a->V + 255) / 256);
+  p.big = (big + 255) / 256 * 200 <= (half + 255) / 256 * 115;
   p.big_dh = a->D > 128;
   p.big_dw = a->D > 128 && tiles(a->V, a->D, 256) >= 256;
   p.ksplit = 1;
@@ -995,7 +1066,7 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
   }
   size_t at = 256;   // [0]: count
   auto take = [&](size_t n) { const size_t o = at; at += align(n); return o; };
-  const long qt = (a->V + (p.big ? 256 : 128) - 1) / (p.big ? 256 : 128);
+  const long qt = (a->V + 255) / 256 * 4;   // pairs per row: one per 64 words
   p.tlogit = take(p.rows * 4);
   p.part = take(p.stream ? (size_t)(STREAM_GRID + 8 * (p.rows / 128)) * 2 * 128 * 8 : (size_t)qt * p.rows * 8);
   if (grad) {
@@ -1018,13 +1089,16 @@ template <int MODE> void launch(CeGemm& g, bool big, long prows, long qcols, hip
   g.ptiles = (int)((prows + b - 1) / b);
   g.qtiles = (int)((qcols + b - 1) / b);
   const unsigned grid = (unsigned)(g.ptiles * g.qtiles * g.ksplit);
-  if (big) hipLaunchKernelGGL((ce_gemm_kernel<MODE, 256, 256, 2, 4>), dim3(grid), dim3(512), 0, st, g);
-  else hipLaunchKernelGGL((ce_gemm_kernel<MODE, 128, 128, 2, 2>), dim3(grid), dim3(256), 0, st, g);
+  if (big) hipLaunchKernelGGL((ce_product_kernel<MODE, 256, 256, 2, 4>), dim3(grid), dim3(512), 0, st, g);
+  else hipLaunchKernelGGL((ce_product_kernel<MODE, 128, 128, 2, 2>), dim3(grid), dim3(256), 0, st, g);
 }
-
-template <int MODE> void launch_logits(CeGemm& g, const CePlan& p, long prows, long qcols, hipStream_t st) {
-  if (p.stream) hipLaunchKernelGGL((ce_stream_kernel<MODE>), dim3(STREAM_GRID), dim3(256), 0, st, g);
-  else launch<MODE>(g, p.big, prows, qcols, st);
+template <int MODE> void launch_logits(CeGemm& g, const CePlan& p, hipStream_t st) {
+  g.qtiles = (g.Qn + 255) / 256;
+  if (p.big) hipLaunchKernelGGL((ce_logits_kernel<MODE, 256, 256, 2, 4>), dim3(TILE_GRID), dim3(512), 0, st, g);
+  else hipLaunchKernelGGL((ce_logits_kernel<MODE, 128, 256, 2, 4>), dim3(TILE_GRID), dim3(512), 0, st, g);
+}
+template <int MODE> void launch_stream(CeGemm& g, hipStream_t st) {
+  hipLaunchKernelGGL((ce_stream_kernel<MODE>), dim3(STREAM_GRID), dim3(256), 0, st, g);
 }
 
 }  // namespace
@@ -1058,9 +1132,10 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
   logit.rows_max = (int)p.rows;
   if (!grad) {
     logit.P = (const bf16*)A.h; logit.ldp = A.ldh; logit.rows_max = N; logit.Pn = N;
-    launch_logits<LOGIT_STATS>(logit, p, N, V, st);
+    if (p.stream) launch_stream<LOGIT_STATS>(logit, st);
+    else launch_logits<LOGIT_STATS>(logit, p, st);
     MMST_CHECK_LAUNCH();
-    hipLaunchKernelGGL(ce_rows_kernel, dim3((N + 15) / 16), dim3(256), 0, st, logit.part, logit.qtiles, N, p.stream ? STREAM_GRID : 0, nullptr, 0, N,
+    hipLaunchKernelGGL(ce_rows_kernel, dim3((N + 15) / 16), dim3(256), 0, st, logit.part, logit.qtiles * 4, N, p.stream ? STREAM_GRID : 0, nullptr, 0, N,
                        nullptr, A.target, A.ignore_index, V, logit.tlogit, nullptr, A.loss, A.lse);
     MMST_CHECK_LAUNCH();
     return MMST_OK;
@@ -1085,15 +1160,17 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
     MMST_CHECK_LAUNCH();
     logit.P = hc; logit.ldp = D; logit.Pn = rows_max; logit.count = count; logit.row0 = row0; logit.index = index + row0;
     logit.word = words + row0;
-    launch_logits<LOGIT_STATS>(logit, p, p.rows, V, st);
+    logit.g = gbuf; logit.ldg = p.Vp;
+    if (p.stream) launch_stream<LOGIT_STATS>(logit, st);
+    else launch_logits<LOGIT_EXP>(logit, p, st);
     MMST_CHECK_LAUNCH();
-    hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)(p.rows / 16)), dim3(256), 0, st, logit.part, logit.qtiles, rows_max,
+    hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)(p.rows / 16)), dim3(256), 0, st, logit.part, logit.qtiles * 4, rows_max,
                        p.stream ? STREAM_GRID : 0, count,
                        row0, rows_max, index, A.target, A.ignore_index, V, logit.tlogit, lse_c, A.loss, A.lse);
     MMST_CHECK_LAUNCH();
-    CeGemm gr = logit;
-    gr.lse = lse_c; gr.weight = weight; gr.g = gbuf; gr.ldg = p.Vp;
-    launch_logits<LOGIT_GRAD>(gr, p, p.rows, p.Vp, st);
+    logit.lse = lse_c; logit.weight = weight;
+    if (p.stream) launch_stream<LOGIT_GRAD>(logit, st);
+    else hipLaunchKernelGGL(ce_scale_kernel, dim3((unsigned)((p.Vp + 2047) / 2048 * (p.rows / 4))), dim3(256), 0, st, logit, 64);
     MMST_CHECK_LAUNCH();
 
     CeGemm dh = {};
