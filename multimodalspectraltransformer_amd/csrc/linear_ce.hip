@@ -299,6 +299,18 @@ struct CeTile {
              pw0, qw0, lane);
       }
       barrier();
+    } else if constexpr (NS == 3) {
+      int rd = 0, wr = NS - 1;
+      for (int s = 0; s < nsteps; ++s) {
+        if (s) {
+          dma_done();
+          asm volatile("s_barrier" ::: "memory");
+        }
+        step(acc, p, q, lds + wr * STAGE, lds + rd * STAGE, true, kbeg + (s + NS - 1) * BK, tid, wave, pw0, qw0, lane);
+        wr = rd;
+        rd = rd + 1 == NS ? 0 : rd + 1;
+      }
+      barrier();
     } else {
       int rd = 0, wr = NS - 1;
       if (wave < 4) {
@@ -946,8 +958,23 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(const float2* part, int ti
     s = s * __builtin_amdgcn_exp2f(m - at) + p.y * __builtin_amdgcn_exp2f(p.x - at);
     m = top;
   };
-  if (r < rows && !grid)
-    for (int q = j; q < tiles; q += 16) join(part[(size_t)q * ld + r]);
+  if (r < rows && !grid) {
+    int q = j;
+    for (; q + 112 < tiles; q += 128) {   // eight at a time: their loads are in flight together, and one new maximum
+      float2 p[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) p[k] = part[(size_t)(q + 16 * k) * ld + r];
+      float top = m;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) top = fmaxf(top, p[k].x);
+      const float at = top == -INFINITY ? 0.f : top;
+      s *= __builtin_amdgcn_exp2f(m - at);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += p[k].y * __builtin_amdgcn_exp2f(p[k].x - at);
+      m = top;
+    }
+    for (; q < tiles; q += 16) join(part[(size_t)q * ld + r]);
+  }
   if (r < rows && grid) {   // lane j: part j / 2 (or j of 16 lanes the only one), half j & 1 of the columns
     CeStream st(rows, V, grid);
     const int pt = (int)blockIdx.x / 8, x = st.parts == 8 ? j >> 1 : 0;
