@@ -142,7 +142,7 @@ template <int MODE, int BP, int BQ, int WP, int WQ>
 struct CeTile {
   static constexpr int NW = WP * WQ, NTHR = NW * 64, MT = BP / WP / 16, NT = BQ / WQ / 16;
   static constexpr bool TP = MODE == DW, TQ = MODE == DH || MODE == DW;
-  static constexpr int BK = 64, NS = NW == 8 && BP + BQ <= 384 ? 3 : 2;   // a step of the contraction; stages
+  static constexpr int BK = 64, NS = 2;   // a step of the contraction; stages
   using OpP = Operand<TP, false, BP, NTHR, BK>;
   using OpQ = Operand<TQ, true, BQ, NTHR, BK>;
   static constexpr int STAGE = OpP::BYTES + OpQ::BYTES, SMEM = NS * STAGE;
@@ -299,18 +299,6 @@ struct CeTile {
              pw0, qw0, lane);
       }
       barrier();
-    } else if constexpr (NS == 3) {
-      int rd = 0, wr = NS - 1;
-      for (int s = 0; s < nsteps; ++s) {
-        if (s) {
-          dma_done();
-          asm volatile("s_barrier" ::: "memory");
-        }
-        step(acc, p, q, lds + wr * STAGE, lds + rd * STAGE, true, kbeg + (s + NS - 1) * BK, tid, wave, pw0, qw0, lane);
-        wr = rd;
-        rd = rd + 1 == NS ? 0 : rd + 1;
-      }
-      barrier();
     } else {
       int rd = 0, wr = NS - 1;
       if (wave < 4) {
@@ -442,7 +430,7 @@ __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_
 // this tile's softmax, which a wave does for its 64 columns alone.  LOGIT_STATS: (max, sum of exponentials) per row and 64 words.  LOGIT_EXP: these, and the exponentials
 // themselves in bf16, for the gradient.
 template <int MODE, int BP, int BQ, int WP, int WQ>
-__global__ __launch_bounds__(512, 2) void ce_logits_kernel(const CeGemm a) {
+__global__ __launch_bounds__(WP * WQ * 64, 2) void ce_logits_kernel(const CeGemm a) {
   using Tile = CeTile<MODE, BP, BQ, WP, WQ>;
   constexpr int MT = Tile::MT, NT = Tile::NT;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[Tile::SMEM];
@@ -1038,12 +1026,13 @@ __global__ __launch_bounds__(256) void ce_zero_rows_kernel(const int64_t* target
 struct CePlan {
   long rows;          // per piece, a multiple of 256
   int pieces, ksplit;
-  bool stream, big;   // logits: ce_stream_kernel, or tiles of 256 x 256 (otherwise 128 x 256)
+  bool stream, big;   // logits: ce_stream_kernel, or tiles of 256 x 256 (otherwise 128 x 128)
   bool big_dh, big_dw;
   long Vp;
   size_t index, words, tlogit, lse, weight, part, hc, g, slab, dwacc, dbacc, total;
 };
 
+constexpr int BIG_TILES = 1024;
 constexpr int STREAM_GRID = 512, TILE_GRID = 256;   // two workgroups per CU, one
 constexpr size_t PIECE_BYTES = (size_t)4 << 30;   // g of a piece, unless the caller says how many rows
 
@@ -1079,9 +1068,7 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
   p.pieces = grad && all ? (int)((all + p.rows - 1) / p.rows) : 1;
   auto tiles = [](long n, long m, int b) { return ((n + b - 1) / b) * ((m + b - 1) / b); };
   p.stream = a->D <= 128;
-  // Tiles of 256 x 256 make the better use of a CU, 128 x 256 (15 % more per logit) leave fewer idle in the last round.
-  const long n = a->N < p.rows ? a->N : p.rows, big = tiles(n, a->V, 256), half = (n + 127) / 128 * ((a->V + 255) / 256);
-  p.big = (big + 255) / 256 * 200 <= (half + 255) / 256 * 115;
+  p.big = tiles(a->N < p.rows ? a->N : p.rows, a->V, 256) >= BIG_TILES;
   p.big_dh = a->D > 128;
   p.big_dw = a->D > 128 && tiles(a->V, a->D, 256) >= 256;
   p.ksplit = 1;
@@ -1093,7 +1080,7 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
   }
   size_t at = 256;   // [0]: count
   auto take = [&](size_t n) { const size_t o = at; at += align(n); return o; };
-  const long qt = (a->V + 255) / 256 * 4;   // pairs per row: one per 64 words
+  const long qt = (a->V + 255) / 256 * 4;
   p.tlogit = take(p.rows * 4);
   p.part = take(p.stream ? (size_t)(STREAM_GRID + 8 * (p.rows / 128)) * 2 * 128 * 8 : (size_t)qt * p.rows * 8);
   if (grad) {
@@ -1120,9 +1107,10 @@ template <int MODE> void launch(CeGemm& g, bool big, long prows, long qcols, hip
   else hipLaunchKernelGGL((ce_product_kernel<MODE, 128, 128, 2, 2>), dim3(grid), dim3(256), 0, st, g);
 }
 template <int MODE> void launch_logits(CeGemm& g, const CePlan& p, hipStream_t st) {
-  g.qtiles = (g.Qn + 255) / 256;
+  const int b = p.big ? 256 : 128;
+  g.qtiles = (g.Qn + b - 1) / b;
   if (p.big) hipLaunchKernelGGL((ce_logits_kernel<MODE, 256, 256, 2, 4>), dim3(TILE_GRID), dim3(512), 0, st, g);
-  else hipLaunchKernelGGL((ce_logits_kernel<MODE, 128, 256, 2, 4>), dim3(TILE_GRID), dim3(512), 0, st, g);
+  else hipLaunchKernelGGL((ce_logits_kernel<MODE, 128, 128, 2, 2>), dim3(2 * TILE_GRID), dim3(256), 0, st, g);
 }
 template <int MODE> void launch_stream(CeGemm& g, hipStream_t st) {
   hipLaunchKernelGGL((ce_stream_kernel<MODE>), dim3(STREAM_GRID), dim3(256), 0, st, g);
@@ -1152,6 +1140,7 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
   const bf16* w = (const bf16*)A.w;
   const int D = A.D, V = A.V, N = A.N, D8 = D / 8;
 
+  const int pairs = p.big ? (V + 255) / 256 * 4 : (V + 127) / 128 * 2;   // per row: one per 64 words
   CeGemm logit = {};
   logit.Q = w; logit.ldq = A.ldw; logit.Qn = V; logit.K = D; logit.ksplit = 1;
   logit.bias = A.bias; logit.target = A.target;
@@ -1162,7 +1151,7 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
     if (p.stream) launch_stream<LOGIT_STATS>(logit, st);
     else launch_logits<LOGIT_STATS>(logit, p, st);
     MMST_CHECK_LAUNCH();
-    hipLaunchKernelGGL(ce_rows_kernel, dim3((N + 15) / 16), dim3(256), 0, st, logit.part, logit.qtiles * 4, N, p.stream ? STREAM_GRID : 0, nullptr, 0, N,
+    hipLaunchKernelGGL(ce_rows_kernel, dim3((N + 15) / 16), dim3(256), 0, st, logit.part, pairs, N, p.stream ? STREAM_GRID : 0, nullptr, 0, N,
                        nullptr, A.target, A.ignore_index, V, logit.tlogit, nullptr, A.loss, A.lse);
     MMST_CHECK_LAUNCH();
     return MMST_OK;
@@ -1191,7 +1180,7 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
     if (p.stream) launch_stream<LOGIT_STATS>(logit, st);
     else launch_logits<LOGIT_EXP>(logit, p, st);
     MMST_CHECK_LAUNCH();
-    hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)(p.rows / 16)), dim3(256), 0, st, logit.part, logit.qtiles * 4, rows_max,
+    hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)(p.rows / 16)), dim3(256), 0, st, logit.part, pairs, rows_max,
                        p.stream ? STREAM_GRID : 0, count,
                        row0, rows_max, index, A.target, A.ignore_index, V, logit.tlogit, lse_c, A.loss, A.lse);
     MMST_CHECK_LAUNCH();

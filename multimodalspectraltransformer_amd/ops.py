@@ -147,24 +147,32 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _call(name, device, *args):
     """One call on the current stream of `device` (the tensors' own, which need not be the current one)."""
     f = _functions.get(name) or _function(name)
     index = device.index
-    if index != torch.cuda.current_device():
+    if index == _current_device():
+        rc = f(*args, _raw_stream(index))
+    else:
         with torch.cuda.device(index):
             rc = f(*args, _raw_stream(index))
-    else:
-        rc = f(*args, _raw_stream(index))
     if rc != 0:
         raise L.MMSTError(f"{name} failed with code {rc}")
+
+
+def _new_like(t):
+    """A contiguous tensor of t's shape, type and device."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _rows(t, like, name, out=False):
     """(tensor, row stride) of a tensor of the shape, type and device of `like`, whose leading dimensions can be counted
     through with one stride and whose columns follow one another.  An input of another layout is copied, an output refused."""
     shape = like.shape
-    if t.dtype != like.dtype or t.shape != shape or t.device != like.device:
+    if t is not like and (t.dtype is not like.dtype or t.shape != shape or t.device != like.device):
         raise L.MMSTError(f"{name}: {tuple(shape)} {like.dtype} on {like.device} expected, got {tuple(t.shape)} {t.dtype} on {t.device}")
     cols = shape[-1]
     if t.is_contiguous():
@@ -184,7 +192,7 @@ def _rows(t, like, name, out=False):
 def _vector(t, n, device, name):
     if t is None:
         return None
-    if t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous() or t.device != device:
+    if t.dtype is not torch.float32 or t.shape != (n,) or not t.is_contiguous() or t.device != device:
         raise L.MMSTError(f"{name}: contiguous fp32 [{n}] on {device} expected, got {tuple(t.shape)} {t.dtype} on {t.device}")
     return t.data_ptr()
 
@@ -211,7 +219,7 @@ def dropout(x, p, seed, offset=0, out=None):
     dt = _dtype_of(x, "dropout")
     _check_mask(p, seed, offset, "dropout")
     if out is None:
-        y = out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        y = out = _new_like(x)
         ldy = x.shape[-1]
     else:
         y, ldy = _rows(out, x, "dropout: out", out=True)
@@ -242,7 +250,7 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, residual=None, p=0.0, seed=0,
         rp = residual.data_ptr()
     ldy = ldz = cols
     if out is None:
-        y = torch.empty_like(x, memory_format=torch.contiguous_format)
+        y = _new_like(x)
     else:
         y, ldy = _rows(out, x, "layer_norm: out", out=True)
     z, zp = x, None
@@ -250,9 +258,9 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, residual=None, p=0.0, seed=0,
         z, ldz = _rows(z_out, x, "layer_norm: z_out", out=True)
         zp = z.data_ptr()
     elif rp is not None or p > 0.0:
-        z = torch.empty_like(x, memory_format=torch.contiguous_format)
+        z = _new_like(x)
         zp = z.data_ptr()
-    stats = torch.empty(shape[:-1] + (2,), dtype=torch.float32, device=device)
+    stats = x.new_empty(shape[:-1] + (2,), dtype=torch.float32)
     _call("mmst_layer_norm", device, x2.data_ptr(), ldx, rp, ldr, gp, bp, y.data_ptr(), ldy, zp, ldz, stats.data_ptr(), dt,
           x.numel() // cols, cols, eps, p, seed, offset)
     return y, z, stats
@@ -298,7 +306,7 @@ def layer_norm_bwd(dy, z, stats, gamma=None, dz_in=None, p=0.0, seed=0, offset=0
         accumulate = 1
         dgp = _vector(dgamma, cols, device, "layer_norm_bwd: dgamma")
         dbp = _vector(dbeta, cols, device, "layer_norm_bwd: dbeta")
-    dz = torch.empty_like(dy, memory_format=torch.contiguous_format)
+    dz = _new_like(dy)
     dx = torch.empty_like(dz) if int(p * 65536.0 + 0.5) > 0 else dz
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     _call("mmst_layer_norm_bwd", device, dy2.data_ptr(), lddy, z2.data_ptr(), ldz, stats.data_ptr(), gp, ap, ldadd,
