@@ -445,14 +445,15 @@ int mmst_layer_norm_bwd_ws(int dtype, long rows, int cols, size_t* bytes);
  * sum_n grad_scale dloss[n] loss[n], the gradients dh, dw and dbias.
  *   - rows whose target is ignore_index do not count: loss, lse and dh 0, nothing in dw, whatever h holds there, and no
  *     work in the products.  A target that is no word and not ignore_index gives loss and lse NaN and no gradient.
- *   - masked words: bias may be -infinity or the lowest float (finite values count as at least -2^127).  A row whose every logit is -infinity has lse -infinity,
- *     loss +infinity and no gradient.
+ *   - masked words: bias may be -infinity or the lowest float (finite values count as at least -2^127).  A row whose every
+ *     logit is -infinity has lse -infinity, loss +infinity and no gradient.
  *   - h, w, dh, dw rows 16-byte aligned; D a multiple of 8.  dw [V][D] and dbias [V] (both without a stride) in bf16,
  *     overwritten, or with grad_f32 in fp32, added to (as the other parameter gradients of this library).  All sums run in
  *     a fixed order: equal calls give equal bits.
  *   - the gradient works through the rows in pieces; the workspace holds the logits' gradient of one piece in bf16
- *     (rows_per_piece x V, rounded up to multiples of 256; 0: as many rows as 4 GiB hold) and its gathered rows, with
- *     bf16 gradients of more than one piece also their fp32 sums.  mmst_linear_ce_ws says how many bytes (its pointers may
+ *     (rows_per_piece x V, rounded up to multiples of 256; 0: as many rows as 4 GiB hold; never more than 64 GiB) and its
+ *     gathered rows of h (never more than 16 GiB), with bf16 gradients of more than one piece also their fp32 sums.  The loss
+ *     alone needs 8 bytes per row and 64 words, 1 GiB at most.  mmst_linear_ce_ws says how many bytes (its pointers may
  *     be unset except dbias, which only has to say whether there is one); it has to be 256-byte aligned. */
 #define MMST_LINEAR_CE_MAX_ROWS (1 << 24)
 #define MMST_LINEAR_CE_MAX_VOCAB (1 << 22)

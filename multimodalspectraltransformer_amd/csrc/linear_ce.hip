@@ -3,12 +3,15 @@
 //   l[n][v] = sum_d h[n][d] w[v][d] + bias[v]          lse[n] = log sum_v exp l[n][v]       loss[n] = lse[n] - l[n][t_n]
 //   g[n][v] = dloss[n] (exp(l[n][v] - lse[n]) - [v == t_n])        dh = g w        dw = g^T h        dbias = sum_n g
 //
-// All of it is matrix products over tiles of 256 x 256 (or 128 x 128 where those are too few) on
-// v_mfma_f32_16x16x32_bf16 with fp32 accumulation; a softmax never leaves the tile that made its logits:
-//   stats  a tile of logits becomes (max, sum exp) per row: 8 bytes per row and tile of the vocabulary
+// All of it is matrix products over tiles of 256 x 256 (or 128 x 128, see large_tiles) on v_mfma_f32_16x16x32_bf16 with
+// fp32 accumulation; the softmax is made from the tile's logits while they are in registers:
+//   logits a tile becomes (max, sum exp) per row and 64 words, 8 bytes; for the gradient also its exponentials, in bf16
 //   rows   a row's pairs are joined into lse and the loss
-//   grad   the tile of logits once more, now as g in bf16
+//   scale  the exponentials become g, in place
 //   dh, dw products with g, whose operands lie along the wrong axis and are read through transposing LDS reads
+// Three products, then, where computing the logits twice would take four; the price is one more rounding to bf16 of a
+// probability (an exponential in [0, 1] relative to its 64 words' maximum, 2^-8 of itself) and one pass over g.  With a short
+// contraction the pass would cost more than the product: those layers compute the logits twice (ce_stream_kernel).
 // The gradient goes in pieces of the ROWS: a piece's g [rows][V] is the only large buffer.  Rows that do not count
 // (ignore_index) are left out at the start: the others are numbered through on the device and gathered, so a padded batch
 // costs what its tokens cost, and what padding holds (NaN, infinities) reaches nothing.
@@ -27,8 +30,7 @@ constexpr int VT = 256;   // g is padded to whole tiles of the vocabulary, its r
 // -2^127 (the logits beside it are still at an infinite distance for exp).
 __device__ __forceinline__ float word_bias(float b) { return b < -0x1p127f && b > -INFINITY ? -0x1p127f : b; }
 
-enum { LOGIT_STATS = 0, LOGIT_GRAD = 1, DH = 2, DW = 3, LOGIT_EXP = 4 };
-
+enum { LOGIT_STATS = 0, LOGIT_GRAD = 1, DH = 2, DW = 3, LOGIT_EXP = 4, LOGIT_LOSS = 5 };
 
 struct CeGemm {
   const bf16* P; const bf16* Q;      // operands; the token / vocabulary side of the output's rows, and its columns
@@ -36,15 +38,16 @@ struct CeGemm {
   int Pn, Qn, K;                     // extents; K for DH is the vocabulary
   const int* count;                  // device: rows that count; the piece holds clamp(count - row0, 0, rows_max) of them
   int row0, rows_max;                // (count == NULL: rows_max rows)
-  int ptiles, qtiles, ksplit;
+  int ptiles, qtiles, ksplit;        // ksplit: parts of the contraction
   // logits
   const float* bias; const int64_t* target; const int* index;
   const int* word;                   // the targets of the rows that count (gradient; NULL: target[row])
-  float2* part; float* tlogit;       // per (tile column, row): max, sum of exp; the target's logit
+  float2* part; float* tlogit;       // per 64 words and row: max, sum of exp; the target's logit
   const float* lse; const float* weight; bf16* g; long ldg;
+  float* loss_out; float* lse_out; int64_t ignore;   // LOGIT_LOSS
   // products
   void* out; long ldo; int out_f32; int accumulate;   // out_f32: fp32, else bf16; accumulate: added to
-  const float* acc_in; float* slab;
+  const float* acc_in; float* slab; float* slab_bias;   // slabs: [ksplit][Pn][Qn], [ksplit][Pn]
   void* dbias; const float* dbias_in;                 // DW: sums of g over the rows, in out's type; added to dbias_in
 };
 
@@ -331,19 +334,24 @@ __device__ __forceinline__ void tile_of(int id, int ptiles, int qtiles, int& pt,
 }
 
 // ---------------------------------------------------------------------------------------------------- products with g
+// dh of a piece or dw, one tile per workgroup.  Bound by the matrix units at the clock that the card's power leaves them:
+// 8192 x 2048 x 65536 takes 1.88 ms for dh and 1.83 ms for dw, 1.17 and 1.20 PFLOP/s in 256 x 256 tiles (2.15 and 2.2 ms with
+// four waves of 128 x 128 each, that issue their DMA, read and multiply one after another).  In narrow layers (3032 x 128 x
+// 32000: 40 and 46 us) by reading g.
 template <int MODE, int BP, int BQ, int WP, int WQ>
 __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_product_kernel(const CeGemm a) {
   using Tile = CeTile<MODE, BP, BQ, WP, WQ>;
   constexpr int MT = Tile::MT, NT = Tile::NT;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[Tile::SMEM];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int id, ks_id = 0;   // consecutive tiles to one XCD (workgroups go round the eight of them)
+  int id;   // consecutive tiles to one XCD (workgroups go round the eight of them)
   {
     const int n = gridDim.x, q8 = n >> 3, r8 = n & 7, x = blockIdx.x & 7;
     id = (x < r8 ? x * (q8 + 1) : r8 * (q8 + 1) + (x - r8) * q8) + ((int)blockIdx.x >> 3);
   }
   const int per = a.ptiles * a.qtiles;
-  if (MODE == DH) { ks_id = id / per; id -= ks_id * per; }
+  const int ks_id = id / per;
+  id -= ks_id * per;
   int pt, qt;
   tile_of(id, a.ptiles, a.qtiles, pt, qt);
   const int rows = piece_rows(a);
@@ -351,7 +359,7 @@ __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_
   const int K = MODE == DW ? rows : a.K, Pn = MODE == DW ? a.Pn : rows;
   if (MODE == DH && p0 >= rows) return;   // (uniform: before any barrier)
   int kbeg = 0, nsteps = (K + Tile::BK - 1) / Tile::BK;
-  if (MODE == DH && a.ksplit > 1) {
+  if (a.ksplit > 1) {
     const int s0 = (int)((long)nsteps * ks_id / a.ksplit), s1 = (int)((long)nsteps * (ks_id + 1) / a.ksplit);
     kbeg = s0 * Tile::BK;
     nsteps = s1 - s0;
@@ -377,8 +385,9 @@ __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_
     for (int mt = 0; mt < MT; ++mt) {
       const int v = p0 + pw0 + mt * 16 + (lane & 15);
       if (lane < 16 && v < Pn) {
-        const float x = sums.sum[MODE == DW ? mt : 0][0] + (a.dbias_in ? a.dbias_in[v] : 0.f);
-        if (a.out_f32) ((float*)a.dbias)[v] = x;
+        const float x = sums.sum[MODE == DW ? mt : 0][0] + (a.dbias_in && !a.slab ? a.dbias_in[v] : 0.f);
+        if (a.slab) a.slab_bias[(size_t)ks_id * Pn + v] = x;
+        else if (a.out_f32) ((float*)a.dbias)[v] = x;
         else ((bf16*)a.dbias)[v] = (bf16)x;
       }
 #pragma unroll
@@ -399,8 +408,8 @@ __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_
       const int c = q0 + qw0 + tp * 32 + 8 * j4;
       if (c >= a.Qn) continue;   // (Qn is a multiple of 8)
       f32x4 lo = acc[mt][2 * tp], hi = acc[mt][2 * tp + 1];
-      if (MODE == DH && a.slab) {
-        float* d = a.slab + ((size_t)ks_id * a.rows_max + m) * a.Qn + c;
+      if (a.slab) {
+        float* d = a.slab + ((size_t)ks_id * a.Pn + m) * a.Qn + c;
         *reinterpret_cast<f32x4*>(d) = lo;
         *reinterpret_cast<f32x4*>(d + 4) = hi;
         continue;
@@ -426,9 +435,11 @@ __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_
 }
 
 // ---------------------------------------------------------------------------------------------------- logits, tile by tile
-// One workgroup per CU walks over tiles of the logits; the first steps of the next tile's contraction are requested before
-// this tile's softmax, which a wave does for its 64 columns alone.  LOGIT_STATS: (max, sum of exponentials) per row and 64 words.  LOGIT_EXP: these, and the exponentials
-// themselves in bf16, for the gradient.
+// A workgroup walks over tiles of the logits (one workgroup per CU with large tiles, two with small ones); the first steps of
+// the next tile's contraction are requested before this tile's softmax, which a wave does for its 64 columns alone.
+// LOGIT_STATS: (max, sum of exponentials) per row and 64 words.  LOGIT_EXP: these, and the exponentials themselves.  8192 x
+// 2048 x 65536: 2.09 ms with the exponentials, 1.05 PFLOP/s, bound by the matrix units and, for 1.1 GB of exponentials at
+// the ends of the tiles, by the softmax that nothing multiplies beside; 333 x 1024 x 50001 (three rounds of small tiles): 50 us.
 template <int MODE, int BP, int BQ, int WP, int WQ>
 __global__ __launch_bounds__(WP * WQ * 64, 2) void ce_logits_kernel(const CeGemm a) {
   using Tile = CeTile<MODE, BP, BQ, WP, WQ>;
@@ -556,12 +567,12 @@ __global__ __launch_bounds__(WP * WQ * 64, 2) void ce_logits_kernel(const CeGemm
 }
 
 // g from the exponentials of a piece, in place: a tile's times exp2(its maximum - the row's lse) and the weight, minus the
-// weight where the word is the target.  Four rows per workgroup and 2048 columns, 16 bytes per lane; bound by HBM.
-__global__ __launch_bounds__(256) void ce_scale_kernel(const CeGemm a, int tile) {
+// weight where the word is the target.  Four rows per workgroup and 2048 columns, 16 bytes per lane; bound by HBM: 2.1 GB in 0.41 ms,
+// 5.2 TB/s.
+__global__ __launch_bounds__(256) void ce_scale_kernel(const CeGemm a) {
   const int rows = piece_rows(a), across = (int)((a.ldg + 2047) / 2048), r0 = (int)(blockIdx.x / across) * 4;
   const int c = (int)(blockIdx.x % across) * 2048 + (int)threadIdx.x * 8;
   if (r0 >= rows || c >= a.Qn) return;
-  const int qt = c / tile;
   bf16x8 x[4];
   float scale[4], wt[4];
   int hit[4];
@@ -574,7 +585,7 @@ __global__ __launch_bounds__(256) void ce_scale_kernel(const CeGemm a, int tile)
     hit[i] = a.word[r] - c;
     // a row whose every logit is masked has no gradient
     if (l == -INFINITY) wt[i] = 0.f;
-    scale[i] = l == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(a.part[(size_t)qt * a.rows_max + r].x - l * LOG2E) * wt[i];
+    scale[i] = l == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(a.part[(size_t)(c / 64) * a.rows_max + r].x - l * LOG2E) * wt[i];
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -586,13 +597,14 @@ __global__ __launch_bounds__(256) void ce_scale_kernel(const CeGemm a, int tile)
 }
 
 // ---------------------------------------------------------------------------------------------------- logits, streamed
-// The logits of a narrow layer (D <= 128, the width of this library's own layers): a tile has so few products that loading
+// The logits of narrow layers (D <= 128, the width of this library's own layers): a tile has so few products that loading
 // it, its softmax and its stores are what counts.  The tiles, 128 x 128, are dealt out to G workgroups in equal runs along the
 // vocabulary; a wave keeps its 64 rows of h in registers for the run, and the words of the next tile arrive by LDS-DMA
 // while this one is multiplied and exponentiated: one barrier per tile.  A lane keeps the running maximum and sum of its
 // own columns of a row over the whole run; lanes, waves and workgroups are joined at its end.  Two workgroups per CU: one's
 // vector instructions (max, fused multiply-add, exponential and sum per logit, what bounds this kernel) run beside the
-// other's products.  (As single tiles, each beginning with an empty pipeline: 109 us for the stats of 3032 x 128 x 32000.)
+// other's products.  Stats of 3032 x 128 x 32000: 42 us, g 61 us (as
+// single tiles, each beginning with an empty pipeline, the stats took 109 us).
 // A large vocabulary is cut into eight parts, one per XCD, so that the words that an XCD's workgroups read over and over stay
 // in its L2 (all of 32000 x 128 from everywhere: 48 us, at the rate of the memory behind the L2s).
 struct CeStream {
@@ -629,7 +641,10 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
   constexpr int MT = 4, NT = 4, KS = 4;   // 64 x 64 per wave, 128 of the contraction
   using OpQ = Operand<false, true, 128, 256, 64>;
   constexpr int STAGE = 2 * OpQ::BYTES;   // the two halves of the contraction
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * STAGE + 1024];
+  constexpr bool STATS = MODE != LOGIT_GRAD;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * STAGE];
+  __shared__ float2 pair[MODE == LOGIT_LOSS ? 256 : 1];   // (max, sum) of a row's halves, its target's logit
+  __shared__ float hit[MODE == LOGIT_LOSS ? 128 : 1];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rows = piece_rows(a);
   CeStream st(rows, a.Qn, gridDim.x);
@@ -673,8 +688,7 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
   float raw[NT / 2][8];
   const __amdgpu_buffer_rsrc_t bias_rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)a.bias, 0, a.bias ? a.Qn * 4 : 0, 0x00020000);
   auto load_bias = [&](int q, int i) {   // instruction i of four
-    typedef int i32x4 __attribute__((ext_vector_type(4)));
-    const f32x4 v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(bias_rsrc, (qw0 + 8 * j4) * 4 + (i >> 1) * 128 + (i & 1) * 16, q * 512, 0));
+    const f32x4 v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(bias_rsrc, (q * 128 + qw0 + 8 * j4) * 4 + (i >> 1) * 128 + (i & 1) * 16, 0, 0));
 #pragma unroll
     for (int e = 0; e < 4; ++e) raw[i >> 1][(i & 1) * 4 + e] = v[e];
   };
@@ -798,7 +812,7 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
     const bool targets = __ballot(any) != 0;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      if constexpr (MODE == LOGIT_STATS) {
+      if constexpr (STATS) {
         float v = acc[mt][0][0];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -829,7 +843,7 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
     // to be done here); waited for here and not at the barrier, which would wait for the following stores as well.
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      if constexpr (MODE == LOGIT_STATS) asm volatile("" : "+v"(sum[mt]), "+v"(m2[mt]));
+      if constexpr (STATS) asm volatile("" : "+v"(sum[mt]), "+v"(m2[mt]));
       else
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) asm volatile("" : "+v"(acc[mt][nt]));
@@ -839,14 +853,17 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       const int m = pt * 128 + pw0 + mt * 16 + i16;
-      if constexpr (MODE == LOGIT_STATS) {
+      if constexpr (STATS) {
         if (targets) {
           float x = 0.f;
 #pragma unroll
           for (int tp = 0; tp < NT / 2; ++tp)
 #pragma unroll
             for (int e = 0; e < 8; ++e) x = target[mt] - base == tp * 32 + e ? acc[mt][2 * tp + (e >> 2)][e & 3] : x;
-          if (((target[mt] - base) & ~39) == 0) a.tlogit[m] = x;
+          if (((target[mt] - base) & ~39) == 0) {
+            if (MODE == LOGIT_LOSS) hit[pw0 + mt * 16 + i16] = x;
+            else a.tlogit[m] = x;
+          }
         }
       } else if (m < rows) {
 #pragma unroll
@@ -859,12 +876,29 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
       }
     }
     if (new_rows || !more) {
-      if constexpr (MODE == LOGIT_STATS) {
+      if constexpr (STATS) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
           const float top = xor32_max(xor16_max(m2[mt])), at = top == -INFINITY ? 0.f : top;
           const float x = xor32_sum(xor16_sum(sum[mt] * __builtin_amdgcn_exp2f(m2[mt] - at)));
-          if (j4 == 0) a.part[st.slot(vocab_part, b, pt, wave & 1) + pw0 + mt * 16 + i16] = make_float2(top, x);
+          if (j4 == 0) {
+            float2* to = MODE == LOGIT_LOSS ? pair + (wave & 1) * 128 : a.part + st.slot(vocab_part, b, pt, wave & 1);
+            to[pw0 + mt * 16 + i16] = make_float2(top, x);
+          }
+        }
+        if (MODE == LOGIT_LOSS) {   // (the next tile's barrier keeps its pairs from overtaking these)
+          __syncthreads();
+          const int m = pt * 128 + tid;
+          if (tid < 128 && m < rows) {
+            const float2 p = pair[tid], q = pair[128 + tid];
+            const float top = fmaxf(p.x, q.x), at = top == -INFINITY ? 0.f : top;
+            const float x = p.y * __builtin_amdgcn_exp2f(p.x - at) + q.y * __builtin_amdgcn_exp2f(q.x - at);
+            const float l = __builtin_fmaf(at, LN2, logf(x));
+            const int64_t t = a.target[m];
+            const bool none = t == a.ignore, word = t >= 0 && t < a.Qn;
+            a.loss_out[m] = none ? 0.f : !word ? __builtin_nanf("") : l == -INFINITY ? INFINITY : l - hit[tid];
+            if (a.lse_out) a.lse_out[m] = none ? 0.f : !word ? __builtin_nanf("") : l;
+          }
         }
       }
       if (more) load_rows(pt1);
@@ -913,10 +947,20 @@ __global__ __launch_bounds__(1024) void ce_index_kernel(const int64_t* target, i
   if (threadIdx.x == 0) *count = done;
 }
 
-// A piece's rows, one after another (16 bytes per lane), and their weights
+// A piece's rows, one after another (16 bytes per lane), and their weights; behind its `gather` workgroups those that clear dh
+// of the rows that do not count, 16 rows each.
 __global__ __launch_bounds__(256) void ce_gather_kernel(const bf16* h, long ldh, int D8, const int* index, const int* count,
                                                         int row0, int rows_max, const float* dloss, float scale, bf16* out,
-                                                        float* weight) {
+                                                        float* weight, unsigned gather, const int64_t* target, int64_t ignore,
+                                                        int N, int V, bf16* dh, long lddh) {
+  if (blockIdx.x >= gather) {
+    const long n = (long)(blockIdx.x - gather) * 16 + (threadIdx.x >> 4);
+    if (n >= N) return;
+    const int64_t t = target[n];
+    if (t != ignore && t >= 0 && t < V) return;
+    for (int c = threadIdx.x & 15; c < D8; c += 16) reinterpret_cast<uint4*>(dh + n * lddh)[c] = make_uint4(0, 0, 0, 0);
+    return;
+  }
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
   const int r = (int)(i / D8), c = (int)(i - (long)r * D8);
   int rows = *count - row0;
@@ -993,48 +1037,53 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(const float2* part, int ti
   if (lse) lse[n] = l;
 }
 
-// dh of a piece from the slabs of its split contraction
-__global__ __launch_bounds__(256) void ce_slabs_kernel(const float* slab, int n, int rows_max, const int* index,
-                                                       const int* count, int row0, int D4, bf16* dh, long lddh) {
+// The results of a product from the slabs of its split contraction: 4 columns per lane, behind them the words of dbias
+template <int MODE> __global__ __launch_bounds__(256) void ce_slabs_kernel(const CeGemm a) {
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  const int r = (int)(i / D4), c = (int)(i - (long)r * D4) * 4;
-  int rows = *count - row0;
-  rows = rows < rows_max ? rows : rows_max;
-  if (r >= rows) return;
-  const size_t stride = (size_t)rows_max * D4 * 4;
-  const float* p = slab + (size_t)r * D4 * 4 + c;
-  f32x4 s = *reinterpret_cast<const f32x4*>(p);
-  for (int k = 1; k < n; ++k) s += *reinterpret_cast<const f32x4*>(p + k * stride);
-  bf16x4 o;
+  const int D4 = a.Qn / 4, rows = MODE == DH ? piece_rows(a) : a.Pn;
+  const long r = i / D4;
+  const size_t c = (size_t)(i - r * D4) * 4, stride = (size_t)a.Pn * a.Qn;
+  if (r < rows) {
+    const float* p = a.slab + (size_t)r * a.Qn + c;
+    f32x4 s = *reinterpret_cast<const f32x4*>(p);
+    for (int k = 1; k < a.ksplit; ++k) s += *reinterpret_cast<const f32x4*>(p + k * stride);
+    if (MODE == DW && a.acc_in) s += *reinterpret_cast<const f32x4*>(a.acc_in + (size_t)r * a.Qn + c);
+    const size_t at = (size_t)(MODE == DH ? a.index[r] : (int)r) * a.ldo + c;
+    if (MODE == DW && a.out_f32) {
+      *reinterpret_cast<f32x4*>((float*)a.out + at) = s;
+    } else {
+      bf16x4 o;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) o[e] = (bf16)s[e];
-  *reinterpret_cast<bf16x4*>(dh + (long)index[row0 + r] * lddh + c) = o;
-}
-
-// dh of the rows that do not count
-__global__ __launch_bounds__(256) void ce_zero_rows_kernel(const int64_t* target, int64_t ignore, int N, int V, int D8,
-                                                           bf16* dh, long lddh) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  const int n = (int)(i / D8), c = (int)(i - (long)n * D8);
-  if (n >= N) return;
-  const int64_t t = target[n];
-  if (t != ignore && t >= 0 && t < V) return;
-  reinterpret_cast<uint4*>(dh + (long)n * lddh)[c] = make_uint4(0, 0, 0, 0);
+      for (int e = 0; e < 4; ++e) o[e] = (bf16)s[e];
+      *reinterpret_cast<bf16x4*>((bf16*)a.out + at) = o;
+    }
+  }
+  if (MODE == DW && a.dbias) {
+    const long v = i - (long)a.Pn * D4;
+    if (v < 0 || v >= a.Pn) return;
+    float s = a.slab_bias[v];
+    for (int k = 1; k < a.ksplit; ++k) s += a.slab_bias[(size_t)k * a.Pn + v];
+    if (a.dbias_in) s += a.dbias_in[v];
+    if (a.out_f32) ((float*)a.dbias)[v] = s;
+    else ((bf16*)a.dbias)[v] = (bf16)s;
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------- host
 struct CePlan {
   long rows;          // per piece, a multiple of 256
-  int pieces, ksplit;
-  bool stream, big;   // logits: ce_stream_kernel, or tiles of 256 x 256 (otherwise 128 x 128)
+  int pieces, split_dh, split_dw;
+  bool stream, whole; // logits: ce_stream_kernel; with the loss in it
+  bool big;           // or tiles of 256 x 256 (otherwise 128 x 128)
   bool big_dh, big_dw;
   long Vp;
-  size_t index, words, tlogit, lse, weight, part, hc, g, slab, dwacc, dbacc, total;
+  size_t index, words, tlogit, lse, weight, part, hc, g, slab, slab_bias, dwacc, dbacc, total;
 };
 
-constexpr int BIG_TILES = 1024;
 constexpr int STREAM_GRID = 512, TILE_GRID = 256;   // two workgroups per CU, one
 constexpr size_t PIECE_BYTES = (size_t)4 << 30;   // g of a piece, unless the caller says how many rows
+constexpr size_t PIECE_MAX = (size_t)64 << 30, HC_MAX = (size_t)16 << 30;   // g and the rows of h, in any case
+constexpr size_t PAIR_BYTES = (size_t)1 << 30;    // pairs of a piece, where only the loss is asked for
 
 bool sizes_ok(const mmst_linear_ce_args* a) {
   return a && a->N >= 0 && a->N <= MMST_LINEAR_CE_MAX_ROWS && a->V >= 1 && a->V <= MMST_LINEAR_CE_MAX_VOCAB && a->D >= 8 &&
@@ -1055,34 +1104,72 @@ bool args_ok(const mmst_linear_ce_args* a, bool grad) {
 
 size_t align(size_t x) { return (x + 255) & ~(size_t)255; }
 
+long tiles(long n, long m, int b) { return ((n + b - 1) / b) * ((m + b - 1) / b); }
+
+// 256 x 256 tiles, one workgroup per CU, or 128 x 128, two: whichever is done first.  A round of the small ones (512, half as
+// much work) takes 7 / 13 of a round of the large ones, whose steps feed the matrix units better; what a last, partly filled
+// round wastes decides.  Measured, large / small: the loss at 2048 x 1024 x 16384 (rows, width, words; 2 rounds against 4)
+// 70 / 78 us, at 333 x 1024 x 50001 (2 against 3) 68 / 55 us; all of the gradient with dw by either at 8192 x 1024 x 32000 (2
+// against 4) 1696 / 1820 us, at 4096 x 256 x 8192 (1 against 1) 192 / 158 us.
+bool large_tiles(long n, long m) {
+  auto rounds = [](long t, long slots) { return (t + slots - 1) / slots; };
+  return 13 * rounds(tiles(n, m, 256), TILE_GRID) <= 7 * rounds(tiles(n, m, 128), 2 * TILE_GRID);
+}
+
+// dh has the vocabulary as its contraction, which is cut into parts where there are too few tiles; the more parts, the more
+// fp32 slabs to write and read, and small tiles need half as many.  Measured, large / small: 16 tiles (2048 x 512 x 32000)
+// 311 / 300 us, 24 (1400 x 1024 x 50001) 533 / 548 us, 128 (8192 x 1024 x 32000) 1696 / 1791 us.
+constexpr int DH_SMALL = 16;
+
+// Parts of a contraction: as many as keep every CU busy, of at least eight steps (of four: within 2 us either way).
+// Uncut: dh of 3000 x 128 x 32000 (16 parts; 8: 55 us, 16: 46) and dw of 4032 x 128 x 43 (7 parts; the whole gradient 72
+// us uncut and 45 in parts).
+int parts(long t, bool big, long contraction) {
+  const long slots = big ? TILE_GRID : 2 * TILE_GRID, steps = contraction / 64;
+  long s = t < slots ? slots / (t ? t : 1) : 1;
+  if (s > steps / 8) s = steps / 8;
+  return (int)(s < 1 ? 1 : s > 32 ? 32 : s);
+}
+
+// Narrow layers: the stream where a workgroup gets more than two tiles of it, for which it computes the logits twice and
+// reads no exponentials back.  Measured, stream / tiles, loss and gradient: 3000 x 128 x 8000 (1512 tiles) 19 / 23 and 93 / 97
+// us, 3000 x 128 x 32000 42 / 65 and 193 / 239, 2000 x 128 x 8000 (1008) 19 / 16 and 80 / 79, 512 x 128 x 4000 (128) 15 / 14
+// and 55 / 47.
+bool streams(long n, const mmst_linear_ce_args* a) { return a->D <= 128 && tiles(n, a->V, 128) > 2 * STREAM_GRID; }
+
 CePlan plan(const mmst_linear_ce_args* a, bool grad) {
   CePlan p = {};
   p.Vp = ((long)a->V + VT - 1) / VT * VT;
-  const long all = ((long)a->N + 255) / 256 * 256;
+  const long all = ((long)a->N + 255) / 256 * 256, pairs = (a->V + 255) / 256 * 4;
+  auto limit = [&](size_t bytes, size_t row) {   // rows of a piece, so that `row` bytes of each are no more than `bytes`
+    const long fit = (long)(bytes / row) / 256 * 256;
+    p.rows = p.rows < fit ? p.rows : fit < 256 ? 256 : fit;
+  };
   p.rows = all ? all : 256;
+  p.whole = !grad && a->D <= 128 && a->V <= 128;
+  p.stream = p.whole || (!grad && streams(a->N, a));
   if (grad) {
-    long fit = a->rows_per_piece ? ((long)a->rows_per_piece + 255) / 256 * 256 : (long)(PIECE_BYTES / (p.Vp * 2)) / 256 * 256;
-    if (fit < 256) fit = 256;
-    if (p.rows > fit) p.rows = fit;
+    if (a->rows_per_piece) limit(((size_t)a->rows_per_piece + 255) / 256 * 256, 1);
+    else limit(PIECE_BYTES, p.Vp * 2);
+    limit(PIECE_MAX, p.Vp * 2);
+    limit(HC_MAX, (size_t)a->D * 2);
+  } else if (!p.stream) {
+    limit(PAIR_BYTES, pairs * 8);
   }
-  p.pieces = grad && all ? (int)((all + p.rows - 1) / p.rows) : 1;
-  auto tiles = [](long n, long m, int b) { return ((n + b - 1) / b) * ((m + b - 1) / b); };
-  p.stream = a->D <= 128;
-  p.big = tiles(a->N < p.rows ? a->N : p.rows, a->V, 256) >= BIG_TILES;
-  p.big_dh = a->D > 128;
-  p.big_dw = a->D > 128 && tiles(a->V, a->D, 256) >= 256;
-  p.ksplit = 1;
+  p.pieces = all ? (int)((all + p.rows - 1) / p.rows) : 1;
+  const long rows = a->N < p.rows ? a->N : p.rows;
+  p.big = large_tiles(rows, a->V);
   if (grad) {
-    const long t = tiles(p.rows, a->D, p.big_dh ? 256 : 128), steps = p.Vp / 64;
-    long s = 256 / (t < 256 ? t : 256);
-    if (s > steps / 8) s = steps / 8;
-    p.ksplit = (int)(s < 1 ? 1 : s > 32 ? 32 : s);
+    p.stream = streams(rows, a);
+    p.big_dh = tiles(rows, a->D, 256) > DH_SMALL;
+    p.big_dw = large_tiles(a->V, a->D);
+    p.split_dh = parts(tiles(rows, a->D, p.big_dh ? 256 : 128), p.big_dh, a->V);
+    p.split_dw = parts(tiles(a->V, a->D, p.big_dw ? 256 : 128), p.big_dw, rows);
   }
   size_t at = 256;   // [0]: count
   auto take = [&](size_t n) { const size_t o = at; at += align(n); return o; };
-  const long qt = (a->V + 255) / 256 * 4;
   p.tlogit = take(p.rows * 4);
-  p.part = take(p.stream ? (size_t)(STREAM_GRID + 8 * (p.rows / 128)) * 2 * 128 * 8 : (size_t)qt * p.rows * 8);
+  p.part = take(p.stream ? (size_t)(STREAM_GRID + 8 * (p.rows / 128)) * 2 * 128 * 8 : (size_t)pairs * p.rows * 8);
   if (grad) {
     p.index = take((size_t)(all + 256) * 4);
     p.words = take((size_t)(all + 256) * 4);
@@ -1090,7 +1177,9 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
     p.weight = take(p.rows * 4);
     p.hc = take((size_t)p.rows * a->D * 2);
     p.g = take((size_t)p.rows * p.Vp * 2);
-    if (p.ksplit > 1) p.slab = take((size_t)p.ksplit * p.rows * a->D * 4);
+    const size_t dh = p.split_dh > 1 ? (size_t)p.split_dh * p.rows : 0, dw = p.split_dw > 1 ? (size_t)p.split_dw * a->V : 0;
+    if (dh || dw) p.slab = take((dh > dw ? dh : dw) * a->D * 4);   // (one after the other)
+    if (dw) p.slab_bias = take(dw * 4);
     if (p.pieces > 1 && !a->grad_f32) p.dwacc = take((size_t)a->V * a->D * 4);
     if (p.pieces > 1 && !a->grad_f32 && a->dbias) p.dbacc = take((size_t)a->V * 4);
   }
@@ -1098,13 +1187,19 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
   return p;
 }
 
-template <int MODE> void launch(CeGemm& g, bool big, long prows, long qcols, hipStream_t st) {
+template <int MODE> int launch(CeGemm& g, bool big, hipStream_t st) {
   const int b = big ? 256 : 128;
-  g.ptiles = (int)((prows + b - 1) / b);
-  g.qtiles = (int)((qcols + b - 1) / b);
+  g.ptiles = (g.Pn + b - 1) / b;
+  g.qtiles = (g.Qn + b - 1) / b;
   const unsigned grid = (unsigned)(g.ptiles * g.qtiles * g.ksplit);
   if (big) hipLaunchKernelGGL((ce_product_kernel<MODE, 256, 256, 2, 4>), dim3(grid), dim3(512), 0, st, g);
   else hipLaunchKernelGGL((ce_product_kernel<MODE, 128, 128, 2, 2>), dim3(grid), dim3(256), 0, st, g);
+  MMST_CHECK_LAUNCH();
+  if (g.ksplit == 1) return MMST_OK;
+  const long lanes = (long)g.Pn * (g.Qn / 4) + (g.dbias ? g.Pn : 0);
+  hipLaunchKernelGGL(ce_slabs_kernel<MODE>, dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, st, g);
+  MMST_CHECK_LAUNCH();
+  return MMST_OK;
 }
 template <int MODE> void launch_logits(CeGemm& g, const CePlan& p, hipStream_t st) {
   const int b = p.big ? 256 : 128;
@@ -1147,23 +1242,30 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
   logit.part = (float2*)(ws + p.part); logit.tlogit = (float*)(ws + p.tlogit);
   logit.rows_max = (int)p.rows;
   if (!grad) {
-    logit.P = (const bf16*)A.h; logit.ldp = A.ldh; logit.rows_max = N; logit.Pn = N;
-    if (p.stream) launch_stream<LOGIT_STATS>(logit, st);
-    else launch_logits<LOGIT_STATS>(logit, p, st);
-    MMST_CHECK_LAUNCH();
-    hipLaunchKernelGGL(ce_rows_kernel, dim3((N + 15) / 16), dim3(256), 0, st, logit.part, pairs, N, p.stream ? STREAM_GRID : 0, nullptr, 0, N,
-                       nullptr, A.target, A.ignore_index, V, logit.tlogit, nullptr, A.loss, A.lse);
-    MMST_CHECK_LAUNCH();
+    for (int i = 0; i < p.pieces; ++i) {
+      const long row0 = i * p.rows;
+      const int rows = (int)(N - row0 < p.rows ? N - row0 : p.rows);
+      logit.P = (const bf16*)A.h + row0 * A.ldh; logit.ldp = A.ldh; logit.rows_max = rows; logit.Pn = rows;
+      logit.target = A.target + row0;
+      if (p.whole) {
+        logit.loss_out = A.loss; logit.lse_out = A.lse; logit.ignore = A.ignore_index;
+        launch_stream<LOGIT_LOSS>(logit, st);
+        MMST_CHECK_LAUNCH();
+        return MMST_OK;
+      }
+      if (p.stream) launch_stream<LOGIT_STATS>(logit, st);
+      else launch_logits<LOGIT_STATS>(logit, p, st);
+      MMST_CHECK_LAUNCH();
+      hipLaunchKernelGGL(ce_rows_kernel, dim3((rows + 15) / 16), dim3(256), 0, st, logit.part, pairs, rows,
+                         p.stream ? STREAM_GRID : 0, nullptr, 0, rows, nullptr, logit.target, A.ignore_index, V, logit.tlogit,
+                         nullptr, A.loss + row0, A.lse ? A.lse + row0 : nullptr);
+      MMST_CHECK_LAUNCH();
+    }
     return MMST_OK;
   }
 
   hipLaunchKernelGGL(ce_index_kernel, dim3(1), dim3(1024), 0, st, A.target, A.ignore_index, N, V, index, words, count, A.loss, A.lse);
   MMST_CHECK_LAUNCH();
-  if (N > 0) {
-    hipLaunchKernelGGL(ce_zero_rows_kernel, dim3((unsigned)(((long)N * D8 + 255) / 256)), dim3(256), 0, st, A.target,
-                       A.ignore_index, N, V, D8, (bf16*)A.dh, A.lddh);
-    MMST_CHECK_LAUNCH();
-  }
   bf16* hc = (bf16*)(ws + p.hc);
   bf16* gbuf = (bf16*)(ws + p.g);
   float* lse_c = (float*)(ws + p.lse);
@@ -1171,8 +1273,10 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
   for (int i = 0; i < p.pieces; ++i) {
     const int row0 = (int)(i * p.rows);
     const int rows_max = (int)p.rows;
-    hipLaunchKernelGGL(ce_gather_kernel, dim3((unsigned)((p.rows * D8 + 255) / 256)), dim3(256), 0, st, (const bf16*)A.h, A.ldh,
-                       D8, index, count, row0, rows_max, A.dloss, A.grad_scale, hc, weight);
+    const unsigned gather = (unsigned)((p.rows * D8 + 255) / 256);
+    hipLaunchKernelGGL(ce_gather_kernel, dim3(gather + (i ? 0 : (N + 15) / 16)), dim3(256), 0, st, (const bf16*)A.h, A.ldh, D8,
+                       index, count, row0, rows_max, A.dloss, A.grad_scale, hc, weight, gather, A.target, A.ignore_index, N, V,
+                       (bf16*)A.dh, A.lddh);
     MMST_CHECK_LAUNCH();
     logit.P = hc; logit.ldp = D; logit.Pn = rows_max; logit.count = count; logit.row0 = row0; logit.index = index + row0;
     logit.word = words + row0;
@@ -1186,26 +1290,21 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
     MMST_CHECK_LAUNCH();
     logit.lse = lse_c; logit.weight = weight;
     if (p.stream) launch_stream<LOGIT_GRAD>(logit, st);
-    else hipLaunchKernelGGL(ce_scale_kernel, dim3((unsigned)((p.Vp + 2047) / 2048 * (p.rows / 4))), dim3(256), 0, st, logit, 64);
+    else hipLaunchKernelGGL(ce_scale_kernel, dim3((unsigned)((p.Vp + 2047) / 2048 * (p.rows / 4))), dim3(256), 0, st, logit);
     MMST_CHECK_LAUNCH();
 
     CeGemm dh = {};
     dh.P = gbuf; dh.ldp = p.Vp; dh.Pn = rows_max; dh.Q = w; dh.ldq = A.ldw; dh.Qn = D; dh.K = V;
-    dh.count = count; dh.row0 = row0; dh.rows_max = rows_max; dh.index = index + row0; dh.ksplit = p.ksplit;
-    dh.out = A.dh; dh.ldo = A.lddh; dh.slab = p.ksplit > 1 ? (float*)(ws + p.slab) : nullptr;
-    launch<DH>(dh, p.big_dh, p.rows, D, st);
-    MMST_CHECK_LAUNCH();
-    if (p.ksplit > 1) {
-      hipLaunchKernelGGL(ce_slabs_kernel, dim3((unsigned)((p.rows * (D / 4) + 255) / 256)), dim3(256), 0, st,
-                         (const float*)dh.slab, p.ksplit, rows_max, index, count, row0, D / 4, (bf16*)A.dh, A.lddh);
-      MMST_CHECK_LAUNCH();
-    }
+    dh.count = count; dh.row0 = row0; dh.rows_max = rows_max; dh.index = index + row0; dh.ksplit = p.split_dh;
+    dh.out = A.dh; dh.ldo = A.lddh; dh.slab = p.split_dh > 1 ? (float*)(ws + p.slab) : nullptr;
+    if (launch<DH>(dh, p.big_dh, st) != MMST_OK) return MMST_ERR_LAUNCH;
 
     // dw and dbias: in fp32 added to what is there; in bf16 written once, behind sums in fp32 where there are more pieces
     const bool last = i + 1 == p.pieces;
     CeGemm dw = {};
     dw.P = gbuf; dw.ldp = p.Vp; dw.Pn = V; dw.Q = hc; dw.ldq = D; dw.Qn = D;
-    dw.count = count; dw.row0 = row0; dw.rows_max = rows_max; dw.ksplit = 1;
+    dw.count = count; dw.row0 = row0; dw.rows_max = rows_max; dw.ksplit = p.split_dw;
+    dw.slab = p.split_dw > 1 ? (float*)(ws + p.slab) : nullptr; dw.slab_bias = (float*)(ws + p.slab_bias);
     float* acc = (float*)(ws + p.dwacc);
     dw.ldo = D;
     float* bacc = (float*)(ws + p.dbacc);
@@ -1216,8 +1315,7 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
       dw.out = last ? A.dw : (void*)acc; dw.out_f32 = last ? 0 : 1; dw.acc_in = i > 0 ? acc : nullptr;
       if (A.dbias) { dw.dbias = last ? A.dbias : (void*)bacc; dw.dbias_in = i > 0 ? bacc : nullptr; }
     }
-    launch<DW>(dw, p.big_dw, V, D, st);
-    MMST_CHECK_LAUNCH();
+    if (launch<DW>(dw, p.big_dw, st) != MMST_OK) return MMST_ERR_LAUNCH;
   }
   return MMST_OK;
 }

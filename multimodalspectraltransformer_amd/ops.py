@@ -331,8 +331,9 @@ def _linear_ce_args(h, w, target, bias, ignore_index, what):
             and h.dim() == w.dim() == 2 and h.device == w.device and h.shape[1] == w.shape[1]):
         raise L.MMSTError(f"{what}: h [N, D] and w [V, D] in bf16 on one GPU expected (there is no CPU path)")
     device, (n, d), v = h.device, h.shape, w.shape[0]
-    if v < 1 or d < 8 or d % 8:
-        raise L.MMSTError(f"{what}: a vocabulary and a width that is a multiple of 8 expected, got {v} and {d}")
+    if not 1 <= v <= 1 << 22 or not 8 <= d <= 32768 or d % 8 or n > 1 << 24:
+        raise L.MMSTError(f"{what}: at most 2^24 rows, 1 to 2^22 words and a width that is a multiple of 8 and at most 32768 "
+                          f"expected, got {n}, {v} and {d}")
     if target.dtype != torch.int64 or target.shape != (n,) or target.device != device:
         raise L.MMSTError(f"{what}: target as int64 [{n}] on {device} expected, got {target.dtype} {tuple(target.shape)} on {target.device}")
     h, ldh = _matrix(h, d, what)
@@ -377,8 +378,8 @@ def linear_ce_grad(h, w, target, bias=None, dloss=None, grad_scale=1.0, ignore_i
     without a bias.  rows_per_piece bounds the workspace: that many rows' gradient of the logits, in bf16, at a time."""
     a, keep = _linear_ce_args(h, w, target, bias, ignore_index, "linear_ce_grad")
     device, n, d, v = h.device, a.N, a.D, a.V
-    if rows_per_piece < 0:
-        raise L.MMSTError("linear_ce_grad: rows_per_piece must not be negative")
+    if not 0 <= rows_per_piece <= 1 << 24:
+        raise L.MMSTError("linear_ce_grad: rows_per_piece between 0 and 2^24 expected")
     loss, lse = torch.empty((2, n), dtype=torch.float32, device=device).unbind(0)
     dh = torch.empty((n, d), dtype=torch.bfloat16, device=device)
     a.loss, a.dh, a.lddh = loss.data_ptr(), dh.data_ptr(), d

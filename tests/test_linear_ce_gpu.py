@@ -347,6 +347,77 @@ def test_gradient_of_logits_past_32_bits():
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("n,v", [(70001, 43), (66000, 128), (66000, 129)])
+def test_loss_of_few_words_over_many_rows(n, v):
+    """More tiles of rows than workgroups; a bias and weights of the loss that start at any float."""
+    h, w, b, t, dl = make(n, 64, v, seed=n + v, ignored=n // 9)
+    t[5], t[n - 1] = v, -3
+    b[1] = float("-inf")
+    t[7] = 1
+    o = oracle(h, w, b, t, dl)
+    b1, dl1 = torch.empty(v + 1, device=DEV), torch.empty(n + 1, device=DEV)
+    b1[1:], dl1[1:] = b.to(DEV), dl.to(DEV)
+    check_loss(o, *ops.linear_ce(*dev(h, w, t), bias=b1[1:]))
+    out = ops.linear_ce_grad(*dev(h, w, t), bias=b1[1:], dloss=dl1[1:])
+    check_loss(o, *out[:2])
+    check_grad(o, *out[2:])
+
+
+def test_loss_whose_pairs_need_pieces():
+    """More than 2^30 bytes of (maximum, sum) pairs: rows on both sides of the cut, and the last ones, by value."""
+    n, d, v = 8192 + 300, 136, 1 << 20
+    g = torch.Generator(device=DEV).manual_seed(2)
+    h = torch.randn(n, d, device=DEV, generator=g).bfloat16()
+    w = (0.1 * torch.randn(v, d, device=DEV, generator=g)).bfloat16()
+    t = torch.randint(0, v, (n,), device=DEV, generator=g)
+    t[8190] = IGN
+    loss, lse = ops.linear_ce(h, w, t)
+    pick = [0, 8189, 8190, 8191, 8192, 8193, n - 1]
+    o = oracle(h[pick].cpu(), w.cpu(), None, t[pick].cpu(), None)
+    check_loss(o, loss[pick], lse[pick])
+    assert torch.isfinite(loss).all() and int((loss == 0).sum()) == 1
+
+
+@pytest.mark.parametrize("n,d,v,ignored", [(1000, 128, 20001, 77), (1300, 40, 13000, 5), (140, 128, 70001, 0), (66000, 64, 300, 9), (33100, 8, 513, 33000)])
+def test_narrow_layers_as_a_stream(n, d, v, ignored):
+    """More than two tiles per workgroup, one part of the vocabulary or eight: masked words, targets that are none, padding."""
+    h, w, b, t, dl = make(n, d, v, seed=n + 1, ignored=ignored)
+    b[v // 3:v // 2] = float("-inf")
+    b[v - 2] = torch.finfo(torch.float32).min
+    t[t >= 0] = t[t >= 0] % (v // 3)
+    t[11], t[n - 2], t[n // 2] = -1, v, 1 << 33
+    h[(t == IGN).nonzero()[:1, 0]] = float("nan")
+    o = oracle(h, w, b, t, dl)
+    loss, lse, dh, dw, db = ops.linear_ce_grad(*dev(h, w, t), bias=dev(b)[0], dloss=dev(dl)[0])
+    check_loss(o, loss, lse)
+    check_grad(o, dh, dw, db)
+    assert (dh[(t == IGN).to(DEV)] == 0).all() and (dw[v // 3:v // 2] == 0).all()
+    check_loss(o, *ops.linear_ce(*dev(h, w, t), bias=dev(b)[0]))
+    o = oracle(h, w, None, t, dl)
+    out = ops.linear_ce_grad(*dev(h, w, t), dloss=dev(dl)[0])
+    check_loss(o, *out[:2])
+    check_grad(o, *out[2:])
+    check_loss(o, *ops.linear_ce(*dev(h, w, t)))
+
+
+@pytest.mark.parametrize("n,d,v", [(300, 512, 32000), (1024, 136, 16000), (2100, 520, 6000), (4100, 136, 7000), (3000, 264, 40)])
+def test_every_tile_size_and_split(n, d, v):
+    """Large tiles of dw; of the logits, one round; of the logits and of dh, split; two rounds; dw split over the rows."""
+    h, w, b, t, dl = make(n, d, v, seed=n + v, ignored=n // 5)
+    b[v // 2] = float("-inf")
+    o = oracle(h, w, b, t, dl)
+    out = ops.linear_ce_grad(*dev(h, w, t), bias=dev(b)[0], dloss=dev(dl)[0])
+    check_loss(o, *out[:2])
+    check_grad(o, *out[2:])
+    again = ops.linear_ce_grad(*dev(h, w, t), bias=dev(b)[0], dloss=dev(dl)[0])
+    assert all(torch.equal(x, y) for x, y in zip(out, again))
+    check_loss(o, *ops.linear_ce(*dev(h, w, t), bias=dev(b)[0]))
+    f32 = torch.ones(v, d, device=DEV), torch.ones(v, device=DEV)
+    ops.linear_ce_grad(*dev(h, w, t), bias=dev(b)[0], dloss=dev(dl)[0], dw=f32[0], dbias=f32[1])
+    inside(f32[0] - 1, o["dw"], o["ddw"] + 8 * U * (1 + o["dw"].abs()), "dw added to")
+    inside(f32[1] - 1, o["db"], o["ddb"] + 8 * U * (1 + o["db"].abs()), "dbias added to")
+
+
 def test_wrappers_refuse():
     h, w, b, t, dl = dev(*make(20, 64, 100))
     bad = [lambda: ops.linear_ce(h.float(), w, t), lambda: ops.linear_ce(h, w.half(), t), lambda: ops.linear_ce(h, w, t.int()),
@@ -356,7 +427,9 @@ def test_wrappers_refuse():
            lambda: ops.linear_ce_grad(h, w, t, dw=torch.zeros(100, 64, device=DEV).bfloat16()),
            lambda: ops.linear_ce_grad(h, w, t, dw=torch.zeros(100, 63, device=DEV)),
            lambda: ops.linear_ce_grad(h, w, t, bias=b, dw=torch.zeros(100, 64, device=DEV)),
-           lambda: ops.linear_ce_grad(h, w, t, dbias=b), lambda: ops.linear_ce_grad(h, w, t, rows_per_piece=-1)]
+           lambda: ops.linear_ce_grad(h, w, t, dbias=b), lambda: ops.linear_ce_grad(h, w, t, rows_per_piece=-1),
+           lambda: ops.linear_ce_grad(h, w, t, rows_per_piece=1 << 32),
+           lambda: ops.linear_ce(h[:1].expand((1 << 32) + 20, 64), w, t[:1].expand((1 << 32) + 20))]
     for i, call in enumerate(bad):
         with pytest.raises(L.MMSTError):
             call()
