@@ -23,12 +23,23 @@ namespace {
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef LDS_AS unsigned char lds_byte;
 typedef __attribute__((address_space(3))) void* lptr_t;
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float LOG2E = 1.4426950408889634f;
+// exp(x - m) is one fused multiply-add, exp2(x log2 e - m log2 e), and one exponential; the rounding of m log2 e costs digits
+// where m is large (and everything where it is a mask's -1e30), so beyond this the difference is taken first.
+constexpr float FAR = 4096.f;
 constexpr int VT = 256;   // g is padded to whole tiles of the vocabulary, its rows to whole tiles as well
 
-// Exponents are taken in units of log 2; a bias that masks with the lowest float would overflow there, so finite ones end at
-// -2^127 (the logits beside it are still at an infinite distance for exp).
-__device__ __forceinline__ float word_bias(float b) { return b < -0x1p127f && b > -INFINITY ? -0x1p127f : b; }
+// Exponentials on their way to g, two in 32 bits.  They lie in [0, 2), so neither the sign nor the top bit of a float's exponent
+// says anything: bits 29..14 are 7 of the exponent and 9 of the mantissa, two more than bf16 keeps.  They are rounded by 2^-10
+// here and by 2^-8 as g, all but as if g had been rounded alone; in bf16 the errors of dbias were 1.4 times as large.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ uint32_t pack_exp(float lo, float hi) {
+  const uint32_t a = (__builtin_bit_cast(uint32_t, lo) << 2) + 0x8000u, b = (__builtin_bit_cast(uint32_t, hi) << 2) + 0x8000u;
+  return __builtin_amdgcn_perm(b, a, 0x07060302);   // the upper halves
+}
+__device__ __forceinline__ float unpack_exp(uint32_t w, int upper) {
+  return __builtin_bit_cast(float, (upper ? w >> 2 : w << 14) & 0x3FFFC000u);
+}
 
 enum { LOGIT_STATS = 0, LOGIT_GRAD = 1, DH = 2, DW = 3, LOGIT_EXP = 4, LOGIT_LOSS = 5 };
 
@@ -43,7 +54,7 @@ struct CeGemm {
   const float* bias; const int64_t* target; const int* index;
   const int* word;                   // the targets of the rows that count (gradient; NULL: target[row])
   float2* part; float* tlogit;       // per 64 words and row: max, sum of exp; the target's logit
-  const float* lse; const float* weight; bf16* g; long ldg;
+  const float2* lse; const float* weight; bf16* g; long ldg;   // lse: the row's maximum, and log2 of its sum of exponentials
   float* loss_out; float* lse_out; int64_t ignore;   // LOGIT_LOSS
   // products
   void* out; long ldo; int out_f32; int accumulate;   // out_f32: fp32, else bf16; accumulate: added to
@@ -504,7 +515,7 @@ __global__ __launch_bounds__(WP * WQ * 64, 2) void ce_logits_kernel(const CeGemm
     for (int tp = 0; tp < NT / 2; ++tp)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        float b = a.bias ? word_bias(raw[tp][e]) : 0.f;
+        float b = raw[tp][e];
         if (edge && q0 + qw0 + tp * 32 + 8 * j4 + e >= a.Qn) b = -INFINITY;   // past the vocabulary
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) acc[mt][2 * tp + (e >> 2)][e & 3] += b;
@@ -535,7 +546,15 @@ __global__ __launch_bounds__(WP * WQ * 64, 2) void ce_logits_kernel(const CeGemm
     }
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      const float top = mx[mt] * LOG2E, at = top == -INFINITY ? 0.f : top;   // nothing but masked words: exp(-inf - 0), not of NaN
+      float at = mx[mt] == -INFINITY ? 0.f : mx[mt];   // nothing but masked words: exp(-inf - 0), not of NaN
+      if (__ballot(fabsf(at) > FAR)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[mt][nt][e] -= at;
+        at = 0.f;
+      }
+      at *= LOG2E;
       float x = 0.f;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -546,17 +565,17 @@ __global__ __launch_bounds__(WP * WQ * 64, 2) void ce_logits_kernel(const CeGemm
         }
       x = xor32_sum(xor16_sum(x));
       const int m = p0 + pw0 + mt * 16 + i16;
-      if (j4 == 0 && m < rows) a.part[(size_t)(qt * WQ + wave % WQ) * a.rows_max + m] = make_float2(top, x);
+      if (j4 == 0 && m < rows) a.part[(size_t)(qt * WQ + wave % WQ) * a.rows_max + m] = make_float2(mx[mt], x);
     }
     if constexpr (MODE == LOGIT_EXP) {   // whole tiles: g has rows and columns for them
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int tp = 0; tp < NT / 2; ++tp) {
-          bf16x8 o;
+          u32x4 o;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) o[e] = (bf16)acc[mt][2 * tp + (e >> 2)][e & 3];
-          *reinterpret_cast<bf16x8*>(a.g + (size_t)(p0 + pw0 + mt * 16 + i16) * a.ldg + q0 + qw0 + tp * 32 + 8 * j4) = o;
+          for (int e = 0; e < 4; ++e) o[e] = pack_exp(acc[mt][2 * tp + (e >> 1)][(2 * e) & 3], acc[mt][2 * tp + (e >> 1)][(2 * e + 1) & 3]);
+          *reinterpret_cast<u32x4*>(a.g + (size_t)(p0 + pw0 + mt * 16 + i16) * a.ldg + q0 + qw0 + tp * 32 + 8 * j4) = o;
         }
     }
     if (next >= end) return;
@@ -573,26 +592,28 @@ __global__ __launch_bounds__(256) void ce_scale_kernel(const CeGemm a) {
   const int rows = piece_rows(a), across = (int)((a.ldg + 2047) / 2048), r0 = (int)(blockIdx.x / across) * 4;
   const int c = (int)(blockIdx.x % across) * 2048 + (int)threadIdx.x * 8;
   if (r0 >= rows || c >= a.Qn) return;
-  bf16x8 x[4];
+  u32x4 x[4];
   float scale[4], wt[4];
   int hit[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = r0 + i < rows ? r0 + i : rows - 1;
-    x[i] = *reinterpret_cast<const bf16x8*>(a.g + (size_t)r * a.ldg + c);
-    const float l = a.lse[r];
+    x[i] = *reinterpret_cast<const u32x4*>(a.g + (size_t)r * a.ldg + c);
+    const float2 l = a.lse[r];
     wt[i] = a.weight[r];
     hit[i] = a.word[r] - c;
     // a row whose every logit is masked has no gradient
-    if (l == -INFINITY) wt[i] = 0.f;
-    scale[i] = l == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(a.part[(size_t)(c / 64) * a.rows_max + r].x - l * LOG2E) * wt[i];
+    if (l.y == -INFINITY) wt[i] = 0.f;
+    const float top = a.part[(size_t)(c / 64) * a.rows_max + r].x;
+    scale[i] = l.y == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((top - l.x) * LOG2E - l.y) * wt[i];
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (r0 + i >= rows) break;
+    bf16x8 o;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[i][e] = (bf16)((float)x[i][e] * scale[i] - (hit[i] == e ? wt[i] : 0.f));
-    *reinterpret_cast<bf16x8*>(a.g + (size_t)(r0 + i) * a.ldg + c) = x[i];
+    for (int e = 0; e < 8; ++e) o[e] = (bf16)(unpack_exp(x[i][e >> 1], e & 1) * scale[i] - (hit[i] == e ? wt[i] : 0.f));
+    *reinterpret_cast<bf16x8*>(a.g + (size_t)(r0 + i) * a.ldg + c) = o;
   }
 }
 
@@ -692,8 +713,9 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) raw[i >> 1][(i & 1) * 4 + e] = v[e];
   };
-  float m2[MT], sum[MT], lse2[MT], wt[MT];   // running maximum in units of log 2, running sum; lse and weight (gradient)
+  float m2[MT], sum[MT], lse2[MT], wt[MT];   // running maximum and sum; lse in units of log 2 and weight (gradient)
   int target[MT];
+  bool far = false;   // the rows' maxima are too large for one multiply-add
   bf16x8 pf[MT][KS];
   auto load_rows = [&](int p) {   // (no branch around a load: each would be waited for before the next)
     const int left = rows - p * 128, n = left < 128 ? left : 128;
@@ -707,17 +729,24 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
         pf[mt][ks] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rsrc, k < a.K ? (r * (int)a.ldp + k) * 2 : (int)OpQ::OUT, 0, 0));
       }
       target[mt] = a.word ? a.word[m] : (int)(a.target[m] >= 0 && a.target[m] < a.Qn ? a.target[m] : -1);
-      if (MODE == LOGIT_GRAD) { lse2[mt] = a.lse[m]; wt[mt] = a.weight[m]; }
+      if (MODE == LOGIT_GRAD) {
+        const float2 l = a.lse[m];
+        lse2[mt] = l.x;
+        sum[mt] = l.y;
+        wt[mt] = a.weight[m];
+      }
     }
+    far = false;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       const bool there = pw0 + mt * 16 + i16 < n;
       m2[mt] = -INFINITY;
-      sum[mt] = 0.f;
+      if (STATS) sum[mt] = 0.f;
       target[mt] = there && target[mt] >= 0 ? target[mt] : -1 << 30;
       if (MODE == LOGIT_GRAD) {   // a row that is not there, or whose every logit is masked: no gradient
-        const bool live = there && lse2[mt] != -INFINITY;
-        lse2[mt] = live ? lse2[mt] * LOG2E : INFINITY;
+        const bool live = there && sum[mt] != -INFINITY;
+        far |= live && fabsf(lse2[mt]) > FAR;
+        lse2[mt] = live ? __builtin_fmaf(lse2[mt], LOG2E, sum[mt]) : INFINITY;
         wt[mt] = live ? wt[mt] : 0.f;
       }
     }
@@ -747,24 +776,8 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
     const int q0 = qt * 128;
     const bool new_rows = qt + 1 == qend, more = t + 1 < ntiles;
     const int pt1 = new_rows ? pt + 1 : pt, qt1 = new_rows ? st.q0 : qt + 1;
-    // The products start from the bias: -infinity past the vocabulary, which leaves those columns out of everything.  The
-    // lowest float is rare enough to look for first.
+    // The products start from the bias: -infinity past the vocabulary, which leaves those columns out of everything.
     f32x4 start[NT];
-    if (a.bias) {
-      uint32_t low = 0;   // of the bits + 2^23 only numbers below -2^127 pass 0xFF800000 (-infinity becomes 0)
-#pragma unroll
-      for (int tp = 0; tp < NT / 2; ++tp)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t u = __builtin_bit_cast(uint32_t, raw[tp][e]) + 0x00800000u;
-          low = u > low ? u : low;
-        }
-      if (__ballot(low > 0xFF800000u))
-#pragma unroll
-        for (int tp = 0; tp < NT / 2; ++tp)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) raw[tp][e] = word_bias(raw[tp][e]);
-    }
     if (q0 + 128 > a.Qn)
 #pragma unroll
       for (int tp = 0; tp < NT / 2; ++tp)
@@ -818,20 +831,38 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) v = fmaxf(v, acc[mt][nt][e]);
-        const float top = fmaxf(m2[mt], v * LOG2E), at = top == -INFINITY ? 0.f : top;   // nothing but masked words so far
-        float x = sum[mt] * __builtin_amdgcn_exp2f(m2[mt] - at);
+        const float top = fmaxf(m2[mt], v), at = top == -INFINITY ? 0.f : top;   // nothing but masked words so far
+        float x = sum[mt] * __builtin_amdgcn_exp2f((m2[mt] - at) * LOG2E);
+        if (__ballot(fabsf(at) > FAR)) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mt][nt][e], LOG2E, -at));
+            for (int e = 0; e < 4; ++e) x += __builtin_amdgcn_exp2f((acc[mt][nt][e] - at) * LOG2E);
+        } else {
+          const float at2 = at * LOG2E;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mt][nt][e], LOG2E, -at2));
+        }
         m2[mt] = top;
         sum[mt] = x;
       } else {
+        float l2 = lse2[mt];
+        if (__ballot(far)) {   // (the lse again, its two parts)
+          const int m = pt * 128 + pw0 + mt * 16 + i16;
+          const float2 l = a.lse[m < rows ? m : rows - 1];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[mt][nt][e] -= l.x == -INFINITY ? 0.f : l.x;
+          l2 = l2 == INFINITY ? l2 : l.y;
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            acc[mt][nt][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mt][nt][e], LOG2E, -lse2[mt])) * wt[mt];
+            acc[mt][nt][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mt][nt][e], LOG2E, -l2)) * wt[mt];
         if (targets)
 #pragma unroll
           for (int tp = 0; tp < NT / 2; ++tp)
@@ -880,7 +911,7 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
           const float top = xor32_max(xor16_max(m2[mt])), at = top == -INFINITY ? 0.f : top;
-          const float x = xor32_sum(xor16_sum(sum[mt] * __builtin_amdgcn_exp2f(m2[mt] - at)));
+          const float x = xor32_sum(xor16_sum(sum[mt] * __builtin_amdgcn_exp2f((m2[mt] - at) * LOG2E)));
           if (j4 == 0) {
             float2* to = MODE == LOGIT_LOSS ? pair + (wave & 1) * 128 : a.part + st.slot(vocab_part, b, pt, wave & 1);
             to[pw0 + mt * 16 + i16] = make_float2(top, x);
@@ -892,11 +923,11 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
           if (tid < 128 && m < rows) {
             const float2 p = pair[tid], q = pair[128 + tid];
             const float top = fmaxf(p.x, q.x), at = top == -INFINITY ? 0.f : top;
-            const float x = p.y * __builtin_amdgcn_exp2f(p.x - at) + q.y * __builtin_amdgcn_exp2f(q.x - at);
-            const float l = __builtin_fmaf(at, LN2, logf(x));
+            const float x = p.y * __builtin_amdgcn_exp2f((p.x - at) * LOG2E) + q.y * __builtin_amdgcn_exp2f((q.x - at) * LOG2E);
+            const float s = logf(x), l = at + s;
             const int64_t t = a.target[m];
             const bool none = t == a.ignore, word = t >= 0 && t < a.Qn;
-            a.loss_out[m] = none ? 0.f : !word ? __builtin_nanf("") : l == -INFINITY ? INFINITY : l - hit[tid];
+            a.loss_out[m] = none ? 0.f : !word ? __builtin_nanf("") : l == -INFINITY ? INFINITY : s + (at - hit[tid]);
             if (a.lse_out) a.lse_out[m] = none ? 0.f : !word ? __builtin_nanf("") : l;
           }
         }
@@ -971,11 +1002,11 @@ __global__ __launch_bounds__(256) void ce_gather_kernel(const bf16* h, long ldh,
   reinterpret_cast<uint4*>(out)[(long)r * D8 + c] = reinterpret_cast<const uint4*>(h + (long)n * ldh)[c];
 }
 
-// A row's pairs (maximum in units of log 2, sum) -> lse and loss: 16 rows per workgroup, 16 lanes each.  The pairs are those
+// A row's pairs (maximum, sum) -> lse and loss: 16 rows per workgroup, 16 lanes each.  The pairs are those
 // of every 64 words, [.][ld], or (grid != 0) those that the workgroups of ce_stream_kernel left.
 __global__ __launch_bounds__(256) void ce_rows_kernel(const float2* part, int tiles, int ld, int grid, const int* count, int row0,
                                                       int rows_max, const int* index, const int64_t* target, int64_t ignore,
-                                                      int V, const float* tlogit, float* lse_c, float* loss, float* lse) {
+                                                      int V, const float* tlogit, float2* lse_c, float* loss, float* lse) {
   __shared__ float rm[16][16], rs[16][16];
   int rows = rows_max;
   if (count) {
@@ -987,7 +1018,7 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(const float2* part, int ti
   float m = -INFINITY, s = 0.f;
   auto join = [&](const float2 p) {
     const float top = fmaxf(m, p.x), at = top == -INFINITY ? 0.f : top;
-    s = s * __builtin_amdgcn_exp2f(m - at) + p.y * __builtin_amdgcn_exp2f(p.x - at);
+    s = s * __builtin_amdgcn_exp2f((m - at) * LOG2E) + p.y * __builtin_amdgcn_exp2f((p.x - at) * LOG2E);
     m = top;
   };
   if (r < rows && !grid) {
@@ -1000,9 +1031,9 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(const float2* part, int ti
 #pragma unroll
       for (int k = 0; k < 8; ++k) top = fmaxf(top, p[k].x);
       const float at = top == -INFINITY ? 0.f : top;
-      s *= __builtin_amdgcn_exp2f(m - at);
+      s *= __builtin_amdgcn_exp2f((m - at) * LOG2E);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) s += p[k].y * __builtin_amdgcn_exp2f(p[k].x - at);
+      for (int k = 0; k < 8; ++k) s += p[k].y * __builtin_amdgcn_exp2f((p[k].x - at) * LOG2E);
       m = top;
     }
     for (; q < tiles; q += 16) join(part[(size_t)q * ld + r]);
@@ -1025,14 +1056,15 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(const float2* part, int ti
   const float at = top == -INFINITY ? 0.f : top;
   float all = 0.f;
 #pragma unroll
-  for (int k = 0; k < 16; ++k) all += rs[k][i] * __builtin_amdgcn_exp2f(rm[k][i] - at);
-  float l = __builtin_fmaf(at, LN2, logf(all));   // all == 0: -inf, every logit of the row is masked
-  if (lse_c) lse_c[r] = l;
+  for (int k = 0; k < 16; ++k) all += rs[k][i] * __builtin_amdgcn_exp2f((rm[k][i] - at) * LOG2E);
+  const float ls = logf(all);
+  float l = at + ls;   // all == 0: -inf, every logit of the row is masked
+  if (lse_c) lse_c[r] = make_float2(top, log2f(all));
   const int n = index ? index[row0 + r] : r;
   float x;
   const int64_t t = target[n];
   if (!index && (t == ignore || t < 0 || t >= V)) x = l = t == ignore ? 0.f : __builtin_nanf("");
-  else x = l == -INFINITY ? INFINITY : l - tlogit[r];
+  else x = l == -INFINITY ? INFINITY : ls + (at - tlogit[r]);   // (at and the logit may be far larger than the loss)
   loss[n] = x;
   if (lse) lse[n] = l;
 }
@@ -1173,7 +1205,7 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
   if (grad) {
     p.index = take((size_t)(all + 256) * 4);
     p.words = take((size_t)(all + 256) * 4);
-    p.lse = take(p.rows * 4);
+    p.lse = take(p.rows * 8);
     p.weight = take(p.rows * 4);
     p.hc = take((size_t)p.rows * a->D * 2);
     p.g = take((size_t)p.rows * p.Vp * 2);
@@ -1268,7 +1300,7 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
   MMST_CHECK_LAUNCH();
   bf16* hc = (bf16*)(ws + p.hc);
   bf16* gbuf = (bf16*)(ws + p.g);
-  float* lse_c = (float*)(ws + p.lse);
+  float2* lse_c = (float2*)(ws + p.lse);
   float* weight = (float*)(ws + p.weight);
   for (int i = 0; i < p.pieces; ++i) {
     const int row0 = (int)(i * p.rows);

@@ -44,14 +44,16 @@ template <typename T> __device__ __forceinline__ void store_vec(T* p, const floa
 struct DropArgs {
   const void* x; void* y;
   uint64_t n, cols, ldx, ldy;   // n = rows * cols
+  uint64_t wg0;                 // workgroups of the launches before this one
   DropKey key;
 };
 
-// blocks of eight elements that lie inside one row; FLAT: rows follow one another
+// blocks of eight elements that lie inside one row; FLAT: rows follow one another.  37248 x 2048 in bf16: 56 us, 5.4 TB/s, as
+// fast as a copy; two blocks per lane of a 16-bit type keep 32 bytes per lane in flight as one does of fp32.
 template <typename T, bool FLAT, int U>
 __global__ __launch_bounds__(256) void dropout_vec_kernel(const DropArgs a) {
   const uint64_t nb = a.n >> 3, per_row = a.cols >> 3;
-  const uint64_t b0 = (uint64_t)blockIdx.x * (256 * U) + threadIdx.x;
+  const uint64_t b0 = (a.wg0 + blockIdx.x) * (256 * U) + threadIdx.x;
   Vec8<T> in[U];
   uint64_t oy[U];
 #pragma unroll
@@ -80,7 +82,7 @@ __global__ __launch_bounds__(256) void dropout_vec_kernel(const DropArgs a) {
   }
   if constexpr (FLAT) {   // the last n % 8 elements
     const uint64_t i = (nb << 3) + threadIdx.x;
-    if (blockIdx.x == 0 && i < a.n) {
+    if (blockIdx.x == 0 && a.wg0 == 0 && i < a.n) {
       const uint4 w = philox_block(nb, a.key);
       const uint32_t word = threadIdx.x < 2 ? w.x : threadIdx.x < 4 ? w.y : threadIdx.x < 6 ? w.z : w.w;
       const uint32_t bits = threadIdx.x & 1 ? word >> 16 : word & 0xFFFFu;
@@ -91,12 +93,12 @@ __global__ __launch_bounds__(256) void dropout_vec_kernel(const DropArgs a) {
 }
 
 // rows of an odd width that do not follow one another, so that a block may lie in two or more: a wave owns 512 consecutive
-// elements, a lane one element per access
+// elements, a lane one element per access (1023 x 4099 of fp32, rows 4112 apart: 8.7 us, 3.9 TB/s)
 template <typename T>
 __global__ __launch_bounds__(256) void dropout_elem_kernel(const DropArgs a) {
   __shared__ uint4 slots[4][65];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint64_t first = ((uint64_t)blockIdx.x * 4 + wave) * 512;
+  const uint64_t first = ((a.wg0 + blockIdx.x) * 4 + wave) * 512;
   float v[8];
   uint64_t oy[8];
   uint64_t i = first + lane;
@@ -122,20 +124,19 @@ __global__ __launch_bounds__(256) void dropout_elem_kernel(const DropArgs a) {
     if (first + j * 64 + lane < a.n) ((T*)a.y)[oy[j]] = (T)v[j];
 }
 
-template <typename T> int launch_dropout(const DropArgs& a, hipStream_t st) {
-  const bool flat = a.ldx == a.cols && a.ldy == a.cols;
+template <typename T> int launch_dropout(DropArgs& a, hipStream_t st) {
+  const bool flat = a.ldx == a.cols && a.ldy == a.cols, vec = flat || a.cols % 8 == 0;
   constexpr int U = sizeof(T) == 4 ? 1 : 2;
-  if (flat || a.cols % 8 == 0) {
-    const uint64_t grid = (a.n / 8 + 256 * U - 1) / (256 * U);
-    if (grid > 0x7FFFFFFFu) return MMST_ERR_ARG;
-    if (flat) hipLaunchKernelGGL((dropout_vec_kernel<T, true, U>), dim3(grid ? (unsigned)grid : 1u), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((dropout_vec_kernel<T, false, U>), dim3((unsigned)grid), dim3(256), 0, st, a);
-  } else {
-    const uint64_t grid = (a.n + 2047) / 2048;
-    if (grid > 0x7FFFFFFFu) return MMST_ERR_ARG;
-    hipLaunchKernelGGL((dropout_elem_kernel<T>), dim3((unsigned)grid), dim3(256), 0, st, a);
-  }
-  MMST_CHECK_LAUNCH();
+  const uint64_t all = vec ? (a.n / 8 + 256 * U - 1) / (256 * U) : (a.n + 2047) / 2048, most = 1u << 20;
+  do {   // (a launch has less than 2^32 threads)
+    const uint64_t left = all - a.wg0;
+    const dim3 grid(left > most ? (unsigned)most : left ? (unsigned)left : 1u);
+    if (flat) hipLaunchKernelGGL((dropout_vec_kernel<T, true, U>), grid, dim3(256), 0, st, a);
+    else if (vec) hipLaunchKernelGGL((dropout_vec_kernel<T, false, U>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((dropout_elem_kernel<T>), grid, dim3(256), 0, st, a);
+    MMST_CHECK_LAUNCH();
+    a.wg0 += most;
+  } while (a.wg0 < all);
   return MMST_OK;
 }
 
@@ -369,7 +370,7 @@ __global__ __launch_bounds__(BLK) void ln_bwd_kernel(const LnArgs a) {
 }
 
 // dgamma / dbeta = sum over the n workgroups' column sums, in order: 16 columns per workgroup, 64 slices of the rows, so
-// that the up to 1024 rows of a narrow layer norm are 16 loads deep (with 64 columns and 16 slices: 6.0 us at 1024 x 256)
+// that the up to 512 rows of a narrow layer norm are 8 loads deep (4.3 us; with 64 columns and 16 slices 6.0 us)
 __global__ __launch_bounds__(1024) void ln_cols_kernel(const float* part, int n, int cols, float* dgamma, float* dbeta,
                                                        int accumulate) {
   __shared__ float red[64][17];
@@ -395,8 +396,10 @@ __global__ __launch_bounds__(1024) void ln_cols_kernel(const float* part, int n,
 
 struct LnShape { int tpr, nv, blk, grid; };
 
-// Lanes per row: eight columns per lane and access up to a wave, then two accesses, then wider workgroups: a row is one
-// or two accesses deep, so that its loads are in flight together and its registers leave room for other rows.
+// Lanes per row: as few as hold it in one access each (16 for 128 columns: 45 us for 262144 x 128 bf16 with a residual, 32
+// lanes 58), two accesses before a row goes over several waves (32768 x 1024: 42 us, one access of 128 lanes in a workgroup of
+// 256 49), four before a workgroup of 1024 (8192 x 4096: 43 us, 1024 lanes 79; 4096 x 8192: 44 and 57).  6 TB/s of bf16, 5 of
+// fp32.  Workgroups take rows in turn beyond 4096 (2048: up to 10 % slower for odd widths, which wait longer per row).
 LnShape ln_fwd_shape(long rows, int cols) {
   LnShape s;
   s.blk = cols <= 8192 ? 256 : 1024;
@@ -406,8 +409,12 @@ LnShape ln_fwd_shape(long rows, int cols) {
   s.grid = (int)(need < 4096 ? need : 4096);
   return s;
 }
-// The backward pass keeps two sums per column besides the row: two accesses per lane only where the 128 registers of a
-// 1024-lane workgroup hold that (16-bit types, even widths), or where there is no wider workgroup.
+// The backward pass keeps two sums per column besides the row, and each workgroup leaves them for ln_cols_kernel: two
+// workgroups of 256 per CU, or one of 1024 (four and two: 5 % faster to 7 % slower, and 15 to 45 % slower from 4096 columns on,
+// where the sums themselves are most of what is written).  Up to 1024 columns a wave per row with two accesses (32768 x 1024
+// bf16: 38 us; four waves of a larger workgroup 49).  Beyond, two accesses per lane only where the 128 registers of a 1024-lane
+// workgroup hold that (16-bit types, even widths: 8192 x 4096 39 us, 42 with one; 4096 x 8192 43 and 53), or where there is no
+// wider workgroup.
 LnShape ln_bwd_shape(long rows, int cols, int dtype) {
   LnShape s;
   const bool one = cols % 8 || dtype == MMST_F32;
@@ -415,7 +422,7 @@ LnShape ln_bwd_shape(long rows, int cols, int dtype) {
   s.tpr = cols <= 128 ? 16 : cols <= 256 ? 32 : cols <= 1024 ? 64 : cols <= 2048 ? 256 : cols <= 4096 ? (one ? 512 : 256)
         : cols <= 8192 ? (one ? 1024 : 512) : 1024;
   s.nv = (cols + s.tpr * 8 - 1) / (s.tpr * 8);
-  const long need = (rows + s.blk / s.tpr - 1) / (s.blk / s.tpr), most = s.blk == 256 ? 1024 : 256;
+  const long need = (rows + s.blk / s.tpr - 1) / (s.blk / s.tpr), most = s.blk == 256 ? 512 : 256;
   s.grid = (int)(need < most ? need : most);
   return s;
 }
@@ -474,7 +481,7 @@ int mmst_dropout(const void* x, long ldx, void* y, long ldy, int dtype, long row
   if (!x || !y || !ld_ok(x, ldx, cols, rows) || !ld_ok(y, ldy, cols, rows)) return MMST_ERR_ARG;
   if (rows > (long)(0x7FFFFFFFFFFFL / cols)) return MMST_ERR_ARG;
   if (rows == 1) ldx = ldy = cols;
-  DropArgs a{x, y, (uint64_t)rows * (uint64_t)cols, (uint64_t)cols, (uint64_t)ldx, (uint64_t)ldy, drop_key(p, seed, offset)};
+  DropArgs a{x, y, (uint64_t)rows * (uint64_t)cols, (uint64_t)cols, (uint64_t)ldx, (uint64_t)ldy, 0, drop_key(p, seed, offset)};
   if (dtype == MMST_F32) return launch_dropout<float>(a, (hipStream_t)stream);
   if (dtype == MMST_BF16) return launch_dropout<bf16>(a, (hipStream_t)stream);
   return launch_dropout<f16>(a, (hipStream_t)stream);

@@ -4,8 +4,8 @@ Tolerances count roundings (u = 2^-24, half = finfo(bf16).eps / 2 = 2^-8).  A lo
 in any order: at most D u sum |h w| off, plus the bias's addition; call the worst of a row E.  The exponent differences
 carry two more roundings of the row's largest magnitude M, so a probability is off by the factor exp(2 E + 4 u M + 8 u)
 (exp2's and the sums' own roundings: each term's at most V / 16 + 300 partial sums are bounded by u * that many), and lse by
-E + that.  The gradient of the logits is rounded to bf16 once (twice where it is made from the exponentials of a tile, which
-are kept in bf16): 2 half each term, and products of N (dw) or V (dh) such terms in fp32."""
+E + that.  The gradient of the logits is rounded to bf16 once (twice where it is made from the exponentials of a tile, which are
+kept in 16 bits of their own, 2^-10): within 2 half each term, and products of N (dw) or V (dh) such terms in fp32."""
 import pytest
 import torch
 
@@ -416,6 +416,62 @@ def test_every_tile_size_and_split(n, d, v):
     ops.linear_ce_grad(*dev(h, w, t), bias=dev(b)[0], dloss=dev(dl)[0], dw=f32[0], dbias=f32[1])
     inside(f32[0] - 1, o["dw"], o["ddw"] + 8 * U * (1 + o["dw"].abs()), "dw added to")
     inside(f32[1] - 1, o["db"], o["ddb"] + 8 * U * (1 + o["db"].abs()), "dbias added to")
+
+
+@pytest.mark.parametrize("low", [-2.0 ** 14, -1e9, -1e10, -1e30, torch.finfo(torch.float32).min])
+@pytest.mark.parametrize("n,d,v", [(200, 128, 3000), (140, 64, 70001), (300, 200, 2100), (150, 64, 100)])
+def test_masks_of_large_finite_numbers(n, d, v, low):
+    """Words masked by a low finite bias, whole tiles of them."""
+    h, w, b, t, dl = make(n, d, v, seed=n)
+    b[v // 4:] = low
+    t = t % (v // 4)
+    o = oracle(h, w, b, t, dl)
+    loss, lse, dh, dw, db = ops.linear_ce_grad(*dev(h, w, t), bias=dev(b)[0], dloss=dev(dl)[0])
+    # the oracle's bound of the whole row counts the mask's magnitude, which reaches nothing: that of the unmasked words
+    u = oracle(h, w[:v // 4], b[:v // 4], t, dl)
+    check_loss(dict(loss=o["loss"], lse=o["lse"], dloss=u["dloss"] + v * U), loss, lse)
+    inside(dh, u["dh"], u["ddh"] + u["dh"].abs() * HALF * 1.01, "dh")
+    inside(dw[:v // 4], u["dw"], u["ddw"] + u["dw"].abs() * HALF * 1.01, "dw")
+    assert (dw[v // 4:] == 0).all() and (db[v // 4:] == 0).all()
+    check_loss(dict(loss=o["loss"], lse=o["lse"], dloss=u["dloss"] + v * U), *ops.linear_ce(*dev(h, w, t), bias=dev(b)[0]))
+
+
+@pytest.mark.parametrize("n,d,v", [(200, 128, 3000), (140, 64, 70001), (300, 200, 2100), (150, 64, 100)])
+@pytest.mark.parametrize("low", [-2.0 ** 40, 2.0 ** 40, -1e30, torch.finfo(torch.float32).min])
+def test_rows_of_nothing_but_a_large_finite_mask(n, d, v, low):
+    """low + l is low in fp32 for every word (|l| < 2^10, half a step of 2^40 is 2^16): equally likely words, so loss log v
+    and g = dloss (1 / v - [target]).  The loss is off by log's and the sum's rounding, g by bf16's and those."""
+    h, w, b, t, dl = make(n, d, v, seed=n)
+    b[:] = low
+    loss, lse, dh, dw, db = ops.linear_ce_grad(*dev(h, w, t), bias=dev(b)[0], dloss=dev(dl)[0])
+    rel = (v / 16 + 308) * U
+    want = torch.full((n,), float(torch.tensor(v, dtype=torch.float64).log()), dtype=torch.float64)
+    for x in (loss, ops.linear_ce(*dev(h, w, t), bias=dev(b)[0])[0]):
+        inside(x, want, want * 0 + rel + 4 * U * want, "loss")
+    inside(lse, want * 0 + low, want * 0 + abs(low) * U * 2, "lse")
+    hd, wd, wt = h.double(), w.double(), dl.double()[:, None]
+    p = torch.full((n, v), 1.0 / v, dtype=torch.float64)
+    g = (p - torch.nn.functional.one_hot(t, v)) * wt
+    dg = 1.01 * (p * (rel + HALF + 3 * U) * wt + g.abs() * (HALF + 2 * U))
+    o = dict(dh=g @ wd, dw=g.t() @ hd, db=g.sum(0), ddh=dg @ wd.abs() + (v + 40) * U * (g.abs() @ wd.abs()),
+             ddw=dg.t() @ hd.abs() + (n + 8) * U * (g.abs().t() @ hd.abs()), ddb=dg.sum(0) + (n + 8) * U * g.abs().sum(0))
+    check_grad(o, dh, dw, db)
+
+
+def test_tiles_keep_more_than_bf16_of_a_probability():
+    """dbias of words that are no row's target is a sum of probabilities.  A rounding to bf16 has steps of 2^-7 of a number's
+    power of two: its relative error has the standard deviation 2^-7 / sqrt(12) times the root of the mean of 1 / x^2 over x in
+    [1, 2) (mantissas spread over their logarithm: 3 / (8 log 2)), 0.00166; the one to 9 bits before it a quarter of that.
+    Together 0.00171, of the root of the sum of p^2; over 990 words the mean of that has a deviation of 1 / sqrt(2 * 990) =
+    2.2 %, five of which leave it below 0.0019.  (Two roundings to bf16 would be at 0.00235.)"""
+    n, d, v = 2000, 136, 1000
+    h, w, b, t, _ = make(n, d, v, seed=31)
+    t = t % 10
+    s = torch.zeros(v, device=DEV)
+    ops.linear_ce_grad(*dev(h, w, t), bias=dev(b)[0], dw=torch.zeros(v, d, device=DEV), dbias=s)
+    p = torch.softmax(h.double() @ w.double().t() + b.double(), 1)[:, 10:]
+    off = (s.cpu().double()[10:] - p.sum(0)) / p.pow(2).sum(0).sqrt()
+    assert float(off.pow(2).mean().sqrt()) < 0.0019
 
 
 def test_wrappers_refuse():
