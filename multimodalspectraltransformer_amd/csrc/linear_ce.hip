@@ -15,6 +15,9 @@
 // The gradient goes in pieces of the ROWS: a piece's g [rows][V] is the only large buffer.  Rows that do not count
 // (ignore_index) are left out at the start: the others are numbered through on the device and gathered, so a padded batch
 // costs what its tokens cost, and what padding holds (NaN, infinities) reaches nothing.
+// g is made for weights relative to the largest one, which the products' results are multiplied with in fp32: weights that are
+// all the same (a mean's 1 / rows) are 1 then, and g of a target, near -1 in most rows, is near -1 in bf16 as well.  Rounded with
+// 1 / rows inside, all of them would be off by the same 2^-8 at worst, and so would their sum.
 #include "../../include/mmst.h"
 #include "common.h"
 
@@ -54,7 +57,8 @@ struct CeGemm {
   const float* bias; const int64_t* target; const int* index;
   const int* word;                   // the targets of the rows that count (gradient; NULL: target[row])
   float2* part; float* tlogit;       // per 64 words and row: max, sum of exp; the target's logit
-  const float2* lse; const float* weight; bf16* g; long ldg;   // lse: the row's maximum, and log2 of its sum of exponentials
+  const float2* lse; const float* weight; const float* unit; bf16* g; long ldg;   // lse: the row's maximum, and log2 of its sum of exponentials;
+                                     // weight: of the rows' losses in g, relative to *unit
   float* loss_out; float* lse_out; int64_t ignore;   // LOGIT_LOSS
   // products
   void* out; long ldo; int out_f32; int accumulate;   // out_f32: fp32, else bf16; accumulate: added to
@@ -396,7 +400,7 @@ __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_
     for (int mt = 0; mt < MT; ++mt) {
       const int v = p0 + pw0 + mt * 16 + (lane & 15);
       if (lane < 16 && v < Pn) {
-        const float x = sums.sum[MODE == DW ? mt : 0][0] + (a.dbias_in && !a.slab ? a.dbias_in[v] : 0.f);
+        const float x = sums.sum[MODE == DW ? mt : 0][0] * (a.slab ? 1.f : *a.unit) + (a.dbias_in && !a.slab ? a.dbias_in[v] : 0.f);
         if (a.slab) a.slab_bias[(size_t)ks_id * Pn + v] = x;
         else if (a.out_f32) ((float*)a.dbias)[v] = x;
         else ((bf16*)a.dbias)[v] = (bf16)x;
@@ -410,6 +414,7 @@ __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_
   }
 
   const int i16 = lane & 15, j4 = lane >> 4;
+  const float unit = a.slab ? 1.f : *a.unit;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     const int m = p0 + pw0 + mt * 16 + i16;
@@ -418,7 +423,7 @@ __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_
     for (int tp = 0; tp < NT / 2; ++tp) {
       const int c = q0 + qw0 + tp * 32 + 8 * j4;
       if (c >= a.Qn) continue;   // (Qn is a multiple of 8)
-      f32x4 lo = acc[mt][2 * tp], hi = acc[mt][2 * tp + 1];
+      f32x4 lo = acc[mt][2 * tp] * unit, hi = acc[mt][2 * tp + 1] * unit;
       if (a.slab) {
         float* d = a.slab + ((size_t)ks_id * a.Pn + m) * a.Qn + c;
         *reinterpret_cast<f32x4*>(d) = lo;
@@ -585,15 +590,15 @@ __global__ __launch_bounds__(WP * WQ * 64, 2) void ce_logits_kernel(const CeGemm
   }
 }
 
-// g from the exponentials of a piece, in place: a tile's times exp2(its maximum - the row's lse) and the weight, minus the
-// weight where the word is the target.  Four rows per workgroup and 2048 columns, 16 bytes per lane; bound by HBM: 2.1 GB in 0.41 ms,
-// 5.2 TB/s.
+// g from the exponentials of a piece, in place: a tile's times exp(its maximum - the row's lse) and the weight; of the target's
+// word from its logit, which is there in fp32.  Four rows per workgroup and 2048 columns, 16 bytes per lane; bound by HBM: 2.1
+// GB in 0.41 ms, 5.2 TB/s.
 __global__ __launch_bounds__(256) void ce_scale_kernel(const CeGemm a) {
   const int rows = piece_rows(a), across = (int)((a.ldg + 2047) / 2048), r0 = (int)(blockIdx.x / across) * 4;
   const int c = (int)(blockIdx.x % across) * 2048 + (int)threadIdx.x * 8;
   if (r0 >= rows || c >= a.Qn) return;
   u32x4 x[4];
-  float scale[4], wt[4];
+  float scale[4], wt[4], gt[4];   // gt: g of the target's word, whose 1 would leave an exponential's last digits
   int hit[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -605,6 +610,7 @@ __global__ __launch_bounds__(256) void ce_scale_kernel(const CeGemm a) {
     // a row whose every logit is masked has no gradient
     if (l.y == -INFINITY) wt[i] = 0.f;
     const float top = a.part[(size_t)(c / 64) * a.rows_max + r].x;
+    gt[i] = l.y == -INFINITY ? 0.f : (__builtin_amdgcn_exp2f((a.tlogit[r] - l.x) * LOG2E - l.y) - 1.f) * wt[i];
     scale[i] = l.y == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((top - l.x) * LOG2E - l.y) * wt[i];
   }
 #pragma unroll
@@ -612,7 +618,7 @@ __global__ __launch_bounds__(256) void ce_scale_kernel(const CeGemm a) {
     if (r0 + i >= rows) break;
     bf16x8 o;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = (bf16)(unpack_exp(x[i][e >> 1], e & 1) * scale[i] - (hit[i] == e ? wt[i] : 0.f));
+    for (int e = 0; e < 8; ++e) o[e] = (bf16)(hit[i] == e ? gt[i] : unpack_exp(x[i][e >> 1], e & 1) * scale[i]);
     *reinterpret_cast<bf16x8*>(a.g + (size_t)(r0 + i) * a.ldg + c) = o;
   }
 }
@@ -941,16 +947,23 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
 
 // ---------------------------------------------------------------------------------------------------- rows
 // The rows that count, numbered through in their order (one workgroup: 16 waves look at 1024 targets at a time), and the
-// losses of those that do not: 0 where the target is ignore_index, NaN where it is no word (and no gradient).
+// losses of those that do not: 0 where the target is ignore_index, NaN where it is no word (and no gradient).  The largest weight.
 __global__ __launch_bounds__(1024) void ce_index_kernel(const int64_t* target, int64_t ignore, int N, int V, int* index,
-                                                        int* words, int* count, float* loss, float* lse) {
+                                                        int* words, int* count, float* loss, float* lse, const float* dloss,
+                                                        float scale, float* unit) {
   __shared__ int waves[16];
+  __shared__ float top[16];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   int done = 0;
+  float largest = 0.f;   // (NaN does not count)
   for (int base = 0; base < N; base += 1024) {
     const int n = base + (int)threadIdx.x;
     int64_t t = ignore;
-    if (n < N) t = target[n];
+    float wt = 1.f;
+    if (n < N) {
+      t = target[n];
+      if (dloss) wt = dloss[n];
+    }
     const bool word = t >= 0 && t < V, keep = n < N && t != ignore && word;
     if (n < N && !keep) {
       const float x = t == ignore ? 0.f : __builtin_nanf("");
@@ -969,20 +982,28 @@ __global__ __launch_bounds__(1024) void ce_index_kernel(const int64_t* target, i
       all += c;
     }
     if (keep) {
+      largest = fmaxf(largest, fabsf(scale * wt));
       const int at = done + before + __popcll(b & ((1ull << lane) - 1));
       index[at] = n;
       words[at] = (int)t;
     }
     done += all;
   }
-  if (threadIdx.x == 0) *count = done;
+  largest = wave_max(largest);
+  if (lane == 0) top[w] = largest;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+#pragma unroll
+  for (int i = 1; i < 16; ++i) largest = fmaxf(largest, top[i]);
+  *count = done;
+  *unit = largest > 0.f && largest < INFINITY ? largest : 1.f;   // (a weight of infinity stays with its row)
 }
 
 // A piece's rows, one after another (16 bytes per lane), and their weights; behind its `gather` workgroups those that clear dh
 // of the rows that do not count, 16 rows each.
 __global__ __launch_bounds__(256) void ce_gather_kernel(const bf16* h, long ldh, int D8, const int* index, const int* count,
                                                         int row0, int rows_max, const float* dloss, float scale, bf16* out,
-                                                        float* weight, unsigned gather, const int64_t* target, int64_t ignore,
+                                                        float* weight, const float* unit, unsigned gather, const int64_t* target, int64_t ignore,
                                                         int N, int V, bf16* dh, long lddh) {
   if (blockIdx.x >= gather) {
     const long n = (long)(blockIdx.x - gather) * 16 + (threadIdx.x >> 4);
@@ -998,7 +1019,7 @@ __global__ __launch_bounds__(256) void ce_gather_kernel(const bf16* h, long ldh,
   rows = rows < rows_max ? rows : rows_max;
   if (r >= rows) return;
   const int n = index[row0 + r];
-  if (c == 0) weight[r] = scale * (dloss ? dloss[n] : 1.f);
+  if (c == 0) weight[r] = scale * (dloss ? dloss[n] : 1.f) / *unit;
   reinterpret_cast<uint4*>(out)[(long)r * D8 + c] = reinterpret_cast<const uint4*>(h + (long)n * ldh)[c];
 }
 
@@ -1075,10 +1096,12 @@ template <int MODE> __global__ __launch_bounds__(256) void ce_slabs_kernel(const
   const int D4 = a.Qn / 4, rows = MODE == DH ? piece_rows(a) : a.Pn;
   const long r = i / D4;
   const size_t c = (size_t)(i - r * D4) * 4, stride = (size_t)a.Pn * a.Qn;
+  const float unit = *a.unit;
   if (r < rows) {
     const float* p = a.slab + (size_t)r * a.Qn + c;
     f32x4 s = *reinterpret_cast<const f32x4*>(p);
     for (int k = 1; k < a.ksplit; ++k) s += *reinterpret_cast<const f32x4*>(p + k * stride);
+    s *= unit;
     if (MODE == DW && a.acc_in) s += *reinterpret_cast<const f32x4*>(a.acc_in + (size_t)r * a.Qn + c);
     const size_t at = (size_t)(MODE == DH ? a.index[r] : (int)r) * a.ldo + c;
     if (MODE == DW && a.out_f32) {
@@ -1095,6 +1118,7 @@ template <int MODE> __global__ __launch_bounds__(256) void ce_slabs_kernel(const
     if (v < 0 || v >= a.Pn) return;
     float s = a.slab_bias[v];
     for (int k = 1; k < a.ksplit; ++k) s += a.slab_bias[(size_t)k * a.Pn + v];
+    s *= unit;
     if (a.dbias_in) s += a.dbias_in[v];
     if (a.out_f32) ((float*)a.dbias)[v] = s;
     else ((bf16*)a.dbias)[v] = (bf16)s;
@@ -1198,7 +1222,7 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
     p.split_dh = parts(tiles(rows, a->D, p.big_dh ? 256 : 128), p.big_dh, a->V);
     p.split_dw = parts(tiles(a->V, a->D, p.big_dw ? 256 : 128), p.big_dw, rows);
   }
-  size_t at = 256;   // [0]: count
+  size_t at = 256;   // count, unit
   auto take = [&](size_t n) { const size_t o = at; at += align(n); return o; };
   p.tlogit = take(p.rows * 4);
   p.part = take(p.stream ? (size_t)(STREAM_GRID + 8 * (p.rows / 128)) * 2 * 128 * 8 : (size_t)pairs * p.rows * 8);
@@ -1262,6 +1286,7 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
   hipStream_t st = (hipStream_t)stream;
   char* ws = (char*)A.ws;
   int* count = (int*)ws;
+  float* unit = (float*)ws + 1;
   int* index = (int*)(ws + p.index);
   int* words = (int*)(ws + p.words);
   const bf16* w = (const bf16*)A.w;
@@ -1296,7 +1321,8 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
     return MMST_OK;
   }
 
-  hipLaunchKernelGGL(ce_index_kernel, dim3(1), dim3(1024), 0, st, A.target, A.ignore_index, N, V, index, words, count, A.loss, A.lse);
+  hipLaunchKernelGGL(ce_index_kernel, dim3(1), dim3(1024), 0, st, A.target, A.ignore_index, N, V, index, words, count, A.loss, A.lse,
+                     A.dloss, A.grad_scale, unit);
   MMST_CHECK_LAUNCH();
   bf16* hc = (bf16*)(ws + p.hc);
   bf16* gbuf = (bf16*)(ws + p.g);
@@ -1307,7 +1333,7 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
     const int rows_max = (int)p.rows;
     const unsigned gather = (unsigned)((p.rows * D8 + 255) / 256);
     hipLaunchKernelGGL(ce_gather_kernel, dim3(gather + (i ? 0 : (N + 15) / 16)), dim3(256), 0, st, (const bf16*)A.h, A.ldh, D8,
-                       index, count, row0, rows_max, A.dloss, A.grad_scale, hc, weight, gather, A.target, A.ignore_index, N, V,
+                       index, count, row0, rows_max, A.dloss, A.grad_scale, hc, weight, unit, gather, A.target, A.ignore_index, N, V,
                        (bf16*)A.dh, A.lddh);
     MMST_CHECK_LAUNCH();
     logit.P = hc; logit.ldp = D; logit.Pn = rows_max; logit.count = count; logit.row0 = row0; logit.index = index + row0;
@@ -1328,7 +1354,7 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
     CeGemm dh = {};
     dh.P = gbuf; dh.ldp = p.Vp; dh.Pn = rows_max; dh.Q = w; dh.ldq = A.ldw; dh.Qn = D; dh.K = V;
     dh.count = count; dh.row0 = row0; dh.rows_max = rows_max; dh.index = index + row0; dh.ksplit = p.split_dh;
-    dh.out = A.dh; dh.ldo = A.lddh; dh.slab = p.split_dh > 1 ? (float*)(ws + p.slab) : nullptr;
+    dh.unit = unit; dh.out = A.dh; dh.ldo = A.lddh; dh.slab = p.split_dh > 1 ? (float*)(ws + p.slab) : nullptr;
     if (launch<DH>(dh, p.big_dh, st) != MMST_OK) return MMST_ERR_LAUNCH;
 
     // dw and dbias: in fp32 added to what is there; in bf16 written once, behind sums in fp32 where there are more pieces
@@ -1336,6 +1362,7 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
     CeGemm dw = {};
     dw.P = gbuf; dw.ldp = p.Vp; dw.Pn = V; dw.Q = hc; dw.ldq = D; dw.Qn = D;
     dw.count = count; dw.row0 = row0; dw.rows_max = rows_max; dw.ksplit = p.split_dw;
+    dw.unit = unit;
     dw.slab = p.split_dw > 1 ? (float*)(ws + p.slab) : nullptr; dw.slab_bias = (float*)(ws + p.slab_bias);
     float* acc = (float*)(ws + p.dwacc);
     dw.ldo = D;

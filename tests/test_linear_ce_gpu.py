@@ -474,6 +474,49 @@ def test_tiles_keep_more_than_bf16_of_a_probability():
     assert float(off.pow(2).mean().sqrt()) < 0.0019
 
 
+@pytest.mark.parametrize("n,d,v", [(333, 136, 5000), (3000, 128, 8000)])
+@pytest.mark.parametrize("weights", ["dloss", "scale"])
+def test_equal_weights_are_not_rounded(n, d, v, weights):
+    """The mean's 1 / n, whose nearest bf16 number is up to 2^-8 off: sums of g would all be.  dbias summed over the words that
+    are targets, each of probability below 2^-9, is minus the weights' sum and what their probabilities add: g of a target is
+    off by at most 2^-9 of it (the step below 1 is 2^-8) and by its probability where that rounds away."""
+    h, w, b, t, _ = make(n, d, v, seed=41, scale=0.5)
+    s = torch.zeros(v, device=DEV)
+    kw = dict(dloss=torch.full((n,), 1 / n, device=DEV)) if weights == "dloss" else dict(grad_scale=1 / n)
+    dh = ops.linear_ce_grad(*dev(h, w, t), bias=dev(b)[0], dw=torch.zeros(v, d, device=DEV), dbias=s, **kw)[2]
+    p = torch.softmax(h.double() @ w.double().t() + b.double(), 1)
+    g = (p - torch.nn.functional.one_hot(t, v)) / n
+    pt = p.gather(1, t[:, None])
+    assert float(pt.max()) < 2.0 ** -9
+    hot = torch.zeros(v, dtype=torch.bool)
+    hot[t] = True
+    off = abs(float(s.cpu().double()[hot].sum() - g.sum(0)[hot].sum()))
+    assert off <= float(pt.mean()) * 1.01 + 2.0 ** -8 * float(p[:, hot].sum()) / n + 1e-5
+    # and without a weight the same bits of g: dh is that times the weight, rounded once more
+    one = ops.linear_ce_grad(*dev(h, w, t), bias=dev(b)[0])[2].cpu().double() / n
+    inside(dh, one, one.abs() * 2.02 * HALF, "dh")
+
+
+@pytest.mark.parametrize("n,d,v", [(64, 136, 500), (1000, 64, 20001)])
+def test_weights_of_every_kind(n, d, v):
+    """Zeros, negative ones, and one of infinity or NaN, which stays with its row (and the words, all of which it reaches)."""
+    h, w, b, t, dl = make(n, d, v, seed=43, ignored=n // 8)
+    dl[::3] = 0
+    dl[1::3] *= -1e-3
+    o = oracle(h, w, b, t, dl)
+    check_grad(o, *ops.linear_ce_grad(*dev(h, w, t), bias=dev(b)[0], dloss=dev(dl)[0])[2:])
+    zero = ops.linear_ce_grad(*dev(h, w, t), bias=dev(b)[0], dloss=torch.zeros(n, device=DEV))
+    assert all((x == 0).all() for x in zero[2:])
+    k = int((t != IGN).nonzero()[2, 0])
+    for bad in (float("nan"), float("inf")):
+        dl2 = dl.clone()
+        dl2[k] = bad
+        dh = ops.linear_ce_grad(*dev(h, w, t), bias=dev(b)[0], dloss=dev(dl2)[0])[2].cpu()
+        rest = torch.arange(n) != k
+        inside(dh[rest], o["dh"][rest], (o["ddh"] + o["dh"].abs() * HALF * 1.01)[rest], "dh")
+        assert not torch.isfinite(dh[k]).any()
+
+
 def test_wrappers_refuse():
     h, w, b, t, dl = dev(*make(20, 64, 100))
     bad = [lambda: ops.linear_ce(h.float(), w, t), lambda: ops.linear_ce(h, w.half(), t), lambda: ops.linear_ce(h, w, t.int()),
