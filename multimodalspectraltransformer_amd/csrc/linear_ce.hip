@@ -353,26 +353,27 @@ __device__ __forceinline__ void tile_of(int id, int ptiles, int qtiles, int& pt,
 // 8192 x 2048 x 65536 takes 1.88 ms for dh and 1.83 ms for dw, 1.17 and 1.20 PFLOP/s in 256 x 256 tiles (2.15 and 2.2 ms with
 // four waves of 128 x 128 each, that issue their DMA, read and multiply one after another).  In narrow layers (3032 x 128 x
 // 32000: 40 and 46 us) by reading g.
+// block: the workgroup's number of n
 template <int MODE, int BP, int BQ, int WP, int WQ>
-__global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_product_kernel(const CeGemm a) {
+__device__ __forceinline__ void ce_product(const CeGemm& a, int block, int n, lds_byte* lds) {
   using Tile = CeTile<MODE, BP, BQ, WP, WQ>;
   constexpr int MT = Tile::MT, NT = Tile::NT;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[Tile::SMEM];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int id;   // consecutive tiles to one XCD (workgroups go round the eight of them)
   {
-    const int n = gridDim.x, q8 = n >> 3, r8 = n & 7, x = blockIdx.x & 7;
-    id = (x < r8 ? x * (q8 + 1) : r8 * (q8 + 1) + (x - r8) * q8) + ((int)blockIdx.x >> 3);
+    const int q8 = n >> 3, r8 = n & 7, x = block & 7;
+    id = (x < r8 ? x * (q8 + 1) : r8 * (q8 + 1) + (x - r8) * q8) + (block >> 3);
   }
   const int per = a.ptiles * a.qtiles;
   const int ks_id = id / per;
+  if (ks_id >= a.ksplit) return;   // (uniform, as the next)
   id -= ks_id * per;
   int pt, qt;
   tile_of(id, a.ptiles, a.qtiles, pt, qt);
   const int rows = piece_rows(a);
   const int p0 = pt * BP, q0 = qt * BQ;
   const int K = MODE == DW ? rows : a.K, Pn = MODE == DW ? a.Pn : rows;
-  if (MODE == DH && p0 >= rows) return;   // (uniform: before any barrier)
+  if (MODE == DH && p0 >= rows) return;
   int kbeg = 0, nsteps = (K + Tile::BK - 1) / Tile::BK;
   if (a.ksplit > 1) {
     const int s0 = (int)((long)nsteps * ks_id / a.ksplit), s1 = (int)((long)nsteps * (ks_id + 1) / a.ksplit);
@@ -385,7 +386,6 @@ __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_
   op.init(a.P, a.ldp, p0, Pn, K, tid);
   oq.init(a.Q, a.ldq, q0, a.Qn, K, tid);
 
-  lds_byte* const lds = (lds_byte*)smem;
   typename Tile::template Acc<false> plain;
   f32x4 (&acc)[MT][NT] = plain.v;
   if (nsteps > 0) {
@@ -448,6 +448,20 @@ __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_
       }
     }
   }
+}
+
+template <int MODE, int BP, int BQ, int WP, int WQ>
+__global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_product_kernel(const CeGemm a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[CeTile<MODE, BP, BQ, WP, WQ>::SMEM];
+  ce_product<MODE, BP, BQ, WP, WQ>(a, blockIdx.x, gridDim.x, (lds_byte*)smem);
+}
+
+// Both products in one launch, where both have small tiles: n workgroups (a multiple of 8, so that the others' XCDs are what
+// their numbers say) for dh, the others for dw.  PRODUCTS_MEASURED
+__global__ __launch_bounds__(256, 1) void ce_products_kernel(const CeGemm dh, const CeGemm dw, int n) {
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[CeTile<DW, 128, 128, 2, 2>::SMEM];
+  if ((int)blockIdx.x < n) ce_product<DH, 128, 128, 2, 2>(dh, blockIdx.x, n, (lds_byte*)smem);
+  else ce_product<DW, 128, 128, 2, 2>(dw, (int)blockIdx.x - n, (int)gridDim.x - n, (lds_byte*)smem);
 }
 
 // ---------------------------------------------------------------------------------------------------- logits, tile by tile
@@ -1091,8 +1105,7 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(const float2* part, int ti
 }
 
 // The results of a product from the slabs of its split contraction: 4 columns per lane, behind them the words of dbias
-template <int MODE> __global__ __launch_bounds__(256) void ce_slabs_kernel(const CeGemm a) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+template <int MODE> __device__ __forceinline__ void join_slabs(const CeGemm& a, long i) {
   const int D4 = a.Qn / 4, rows = MODE == DH ? piece_rows(a) : a.Pn;
   const long r = i / D4;
   const size_t c = (size_t)(i - r * D4) * 4, stride = (size_t)a.Pn * a.Qn;
@@ -1125,6 +1138,11 @@ template <int MODE> __global__ __launch_bounds__(256) void ce_slabs_kernel(const
   }
 }
 
+__global__ __launch_bounds__(256) void ce_slabs_kernel(const CeGemm dh, const CeGemm dw, unsigned n) {   // n workgroups for dh
+  if (blockIdx.x < n) join_slabs<DH>(dh, (long)blockIdx.x * 256 + threadIdx.x);
+  else join_slabs<DW>(dw, (long)(blockIdx.x - n) * 256 + threadIdx.x);
+}
+
 // ---------------------------------------------------------------------------------------------------- host
 struct CePlan {
   long rows;          // per piece, a multiple of 256
@@ -1133,7 +1151,7 @@ struct CePlan {
   bool big;           // or tiles of 256 x 256 (otherwise 128 x 128)
   bool big_dh, big_dw;
   long Vp;
-  size_t index, words, tlogit, lse, weight, part, hc, g, slab, slab_bias, dwacc, dbacc, total;
+  size_t index, words, tlogit, lse, weight, part, hc, g, slab_dh, slab_dw, slab_bias, dwacc, dbacc, total;
 };
 
 constexpr int STREAM_GRID = 512, TILE_GRID = 256;   // two workgroups per CU, one
@@ -1154,7 +1172,10 @@ bool args_ok(const mmst_linear_ce_args* a, bool grad) {
   };
   if (!rows_ok(a->w, a->ldw, a->V)) return false;
   if (a->N > 0 && (!rows_ok(a->h, a->ldh, a->N) || !a->target || !a->loss)) return false;
+  auto aligned = [](const void* p, size_t n) { return (uintptr_t)p % n == 0; };   // (NULL is)
+  if (!aligned(a->target, 8) || !aligned(a->bias, 4) || !aligned(a->loss, 4) || !aligned(a->lse, 4)) return false;
   if (!grad) return true;
+  if (!aligned(a->dloss, 4) || !aligned(a->dbias, a->grad_f32 ? 4 : 2)) return false;
   return (a->N == 0 || rows_ok(a->dh, a->lddh, a->N)) && a->dw && (uintptr_t)a->dw % 16 == 0;
 }
 
@@ -1234,7 +1255,8 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
     p.hc = take((size_t)p.rows * a->D * 2);
     p.g = take((size_t)p.rows * p.Vp * 2);
     const size_t dh = p.split_dh > 1 ? (size_t)p.split_dh * p.rows : 0, dw = p.split_dw > 1 ? (size_t)p.split_dw * a->V : 0;
-    if (dh || dw) p.slab = take((dh > dw ? dh : dw) * a->D * 4);   // (one after the other)
+    if (dh) p.slab_dh = take(dh * a->D * 4);
+    if (dw) p.slab_dw = take(dw * a->D * 4);
     if (dw) p.slab_bias = take(dw * 4);
     if (p.pieces > 1 && !a->grad_f32) p.dwacc = take((size_t)a->V * a->D * 4);
     if (p.pieces > 1 && !a->grad_f32 && a->dbias) p.dbacc = take((size_t)a->V * 4);
@@ -1243,18 +1265,35 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
   return p;
 }
 
-template <int MODE> int launch(CeGemm& g, bool big, hipStream_t st) {
-  const int b = big ? 256 : 128;
-  g.ptiles = (g.Pn + b - 1) / b;
-  g.qtiles = (g.Qn + b - 1) / b;
-  const unsigned grid = (unsigned)(g.ptiles * g.qtiles * g.ksplit);
+template <int MODE> void launch_product(const CeGemm& g, bool big, unsigned grid, hipStream_t st) {
   if (big) hipLaunchKernelGGL((ce_product_kernel<MODE, 256, 256, 2, 4>), dim3(grid), dim3(512), 0, st, g);
   else hipLaunchKernelGGL((ce_product_kernel<MODE, 128, 128, 2, 2>), dim3(grid), dim3(256), 0, st, g);
+}
+int launch_products(CeGemm& dh, CeGemm& dw, const CePlan& p, hipStream_t st) {
+  auto grid = [](CeGemm& g, bool big) {
+    const int b = big ? 256 : 128;
+    g.ptiles = (g.Pn + b - 1) / b;
+    g.qtiles = (g.Qn + b - 1) / b;
+    return (unsigned)(g.ptiles * g.qtiles * g.ksplit);
+  };
+  const unsigned n = grid(dh, p.big_dh), m = grid(dw, p.big_dw);
+  if (!p.big_dh && !p.big_dw) {
+    const unsigned n8 = (n + 7) & ~7u;
+    hipLaunchKernelGGL(ce_products_kernel, dim3(n8 + m), dim3(256), 0, st, dh, dw, (int)n8);
+  } else {
+    launch_product<DH>(dh, p.big_dh, n, st);
+    MMST_CHECK_LAUNCH();
+    launch_product<DW>(dw, p.big_dw, m, st);
+  }
   MMST_CHECK_LAUNCH();
-  if (g.ksplit == 1) return MMST_OK;
-  const long lanes = (long)g.Pn * (g.Qn / 4) + (g.dbias ? g.Pn : 0);
-  hipLaunchKernelGGL(ce_slabs_kernel<MODE>, dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, st, g);
-  MMST_CHECK_LAUNCH();
+  auto lanes = [](const CeGemm& g) -> unsigned {   // workgroups of 256 that join its slabs
+    return g.ksplit > 1 ? (unsigned)(((long)g.Pn * (g.Qn / 4) + (g.dbias ? g.Pn : 0) + 255) / 256) : 0u;
+  };
+  const unsigned a = lanes(dh), b = lanes(dw);
+  if (a + b) {
+    hipLaunchKernelGGL(ce_slabs_kernel, dim3(a + b), dim3(256), 0, st, dh, dw, a);
+    MMST_CHECK_LAUNCH();
+  }
   return MMST_OK;
 }
 template <int MODE> void launch_logits(CeGemm& g, const CePlan& p, hipStream_t st) {
@@ -1354,8 +1393,7 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
     CeGemm dh = {};
     dh.P = gbuf; dh.ldp = p.Vp; dh.Pn = rows_max; dh.Q = w; dh.ldq = A.ldw; dh.Qn = D; dh.K = V;
     dh.count = count; dh.row0 = row0; dh.rows_max = rows_max; dh.index = index + row0; dh.ksplit = p.split_dh;
-    dh.unit = unit; dh.out = A.dh; dh.ldo = A.lddh; dh.slab = p.split_dh > 1 ? (float*)(ws + p.slab) : nullptr;
-    if (launch<DH>(dh, p.big_dh, st) != MMST_OK) return MMST_ERR_LAUNCH;
+    dh.unit = unit; dh.out = A.dh; dh.ldo = A.lddh; dh.slab = p.split_dh > 1 ? (float*)(ws + p.slab_dh) : nullptr;
 
     // dw and dbias: in fp32 added to what is there; in bf16 written once, behind sums in fp32 where there are more pieces
     const bool last = i + 1 == p.pieces;
@@ -1363,7 +1401,7 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
     dw.P = gbuf; dw.ldp = p.Vp; dw.Pn = V; dw.Q = hc; dw.ldq = D; dw.Qn = D;
     dw.count = count; dw.row0 = row0; dw.rows_max = rows_max; dw.ksplit = p.split_dw;
     dw.unit = unit;
-    dw.slab = p.split_dw > 1 ? (float*)(ws + p.slab) : nullptr; dw.slab_bias = (float*)(ws + p.slab_bias);
+    dw.slab = p.split_dw > 1 ? (float*)(ws + p.slab_dw) : nullptr; dw.slab_bias = (float*)(ws + p.slab_bias);
     float* acc = (float*)(ws + p.dwacc);
     dw.ldo = D;
     float* bacc = (float*)(ws + p.dbacc);
@@ -1374,7 +1412,7 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
       dw.out = last ? A.dw : (void*)acc; dw.out_f32 = last ? 0 : 1; dw.acc_in = i > 0 ? acc : nullptr;
       if (A.dbias) { dw.dbias = last ? A.dbias : (void*)bacc; dw.dbias_in = i > 0 ? bacc : nullptr; }
     }
-    if (launch<DW>(dw, p.big_dw, st) != MMST_OK) return MMST_ERR_LAUNCH;
+    if (launch_products(dh, dw, p, st) != MMST_OK) return MMST_ERR_LAUNCH;
   }
   return MMST_OK;
 }

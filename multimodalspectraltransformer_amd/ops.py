@@ -384,6 +384,8 @@ def linear_ce_grad(h, w, target, bias=None, dloss=None, grad_scale=1.0, ignore_i
     dh = torch.empty((n, d), dtype=torch.bfloat16, device=device)
     a.loss, a.dh, a.lddh = loss.data_ptr(), dh.data_ptr(), d
     a.lse = a.loss + 4 * n if n else None
+    if isinstance(dloss, torch.Tensor) and not dloss.is_contiguous():   # a mean's gradient is one number, expanded
+        dloss = dloss.contiguous()
     a.dloss = _vector(dloss, n, device, "linear_ce_grad: dloss")
     a.grad_scale, a.rows_per_piece = grad_scale, rows_per_piece
     if dw is None:

@@ -39,6 +39,15 @@ def test_linear_ce_gradient_refusals(kw):
     assert _call(1, **kw) == -1
 
 
+@pytest.mark.parametrize("kw", [dict(target=3 * P + 4), dict(bias=8 * P + 2), dict(loss=4 * P + 1), dict(lse=8 * P + 2)])
+def test_linear_ce_refuses_misaligned_vectors(kw):
+    assert _call(0, **kw) == -1
+    assert _call(1, **kw) == -1
+    assert _call(1, dloss=8 * P + 2) == -1
+    assert _call(1, dbias=8 * P + 1) == -1
+    assert _call(1, dbias=8 * P + 2, grad_f32=1) == -1
+
+
 def test_linear_ce_workspace():
     def need(grad, **kw):
         n = C.c_size_t()

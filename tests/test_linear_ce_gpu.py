@@ -517,6 +517,14 @@ def test_weights_of_every_kind(n, d, v):
         assert not torch.isfinite(dh[k]).any()
 
 
+def test_an_expanded_gradient_of_the_loss():
+    """What autograd hands back for a mean: one number with a stride of 0."""
+    h, w, b, t, _ = make(150, 64, 700, seed=44, ignored=9)
+    want = ops.linear_ce_grad(*dev(h, w, t), bias=dev(b)[0], dloss=torch.full((150,), 0.125, device=DEV))
+    got = ops.linear_ce_grad(*dev(h, w, t), bias=dev(b)[0], dloss=torch.tensor(0.125, device=DEV).expand(150))
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 def test_wrappers_refuse():
     h, w, b, t, dl = dev(*make(20, 64, 100))
     bad = [lambda: ops.linear_ce(h.float(), w, t), lambda: ops.linear_ce(h, w.half(), t), lambda: ops.linear_ce(h, w, t.int()),
