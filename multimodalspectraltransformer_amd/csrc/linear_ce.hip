@@ -457,7 +457,8 @@ __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_
 }
 
 // Both products in one launch, where both have small tiles: n workgroups (a multiple of 8, so that the others' XCDs are what
-// their numbers say) for dh, the others for dw.  PRODUCTS_MEASURED
+// their numbers say) for dh, the others for dw.  All of the gradient of 4032 x 128 x 43: 42 us with a launch each and 36 with one; of 2000 x
+// 128 x 8000: 80 and 65; of 3032 x 128 x 32000: 203 and, with parts for 256 workgroups of each, 167.
 __global__ __launch_bounds__(256, 1) void ce_products_kernel(const CeGemm dh, const CeGemm dw, int n) {
   __shared__ __attribute__((aligned(1024))) unsigned char smem[CeTile<DW, 128, 128, 2, 2>::SMEM];
   if ((int)blockIdx.x < n) ce_product<DH, 128, 128, 2, 2>(dh, blockIdx.x, n, (lds_byte*)smem);
@@ -1198,11 +1199,13 @@ bool large_tiles(long n, long m) {
 // 311 / 300 us, 24 (1400 x 1024 x 50001) 533 / 548 us, 128 (8192 x 1024 x 32000) 1696 / 1791 us.
 constexpr int DH_SMALL = 16;
 
-// Parts of a contraction: as many as keep every CU busy, of at least eight steps (of four: within 2 us either way).
-// Uncut: dh of 3000 x 128 x 32000 (16 parts; 8: 55 us, 16: 46) and dw of 4032 x 128 x 43 (7 parts; the whole gradient 72
-// us uncut and 45 in parts).
-int parts(long t, bool big, long contraction) {
-  const long slots = big ? TILE_GRID : 2 * TILE_GRID, steps = contraction / 64;
+// Parts of a contraction: as many as make the product's share of the workgroups that run at once, each of at least eight steps
+// (of four: within 2 us either way).  `slots`: one workgroup per CU with large tiles; with small ones two, or one of each
+// product where both are in one launch.  All of the gradient of 4032 x 128 x 43: 72 us with dw uncut, 45 in 7 parts (in launches
+// of their own); of 3032 x 128 x 32000 in one launch: 189 us for 128 slots each, 167 for 256, 197 for 512; of 333 x 1024 x
+// 50001: 196, 181, 203.
+int parts(long t, long slots, long contraction) {
+  const long steps = contraction / 64;
   long s = t < slots ? slots / (t ? t : 1) : 1;
   if (s > steps / 8) s = steps / 8;
   return (int)(s < 1 ? 1 : s > 32 ? 32 : s);
@@ -1240,8 +1243,9 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
     p.stream = streams(rows, a);
     p.big_dh = tiles(rows, a->D, 256) > DH_SMALL;
     p.big_dw = large_tiles(a->V, a->D);
-    p.split_dh = parts(tiles(rows, a->D, p.big_dh ? 256 : 128), p.big_dh, a->V);
-    p.split_dw = parts(tiles(a->V, a->D, p.big_dw ? 256 : 128), p.big_dw, rows);
+    const long slots = p.big_dh == p.big_dw ? TILE_GRID : 2 * TILE_GRID;   // of a small product: both run at once, or it alone
+    p.split_dh = parts(tiles(rows, a->D, p.big_dh ? 256 : 128), p.big_dh ? TILE_GRID : slots, a->V);
+    p.split_dw = parts(tiles(a->V, a->D, p.big_dw ? 256 : 128), p.big_dw ? TILE_GRID : slots, rows);
   }
   size_t at = 256;   // count, unit
   auto take = [&](size_t n) { const size_t o = at; at += align(n); return o; };
