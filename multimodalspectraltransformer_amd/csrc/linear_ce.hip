@@ -467,10 +467,11 @@ __global__ __launch_bounds__(256, 1) void ce_products_kernel(const CeGemm dh, co
 
 // ---------------------------------------------------------------------------------------------------- logits, tile by tile
 // A workgroup walks over tiles of the logits (one workgroup per CU with large tiles, two with small ones); the first steps of
-// the next tile's contraction are requested before this tile's softmax, which a wave does for its 64 columns alone.
-// LOGIT_STATS: (max, sum of exponentials) per row and 64 words.  LOGIT_EXP: these, and the exponentials themselves.  8192 x
+// the next tile's contraction are requested before this tile's softmax, which a wave does for its 64 columns (or 160) alone.
+// LOGIT_STATS: (max, sum of exponentials) per row and 64 words (160).  LOGIT_EXP: these, and the exponentials themselves.  8192 x
 // 2048 x 65536: 2.09 ms with the exponentials, 1.05 PFLOP/s, bound by the matrix units and, for 1.1 GB of exponentials at
-// the ends of the tiles, by the softmax that nothing multiplies beside; 333 x 1024 x 50001 (three rounds of small tiles): 50 us.
+// the ends of the tiles, by the softmax that nothing multiplies beside; 333 x 1024 x 50001: 48 us in two rounds of 128 x
+// 160, 54 in three of 128 x 128.
 template <int MODE, int BP, int BQ, int WP, int WQ>
 __global__ __launch_bounds__(WP * WQ * 64, 2) void ce_logits_kernel(const CeGemm a) {
   using Tile = CeTile<MODE, BP, BQ, WP, WQ>;
@@ -541,9 +542,10 @@ __global__ __launch_bounds__(WP * WQ * 64, 2) void ce_logits_kernel(const CeGemm
         for (int mt = 0; mt < MT; ++mt) acc[mt][2 * tp + (e >> 2)][e & 3] += b;
       }
     const int base = q0 + qw0 + 8 * j4;
+    auto mine = [&](int word) { return (unsigned)(word - base) < NT * 16u && ((word - base) & 24) == 0; };   // 32 tp + 0..7
     bool any = false;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) any |= ((target[mt] - base) & ~39) == 0;   // the lane's columns are 0..7 and 32..39 of the wave's
+    for (int mt = 0; mt < MT; ++mt) any |= mine(target[mt]);
     const bool targets = __ballot(any) != 0;
     float mx[MT];
 #pragma unroll
@@ -561,7 +563,7 @@ __global__ __launch_bounds__(WP * WQ * 64, 2) void ce_logits_kernel(const CeGemm
         for (int tp = 0; tp < NT / 2; ++tp)
 #pragma unroll
           for (int e = 0; e < 8; ++e) x = target[mt] - base == tp * 32 + e ? acc[mt][2 * tp + (e >> 2)][e & 3] : x;
-        if (((target[mt] - base) & ~39) == 0 && m < rows) a.tlogit[m] = x;
+        if (mine(target[mt]) && m < rows) a.tlogit[m] = x;
       }
     }
 #pragma unroll
@@ -1149,7 +1151,7 @@ struct CePlan {
   long rows;          // per piece, a multiple of 256
   int pieces, split_dh, split_dw;
   bool stream, whole; // logits: ce_stream_kernel; with the loss in it
-  bool big;           // or tiles of 256 x 256 (otherwise 128 x 128)
+  bool big, wide;     // or tiles of 256 x 256, of 128 x 160 (loss); otherwise 128 x 128
   bool big_dh, big_dw;
   long Vp;
   size_t index, words, tlogit, lse, weight, part, hc, g, slab_dh, slab_dw, slab_bias, dwacc, dbacc, total;
@@ -1184,14 +1186,26 @@ size_t align(size_t x) { return (x + 255) & ~(size_t)255; }
 
 long tiles(long n, long m, int b) { return ((n + b - 1) / b) * ((m + b - 1) / b); }
 
-// 256 x 256 tiles, one workgroup per CU, or 128 x 128, two: whichever is done first.  A round of the small ones (512, half as
-// much work) takes 7 / 13 of a round of the large ones, whose steps feed the matrix units better; what a last, partly filled
-// round wastes decides.  Measured, large / small: the loss at 2048 x 1024 x 16384 (rows, width, words; 2 rounds against 4)
-// 70 / 78 us, at 333 x 1024 x 50001 (2 against 3) 68 / 55 us; all of the gradient with dw by either at 8192 x 1024 x 32000 (2
-// against 4) 1696 / 1820 us, at 4096 x 256 x 8192 (1 against 1) 192 / 158 us.
-bool large_tiles(long n, long m) {
-  auto rounds = [](long t, long slots) { return (t + slots - 1) / slots; };
-  return 13 * rounds(tiles(n, m, 256), TILE_GRID) <= 7 * rounds(tiles(n, m, 128), 2 * TILE_GRID);
+// 256 x 256 tiles, one workgroup per CU, or 128 x 128, two: whichever is done first.  A round of the small ones (512 tiles,
+// half as much work) takes 14 / 26 of a round of the large ones, whose steps feed the matrix units better, and three fifths of
+// that where no CU has more than one; what a last, partly filled round wastes decides.  Measured, large / small: the loss at
+// 2048 x 1024 x 16384 (rows, width, words; 2 rounds against 4) 70 / 78 us, at 333 x 1024 x 50001 (2 against 2 and 149 tiles) 68 /
+// 55 us; all of the gradient with dw by either at 8192 x 1024 x 32000 (2 against 4) 1696 / 1820 us, at 4096 x 256 x 8192 (1
+// against 128 tiles) 192 / 158 us.
+long fifths(long t) {   // of a round of two workgroups per CU
+  const long rest = t % (2 * TILE_GRID);
+  return t / (2 * TILE_GRID) * 5 + (rest == 0 ? 0 : rest <= TILE_GRID ? 3 : 5);
+}
+long cost_large(long n, long m) { return 26 * 5 * ((tiles(n, m, 256) + TILE_GRID - 1) / TILE_GRID); }
+long cost_small(long n, long m) { return 14 * fifths(tiles(n, m, 128)); }
+bool large_tiles(long n, long m) { return cost_large(n, m) <= cost_small(n, m); }
+
+// For the loss alone also 128 rows x 160 words, whose rounds take 17 / 26: measured, 160 words / 128: 333 x 1024 x 50001 (2 rounds)
+// 47 / 51 us, 1000 x 1024 x 50001 (5 against 6 and 56 tiles) 107 / 111; against 256 x 256 at 1400 x 1024 x 50001 (7 against 5) 147
+// / 159.
+bool wide_tiles(long n, long m) {
+  const long wide = 17 * fifths((n + 127) / 128 * ((m + 159) / 160));
+  return wide < cost_large(n, m) && wide < cost_small(n, m);
 }
 
 // dh has the vocabulary as its contraction, which is cut into parts where there are too few tiles; the more parts, the more
@@ -1239,6 +1253,7 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
   p.pieces = all ? (int)((all + p.rows - 1) / p.rows) : 1;
   const long rows = a->N < p.rows ? a->N : p.rows;
   p.big = large_tiles(rows, a->V);
+  p.wide = !grad && wide_tiles(rows, a->V);
   if (grad) {
     p.stream = streams(rows, a);
     p.big_dh = tiles(rows, a->D, 256) > DH_SMALL;
@@ -1301,8 +1316,13 @@ int launch_products(CeGemm& dh, CeGemm& dw, const CePlan& p, hipStream_t st) {
   return MMST_OK;
 }
 template <int MODE> void launch_logits(CeGemm& g, const CePlan& p, hipStream_t st) {
-  const int b = p.big ? 256 : 128;
+  const int b = p.wide ? 160 : p.big ? 256 : 128;
   g.qtiles = (g.Qn + b - 1) / b;
+  if constexpr (MODE == LOGIT_STATS)
+    if (p.wide) {
+      hipLaunchKernelGGL((ce_logits_kernel<MODE, 128, 160, 4, 1>), dim3(2 * TILE_GRID), dim3(256), 0, st, g);
+      return;
+    }
   if (p.big) hipLaunchKernelGGL((ce_logits_kernel<MODE, 256, 256, 2, 4>), dim3(TILE_GRID), dim3(512), 0, st, g);
   else hipLaunchKernelGGL((ce_logits_kernel<MODE, 128, 128, 2, 2>), dim3(2 * TILE_GRID), dim3(256), 0, st, g);
 }
@@ -1335,7 +1355,8 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
   const bf16* w = (const bf16*)A.w;
   const int D = A.D, V = A.V, N = A.N, D8 = D / 8;
 
-  const int pairs = p.big ? (V + 255) / 256 * 4 : (V + 127) / 128 * 2;   // per row: one per 64 words
+  // per row: one per 64 words, or 160
+  const int pairs = p.wide ? (V + 159) / 160 : p.big ? (V + 255) / 256 * 4 : (V + 127) / 128 * 2;
   CeGemm logit = {};
   logit.Q = w; logit.ldq = A.ldw; logit.Qn = V; logit.K = D; logit.ksplit = 1;
   logit.bias = A.bias; logit.target = A.target;

@@ -525,6 +525,20 @@ def test_an_expanded_gradient_of_the_loss():
     assert all(torch.equal(x, y) for x, y in zip(got, want))
 
 
+@pytest.mark.parametrize("n,d,v", [(333, 136, 50001), (300, 200, 50000)])
+def test_loss_of_wide_tiles(n, d, v):
+    """Tiles of 160 words: targets in every part of them, masked words, an odd end."""
+    h, w, b, t, _ = make(n, d, v, seed=n, ignored=n // 10)
+    b[:170] = float("-inf")
+    b[v // 2] = torch.finfo(torch.float32).min
+    t[t >= 0] = t[t >= 0].clamp(min=170)
+    t[:160] = 10400 + torch.arange(160)   # every column of a tile
+    t[200], t[201] = v, v - 1
+    o = oracle(h, w, b, t, None)
+    check_loss(o, *ops.linear_ce(*dev(h, w, t), bias=dev(b)[0]))
+    check_loss(oracle(h, w, None, t, None), *ops.linear_ce(*dev(h, w, t)))
+
+
 def test_wrappers_refuse():
     h, w, b, t, dl = dev(*make(20, 64, 100))
     bad = [lambda: ops.linear_ce(h.float(), w, t), lambda: ops.linear_ce(h, w.half(), t), lambda: ops.linear_ce(h, w, t.int()),
