@@ -350,9 +350,9 @@ __device__ __forceinline__ void tile_of(int id, int ptiles, int qtiles, int& pt,
 
 // ---------------------------------------------------------------------------------------------------- products with g
 // dh of a piece or dw, one tile per workgroup.  Bound by the matrix units at the clock that the card's power leaves them:
-// 8192 x 2048 x 65536 takes 1.88 ms for dh and 1.83 ms for dw, 1.17 and 1.20 PFLOP/s in 256 x 256 tiles (2.15 and 2.2 ms with
-// four waves of 128 x 128 each, that issue their DMA, read and multiply one after another).  In narrow layers (3032 x 128 x
-// 32000: 40 and 46 us) by reading g.
+// 8192 x 2048 x 65536 takes 1.81 ms for dh and 1.76 ms for dw, 1.21 and 1.25 PFLOP/s in 256 x 256 tiles (2.15 and 2.2 ms with
+// four waves of 128 x 128 each, that issue their DMA, read and multiply one after another).  In narrow layers by reading g: 3032
+// x 128 x 32000 takes 66 us for both, 388 MB at 5.9 TB/s.
 // block: the workgroup's number of n
 template <int MODE, int BP, int BQ, int WP, int WQ>
 __device__ __forceinline__ void ce_product(const CeGemm& a, int block, int n, lds_byte* lds) {
@@ -469,9 +469,9 @@ __global__ __launch_bounds__(256, 1) void ce_products_kernel(const CeGemm dh, co
 // A workgroup walks over tiles of the logits (one workgroup per CU with large tiles, two with small ones); the first steps of
 // the next tile's contraction are requested before this tile's softmax, which a wave does for its 64 columns (or 160) alone.
 // LOGIT_STATS: (max, sum of exponentials) per row and 64 words (160).  LOGIT_EXP: these, and the exponentials themselves.  8192 x
-// 2048 x 65536: 2.09 ms with the exponentials, 1.05 PFLOP/s, bound by the matrix units and, for 1.1 GB of exponentials at
-// the ends of the tiles, by the softmax that nothing multiplies beside; 333 x 1024 x 50001: 48 us in two rounds of 128 x
-// 160, 54 in three of 128 x 128.
+// 2048 x 65536: 2.02 ms with the exponentials, 1.09 PFLOP/s, bound by the matrix units and, for 1.1 GB of exponentials at
+// the ends of the tiles, by the softmax that nothing multiplies beside; 333 x 1024 x 50001: 45 us in two rounds of 128 x
+// 160, 50 in three of 128 x 128.
 template <int MODE, int BP, int BQ, int WP, int WQ>
 __global__ __launch_bounds__(WP * WQ * 64, 2) void ce_logits_kernel(const CeGemm a) {
   using Tile = CeTile<MODE, BP, BQ, WP, WQ>;
