@@ -445,8 +445,8 @@ int mmst_layer_norm_bwd_ws(int dtype, long rows, int cols, size_t* bytes);
  * sum_n grad_scale dloss[n] loss[n], the gradients dh, dw and dbias.
  *   - rows whose target is ignore_index do not count: loss, lse and dh 0, nothing in dw, whatever h holds there, and no
  *     work in the products.  A target that is no word and not ignore_index gives loss and lse NaN and no gradient.
- *   - masked words: bias may be -infinity or any low number.  A row whose every
- *     logit is -infinity has lse -infinity, loss +infinity and no gradient.
+ *   - masked words: bias may be -infinity or any low number.  A row whose every logit is -infinity has lse -infinity, loss
+ *     +infinity and no gradient.
  *   - h, w, dh, dw rows 16-byte aligned; D a multiple of 8.  dw [V][D] and dbias [V] (both without a stride) in bf16,
  *     overwritten, or with grad_f32 in fp32, added to (as the other parameter gradients of this library).  All sums run in
  *     a fixed order: equal calls give equal bits.

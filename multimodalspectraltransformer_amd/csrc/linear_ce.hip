@@ -57,8 +57,9 @@ struct CeGemm {
   const float* bias; const int64_t* target; const int* index;
   const int* word;                   // the targets of the rows that count (gradient; NULL: target[row])
   float2* part; float* tlogit;       // per 64 words and row: max, sum of exp; the target's logit
-  const float2* lse; const float* weight; const float* unit; bf16* g; long ldg;   // lse: the row's maximum, and log2 of its sum of exponentials;
-                                     // weight: of the rows' losses in g, relative to *unit
+  const float2* lse;                 // the row's maximum, and log2 of its sum of exponentials
+  const float* weight;               // of the rows' losses in g, relative to *unit
+  const float* unit; bf16* g; long ldg;
   float* loss_out; float* lse_out; int64_t ignore;   // LOGIT_LOSS
   // products
   void* out; long ldo; int out_f32; int accumulate;   // out_f32: fp32, else bf16; accumulate: added to
@@ -82,7 +83,7 @@ template <bool T, bool QSIDE, int B, int NTHR, int BK> struct Operand {
   static constexpr int PIECES = B * BK / 8, NI = PIECES / NTHR;   // 16-byte pieces; DMA instructions per thread and step
   static constexpr int BYTES = B * BK * 2, ROW = BK / 8;          // pieces per row (!T)
   static constexpr uint32_t OUT = 0xFFFFFFF0u;
-  static_assert(PIECES % NTHR == 0 && (BK == 32 || BK == 64), "tile shape");
+  static_assert(PIECES % NTHR == 0 && BK == 64, "tile shape");
   uint32_t off[NI];
   const bf16* base;
   long ld;
@@ -92,8 +93,7 @@ template <bool T, bool QSIDE, int B, int NTHR, int BK> struct Operand {
   // a fragment reads 16 rows: r0 + i (P), r0 + 8 (i >> 2) + 4 half + (i & 3) (Q); 64 banks of 4 bytes
   static __device__ __forceinline__ int key(int r) {
     if constexpr (T) return (r & 3) | (((r >> 3) & 1) << 2);
-    else if constexpr (BK == 64) return QSIDE ? (r & 3) | (((r >> 3) & 1) << 2) : r & 7;
-    else return QSIDE ? (r >> 3) & 3 : (r >> 2) & 3;
+    else return QSIDE ? (r & 3) | (((r >> 3) & 1) << 2) : r & 7;
   }
   static __device__ __forceinline__ int piece(int slot) { const int r = slot / ROW; return (slot % ROW) ^ key(r); }   // (!T)
 
@@ -457,8 +457,8 @@ __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_
 }
 
 // Both products in one launch, where both have small tiles: n workgroups (a multiple of 8, so that the others' XCDs are what
-// their numbers say) for dh, the others for dw.  All of the gradient of 4032 x 128 x 43: 42 us with a launch each and 36 with one; of 2000 x
-// 128 x 8000: 80 and 65; of 3032 x 128 x 32000: 203 and, with parts for 256 workgroups of each, 167.
+// their numbers say) for dh, the others for dw.  All of the gradient of 4032 x 128 x 43: 42 us with a launch each and 36 with
+// one; of 2000 x 128 x 8000: 80 and 65; of 3032 x 128 x 32000: 203 and, with parts for 256 workgroups of each, 167.
 __global__ __launch_bounds__(256, 1) void ce_products_kernel(const CeGemm dh, const CeGemm dw, int n) {
   __shared__ __attribute__((aligned(1024))) unsigned char smem[CeTile<DW, 128, 128, 2, 2>::SMEM];
   if ((int)blockIdx.x < n) ce_product<DH, 128, 128, 2, 2>(dh, blockIdx.x, n, (lds_byte*)smem);
@@ -505,7 +505,8 @@ __global__ __launch_bounds__(WP * WQ * 64, 2) void ce_logits_kernel(const CeGemm
     float raw[NT / 2][8];
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      const f32x4 v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(bias_rsrc, (q0 + qw0 + 8 * j4) * 4 + (i >> 1) * 128 + (i & 1) * 16, 0, 0));
+      const int at = (q0 + qw0 + 8 * j4) * 4 + (i >> 1) * 128 + (i & 1) * 16;
+      const f32x4 v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(bias_rsrc, at, 0, 0));
 #pragma unroll
       for (int e = 0; e < 4; ++e) raw[i >> 1][(i & 1) * 4 + e] = v[e];
     }
@@ -732,7 +733,8 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
   float raw[NT / 2][8];
   const __amdgpu_buffer_rsrc_t bias_rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)a.bias, 0, a.bias ? a.Qn * 4 : 0, 0x00020000);
   auto load_bias = [&](int q, int i) {   // instruction i of four
-    const f32x4 v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(bias_rsrc, (q * 128 + qw0 + 8 * j4) * 4 + (i >> 1) * 128 + (i & 1) * 16, 0, 0));
+    const int at = (q * 128 + qw0 + 8 * j4) * 4 + (i >> 1) * 128 + (i & 1) * 16;
+    const f32x4 v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(bias_rsrc, at, 0, 0));
 #pragma unroll
     for (int e = 0; e < 4; ++e) raw[i >> 1][(i & 1) * 4 + e] = v[e];
   };
@@ -742,14 +744,16 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
   bf16x8 pf[MT][KS];
   auto load_rows = [&](int p) {   // (no branch around a load: each would be waited for before the next)
     const int left = rows - p * 128, n = left < 128 ? left : 128;
-    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(a.P + (long)p * 128 * a.ldp), 0, ((n - 1) * (int)a.ldp + a.K) * 2, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(a.P + (long)p * 128 * a.ldp), 0,
+                                                                          ((n - 1) * (int)a.ldp + a.K) * 2, 0x00020000);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       const int r = pw0 + mt * 16 + i16, m = p * 128 + (r < n ? r : n - 1);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const int k = ks * 32 + 8 * j4;
-        pf[mt][ks] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rsrc, k < a.K ? (r * (int)a.ldp + k) * 2 : (int)OpQ::OUT, 0, 0));
+        const int at = k < a.K ? (r * (int)a.ldp + k) * 2 : (int)OpQ::OUT;
+        pf[mt][ks] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, 0));
       }
       target[mt] = a.word ? a.word[m] : (int)(a.target[m] >= 0 && a.target[m] < a.Qn ? a.target[m] : -1);
       if (MODE == LOGIT_GRAD) {
@@ -1020,8 +1024,9 @@ __global__ __launch_bounds__(1024) void ce_index_kernel(const int64_t* target, i
 // of the rows that do not count, 16 rows each.
 __global__ __launch_bounds__(256) void ce_gather_kernel(const bf16* h, long ldh, int D8, const int* index, const int* count,
                                                         int row0, int rows_max, const float* dloss, float scale, bf16* out,
-                                                        float* weight, const float* unit, unsigned gather, const int64_t* target, int64_t ignore,
-                                                        int N, int V, bf16* dh, long lddh) {
+                                                        float* weight, const float* unit, unsigned gather,
+                                                        const int64_t* target, int64_t ignore, int N, int V, bf16* dh,
+                                                        long lddh) {
   if (blockIdx.x >= gather) {
     const long n = (long)(blockIdx.x - gather) * 16 + (threadIdx.x >> 4);
     if (n >= N) return;

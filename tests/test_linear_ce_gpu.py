@@ -539,6 +539,39 @@ def test_loss_of_wide_tiles(n, d, v):
     check_loss(oracle(h, w, None, t, None), *ops.linear_ce(*dev(h, w, t)))
 
 
+@pytest.mark.parametrize("n,d,v", [(3, 32768, 70), (2, 8, 1 << 22), (2, 1032, 1 << 18), (1, 8, 1)])
+def test_largest_widths_and_vocabularies(n, d, v):
+    h, w, b, t, dl = make(n, d, v, seed=45)
+    t[-1] = v - 1
+    o = oracle(h, w, b, t, dl)
+    out = ops.linear_ce_grad(*dev(h, w, t), bias=dev(b)[0], dloss=dev(dl)[0])
+    check_loss(o, *out[:2])
+    check_grad(o, *out[2:])
+    check_loss(o, *ops.linear_ce(*dev(h, w, t), bias=dev(b)[0]))
+
+
+def test_the_most_rows():
+    """2^24 rows, in two pieces: first and last ones by value, every row's loss against the sum of its equal copies."""
+    n, d, v = 1 << 24, 8, 5
+    h, w, b, t, _ = make(1 << 10, d, v, seed=46, ignored=100)
+    many = n >> 10
+    o = oracle(h, w, b, t, torch.ones(1 << 10))
+    hd, td = h.to(DEV).repeat(many, 1), t.to(DEV).repeat(many)
+    s = torch.zeros(v, d, device=DEV), torch.zeros(v, device=DEV)
+    loss, lse, dh, _, _ = ops.linear_ce_grad(hd, w.to(DEV), td, bias=b.to(DEV), dw=s[0], dbias=s[1])
+    for rows in (slice(0, 1 << 10), slice(n - (1 << 10), n)):
+        check_loss(o, loss[rows], lse[rows])
+        inside(dh[rows], o["dh"], o["ddh"] + o["dh"].abs() * HALF * 1.01, "dh")
+    assert torch.equal(loss.view(many, -1), loss[:1 << 10].expand(many, -1))
+    assert torch.equal(dh.view(many, -1), dh[:1 << 10].reshape(-1).expand(many, -1))
+    # a piece of 2^23 rows is summed in 32 parts: at most 2^18 roundings in a row, each of the magnitudes' sum
+    z = h.double() @ w.double().t() + b.double()
+    g = ((torch.softmax(z, 1) - torch.nn.functional.one_hot(t.clamp(min=0), v)) * (t != IGN)[:, None]).abs()
+    inside(s[1] / many, o["db"], o["ddb"] + (2 ** 18 + 100) * U * g.sum(0), "dbias")
+    check_loss(o, *(x[-(1 << 10):] for x in ops.linear_ce(hd, w.to(DEV), td, bias=b.to(DEV))))
+    torch.cuda.empty_cache()
+
+
 def test_wrappers_refuse():
     h, w, b, t, dl = dev(*make(20, 64, 100))
     bad = [lambda: ops.linear_ce(h.float(), w, t), lambda: ops.linear_ce(h, w.half(), t), lambda: ops.linear_ce(h, w, t.int()),
