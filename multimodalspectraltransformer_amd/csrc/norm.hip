@@ -48,27 +48,37 @@ struct DropArgs {
   DropKey key;
 };
 
-// blocks of eight elements that lie inside one row; FLAT: rows follow one another.  37248 x 2048 in bf16: 56 us, 5.4 TB/s, as
-// fast as a copy; two blocks per lane of a 16-bit type keep 32 bytes per lane in flight as one does of fp32.
-template <typename T, bool FLAT, int U>
+// A lane owns blocks of eight elements.  FLAT: rows follow one another, and the tensor is one row.  ROWS: rows of a multiple of
+// eight elements, a block lies inside one.  ANY: of eight elements or more; a block may begin in one row and end in the next, and goes
+// by elements then.  37248 x 2048 in bf16 (FLAT): 56 us, 5.4 TB/s, as fast as a copy; two blocks per lane of a 16-bit type keep
+// 32 bytes per lane in flight as one does of fp32.
+enum { FLAT = 0, ROWS = 1, ANY = 2 };
+template <typename T, int MODE, int U>
 __global__ __launch_bounds__(256) void dropout_vec_kernel(const DropArgs a) {
-  const uint64_t nb = a.n >> 3, per_row = a.cols >> 3;
+  const uint64_t nb = MODE == ANY ? (a.n + 7) >> 3 : a.n >> 3;
   const uint64_t b0 = (a.wg0 + blockIdx.x) * (256 * U) + threadIdx.x;
   Vec8<T> in[U];
-  uint64_t oy[U];
+  uint64_t ox[U], oy[U];
+  int left[U];   // elements before the end of the row (ANY)
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const uint64_t b = b0 + 256 * u;
     if (b >= nb) continue;
-    uint64_t ox = b << 3;
-    oy[u] = ox;
-    if constexpr (!FLAT) {
-      const uint64_t r = (nb >> 32) ? b / per_row : (uint64_t)((uint32_t)b / (uint32_t)per_row);
-      const uint64_t c = (b - r * per_row) << 3;
-      ox = r * a.ldx + c;
+    ox[u] = oy[u] = b << 3;
+    left[u] = 8;
+    if constexpr (MODE != FLAT) {
+      const uint64_t i = b << 3, r = (a.n >> 32) ? i / a.cols : (uint64_t)((uint32_t)i / (uint32_t)a.cols), c = i - r * a.cols;
+      ox[u] = r * a.ldx + c;
       oy[u] = r * a.ldy + c;
+      if constexpr (MODE == ANY) left[u] = a.cols - c < 8 ? (int)(a.cols - c) : 8;
     }
-    load_vec(in[u], (const T*)a.x + ox);
+    if (MODE != ANY || left[u] == 8) {
+      load_vec(in[u], (const T*)a.x + ox[u]);
+    } else {
+      const T* p = (const T*)a.x + ox[u];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) in[u].v[e] = (b << 3) + e < a.n ? p[e < left[u] ? (uint64_t)e : e + a.ldx - a.cols] : (T)0.f;
+    }
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -78,9 +88,16 @@ __global__ __launch_bounds__(256) void dropout_vec_kernel(const DropArgs a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = (float)in[u].v[e];
     if (a.key.thr) drop_block(v, philox_block(b, a.key), a.key);
-    store_vec((T*)a.y + oy[u], v);
+    if (MODE != ANY || left[u] == 8) {
+      store_vec((T*)a.y + oy[u], v);
+    } else {
+      T* p = (T*)a.y + oy[u];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if ((b << 3) + e < a.n) p[e < left[u] ? (uint64_t)e : e + a.ldy - a.cols] = (T)v[e];
+    }
   }
-  if constexpr (FLAT) {   // the last n % 8 elements
+  if constexpr (MODE == FLAT) {   // the last n % 8 elements
     const uint64_t i = (nb << 3) + threadIdx.x;
     if (blockIdx.x == 0 && a.wg0 == 0 && i < a.n) {
       const uint4 w = philox_block(nb, a.key);
@@ -92,8 +109,8 @@ __global__ __launch_bounds__(256) void dropout_vec_kernel(const DropArgs a) {
   }
 }
 
-// rows of an odd width that do not follow one another, so that a block may lie in two or more: a wave owns 512 consecutive
-// elements, a lane one element per access (1023 x 4099 of fp32, rows 4112 apart: 8.7 us, 3.9 TB/s)
+// short rows of an odd width that do not follow one another, so that a block may lie in two or more: a wave owns 512
+// consecutive elements, a lane one element per access
 template <typename T>
 __global__ __launch_bounds__(256) void dropout_elem_kernel(const DropArgs a) {
   __shared__ uint4 slots[4][65];
@@ -124,15 +141,21 @@ __global__ __launch_bounds__(256) void dropout_elem_kernel(const DropArgs a) {
     if (first + j * 64 + lane < a.n) ((T*)a.y)[oy[j]] = (T)v[j];
 }
 
+// Rows of an odd width and a stride of their own: blocks from 32 columns of a 16-bit type and 128 of fp32 on, where few enough of
+// them lie in two rows, single elements below.  Blocks / elements: bf16 17 columns 52 / 48 us, 41 39 / 46, 4099 25 / 46 (of 33 to
+// 36 M elements), fp32 65 columns 55 / 43, 101 39.5 / 38, 501 39 / 43, 4099 41 / 44.
+template <typename T> constexpr uint64_t any_cols() { return sizeof(T) == 2 ? 32 : 128; }
+
 template <typename T> int launch_dropout(DropArgs& a, hipStream_t st) {
-  const bool flat = a.ldx == a.cols && a.ldy == a.cols, vec = flat || a.cols % 8 == 0;
+  const bool flat = a.ldx == a.cols && a.ldy == a.cols, rows = a.cols % 8 == 0, any = a.cols >= any_cols<T>();
   constexpr int U = sizeof(T) == 4 ? 1 : 2;
-  const uint64_t all = vec ? (a.n / 8 + 256 * U - 1) / (256 * U) : (a.n + 2047) / 2048, most = 1u << 20;
+  const uint64_t all = flat || rows || any ? (a.n / 8 + 256 * U) / (256 * U) : (a.n + 2047) / 2048, most = 1u << 20;
   do {   // (a launch has less than 2^32 threads)
     const uint64_t left = all - a.wg0;
-    const dim3 grid(left > most ? (unsigned)most : left ? (unsigned)left : 1u);
-    if (flat) hipLaunchKernelGGL((dropout_vec_kernel<T, true, U>), grid, dim3(256), 0, st, a);
-    else if (vec) hipLaunchKernelGGL((dropout_vec_kernel<T, false, U>), grid, dim3(256), 0, st, a);
+    const dim3 grid(left > most ? (unsigned)most : (unsigned)left);
+    if (flat) hipLaunchKernelGGL((dropout_vec_kernel<T, FLAT, U>), grid, dim3(256), 0, st, a);
+    else if (rows) hipLaunchKernelGGL((dropout_vec_kernel<T, ROWS, U>), grid, dim3(256), 0, st, a);
+    else if (any) hipLaunchKernelGGL((dropout_vec_kernel<T, ANY, U>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((dropout_elem_kernel<T>), grid, dim3(256), 0, st, a);
     MMST_CHECK_LAUNCH();
     a.wg0 += most;

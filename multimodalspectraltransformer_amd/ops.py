@@ -177,6 +177,8 @@ def _rows(t, like, name, out=False):
     cols = shape[-1]
     if t.is_contiguous():
         return t, cols
+    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= cols:
+        return t, t.stride(0)
     if t.stride(-1) == 1 or cols == 1:
         try:
             flat = t.view(-1, cols)

@@ -88,6 +88,25 @@ def test_dropout_strided_in_place_and_unaligned(t, cols, pad, lead):
     inside(ops.dropout(flat[1:], 0.3, 11), want.reshape(-1), tol.reshape(-1), "unaligned start")
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows,cols,pad", [(1003, 31, 2), (1003, 33, 1), (517, 127, 5), (517, 129, 3), (2, 4099, 13), (301, 257, 1), (9, 9, 9), (1, 130, 1)])
+def test_dropout_of_odd_rows(t, rows, cols, pad):
+    """Blocks of eight elements that begin in one row and end in the next, and the widths at which they are taken."""
+    x = rnd(rows, cols, seed=rows).to(t)
+    want = x.double() * factor(x.shape, 0.3, 11, 5)
+    tol = want.abs() * (2 * U + half(t)) + tiny(t)
+    wide = torch.full((rows + 1, cols + pad), float("nan"), dtype=t, device=DEV)
+    out = wide[:rows, :cols]
+    xs = strided(x, pad + 2)
+    ops.dropout(xs, 0.3, 11, 5, out=out)
+    inside(out, want, tol, "strided")
+    assert wide[:, cols:].isnan().all() and wide[rows:].isnan().all()
+    ops.dropout(xs, 0.3, 11, 5, out=xs)
+    inside(xs, want, tol, "in place")
+    y = ops.dropout(strided(x, pad + 2), 0.0, 11)
+    assert torch.equal(y.cpu(), x)
+
+
 def test_dropout_clears_infinities_and_nan():
     x = torch.full((64, 128), float("nan"), device=DEV)
     x[::2] = float("inf")
