@@ -7,9 +7,9 @@
 //               dgamma = sum over rows of dy xh,  dbeta = sum over rows of dy
 //
 // All of it is bound by HBM: every tensor is read or written once and a row stays in registers between the statistics and
-// the output.  TPR lanes own a row (16 lanes for 128 columns up to a workgroup of 1024 for 16384), NV groups of eight
-// columns each, so that a lane's accesses are 16 bytes wide, whatever their alignment; only the last group of a row whose
-// width is no multiple of eight goes by elements.
+// the output.  TPR lanes own a row (4 lanes for 32 columns up to a workgroup of 1024 for 16384), NV groups of eight
+// columns each, so that a lane's accesses are 16 bytes wide, whatever their alignment; the last group of a row whose width
+// is no multiple of eight is read as the last eight columns and moved.
 #include "../../include/mmst.h"
 #include "philox.h"
 
@@ -179,7 +179,11 @@ struct LnArgs {
 // sum over the TPR lanes that own a row, on all of them; wider than a wave: through LDS, two buffers in turn, so that one
 // barrier per sum is enough (a buffer is written again only behind the next sum's barrier)
 template <int TPR, int BLK> __device__ __forceinline__ float row_sum(float v, float (*red)[BLK / 64], int& turn) {
-  if constexpr (TPR == 16) return row16_sum(v);
+  if constexpr (TPR == 4) {
+    v += dpp_f32<0xB1>(v);
+    return v + dpp_f32<0x4E>(v);
+  } else if constexpr (TPR == 8) return row8_sum(v);
+  else if constexpr (TPR == 16) return row16_sum(v);
   else if constexpr (TPR == 32) return xor16_sum(row16_sum(v));
   else {
     v = wave_sum(v);
@@ -196,51 +200,92 @@ template <int TPR, int BLK> __device__ __forceinline__ float row_sum(float v, fl
   }
 }
 
-// Group q of lane t of a row: columns (q * TPR + t) * 8 .. + 7.  ODD: cols is no multiple of eight, so one lane's last
-// group is cut off.
+// Group q of lane t of a row: columns (q * TPR + t) * 8 .. + 7.  ODD: cols is no multiple of eight, so one lane's last group is
+// cut off.  It is loaded as the row's last eight columns, so that nothing behind the row is read, and moved down by the columns
+// that belong to the lane before (ln_fix, when the loads of all tensors are under way: moving needs them).  Column by column:
+// 153 us instead of 52 for the backward pass of 262000 x 127 in bf16.
+template <int N> __device__ __forceinline__ void words_down(uint32_t (&w)[N], int by, bool go) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) w[i] = go ? (i + by < N ? w[i + by] : 0u) : w[i];
+}
+template <typename T> __device__ __forceinline__ void move_down(Vec8<T>& d, int n) {   // n: 1..7 elements, the same in every lane
+  constexpr int N = sizeof(Vec8<T>) / 4;
+  uint32_t w[N];
+  __builtin_memcpy(w, &d, sizeof d);
+  words_down(w, N / 2, n & 4);
+  words_down(w, N / 4, n & 2);
+  if constexpr (N == 8) {
+    words_down(w, 1, n & 1);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = n & 1 ? __builtin_amdgcn_alignbit(i + 1 < N ? w[i + 1] : 0u, w[i], 16) : w[i];
+  }
+  __builtin_memcpy(&d, w, sizeof d);
+}
+template <bool ODD> __device__ __forceinline__ int cut_off(int c, int cols) {   // columns that the group at c lacks
+  return ODD && c + 8 > cols && cols >= 8 ? c + 8 - cols : 0;
+}
+template <typename T, bool ODD> __device__ __forceinline__ void load_group(Vec8<T>& d, const T* row, int c, int cols) {
+  if (!ODD || cols >= 8) {
+    load_vec(d, row + c - cut_off<ODD>(c, cols));
+  } else {   // a row of less than eight columns
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+      if (e < cols) d.v[e] = row[e];
+  }
+}
 template <typename T, bool ODD, int TPR, int NV>
 __device__ __forceinline__ void ln_load(Vec8<T> (&d)[NV], const T* row, int cols, int t, bool ok) {
 #pragma unroll
   for (int q = 0; q < NV; ++q) {
     const int c = (q * TPR + t) * 8;
-    if (ok && c + (ODD ? 7 : 0) < cols) {
-      load_vec(d[q], row + c);
-    } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) d[q].v[e] = (T)0.f;
-      if (ODD && ok && c < cols)
-#pragma unroll
-        for (int e = 0; e < 7; ++e)
-          if (c + e < cols) d[q].v[e] = row[c + e];
-    }
+    for (int e = 0; e < 8; ++e) d[q].v[e] = (T)0.f;
+    if (ok && c < cols) load_group<T, ODD>(d[q], row, c, cols);
   }
+}
+template <typename T, bool ODD, int TPR, int NV> __device__ __forceinline__ void ln_fix(Vec8<T> (&d)[NV], int cols, int t) {
+  if constexpr (ODD)
+#pragma unroll
+    for (int q = 0; q < NV; ++q) {
+      const int c = (q * TPR + t) * 8;
+      if (c < cols && cut_off<ODD>(c, cols)) move_down(d[q], 8 - (cols & 7));
+    }
 }
 template <typename T, bool ODD, int TPR>
 __device__ __forceinline__ void ln_store(T* row, const float (&v)[8], int cols, int q, int t) {
   const int c = (q * TPR + t) * 8;
   if (c + (ODD ? 7 : 0) < cols) {
     store_vec(row + c, v);
-  } else if (ODD && c < cols) {
+  } else if (ODD && c < cols) {   // four, two and one columns
+    const int n = cols & 7;
+    T* p = row + c;
+    float w[4] = {v[0], v[1], v[2], v[3]};
+    if (n & 4) {
 #pragma unroll
-    for (int e = 0; e < 7; ++e)
-      if (c + e < cols) row[c + e] = (T)v[e];
+      for (int e = 0; e < 4; ++e) { p[e] = (T)w[e]; w[e] = v[4 + e]; }
+      p += 4;
+    }
+    if (n & 2) {
+      p[0] = (T)w[0];
+      p[1] = (T)w[1];
+      w[0] = w[2];
+      p += 2;
+    }
+    if (n & 1) p[0] = (T)w[0];
   }
 }
 template <bool ODD, int TPR>
 __device__ __forceinline__ void ln_vec_f32(float (&v)[8], const float* p, float none, int cols, int q, int t) {
   const int c = (q * TPR + t) * 8;
-  if (p && c + (ODD ? 7 : 0) < cols) {
-    Vec8<float> d;
-    load_vec(d, p + c);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = none;
+  if (p && c < cols) {
+    Vec8<float> d = {};
+    load_group<float, ODD>(d, p, c, cols);
+    if (cut_off<ODD>(c, cols)) move_down(d, 8 - (cols & 7));
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = d.v[e];
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = none;
-    if (ODD && p && c < cols)
-#pragma unroll
-      for (int e = 0; e < 7; ++e)
-        if (c + e < cols) v[e] = p[c + e];
   }
 }
 // dropout of group q of row r, whose elements are r * cols + column of the tensor read row by row
@@ -268,6 +313,8 @@ __global__ __launch_bounds__(BLK) void ln_fwd_kernel(const LnArgs a) {
     Vec8<T> x[NV], rs[NV];
     ln_load<T, ODD, TPR, NV>(x, (const T*)a.x + r * a.ldx, cols, t, ok);
     if (a.res) ln_load<T, ODD, TPR, NV>(rs, (const T*)a.res + r * a.ldr, cols, t, ok);
+    ln_fix<T, ODD, TPR, NV>(x, cols, t);
+    if (a.res) ln_fix<T, ODD, TPR, NV>(rs, cols, t);
     float z[NV][8];
     float s = 0.f;
 #pragma unroll
@@ -328,6 +375,9 @@ __global__ __launch_bounds__(BLK) void ln_bwd_kernel(const LnArgs a) {
     ln_load<T, ODD, TPR, NV>(zv, (const T*)a.zin + r * a.ldzin, cols, t, ok);
     if (a.res) ln_load<T, ODD, TPR, NV>(add, (const T*)a.res + r * a.ldr, cols, t, ok);
     const float mean = ok ? a.stats[2 * r] : 0.f, rstd = ok ? a.stats[2 * r + 1] : 0.f;
+    ln_fix<T, ODD, TPR, NV>(dy, cols, t);
+    ln_fix<T, ODD, TPR, NV>(zv, cols, t);
+    if (a.res) ln_fix<T, ODD, TPR, NV>(add, cols, t);
     float xh[NV][8], qv[NV][8];
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
@@ -419,30 +469,33 @@ __global__ __launch_bounds__(1024) void ln_cols_kernel(const float* part, int n,
 
 struct LnShape { int tpr, nv, blk, grid; };
 
-// Lanes per row: as few as hold it in one access each (16 for 128 columns: 45 us for 262144 x 128 bf16 with a residual, 32
-// lanes 58), two accesses before a row goes over several waves (32768 x 1024: 42 us, one access of 128 lanes in a workgroup of
-// 256 49), four before a workgroup of 1024 (8192 x 4096: 43 us, 1024 lanes 79; 4096 x 8192: 44 and 57).  6 TB/s of bf16, 5 of
-// fp32.  Workgroups take rows in turn beyond 4096 (2048: up to 10 % slower for odd widths, which wait longer per row).
+// Lanes per row: as few as hold it with a few accesses each, so that a wave has several rows' loads in flight and few idle
+// lanes.  Forward with a residual, bf16, one shape / the next: 1000000 x 24 4 lanes 32 us, 16 90; 524288 x 64 8 lanes 45, 16 59;
+// 262144 x 128 16 lanes 45, 32 58; 60000 x 520 32 lanes with three accesses 43, 64 with two 50; 25000 x 1200 64 lanes with three
+// 39, 256 with one 47; 16000 x 2048 256 with one 41, 64 with four 42; 8000 x 4099 256 with three 67, with four 92; 4096 x 8192
+// 256 with four 44, 1024 with two 57.  6 TB/s of bf16 and 5 of fp32 at even widths that fill their lanes.  Workgroups take rows
+// in turn beyond 4096 (2048: up to 10 % slower for odd widths, which wait longer per row).
 LnShape ln_fwd_shape(long rows, int cols) {
   LnShape s;
   s.blk = cols <= 8192 ? 256 : 1024;
-  s.tpr = cols <= 128 ? 16 : cols <= 256 ? 32 : cols <= 1024 ? 64 : cols <= 8192 ? 256 : 1024;
-  s.nv = cols <= 512 ? 1 : cols <= 1024 ? 2 : cols <= 2048 ? 1 : cols <= 4096 ? 2 : cols <= 8192 ? 4 : 2;
+  s.tpr = cols <= 32 ? 4 : cols <= 64 ? 8 : cols <= 128 ? 16 : cols <= 768 ? 32 : cols <= 1536 ? 64 : cols <= 8192 ? 256 : 1024;
+  s.nv = (cols + s.tpr * 8 - 1) / (s.tpr * 8);
+  if (s.tpr == 1024) s.nv = 2;
   const long need = (rows + s.blk / s.tpr - 1) / (s.blk / s.tpr);
   s.grid = (int)(need < 4096 ? need : 4096);
   return s;
 }
 // The backward pass keeps two sums per column besides the row, and each workgroup leaves them for ln_cols_kernel: two
 // workgroups of 256 per CU, or one of 1024 (four and two: 5 % faster to 7 % slower, and 15 to 45 % slower from 4096 columns on,
-// where the sums themselves are most of what is written).  Up to 1024 columns a wave per row with two accesses (32768 x 1024
-// bf16: 38 us; four waves of a larger workgroup 49).  Beyond, two accesses per lane only where the 128 registers of a 1024-lane
+// where the sums themselves are most of what is written).  Up to 1536 columns lanes as above, in a wave (60000 x 520
+// bf16: 32 lanes with three accesses 38 us, 64 with two 43; 25000 x 1200: 64 with three 35, 256 of a larger workgroup 42).  Beyond, two accesses per lane only where the 128 registers of a 1024-lane
 // workgroup hold that (16-bit types, even widths: 8192 x 4096 39 us, 42 with one; 4096 x 8192 43 and 53), or where there is no
 // wider workgroup.
 LnShape ln_bwd_shape(long rows, int cols, int dtype) {
   LnShape s;
   const bool one = cols % 8 || dtype == MMST_F32;
-  s.blk = cols <= 1024 ? 256 : 1024;
-  s.tpr = cols <= 128 ? 16 : cols <= 256 ? 32 : cols <= 1024 ? 64 : cols <= 2048 ? 256 : cols <= 4096 ? (one ? 512 : 256)
+  s.blk = cols <= 1536 ? 256 : 1024;
+  s.tpr = cols <= 32 ? 4 : cols <= 64 ? 8 : cols <= 128 ? 16 : cols <= 768 ? 32 : cols <= 1536 ? 64 : cols <= 2048 ? 256 : cols <= 4096 ? (one ? 512 : 256)
         : cols <= 8192 ? (one ? 1024 : 512) : 1024;
   s.nv = (cols + s.tpr * 8 - 1) / (s.tpr * 8);
   const long need = (rows + s.blk / s.tpr - 1) / (s.blk / s.tpr), most = s.blk == 256 ? 512 : 256;
@@ -454,28 +507,39 @@ LnShape ln_bwd_shape(long rows, int cols, int dtype) {
   if (s.tpr == TPR && s.nv == NV && s.blk == BLK) {                                                 \
     if (a.cols % 8) hipLaunchKernelGGL((K<T, true, TPR, NV, BLK>), dim3(s.grid), dim3(BLK), 0, st, a); \
     else hipLaunchKernelGGL((K<T, false, TPR, NV, BLK>), dim3(s.grid), dim3(BLK), 0, st, a);        \
-    return;                                                                                         \
+    return true;                                                                                    \
   }
 #define LN_WIDE(TPR)                                                                                 \
   if (s.tpr == TPR && s.nv == 2) {                                                                  \
     hipLaunchKernelGGL((ln_bwd_kernel<T, false, TPR, 2, 1024>), dim3(s.grid), dim3(1024), 0, st, a); \
-    return;                                                                                         \
+    return true;                                                                                    \
   }
-template <typename T> void launch_ln_fwd(const LnArgs& a, const LnShape& s, hipStream_t st) {
+// (false: a shape without a kernel)
+template <typename T> bool launch_ln_fwd(const LnArgs& a, const LnShape& s, hipStream_t st) {
+  LN_CASE(ln_fwd_kernel, 4, 1, 256)
+  LN_CASE(ln_fwd_kernel, 8, 1, 256)
   LN_CASE(ln_fwd_kernel, 16, 1, 256)
   LN_CASE(ln_fwd_kernel, 32, 1, 256)
-  LN_CASE(ln_fwd_kernel, 64, 1, 256)
+  LN_CASE(ln_fwd_kernel, 32, 2, 256)
+  LN_CASE(ln_fwd_kernel, 32, 3, 256)
   LN_CASE(ln_fwd_kernel, 64, 2, 256)
+  LN_CASE(ln_fwd_kernel, 64, 3, 256)
   LN_CASE(ln_fwd_kernel, 256, 1, 256)
   LN_CASE(ln_fwd_kernel, 256, 2, 256)
+  LN_CASE(ln_fwd_kernel, 256, 3, 256)
   LN_CASE(ln_fwd_kernel, 256, 4, 256)
   LN_CASE(ln_fwd_kernel, 1024, 2, 1024)
+  return false;
 }
-template <typename T> void launch_ln_bwd(const LnArgs& a, const LnShape& s, hipStream_t st) {
+template <typename T> bool launch_ln_bwd(const LnArgs& a, const LnShape& s, hipStream_t st) {
+  LN_CASE(ln_bwd_kernel, 4, 1, 256)
+  LN_CASE(ln_bwd_kernel, 8, 1, 256)
   LN_CASE(ln_bwd_kernel, 16, 1, 256)
   LN_CASE(ln_bwd_kernel, 32, 1, 256)
-  LN_CASE(ln_bwd_kernel, 64, 1, 256)
+  LN_CASE(ln_bwd_kernel, 32, 2, 256)
+  LN_CASE(ln_bwd_kernel, 32, 3, 256)
   LN_CASE(ln_bwd_kernel, 64, 2, 256)
+  LN_CASE(ln_bwd_kernel, 64, 3, 256)
   LN_CASE(ln_bwd_kernel, 256, 1, 1024)
   LN_CASE(ln_bwd_kernel, 1024, 2, 1024)
   if constexpr (sizeof(T) == 2)
@@ -485,6 +549,7 @@ template <typename T> void launch_ln_bwd(const LnArgs& a, const LnShape& s, hipS
     }
   LN_CASE(ln_bwd_kernel, 512, 1, 1024)
   LN_CASE(ln_bwd_kernel, 1024, 1, 1024)
+  return false;
 }
 #undef LN_CASE
 #undef LN_WIDE
@@ -521,9 +586,9 @@ int mmst_layer_norm(const void* x, long ldx, const void* residual, long ldr, con
   LnArgs a{x, residual, nullptr, gamma, beta, y, z, stats, nullptr, rows, cols, ldx, ldr, 0, ldy, ldz,
            eps, 1.0f / (float)cols, drop_key(p, seed, offset)};
   const LnShape s = ln_fwd_shape(rows, cols);
-  if (dtype == MMST_F32) launch_ln_fwd<float>(a, s, (hipStream_t)stream);
-  else if (dtype == MMST_BF16) launch_ln_fwd<bf16>(a, s, (hipStream_t)stream);
-  else launch_ln_fwd<f16>(a, s, (hipStream_t)stream);
+  const hipStream_t st = (hipStream_t)stream;
+  if (!(dtype == MMST_F32 ? launch_ln_fwd<float>(a, s, st) : dtype == MMST_BF16 ? launch_ln_fwd<bf16>(a, s, st) : launch_ln_fwd<f16>(a, s, st)))
+    return MMST_ERR_LAUNCH;
   MMST_CHECK_LAUNCH();
   return MMST_OK;
 }
@@ -550,9 +615,9 @@ int mmst_layer_norm_bwd(const void* dy, long lddy, const void* z, long ldz, cons
       return MMST_ERR_ARG;
     LnArgs a{dy, dz_in, z, gamma, nullptr, dz, dx, const_cast<float*>(stats), sums ? (float*)ws : nullptr, rows, cols,
              lddy, lddz_in, ldz, lddz, lddx, 0.f, 1.0f / (float)cols, key};
-    if (dtype == MMST_F32) launch_ln_bwd<float>(a, s, (hipStream_t)stream);
-    else if (dtype == MMST_BF16) launch_ln_bwd<bf16>(a, s, (hipStream_t)stream);
-    else launch_ln_bwd<f16>(a, s, (hipStream_t)stream);
+    const hipStream_t st = (hipStream_t)stream;
+    if (!(dtype == MMST_F32 ? launch_ln_bwd<float>(a, s, st) : dtype == MMST_BF16 ? launch_ln_bwd<bf16>(a, s, st) : launch_ln_bwd<f16>(a, s, st)))
+      return MMST_ERR_LAUNCH;
     MMST_CHECK_LAUNCH();
   }
   if (sums) {

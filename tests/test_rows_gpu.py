@@ -246,6 +246,28 @@ def test_layer_norm_bwd(t, cols):
         check_backward(dy, z, stats, g, a, p, got)
 
 
+# on both sides of every change of the number of lanes per row and of the accesses per lane
+EDGES = [3, 8, 9, 24, 31, 32, 33, 63, 64, 65, 127, 129, 255, 256, 257, 300, 511, 513, 768, 769, 777, 1025, 1536, 1537, 2047, 2049, 4095,
+         4097, 6144, 6145, 8191]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("cols", EDGES)
+def test_layer_norm_at_the_edges_of_its_shapes(t, cols):
+    rows = 9 if cols > 1024 else 77
+    x, res, dy = (rnd(rows, cols, seed=cols + i, scale=1.5, shift=0.3).to(t) for i in range(3))
+    gamma, beta = 1 + 0.3 * rnd(cols, seed=5), 0.3 * rnd(cols, seed=6)
+    # rows apart, and nothing but NaN between them
+    xs, rs, ds = strided(x, 5), strided(res, 3, 1), strided(dy, 8, 8)
+    y, z, stats = ops.layer_norm(xs, gamma.to(DEV), beta.to(DEV), residual=rs, p=0.2, seed=SEED, offset=OFFSET)
+    check_forward(x, res, gamma, beta, 0.2, y, z, stats)
+    wide = torch.full((rows, cols + 2), float("nan"), dtype=t, device=DEV)
+    again = ops.layer_norm(xs, gamma.to(DEV), beta.to(DEV), residual=rs, p=0.2, seed=SEED, offset=OFFSET, out=wide[:, 1:-1])
+    assert torch.equal(again[0], y) and wide[:, 0].isnan().all() and wide[:, -1].isnan().all()
+    got = ops.layer_norm_bwd(ds, z, stats, gamma.to(DEV), dz_in=rs, p=0.2, seed=SEED, offset=OFFSET)
+    check_backward(dy, z.cpu(), stats.cpu(), gamma, res, 0.2, got)
+
+
 @pytest.mark.parametrize("rows,cols", [(1, 128), (3, 200), (5000, 64), (4100, 1000), (1500, 1536)])
 def test_layer_norm_many_rows_both_passes(rows, cols):
     """More rows than one sweep of the grid; the backward pass from what the forward pass returned."""
