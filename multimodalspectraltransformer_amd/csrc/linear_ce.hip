@@ -44,7 +44,7 @@ __device__ __forceinline__ float unpack_exp(uint32_t w, int upper) {
   return __builtin_bit_cast(float, (upper ? w >> 2 : w << 14) & 0x3FFFC000u);
 }
 
-enum { LOGIT_STATS = 0, LOGIT_GRAD = 1, DH = 2, DW = 3, LOGIT_EXP = 4, LOGIT_LOSS = 5 };
+enum { LOGIT_STATS = 0, LOGIT_GRAD = 1, DH = 2, DW = 3, LOGIT_EXP = 4, LOGIT_LOSS = 5, LOGIT_PART = 6 };
 
 struct CeGemm {
   const bf16* P; const bf16* Q;      // operands; the token / vocabulary side of the output's rows, and its columns
@@ -63,7 +63,8 @@ struct CeGemm {
   float* loss_out; float* lse_out; int64_t ignore;   // LOGIT_LOSS
   // products
   void* out; long ldo; int out_f32; int accumulate;   // out_f32: fp32, else bf16; accumulate: added to
-  const float* acc_in; float* slab; float* slab_bias;   // slabs: [ksplit][Pn][Qn], [ksplit][Pn]
+  const float* acc_in; float* slab; float* slab_bias;   // slabs: [ksplit][Pn][ldslab], [ksplit][Pn]
+  int ldslab;
   void* dbias; const float* dbias_in;                 // DW: sums of g over the rows, in out's type; added to dbias_in
 };
 
@@ -156,11 +157,11 @@ template <bool T, bool QSIDE, int B, int NTHR, int BK> struct Operand {
   }
 };
 
-template <int MODE, int BP, int BQ, int WP, int WQ>
+template <int MODE, int BP, int BQ, int WP, int WQ, int STAGES = 2>
 struct CeTile {
   static constexpr int NW = WP * WQ, NTHR = NW * 64, MT = BP / WP / 16, NT = BQ / WQ / 16;
   static constexpr bool TP = MODE == DW, TQ = MODE == DH || MODE == DW;
-  static constexpr int BK = 64, NS = 2;   // a step of the contraction; stages
+  static constexpr int BK = 64, NS = STAGES;   // a step of the contraction; stages of LDS
   using OpP = Operand<TP, false, BP, NTHR, BK>;
   using OpQ = Operand<TQ, true, BQ, NTHR, BK>;
   static constexpr int STAGE = OpP::BYTES + OpQ::BYTES, SMEM = NS * STAGE;
@@ -310,12 +311,20 @@ struct CeTile {
   static __device__ __forceinline__ void steps(Acc<SUM>& acc, const OpP& p, const OpQ& q, lds_byte* lds, int kbeg, int nsteps,
                                                int tid, int wave, int pw0, int qw0, int lane) {
     if constexpr (NW != 8) {
+      int rd = 0, wr = NS - 1;
       for (int s = 0; s < nsteps; ++s) {
-        // this wave's share of step s has landed; behind the barrier everybody's has, and nobody reads the other stage
-        if (s) asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-        step(acc, p, q, lds + ((s + 1) & 1) * STAGE, lds + (s & 1) * STAGE, s + 1 < nsteps, kbeg + (s + 1) * BK, tid, wave,
-             pw0, qw0, lane);
+        // this wave's share of step s has landed; behind the barrier everybody's has, and nobody reads the stage of step s - 1
+        if (s) {
+          dma_done();
+          asm volatile("s_barrier" ::: "memory");
+        }
+        // (two stages: nothing is requested behind the last step; more: always, so that what is in flight can be counted)
+        step(acc, p, q, lds + wr * STAGE, lds + rd * STAGE, NS > 2 || s + 1 < nsteps, kbeg + (s + NS - 1) * BK, tid, wave, pw0,
+             qw0, lane);
+        wr = rd;
+        rd = rd + 1 == NS ? 0 : rd + 1;
       }
+      if constexpr (NS > 2) all_done();
       barrier();
     } else {
       int rd = 0, wr = NS - 1;
@@ -354,9 +363,9 @@ __device__ __forceinline__ void tile_of(int id, int ptiles, int qtiles, int& pt,
 // four waves of 128 x 128 each, that issue their DMA, read and multiply one after another).  In narrow layers by reading g: 3032
 // x 128 x 32000 takes 66 us for both, 388 MB at 5.9 TB/s.
 // block: the workgroup's number of n
-template <int MODE, int BP, int BQ, int WP, int WQ>
+template <int MODE, int BP, int BQ, int WP, int WQ, int STAGES = 2>
 __device__ __forceinline__ void ce_product(const CeGemm& a, int block, int n, lds_byte* lds) {
-  using Tile = CeTile<MODE, BP, BQ, WP, WQ>;
+  using Tile = CeTile<MODE, BP, BQ, WP, WQ, STAGES>;
   constexpr int MT = Tile::MT, NT = Tile::NT;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int id;   // consecutive tiles to one XCD (workgroups go round the eight of them)
@@ -373,7 +382,7 @@ __device__ __forceinline__ void ce_product(const CeGemm& a, int block, int n, ld
   const int rows = piece_rows(a);
   const int p0 = pt * BP, q0 = qt * BQ;
   const int K = MODE == DW ? rows : a.K, Pn = MODE == DW ? a.Pn : rows;
-  if (MODE == DH && p0 >= rows) return;
+  if (MODE != DW && p0 >= rows) return;
   int kbeg = 0, nsteps = (K + Tile::BK - 1) / Tile::BK;
   if (a.ksplit > 1) {
     const int s0 = (int)((long)nsteps * ks_id / a.ksplit), s1 = (int)((long)nsteps * (ks_id + 1) / a.ksplit);
@@ -422,10 +431,10 @@ __device__ __forceinline__ void ce_product(const CeGemm& a, int block, int n, ld
 #pragma unroll
     for (int tp = 0; tp < NT / 2; ++tp) {
       const int c = q0 + qw0 + tp * 32 + 8 * j4;
-      if (c >= a.Qn) continue;   // (Qn is a multiple of 8)
+      if (c >= a.Qn) continue;   // (Qn is a multiple of 8, or the slabs' rows are padded to one)
       f32x4 lo = acc[mt][2 * tp] * unit, hi = acc[mt][2 * tp + 1] * unit;
       if (a.slab) {
-        float* d = a.slab + ((size_t)ks_id * a.Pn + m) * a.Qn + c;
+        float* d = a.slab + ((size_t)ks_id * a.Pn + m) * a.ldslab + c;
         *reinterpret_cast<f32x4*>(d) = lo;
         *reinterpret_cast<f32x4*>(d + 4) = hi;
         continue;
@@ -450,10 +459,10 @@ __device__ __forceinline__ void ce_product(const CeGemm& a, int block, int n, ld
   }
 }
 
-template <int MODE, int BP, int BQ, int WP, int WQ>
+template <int MODE, int BP, int BQ, int WP, int WQ, int STAGES = 2>
 __global__ __launch_bounds__(WP * WQ * 64, WP * WQ * 64 == 512 ? 2 : 1) void ce_product_kernel(const CeGemm a) {
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[CeTile<MODE, BP, BQ, WP, WQ>::SMEM];
-  ce_product<MODE, BP, BQ, WP, WQ>(a, blockIdx.x, gridDim.x, (lds_byte*)smem);
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[CeTile<MODE, BP, BQ, WP, WQ, STAGES>::SMEM];
+  ce_product<MODE, BP, BQ, WP, WQ, STAGES>(a, blockIdx.x, gridDim.x, (lds_byte*)smem);
 }
 
 // Both products in one launch, where both have small tiles: n workgroups (a multiple of 8, so that the others' XCDs are what
@@ -472,9 +481,9 @@ __global__ __launch_bounds__(256, 1) void ce_products_kernel(const CeGemm dh, co
 // 2048 x 65536: 2.02 ms with the exponentials, 1.09 PFLOP/s, bound by the matrix units and, for 1.1 GB of exponentials at
 // the ends of the tiles, by the softmax that nothing multiplies beside; 333 x 1024 x 50001: 45 us in two rounds of 128 x
 // 160, 50 in three of 128 x 128.
-template <int MODE, int BP, int BQ, int WP, int WQ>
-__global__ __launch_bounds__(WP * WQ * 64, 2) void ce_logits_kernel(const CeGemm a) {
-  using Tile = CeTile<MODE, BP, BQ, WP, WQ>;
+template <int MODE, int BP, int BQ, int WP, int WQ, int STAGES = 2>
+__global__ __launch_bounds__(WP * WQ * 64, STAGES == 2 ? 2 : 1) void ce_logits_kernel(const CeGemm a) {
+  using Tile = CeTile<MODE, BP, BQ, WP, WQ, STAGES>;
   constexpr int MT = Tile::MT, NT = Tile::NT;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[Tile::SMEM];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -605,6 +614,44 @@ __global__ __launch_bounds__(WP * WQ * 64, 2) void ce_logits_kernel(const CeGemm
     id = next;
     pt = pt1;
     qt = qt1;
+  }
+}
+
+// Logits in parts of their contraction (LOGIT_PART: slabs, as of the other split products), for layers so wide and tiles so few
+// that the steps of one tile are what takes the time.  This joins them: 16 rows x 64 words per workgroup, four words per lane,
+// and leaves what the tiles leave otherwise.
+template <int MODE> __global__ __launch_bounds__(256) void ce_join_kernel(const CeGemm a) {
+  const int rows = piece_rows(a), m = blockIdx.y * 16 + (threadIdx.x >> 4), c = blockIdx.x * 64 + (threadIdx.x & 15) * 4;
+  if ((int)blockIdx.y * 16 >= rows) return;
+  const int r = m < rows ? m : rows - 1;
+  f32x4 x = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  if (c < a.Qn) {
+    const float* p = a.slab + (size_t)r * a.ldslab + c;
+    const size_t stride = (size_t)a.Pn * a.ldslab;
+    x = *reinterpret_cast<const f32x4*>(p);
+#pragma unroll 4
+    for (int k = 1; k < a.ksplit; ++k) x += *reinterpret_cast<const f32x4*>(p + k * stride);
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (c + e >= a.Qn) x[e] = -INFINITY;
+    else if (a.bias) x[e] += a.bias[c + e];
+  }
+  const int64_t t = a.word ? a.word[r] : a.target[r];
+  if (t >= c && t < c + 4 && t < a.Qn && m < rows) a.tlogit[m] = t == c ? x[0] : t == c + 1 ? x[1] : t == c + 2 ? x[2] : x[3];
+  const float mx = row16_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]))), at = mx == -INFINITY ? 0.f : mx;
+  float sum = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    x[e] = __builtin_amdgcn_exp2f((x[e] - at) * LOG2E);
+    sum += x[e];
+  }
+  sum = row16_sum(sum);
+  if (m >= rows) return;
+  if ((threadIdx.x & 15) == 0) a.part[(size_t)blockIdx.x * a.rows_max + m] = make_float2(mx, sum);
+  if constexpr (MODE == LOGIT_EXP) {
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    *reinterpret_cast<u32x2*>(a.g + (size_t)m * a.ldg + c) = u32x2{pack_exp(x[0], x[1]), pack_exp(x[2], x[3])};
   }
 }
 
@@ -1116,10 +1163,10 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(const float2* part, int ti
 template <int MODE> __device__ __forceinline__ void join_slabs(const CeGemm& a, long i) {
   const int D4 = a.Qn / 4, rows = MODE == DH ? piece_rows(a) : a.Pn;
   const long r = i / D4;
-  const size_t c = (size_t)(i - r * D4) * 4, stride = (size_t)a.Pn * a.Qn;
+  const size_t c = (size_t)(i - r * D4) * 4, stride = (size_t)a.Pn * a.ldslab;
   const float unit = *a.unit;
   if (r < rows) {
-    const float* p = a.slab + (size_t)r * a.Qn + c;
+    const float* p = a.slab + (size_t)r * a.ldslab + c;
     f32x4 s = *reinterpret_cast<const f32x4*>(p);
     for (int k = 1; k < a.ksplit; ++k) s += *reinterpret_cast<const f32x4*>(p + k * stride);
     s *= unit;
@@ -1157,9 +1204,11 @@ struct CePlan {
   int pieces, split_dh, split_dw;
   bool stream, whole; // logits: ce_stream_kernel; with the loss in it
   bool big, wide;     // or tiles of 256 x 256, of 128 x 160 (loss); otherwise 128 x 128
+  bool few;           // of these at most one per CU: four stages of LDS (loss of 200 x 4096 x 1000 uncut: 41 us, 46 with two)
+  int split_logits;   // or in parts of the contraction, joined by ce_join_kernel
   bool big_dh, big_dw;
   long Vp;
-  size_t index, words, tlogit, lse, weight, part, hc, g, slab_dh, slab_dw, slab_bias, dwacc, dbacc, total;
+  size_t index, words, tlogit, lse, weight, part, hc, g, slab_logits, slab_dh, slab_dw, slab_bias, dwacc, dbacc, total;
 };
 
 constexpr int STREAM_GRID = 512, TILE_GRID = 256;   // two workgroups per CU, one
@@ -1230,6 +1279,17 @@ int parts(long t, long slots, long contraction) {
   return (int)(s < 1 ? 1 : s > 32 ? 32 : s);
 }
 
+// Parts of the logits' contraction (`steps` of it) where t tiles leave most CUs idle: at least eight steps each, and more than 16
+// steps (of half a microsecond) fewer in a row, which pays for the join.  Loss, uncut / in parts: 64 x 4096 x 43 (8 parts) 41 / 17
+// us, 200 x 4096 x 1000 (8) 41 / 20, 16 x 2048 x 8000 (4) 27 / 18, 500 x 2000 x 3000 (2, 16 steps fewer) 26 / 28; with four steps
+// each, 16 parts, 200 x 4096 x 1000 takes 23.
+int logit_parts(long t, long steps) {
+  if (t == 0) return 1;
+  long s = TILE_GRID / t;
+  if (s > steps / 8) s = steps / 8;
+  return s >= 2 && steps - steps / s > 16 ? (int)s : 1;
+}
+
 // Narrow layers: the stream where a workgroup gets more than two tiles of it, for which it computes the logits twice and
 // reads no exponentials back.  Measured, stream / tiles, loss and gradient: 3000 x 128 x 8000 (1512 tiles) 19 / 23 and 93 / 97
 // us, 3000 x 128 x 32000 42 / 65 and 193 / 239, 2000 x 128 x 8000 (1008) 19 / 16 and 80 / 79, 512 x 128 x 4000 (128) 15 / 14
@@ -1257,10 +1317,12 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
   }
   p.pieces = all ? (int)((all + p.rows - 1) / p.rows) : 1;
   const long rows = a->N < p.rows ? a->N : p.rows;
+  if (grad) p.stream = streams(rows, a);
   p.big = large_tiles(rows, a->V);
   p.wide = !grad && wide_tiles(rows, a->V);
+  p.few = tiles(rows, a->V, 128) <= TILE_GRID;
+  p.split_logits = p.stream ? 1 : logit_parts(tiles(rows, a->V, 128), (a->D + 63) / 64);
   if (grad) {
-    p.stream = streams(rows, a);
     p.big_dh = tiles(rows, a->D, 256) > DH_SMALL;
     p.big_dw = large_tiles(a->V, a->D);
     const long slots = p.big_dh == p.big_dw ? TILE_GRID : 2 * TILE_GRID;   // of a small product: both run at once, or it alone
@@ -1269,6 +1331,7 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
   }
   size_t at = 256;   // count, unit
   auto take = [&](size_t n) { const size_t o = at; at += align(n); return o; };
+  if (p.split_logits > 1) p.slab_logits = take((size_t)p.split_logits * p.rows * ((a->V + 7) & ~7) * 4);
   p.tlogit = take(p.rows * 4);
   p.part = take(p.stream ? (size_t)(STREAM_GRID + 8 * (p.rows / 128)) * 2 * 128 * 8 : (size_t)pairs * p.rows * 8);
   if (grad) {
@@ -1298,6 +1361,7 @@ int launch_products(CeGemm& dh, CeGemm& dw, const CePlan& p, hipStream_t st) {
     const int b = big ? 256 : 128;
     g.ptiles = (g.Pn + b - 1) / b;
     g.qtiles = (g.Qn + b - 1) / b;
+    g.ldslab = g.Qn;
     return (unsigned)(g.ptiles * g.qtiles * g.ksplit);
   };
   const unsigned n = grid(dh, p.big_dh), m = grid(dw, p.big_dw);
@@ -1320,7 +1384,17 @@ int launch_products(CeGemm& dh, CeGemm& dw, const CePlan& p, hipStream_t st) {
   }
   return MMST_OK;
 }
-template <int MODE> void launch_logits(CeGemm& g, const CePlan& p, hipStream_t st) {
+template <int MODE> void launch_logits(CeGemm& g, const CePlan& p, char* ws, hipStream_t st) {
+  if (p.split_logits > 1) {
+    g.ptiles = (g.Pn + 127) / 128;
+    g.qtiles = (g.Qn + 127) / 128;
+    g.ksplit = p.split_logits;
+    g.slab = (float*)(ws + p.slab_logits);
+    g.ldslab = (g.Qn + 7) & ~7;
+    hipLaunchKernelGGL((ce_product_kernel<LOGIT_PART, 128, 128, 2, 2, 4>), dim3(g.ptiles * g.qtiles * g.ksplit), dim3(256), 0, st, g);
+    hipLaunchKernelGGL(ce_join_kernel<MODE>, dim3((g.Qn + 63) / 64, (g.Pn + 15) / 16), dim3(256), 0, st, g);
+    return;
+  }
   const int b = p.wide ? 160 : p.big ? 256 : 128;
   g.qtiles = (g.Qn + b - 1) / b;
   if constexpr (MODE == LOGIT_STATS)
@@ -1329,6 +1403,7 @@ template <int MODE> void launch_logits(CeGemm& g, const CePlan& p, hipStream_t s
       return;
     }
   if (p.big) hipLaunchKernelGGL((ce_logits_kernel<MODE, 256, 256, 2, 4>), dim3(TILE_GRID), dim3(512), 0, st, g);
+  else if (p.few) hipLaunchKernelGGL((ce_logits_kernel<MODE, 128, 128, 2, 2, 4>), dim3(TILE_GRID), dim3(256), 0, st, g);
   else hipLaunchKernelGGL((ce_logits_kernel<MODE, 128, 128, 2, 2>), dim3(2 * TILE_GRID), dim3(256), 0, st, g);
 }
 template <int MODE> void launch_stream(CeGemm& g, hipStream_t st) {
@@ -1361,7 +1436,7 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
   const int D = A.D, V = A.V, N = A.N, D8 = D / 8;
 
   // per row: one per 64 words, or 160
-  const int pairs = p.wide ? (V + 159) / 160 : p.big ? (V + 255) / 256 * 4 : (V + 127) / 128 * 2;
+  const int pairs = p.split_logits > 1 ? (V + 63) / 64 : p.wide ? (V + 159) / 160 : p.big ? (V + 255) / 256 * 4 : (V + 127) / 128 * 2;
   CeGemm logit = {};
   logit.Q = w; logit.ldq = A.ldw; logit.Qn = V; logit.K = D; logit.ksplit = 1;
   logit.bias = A.bias; logit.target = A.target;
@@ -1380,7 +1455,7 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
         return MMST_OK;
       }
       if (p.stream) launch_stream<LOGIT_STATS>(logit, st);
-      else launch_logits<LOGIT_STATS>(logit, p, st);
+      else launch_logits<LOGIT_STATS>(logit, p, ws, st);
       MMST_CHECK_LAUNCH();
       hipLaunchKernelGGL(ce_rows_kernel, dim3((rows + 15) / 16), dim3(256), 0, st, logit.part, pairs, rows,
                          p.stream ? STREAM_GRID : 0, nullptr, 0, rows, nullptr, logit.target, A.ignore_index, V, logit.tlogit,
@@ -1409,7 +1484,7 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
     logit.word = words + row0;
     logit.g = gbuf; logit.ldg = p.Vp;
     if (p.stream) launch_stream<LOGIT_STATS>(logit, st);
-    else launch_logits<LOGIT_EXP>(logit, p, st);
+    else launch_logits<LOGIT_EXP>(logit, p, ws, st);
     MMST_CHECK_LAUNCH();
     hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)(p.rows / 16)), dim3(256), 0, st, logit.part, pairs, rows_max,
                        p.stream ? STREAM_GRID : 0, count,

@@ -572,6 +572,30 @@ def test_the_most_rows():
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("n,d,v", [(70, 1032, 45), (200, 4096, 1001), (1, 2000, 300), (130, 1024, 129), (16, 2048, 8003), (600, 8192, 7)])
+def test_logits_in_parts_of_a_long_contraction(n, d, v):
+    h, w, b, t, dl = make(n, d, v, seed=n + d, ignored=n // 6)
+    if v > 40:
+        b[v // 3:v // 3 + 20], b[v - 1] = float("-inf"), -1e30
+        t[t >= 0] %= v // 3
+    if n > 60:
+        t[3], t[50] = v, -7
+        h[(t == IGN).nonzero()[0, 0]] = float("nan")
+    # the oracle's bound counts the mask's magnitude, which reaches nothing
+    b2 = torch.where(b < -1e20, torch.full_like(b, float("-inf")), b)
+    o = oracle(h, w, b2, t, dl)
+    out = ops.linear_ce_grad(*dev(h, w, t), bias=dev(b)[0], dloss=dev(dl)[0])
+    check_loss(o, *out[:2])
+    check_grad(o, *out[2:])
+    check_loss(o, *ops.linear_ce(*dev(h, w, t), bias=dev(b)[0]))
+    again = ops.linear_ce_grad(*dev(h, w, t), bias=dev(b)[0], dloss=dev(dl)[0])
+    assert all(torch.equal(x, y) or x.isnan().any() for x, y in zip(out, again))
+    none = torch.full((v,), float("-inf"))
+    out = ops.linear_ce_grad(*dev(h, w, t), bias=dev(none)[0])
+    keep = ((t >= 0) & (t < v)).to(DEV)
+    assert (out[1][keep] == float("-inf")).all() and (out[2] == 0).all() and (out[3] == 0).all()
+
+
 def test_wrappers_refuse():
     h, w, b, t, dl = dev(*make(20, 64, 100))
     bad = [lambda: ops.linear_ce(h.float(), w, t), lambda: ops.linear_ce(h, w.half(), t), lambda: ops.linear_ce(h, w, t.int()),
