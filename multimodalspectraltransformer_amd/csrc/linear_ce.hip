@@ -60,7 +60,7 @@ struct CeGemm {
   const float2* lse;                 // the row's maximum, and log2 of its sum of exponentials
   const float* weight;               // of the rows' losses in g, relative to *unit
   const float* unit; bf16* g; long ldg;
-  float* loss_out; float* lse_out; int64_t ignore;   // LOGIT_LOSS
+  float* loss_out; float* lse_out; int64_t ignore;   // LOGIT_LOSS; joining scale
   // products
   void* out; long ldo; int out_f32; int accumulate;   // out_f32: fp32, else bf16; accumulate: added to
   const float* acc_in; float* slab; float* slab_bias;   // slabs: [ksplit][Pn][ldslab], [ksplit][Pn]
@@ -658,10 +658,39 @@ template <int MODE> __global__ __launch_bounds__(256) void ce_join_kernel(const 
 // g from the exponentials of a piece, in place: a tile's times exp(its maximum - the row's lse) and the weight; of the target's
 // word from its logit, which is there in fp32.  Four rows per workgroup and 2048 columns, 16 bytes per lane; bound by HBM: 2.1
 // GB in 0.41 ms, 5.2 TB/s.
-__global__ __launch_bounds__(256) void ce_scale_kernel(const CeGemm a) {
+// JOIN: a wave first joins the pairs of one of the rows, which saves the launch of ce_rows_kernel; every 2048 columns do that
+// again, so only up to JOIN_VOCAB words.  All of the gradient, joined here / apart: 4032 x 128 x 43 35 / 37 us, 700 x 136 x 5000
+// 44 / 47, 1000 x 128 x 8000 49 / 54, 2000 x 136 x 16000 107 / 106, 1000 x 256 x 32000 121 / 114.
+template <bool JOIN> __global__ __launch_bounds__(256) void ce_scale_kernel(const CeGemm a, int pairs) {
+  __shared__ float2 joined[4];
   const int rows = piece_rows(a), across = (int)((a.ldg + 2047) / 2048), r0 = (int)(blockIdx.x / across) * 4;
   const int c = (int)(blockIdx.x % across) * 2048 + (int)threadIdx.x * 8;
-  if (r0 >= rows || c >= a.Qn) return;
+  if (r0 >= rows) return;   // (uniform)
+  if constexpr (JOIN) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = r0 + w;
+    if (r < rows) {
+      float m = -INFINITY, s = 0.f;
+      for (int q = lane; q < pairs; q += 64) {
+        const float2 p = a.part[(size_t)q * a.rows_max + r];
+        const float top = fmaxf(m, p.x), at = top == -INFINITY ? 0.f : top;
+        s = s * __builtin_amdgcn_exp2f((m - at) * LOG2E) + p.y * __builtin_amdgcn_exp2f((p.x - at) * LOG2E);
+        m = top;
+      }
+      const float top = wave_max(m), at = top == -INFINITY ? 0.f : top;
+      s = wave_sum(s * __builtin_amdgcn_exp2f((m - at) * LOG2E));
+      if (lane == 0) {
+        joined[w] = make_float2(top, log2f(s));
+        if (blockIdx.x % across == 0) {
+          const int n = a.index[r];
+          const float ls = logf(s), l = at + ls;
+          a.loss_out[n] = l == -INFINITY ? INFINITY : ls + (at - a.tlogit[r]);
+          if (a.lse_out) a.lse_out[n] = l;
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if (c >= a.Qn) return;
   u32x4 x[4];
   float scale[4], wt[4], gt[4];   // gt: g of the target's word, whose 1 would leave an exponential's last digits
   int hit[4];
@@ -669,7 +698,7 @@ __global__ __launch_bounds__(256) void ce_scale_kernel(const CeGemm a) {
   for (int i = 0; i < 4; ++i) {
     const int r = r0 + i < rows ? r0 + i : rows - 1;
     x[i] = *reinterpret_cast<const u32x4*>(a.g + (size_t)r * a.ldg + c);
-    const float2 l = a.lse[r];
+    const float2 l = JOIN ? joined[r - r0] : a.lse[r];
     wt[i] = a.weight[r];
     hit[i] = a.word[r] - c;
     // a row whose every logit is masked has no gradient
@@ -1266,6 +1295,7 @@ bool wide_tiles(long n, long m) {
 // fp32 slabs to write and read, and small tiles need half as many.  Measured, large / small: 16 tiles (2048 x 512 x 32000)
 // 311 / 300 us, 24 (1400 x 1024 x 50001) 533 / 548 us, 128 (8192 x 1024 x 32000) 1696 / 1791 us.
 constexpr int DH_SMALL = 16;
+constexpr int JOIN_VOCAB = 8192;
 
 // Parts of a contraction: as many as make the product's share of the workgroups that run at once, each of at least eight steps
 // (of four: within 2 us either way).  `slots`: one workgroup per CU with large tiles; with small ones two, or one of each
@@ -1486,13 +1516,19 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
     if (p.stream) launch_stream<LOGIT_STATS>(logit, st);
     else launch_logits<LOGIT_EXP>(logit, p, ws, st);
     MMST_CHECK_LAUNCH();
-    hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)(p.rows / 16)), dim3(256), 0, st, logit.part, pairs, rows_max,
-                       p.stream ? STREAM_GRID : 0, count,
-                       row0, rows_max, index, A.target, A.ignore_index, V, logit.tlogit, lse_c, A.loss, A.lse);
-    MMST_CHECK_LAUNCH();
     logit.lse = lse_c; logit.weight = weight;
-    if (p.stream) launch_stream<LOGIT_GRAD>(logit, st);
-    else hipLaunchKernelGGL(ce_scale_kernel, dim3((unsigned)((p.Vp + 2047) / 2048 * (p.rows / 4))), dim3(256), 0, st, logit);
+    logit.loss_out = A.loss; logit.lse_out = A.lse;
+    const dim3 scale((unsigned)((p.Vp + 2047) / 2048 * (p.rows / 4)));
+    if (p.stream || V > JOIN_VOCAB) {
+      hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)(p.rows / 16)), dim3(256), 0, st, logit.part, pairs, rows_max,
+                         p.stream ? STREAM_GRID : 0, count, row0, rows_max, index, A.target, A.ignore_index, V, logit.tlogit,
+                         lse_c, A.loss, A.lse);
+      MMST_CHECK_LAUNCH();
+      if (p.stream) launch_stream<LOGIT_GRAD>(logit, st);
+      else hipLaunchKernelGGL(ce_scale_kernel<false>, scale, dim3(256), 0, st, logit, pairs);
+    } else {
+      hipLaunchKernelGGL(ce_scale_kernel<true>, scale, dim3(256), 0, st, logit, pairs);
+    }
     MMST_CHECK_LAUNCH();
 
     CeGemm dh = {};
