@@ -1121,6 +1121,69 @@ __global__ __launch_bounds__(256) void ce_gather_kernel(const bf16* h, long ldh,
   reinterpret_cast<uint4*>(out)[(long)r * D8 + c] = reinterpret_cast<const uint4*>(h + (long)n * ldh)[c];
 }
 
+// Both of these in one launch, for few rows in one piece: a workgroup has 16 rows, 16 lanes each, and looks at all the
+// targets and weights itself, for the number of rows that count before its own and the largest weight: up to MERGE_ROWS, since that grows with their square.
+// All of the gradient, in one launch / in two: 64 x 128 x 43 24 / 27 us, 4032 x 128 x 43 32 / 35, 8192 x 1024 x 43 63 / 71, 16384 x
+// 128 x 43 61 / 64, 32768 x 128 x 43 98 / 96, 65536 x 128 x 43 211 / 150.
+__global__ __launch_bounds__(256) void ce_index_gather_kernel(const bf16* h, long ldh, int D8, const int64_t* target, int64_t ignore,
+                                                              int N, int V, const float* dloss, float scale, int* index, int* words,
+                                                              int* count, float* unit, float* weight, bf16* out, float* loss,
+                                                              float* lse, bf16* dh, long lddh) {
+  __shared__ int before_of[4], all_of[4];
+  __shared__ float top_of[4];
+  const int tid = threadIdx.x, w = tid >> 6, first = blockIdx.x * 16;
+  int before = 0, all = 0;
+  float largest = 0.f;   // (NaN does not count)
+#pragma unroll 4
+  for (int n = tid; n < N; n += 256) {
+    const int64_t t = target[n];
+    const float wt = fabsf(scale * (dloss ? dloss[n] : 1.f));
+    const bool keep = t != ignore && t >= 0 && t < V;
+    all += keep;
+    before += keep && n < first;
+    largest = fmaxf(largest, keep ? wt : 0.f);
+  }
+  const int lane = tid & 63;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    all += __shfl_xor(all, d);
+    before += __shfl_xor(before, d);
+  }
+  largest = wave_max(largest);
+  if (lane == 0) { all_of[w] = all; before_of[w] = before; top_of[w] = largest; }
+  __syncthreads();
+  largest = fmaxf(fmaxf(top_of[0], top_of[1]), fmaxf(top_of[2], top_of[3]));
+  const float most = largest > 0.f && largest < INFINITY ? largest : 1.f;   // (a weight of infinity stays with its row)
+  if (blockIdx.x == 0 && tid == 0) {
+    *count = all_of[0] + all_of[1] + all_of[2] + all_of[3];
+    *unit = most;
+  }
+  // lane i of each wave knows of row i: which of the 16 count
+  int64_t mine = ignore;
+  if (lane < 16 && first + lane < N) mine = target[first + lane];
+  const unsigned long long rows = __ballot(lane < 16 && first + lane < N && mine != ignore && mine >= 0 && mine < V);
+  const int r = tid >> 4, n = first + r;
+  if (n >= N) return;
+  const int64_t t = target[n];
+  if ((rows >> r) & 1) {
+    const int at = before_of[0] + before_of[1] + before_of[2] + before_of[3] + __popcll(rows & ((1ull << r) - 1));
+    if ((tid & 15) == 0) {
+      index[at] = n;
+      words[at] = (int)t;
+      weight[at] = scale * (dloss ? dloss[n] : 1.f) / most;
+    }
+    for (int c = tid & 15; c < D8; c += 16)
+      reinterpret_cast<uint4*>(out)[(long)at * D8 + c] = reinterpret_cast<const uint4*>(h + (long)n * ldh)[c];
+  } else {
+    if ((tid & 15) == 0) {
+      const float x = t == ignore ? 0.f : __builtin_nanf("");
+      loss[n] = x;
+      if (lse) lse[n] = x;
+    }
+    for (int c = tid & 15; c < D8; c += 16) reinterpret_cast<uint4*>(dh + (long)n * lddh)[c] = make_uint4(0, 0, 0, 0);
+  }
+}
+
 // A row's pairs (maximum, sum) -> lse and loss: 16 rows per workgroup, 16 lanes each.  The pairs are those
 // of every 64 words, [.][ld], or (grid != 0) those that the workgroups of ce_stream_kernel left.
 __global__ __launch_bounds__(256) void ce_rows_kernel(const float2* part, int tiles, int ld, int grid, const int* count, int row0,
@@ -1295,7 +1358,7 @@ bool wide_tiles(long n, long m) {
 // fp32 slabs to write and read, and small tiles need half as many.  Measured, large / small: 16 tiles (2048 x 512 x 32000)
 // 311 / 300 us, 24 (1400 x 1024 x 50001) 533 / 548 us, 128 (8192 x 1024 x 32000) 1696 / 1791 us.
 constexpr int DH_SMALL = 16;
-constexpr int JOIN_VOCAB = 8192;
+constexpr int JOIN_VOCAB = 8192, MERGE_ROWS = 16384;
 
 // Parts of a contraction: as many as make the product's share of the workgroups that run at once, each of at least eight steps
 // (of four: within 2 us either way).  `slots`: one workgroup per CU with large tiles; with small ones two, or one of each
@@ -1495,21 +1558,29 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
     return MMST_OK;
   }
 
-  hipLaunchKernelGGL(ce_index_kernel, dim3(1), dim3(1024), 0, st, A.target, A.ignore_index, N, V, index, words, count, A.loss, A.lse,
-                     A.dloss, A.grad_scale, unit);
-  MMST_CHECK_LAUNCH();
   bf16* hc = (bf16*)(ws + p.hc);
   bf16* gbuf = (bf16*)(ws + p.g);
   float2* lse_c = (float2*)(ws + p.lse);
   float* weight = (float*)(ws + p.weight);
+  const bool merged = p.pieces == 1 && N > 0 && N <= MERGE_ROWS;
+  if (merged)
+    hipLaunchKernelGGL(ce_index_gather_kernel, dim3((N + 15) / 16), dim3(256), 0, st, (const bf16*)A.h, A.ldh, D8, A.target,
+                       A.ignore_index, N, V, A.dloss, A.grad_scale, index, words, count, unit, weight, hc, A.loss, A.lse,
+                       (bf16*)A.dh, A.lddh);
+  else
+    hipLaunchKernelGGL(ce_index_kernel, dim3(1), dim3(1024), 0, st, A.target, A.ignore_index, N, V, index, words, count, A.loss,
+                       A.lse, A.dloss, A.grad_scale, unit);
+  MMST_CHECK_LAUNCH();
   for (int i = 0; i < p.pieces; ++i) {
     const int row0 = (int)(i * p.rows);
     const int rows_max = (int)p.rows;
     const unsigned gather = (unsigned)((p.rows * D8 + 255) / 256);
-    hipLaunchKernelGGL(ce_gather_kernel, dim3(gather + (i ? 0 : (N + 15) / 16)), dim3(256), 0, st, (const bf16*)A.h, A.ldh, D8,
-                       index, count, row0, rows_max, A.dloss, A.grad_scale, hc, weight, unit, gather, A.target, A.ignore_index, N, V,
-                       (bf16*)A.dh, A.lddh);
-    MMST_CHECK_LAUNCH();
+    if (!merged) {
+      hipLaunchKernelGGL(ce_gather_kernel, dim3(gather + (i ? 0 : (N + 15) / 16)), dim3(256), 0, st, (const bf16*)A.h, A.ldh, D8,
+                         index, count, row0, rows_max, A.dloss, A.grad_scale, hc, weight, unit, gather, A.target, A.ignore_index,
+                         N, V, (bf16*)A.dh, A.lddh);
+      MMST_CHECK_LAUNCH();
+    }
     logit.P = hc; logit.ldp = D; logit.Pn = rows_max; logit.count = count; logit.row0 = row0; logit.index = index + row0;
     logit.word = words + row0;
     logit.g = gbuf; logit.ldg = p.Vp;

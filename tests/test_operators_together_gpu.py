@@ -156,3 +156,19 @@ def test_a_run_in_two_replayed_graphs():
             run(ins[k % 2])
             torch.cuda.synchronize()
             assert all(torch.equal(out[n], want[n]) for n in out), f"replay {k}"
+
+
+def test_runs_on_two_streams_at_once():
+    """Two runs enqueued in turn on streams of their own: nothing is shared between calls."""
+    ins = [{k: t.to(DEV) for k, t in make(n, c, v, 20, seed=n).items()} for n, c, v in ((300, 128, 9000), (257, 1000, 517))]
+    want = [run(i) for i in ins]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in ins]
+    got = [[], []]
+    for _ in range(3):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(run(ins[k]))
+    torch.cuda.synchronize()
+    for k, w in enumerate(want):
+        assert all(torch.equal(g[n], w[n]) for g in got[k] for n in w)
