@@ -5,13 +5,13 @@
 //
 // All of it is matrix products over tiles of 256 x 256 (or 128 x 128, see large_tiles) on v_mfma_f32_16x16x32_bf16 with
 // fp32 accumulation; the softmax is made from the tile's logits while they are in registers:
-//   logits a tile becomes (max, sum exp) per row and 64 words, 8 bytes; for the gradient also its exponentials, in bf16
+//   logits a tile becomes (max, sum exp) per row and 64 words, 8 bytes; for the gradient also its exponentials, 16 bits
 //   rows   a row's pairs are joined into lse and the loss
 //   scale  the exponentials become g, in place
 //   dh, dw products with g, whose operands lie along the wrong axis and are read through transposing LDS reads
-// Three products, then, where computing the logits twice would take four; the price is one more rounding to bf16 of a
-// probability (an exponential in [0, 1] relative to its 64 words' maximum, 2^-8 of itself) and one pass over g.  With a short
-// contraction the pass would cost more than the product: those layers compute the logits twice (ce_stream_kernel).
+// Three products, then, where computing the logits twice would take four; the price is one more rounding of a probability
+// (pack_exp, 2^-10 of itself) and one pass over g.  With a short contraction the pass would cost more than the product:
+// those layers compute the logits twice (ce_stream_kernel).
 // The gradient goes in pieces of the ROWS: a piece's g [rows][V] is the only large buffer.  Rows that do not count
 // (ignore_index) are left out at the start: the others are numbered through on the device and gathered, so a padded batch
 // costs what its tokens cost, and what padding holds (NaN, infinities) reaches nothing.
@@ -606,7 +606,10 @@ __global__ __launch_bounds__(WP * WQ * 64, STAGES == 2 ? 2 : 1) void ce_logits_k
         for (int tp = 0; tp < NT / 2; ++tp) {
           u32x4 o;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] = pack_exp(acc[mt][2 * tp + (e >> 1)][(2 * e) & 3], acc[mt][2 * tp + (e >> 1)][(2 * e + 1) & 3]);
+          for (int e = 0; e < 4; ++e) {
+            const f32x4& x = acc[mt][2 * tp + (e >> 1)];
+            o[e] = pack_exp(x[(2 * e) & 3], x[(2 * e + 1) & 3]);
+          }
           *reinterpret_cast<u32x4*>(a.g + (size_t)(p0 + pw0 + mt * 16 + i16) * a.ldg + q0 + qw0 + tp * 32 + 8 * j4) = o;
         }
     }
@@ -746,7 +749,9 @@ struct CeStream {
     each = G ? T / (uint32_t)G : 0;
     extra = T - each * (uint32_t)G;
   }
-  __device__ __forceinline__ uint32_t begin(int b) const { return each * (uint32_t)b + ((uint32_t)b < extra ? (uint32_t)b : extra); }
+  __device__ __forceinline__ uint32_t begin(int b) const {
+    return each * (uint32_t)b + ((uint32_t)b < extra ? (uint32_t)b : extra);
+  }
   __device__ __forceinline__ int owner(uint32_t tile) const {
     const uint32_t longer = (each + 1) * extra;
     return (int)(tile < longer ? tile / (each + 1) : extra + (tile - longer) / each);
@@ -795,7 +800,8 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
     return __builtin_amdgcn_make_buffer_rsrc((void*)(a.Q + (long)q * 128 * a.ldq), 0, ((n - 1) * (int)a.ldq + a.K) * 2, 0x00020000);
   };
   auto issue = [&](const __amdgpu_buffer_rsrc_t rsrc, lds_byte* wr, int h, int i) {   // instruction i of half h
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lptr_t)(wr + h * OpQ::BYTES + i * 4096 + wave * 1024), 16, (int)off[h][i], 0, 0, 0);
+    const lptr_t to = (lptr_t)(wr + h * OpQ::BYTES + i * 4096 + wave * 1024);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, to, 16, (int)off[h][i], 0, 0, 0);
   };
   {
     const __amdgpu_buffer_rsrc_t rsrc = words_of(qt);
@@ -1121,14 +1127,14 @@ __global__ __launch_bounds__(256) void ce_gather_kernel(const bf16* h, long ldh,
   reinterpret_cast<uint4*>(out)[(long)r * D8 + c] = reinterpret_cast<const uint4*>(h + (long)n * ldh)[c];
 }
 
-// Both of these in one launch, for few rows in one piece: a workgroup has 16 rows, 16 lanes each, and looks at all the
-// targets and weights itself, for the number of rows that count before its own and the largest weight: up to MERGE_ROWS, since that grows with their square.
-// All of the gradient, in one launch / in two: 64 x 128 x 43 24 / 27 us, 4032 x 128 x 43 32 / 35, 8192 x 1024 x 43 63 / 71, 16384 x
-// 128 x 43 61 / 64, 32768 x 128 x 43 98 / 96, 65536 x 128 x 43 211 / 150.
-__global__ __launch_bounds__(256) void ce_index_gather_kernel(const bf16* h, long ldh, int D8, const int64_t* target, int64_t ignore,
-                                                              int N, int V, const float* dloss, float scale, int* index, int* words,
-                                                              int* count, float* unit, float* weight, bf16* out, float* loss,
-                                                              float* lse, bf16* dh, long lddh) {
+// Both of these in one launch, for few rows in one piece: a workgroup has 16 rows, 16 lanes each, and looks at all the targets
+// and weights itself, for the number of rows that count before its own and the largest weight.  That grows with the square of
+// the rows, so up to MERGE_ROWS.  All of the gradient, in one launch / in two: 64 x 128 x 43 24 / 27 us, 4032 x 128 x 43 32 /
+// 35, 8192 x 1024 x 43 63 / 71, 16384 x 128 x 43 61 / 64, 32768 x 128 x 43 98 / 96, 65536 x 128 x 43 211 / 150.
+__global__ __launch_bounds__(256) void ce_index_gather_kernel(const bf16* h, long ldh, int D8, const int64_t* target,
+                                                              int64_t ignore, int N, int V, const float* dloss, float scale,
+                                                              int* index, int* words, int* count, float* unit, float* weight,
+                                                              bf16* out, float* loss, float* lse, bf16* dh, long lddh) {
   __shared__ int before_of[4], all_of[4];
   __shared__ float top_of[4];
   const int tid = threadIdx.x, w = tid >> 6, first = blockIdx.x * 16;
@@ -1484,7 +1490,8 @@ template <int MODE> void launch_logits(CeGemm& g, const CePlan& p, char* ws, hip
     g.ksplit = p.split_logits;
     g.slab = (float*)(ws + p.slab_logits);
     g.ldslab = (g.Qn + 7) & ~7;
-    hipLaunchKernelGGL((ce_product_kernel<LOGIT_PART, 128, 128, 2, 2, 4>), dim3(g.ptiles * g.qtiles * g.ksplit), dim3(256), 0, st, g);
+    const dim3 grid(g.ptiles * g.qtiles * g.ksplit);
+    hipLaunchKernelGGL((ce_product_kernel<LOGIT_PART, 128, 128, 2, 2, 4>), grid, dim3(256), 0, st, g);
     hipLaunchKernelGGL(ce_join_kernel<MODE>, dim3((g.Qn + 63) / 64, (g.Pn + 15) / 16), dim3(256), 0, st, g);
     return;
   }
@@ -1529,7 +1536,8 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
   const int D = A.D, V = A.V, N = A.N, D8 = D / 8;
 
   // per row: one per 64 words, or 160
-  const int pairs = p.split_logits > 1 ? (V + 63) / 64 : p.wide ? (V + 159) / 160 : p.big ? (V + 255) / 256 * 4 : (V + 127) / 128 * 2;
+  const int pairs = p.split_logits > 1 ? (V + 63) / 64 : p.wide ? (V + 159) / 160 : p.big ? (V + 255) / 256 * 4
+                                                                                          : (V + 127) / 128 * 2;
   CeGemm logit = {};
   logit.Q = w; logit.ldq = A.ldw; logit.Qn = V; logit.K = D; logit.ksplit = 1;
   logit.bias = A.bias; logit.target = A.target;

@@ -49,9 +49,9 @@ struct DropArgs {
 };
 
 // A lane owns blocks of eight elements.  FLAT: rows follow one another, and the tensor is one row.  ROWS: rows of a multiple of
-// eight elements, a block lies inside one.  ANY: of eight elements or more; a block may begin in one row and end in the next, and goes
-// by elements then.  37248 x 2048 in bf16 (FLAT): 56 us, 5.4 TB/s, as fast as a copy; two blocks per lane of a 16-bit type keep
-// 32 bytes per lane in flight as one does of fp32.
+// eight elements, a block lies inside one.  ANY: of eight elements or more; a block may begin in one row and end in the next,
+// and goes by elements then.  37248 x 2048 in bf16 (FLAT): 56 us, 5.4 TB/s, as fast as a copy; two blocks per lane of a 16-bit
+// type keep 32 bytes per lane in flight as one does of fp32.
 enum { FLAT = 0, ROWS = 1, ANY = 2 };
 template <typename T, int MODE, int U>
 __global__ __launch_bounds__(256) void dropout_vec_kernel(const DropArgs a) {
@@ -328,7 +328,8 @@ __global__ __launch_bounds__(BLK) void ln_fwd_kernel(const LnArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) s += z[q][e];   // columns past the end are zero
     }
-    const float mean = row_sum<TPR, BLK>(s, red, turn) / (float)cols;   // (a product with 1 / cols would not leave a constant row at 0)
+    // (a product with 1 / cols would not leave a constant row at 0)
+    const float mean = row_sum<TPR, BLK>(s, red, turn) / (float)cols;
     float vs = 0.f;   // the variance from the centred row: a large mean costs no digits
 #pragma unroll
     for (int q = 0; q < NV; ++q)
@@ -486,17 +487,17 @@ LnShape ln_fwd_shape(long rows, int cols) {
   return s;
 }
 // The backward pass keeps two sums per column besides the row, and each workgroup leaves them for ln_cols_kernel: two
-// workgroups of 256 per CU, or one of 1024 (four and two: 5 % faster to 7 % slower, and 15 to 45 % slower from 4096 columns on,
-// where the sums themselves are most of what is written).  Up to 1536 columns lanes as above, in a wave (60000 x 520
-// bf16: 32 lanes with three accesses 38 us, 64 with two 43; 25000 x 1200: 64 with three 35, 256 of a larger workgroup 42).  Beyond, two accesses per lane only where the 128 registers of a 1024-lane
-// workgroup hold that (16-bit types, even widths: 8192 x 4096 39 us, 42 with one; 4096 x 8192 43 and 53), or where there is no
-// wider workgroup.
+// workgroups of 256 per CU, or one of 1024 (four and two: 5 % faster to 7 % slower, and 15 to 45 % slower from 4096 columns
+// on, where the sums themselves are most of what is written).  Up to 1536 columns lanes as above, in a wave (60000 x 520
+// bf16: 32 lanes with three accesses 38 us, 64 with two 43; 25000 x 1200: 64 with three 35, 256 of a larger workgroup 42).
+// Beyond, two accesses per lane only where the 128 registers of a 1024-lane workgroup hold that (16-bit types, even widths:
+// 8192 x 4096 39 us, 42 with one; 4096 x 8192 43 and 53), or where there is no wider workgroup.
 LnShape ln_bwd_shape(long rows, int cols, int dtype) {
   LnShape s;
   const bool one = cols % 8 || dtype == MMST_F32;
   s.blk = cols <= 1536 ? 256 : 1024;
-  s.tpr = cols <= 32 ? 4 : cols <= 64 ? 8 : cols <= 128 ? 16 : cols <= 768 ? 32 : cols <= 1536 ? 64 : cols <= 2048 ? 256 : cols <= 4096 ? (one ? 512 : 256)
-        : cols <= 8192 ? (one ? 1024 : 512) : 1024;
+  s.tpr = cols <= 32 ? 4 : cols <= 64 ? 8 : cols <= 128 ? 16 : cols <= 768 ? 32 : cols <= 1536 ? 64 : cols <= 2048 ? 256
+        : cols <= 4096 ? (one ? 512 : 256) : cols <= 8192 ? (one ? 1024 : 512) : 1024;
   s.nv = (cols + s.tpr * 8 - 1) / (s.tpr * 8);
   const long need = (rows + s.blk / s.tpr - 1) / (s.blk / s.tpr), most = s.blk == 256 ? 512 : 256;
   s.grid = (int)(need < most ? need : most);
@@ -587,7 +588,8 @@ int mmst_layer_norm(const void* x, long ldx, const void* residual, long ldr, con
            eps, 1.0f / (float)cols, drop_key(p, seed, offset)};
   const LnShape s = ln_fwd_shape(rows, cols);
   const hipStream_t st = (hipStream_t)stream;
-  if (!(dtype == MMST_F32 ? launch_ln_fwd<float>(a, s, st) : dtype == MMST_BF16 ? launch_ln_fwd<bf16>(a, s, st) : launch_ln_fwd<f16>(a, s, st)))
+  if (!(dtype == MMST_F32 ? launch_ln_fwd<float>(a, s, st) : dtype == MMST_BF16 ? launch_ln_fwd<bf16>(a, s, st)
+                                                                                 : launch_ln_fwd<f16>(a, s, st)))
     return MMST_ERR_LAUNCH;
   MMST_CHECK_LAUNCH();
   return MMST_OK;
@@ -616,7 +618,8 @@ int mmst_layer_norm_bwd(const void* dy, long lddy, const void* z, long ldz, cons
     LnArgs a{dy, dz_in, z, gamma, nullptr, dz, dx, const_cast<float*>(stats), sums ? (float*)ws : nullptr, rows, cols,
              lddy, lddz_in, ldz, lddz, lddx, 0.f, 1.0f / (float)cols, key};
     const hipStream_t st = (hipStream_t)stream;
-    if (!(dtype == MMST_F32 ? launch_ln_bwd<float>(a, s, st) : dtype == MMST_BF16 ? launch_ln_bwd<bf16>(a, s, st) : launch_ln_bwd<f16>(a, s, st)))
+    if (!(dtype == MMST_F32 ? launch_ln_bwd<float>(a, s, st) : dtype == MMST_BF16 ? launch_ln_bwd<bf16>(a, s, st)
+                                                                                   : launch_ln_bwd<f16>(a, s, st)))
       return MMST_ERR_LAUNCH;
     MMST_CHECK_LAUNCH();
   }

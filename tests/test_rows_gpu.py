@@ -246,6 +246,27 @@ def test_layer_norm_bwd(t, cols):
         check_backward(dy, z, stats, g, a, p, got)
 
 
+@pytest.mark.parametrize("rows,cols", [(1 << 20, 4104), ((1 << 22) + 5, 1027)])
+def test_layer_norm_past_32_bits_of_elements(rows, cols):
+    """The last of more than 2^32 elements.  Half of them dropped and the others doubled is exact in bf16, so those rows by
+    themselves, without dropout, have to give the same bits."""
+    t = torch.bfloat16
+    x = rnd(64, cols, seed=1).to(t).to(DEV).repeat(rows // 64 + 1, 1)[:rows]
+    gamma, beta = (1 + 0.2 * rnd(cols, seed=2)).to(DEV), rnd(cols, seed=3).to(DEV)
+    y, z, stats = ops.layer_norm(x, gamma, beta, p=0.5, seed=SEED, offset=OFFSET)
+    k = 5
+    idx = np.arange((rows - k) * cols, rows * cols, dtype=np.uint64)
+    f = torch.from_numpy(factor_at(idx, 0.5, SEED, OFFSET)).reshape(k, cols)
+    assert torch.equal(z[-k:].cpu().double(), x[-k:].cpu().double() * f)
+    alone = ops.layer_norm(z[-k:].contiguous(), gamma, beta)
+    assert torch.equal(y[-k:], alone[0]) and torch.equal(stats[-k:], alone[2])
+    dz, dx = ops.layer_norm_bwd(x, z, stats, gamma, p=0.5, seed=SEED, offset=OFFSET)[:2]
+    want = ops.layer_norm_bwd(x[-k:].contiguous(), z[-k:].contiguous(), stats[-k:].contiguous(), gamma)[0]
+    assert torch.equal(dz[-k:], want) and torch.equal(dx[-k:].cpu().double(), want.cpu().double() * f)
+    del x, y, z, dz, dx
+    torch.cuda.empty_cache()
+
+
 # on both sides of every change of the number of lanes per row and of the accesses per lane
 EDGES = [3, 8, 9, 24, 31, 32, 33, 63, 64, 65, 127, 129, 255, 256, 257, 300, 511, 513, 768, 769, 777, 1025, 1536, 1537, 2047, 2049, 4095,
          4097, 6144, 6145, 8191]
