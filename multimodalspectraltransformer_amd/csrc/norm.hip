@@ -491,8 +491,8 @@ LnShape ln_fwd_shape(long rows, int cols) {
 // on, where the sums themselves are most of what is written).  Up to 1536 columns lanes as above, in a wave (60000 x 520
 // bf16: 32 lanes with three accesses 38 us, 64 with two 43; 25000 x 1200: 64 with three 35, 256 of a larger workgroup 42).
 // Beyond, two accesses per lane only where the 128 registers of a 1024-lane workgroup hold that (16-bit types, even widths:
-// 8192 x 4096 39 us, 42 with one; 4096 x 8192 43 and 53; two accesses in workgroups of 256 at 8000 x 4099 88, one in a workgroup of 1024 79), or where there is
-// no wider workgroup.
+// 8192 x 4096 39 us, 42 with one; 4096 x 8192 43 and 53; two accesses in workgroups of 256 at 8000 x 4099 88, one in a
+// workgroup of 1024 79), or where there is no wider workgroup.
 LnShape ln_bwd_shape(long rows, int cols, int dtype) {
   LnShape s;
   const bool one = cols % 8 || dtype == MMST_F32;
