@@ -1310,6 +1310,7 @@ struct CePlan {
 };
 
 constexpr int STREAM_GRID = 512, TILE_GRID = 256;   // two workgroups per CU, one
+constexpr int JOIN_VOCAB = 8192, MERGE_ROWS = 16384;
 constexpr size_t PIECE_BYTES = (size_t)4 << 30;   // g of a piece, unless the caller says how many rows
 constexpr size_t PIECE_MAX = (size_t)64 << 30, HC_MAX = (size_t)16 << 30;   // g and the rows of h, in any case
 constexpr size_t PAIR_BYTES = (size_t)1 << 30;    // pairs of a piece, where only the loss is asked for
@@ -1360,22 +1361,22 @@ bool wide_tiles(long n, long m) {
   return wide < cost_large(n, m) && wide < cost_small(n, m);
 }
 
-// dh has the vocabulary as its contraction, which is cut into parts where there are too few tiles; the more parts, the more
-// fp32 slabs to write and read, and small tiles need half as many.  Measured, large / small: 16 tiles (2048 x 512 x 32000)
-// 311 / 300 us, 24 (1400 x 1024 x 50001) 533 / 548 us, 128 (8192 x 1024 x 32000) 1696 / 1791 us.
-constexpr int DH_SMALL = 16;
-constexpr int JOIN_VOCAB = 8192, MERGE_ROWS = 16384;
-
-// Parts of a contraction: as many as make the product's share of the workgroups that run at once, each of at least eight steps
-// (of four: within 2 us either way).  `slots`: one workgroup per CU with large tiles; with small ones two, or one of each
-// product where both are in one launch.  All of the gradient of 4032 x 128 x 43: 72 us with dw uncut, 45 in 7 parts (in launches
-// of their own); of 3032 x 128 x 32000 in one launch: 189 us for 128 slots each, 167 for 256, 197 for 512; of 333 x 1024 x
-// 50001: 196, 181, 203.
-int parts(long t, long slots, long contraction) {
-  const long steps = contraction / 64;
-  long s = t < slots ? slots / (t ? t : 1) : 1;
-  if (s > steps / 8) s = steps / 8;
-  return (int)(s < 1 ? 1 : s > 32 ? 32 : s);
+// Parts of a contraction (of dh: the vocabulary, of dw: the rows), each of at least eight steps: as many as are done first,
+// counted in steps of the workgroups that run at once (`slots`: one per CU with large tiles; with small ones two, or one of each
+// product where both are in one launch) and what writing and reading the fp32 slabs takes, 1 / 10 of a step per large tile and
+// part, 1 / 20 per small one.  All of the gradient of 4032 x 128 x 43: 72 us with dw uncut, 45 in 7 parts (in launches of their
+// own); of 3032 x 128 x 32000 in one launch: 189 us for 4 parts of dh, 167 for 8, 197 for 16; of 10878 x 568 x 41518 2970 us for
+// one (129 tiles), 2610 for 3; of 1840 x 680 x 773 67 us for as many as fill the slots once, 46 for the best.
+struct Parts { int n; double steps; };
+Parts parts(long t, bool big, long slots, long contraction) {
+  const long steps = (contraction + 63) / 64;
+  const double join = big ? 1.0 / 10 : 1.0 / 20;
+  Parts best = {1, (double)((t + slots - 1) / slots * steps)};
+  for (long s = 2; s <= 32 && s <= steps / 8; ++s) {
+    const double cost = (double)((t * s + slots - 1) / slots) * (double)steps / (double)s + (double)(t * s) * join;
+    if (cost < best.steps) best = {(int)s, cost};
+  }
+  return best;
 }
 
 // Parts of the logits' contraction (`steps` of it) where t tiles leave most CUs idle: at least eight steps each, and more than 16
@@ -1422,11 +1423,17 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
   p.few = tiles(rows, a->V, 128) <= TILE_GRID;
   p.split_logits = p.stream ? 1 : logit_parts(tiles(rows, a->V, 128), (a->D + 63) / 64);
   if (grad) {
-    p.big_dh = tiles(rows, a->D, 256) > DH_SMALL;
     p.big_dw = large_tiles(a->V, a->D);
-    const long slots = p.big_dh == p.big_dw ? TILE_GRID : 2 * TILE_GRID;   // of a small product: both run at once, or it alone
-    p.split_dh = parts(tiles(rows, a->D, p.big_dh ? 256 : 128), p.big_dh ? TILE_GRID : slots, a->V);
-    p.split_dw = parts(tiles(a->V, a->D, p.big_dw ? 256 : 128), p.big_dw ? TILE_GRID : slots, rows);
+    // A step of small tiles takes 7 / 13 of one of large ones; large ones for dh also where they take 5 % more by that count.
+    // Measured, large / small: 2048 x 512 x 32000 (16 large tiles) 311 / 300 us, 1400 x 1024 x 50001 (24) 533 / 548, 8192 x 1024 x
+    // 32000 (128) 1696 / 1791.
+    const long slots = p.big_dw ? 2 * TILE_GRID : TILE_GRID;   // of small tiles, beside dw or alone
+    const Parts large = parts(tiles(rows, a->D, 256), true, TILE_GRID, a->V);
+    const Parts small = parts(tiles(rows, a->D, 128), false, 2 * TILE_GRID, a->V);
+    p.big_dh = large.steps * 13 <= small.steps * 7 * 1.05;
+    p.split_dh = p.big_dh ? large.n : parts(tiles(rows, a->D, 128), false, slots, a->V).n;
+    p.split_dw = p.big_dw ? parts(tiles(a->V, a->D, 256), true, TILE_GRID, rows).n
+                          : parts(tiles(a->V, a->D, 128), false, p.big_dh ? 2 * TILE_GRID : TILE_GRID, rows).n;
   }
   size_t at = 256;   // count, unit
   auto take = [&](size_t n) { const size_t o = at; at += align(n); return o; };

@@ -217,10 +217,13 @@ def _check_mask(p, seed, offset, what):
 def dropout(x, p, seed, offset=0, out=None):
     """x with each element set to 0 with probability p and scaled by 1 / (1 - p) otherwise (p rounded to a multiple of
     1 / 65536).  The mask is a function of (seed, offset, element of x read row by row) and never stored: the same call on
-    the gradient of the result is the backward pass.  `out` may be x.  fp32, bf16, fp16; any shape."""
+    the gradient of the result is the backward pass.  `out` may be x; without it, x itself is returned where p rounds to 0.
+    fp32, bf16, fp16; any shape."""
     dt = _dtype_of(x, "dropout")
     _check_mask(p, seed, offset, "dropout")
     if out is None:
+        if p * 65536.0 + 0.5 < 1.0:
+            return x
         y = out = _new_like(x)
         ldy = x.shape[-1]
     else:

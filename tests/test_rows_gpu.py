@@ -107,6 +107,14 @@ def test_dropout_of_odd_rows(t, rows, cols, pad):
     assert torch.equal(y.cpu(), x)
 
 
+def test_dropout_of_nothing_dropped_is_its_input():
+    x = rnd(40, 17, seed=1).to(DEV)
+    assert ops.dropout(x, 0.0, 1) is x and ops.dropout(x, 2.0 ** -18, 1) is x
+    out = torch.empty_like(x)
+    assert ops.dropout(x, 0.0, 1, out=out) is out and torch.equal(out, x)
+    assert ops.dropout(x, 2.0 ** -17, 1) is not x
+
+
 def test_dropout_clears_infinities_and_nan():
     x = torch.full((64, 128), float("nan"), device=DEV)
     x[::2] = float("inf")
