@@ -452,9 +452,10 @@ int mmst_layer_norm_bwd_ws(int dtype, long rows, int cols, size_t* bytes);
  *     a fixed order: equal calls give equal bits.
  *   - the gradient works through the rows in pieces; the workspace holds the logits' gradient of one piece in bf16
  *     (rows_per_piece x V, rounded up to multiples of 256; 0: as many rows as 4 GiB hold; never more than 64 GiB) and its
- *     gathered rows of h (never more than 16 GiB), with bf16 gradients of more than one piece also their fp32 sums.  The loss
- *     alone needs 8 bytes per row and 64 words, 1 GiB at most.  mmst_linear_ce_ws says how many bytes (its pointers may
- *     be unset except dbias, which only has to say whether there is one); it has to be 256-byte aligned. */
+ *     gathered rows of h (never more than 16 GiB), with bf16 gradients of more than one piece also their fp32 sums, and the
+ *     fp32 parts of products whose contraction is split.  The loss alone needs 8 bytes per row and 64 words, 1 GiB at most.
+ *     mmst_linear_ce_ws says how many bytes (its pointers may be unset except dbias, which only has to say whether there is
+ *     one); it has to be 256-byte aligned. */
 #define MMST_LINEAR_CE_MAX_ROWS (1 << 24)
 #define MMST_LINEAR_CE_MAX_VOCAB (1 << 22)
 #define MMST_LINEAR_CE_MAX_DIM 32768
