@@ -191,6 +191,25 @@ def _rows(t, like, name, out=False):
     return t.contiguous(), cols
 
 
+def _overlap(a, lda, b, ldb):
+    """Whether two tensors of one shape and type, their rows lda and ldb elements apart, have an element in common."""
+    cols, size = a.shape[-1], a.element_size()
+    if a.numel() == 0:
+        return False
+    rows, gap = a.numel() // cols, b.data_ptr() - a.data_ptr()
+    if gap >= ((rows - 1) * lda + cols) * size or -gap >= ((rows - 1) * ldb + cols) * size:
+        return False
+    if rows == 1 or lda == ldb:   # a row of one begins `at` bytes behind one of the other
+        at = gap % (lda * size)
+        return rows == 1 or at < cols * size or lda * size - at < cols * size
+    first = torch.arange(rows) * (lda * size)
+    other = gap + torch.arange(rows) * (ldb * size)
+    i = torch.searchsorted(first, other, right=True)   # rows of a that begin no later
+    before = other - first[(i - 1).clamp(min=0)]
+    behind = first[i.clamp(max=rows - 1)] - other
+    return bool((((i > 0) & (before < cols * size)) | ((i < rows) & (behind < cols * size))).any())
+
+
 def _vector(t, n, device, name):
     if t is None:
         return None
@@ -239,8 +258,8 @@ def dropout(x, p, seed, offset=0, out=None):
 
 def layer_norm(x, gamma=None, beta=None, eps=1e-5, residual=None, p=0.0, seed=0, offset=0, out=None, z_out=None):
     """(y, z, stats): z = residual + dropout(x) and its layer norm over the last dimension, y = (z - mean) rstd gamma +
-    beta; stats [..., 2] = (mean, rstd) in fp32.  z is x itself where there is neither residual nor dropout.  gamma / beta
-    fp32 or None; at most 16384 columns.  (p, seed, offset) as in dropout()."""
+    beta; stats [..., 2] = (mean, rstd) in fp32.  z is x itself where there is neither residual nor dropout, and a copy of
+    it where `out` overwrites x.  gamma / beta fp32 or None; at most 16384 columns.  (p, seed, offset) as in dropout()."""
     dt = _dtype_of(x, "layer_norm")
     _check_mask(p, seed, offset, "layer_norm")
     shape, device = x.shape, x.device
@@ -265,6 +284,12 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, residual=None, p=0.0, seed=0,
     elif rp is not None or p > 0.0:
         z = _new_like(x)
         zp = z.data_ptr()
+    elif out is not None:   # z is x, unless y is written over it
+        if x2 is not x:
+            z = x2
+        elif _overlap(x, ldx, y, ldy):
+            z = _new_like(x)
+            zp = z.data_ptr()
     stats = x.new_empty(shape[:-1] + (2,), dtype=torch.float32)
     _call("mmst_layer_norm", device, x2.data_ptr(), ldx, rp, ldr, gp, bp, y.data_ptr(), ldy, zp, ldz, stats.data_ptr(), dt,
           x.numel() // cols, cols, eps, p, seed, offset)
