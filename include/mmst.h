@@ -409,7 +409,7 @@ int mmst_fragment_bf16(int n, const mmst_frag_desc* descs, void* stream);
  * What the width-128 launches above fuse into their epilogues, for rows of any width, in fp32, bf16 or fp16 (dtype; sums
  * and statistics always fp32).  Row r of a tensor starts ld* elements behind row r - 1, ld* >= cols; any alignment of an
  * element is served, 16-byte aligned rows of a multiple of 8 columns fastest.  An output may be the same tensor as an
- * input of the same call (same pointer, same stride), other overlaps are not allowed.
+ * input of the same call (same pointer, same stride), other overlaps are not allowed: none of two outputs either.
  *
  * The dropout mask is Philox4x32-10 of (seed, offset, element), see csrc/philox.h: element i = r * cols + c of the tensor
  * read row by row, whatever its strides and type, and the same in mmst_dropout, mmst_layer_norm and mmst_layer_norm_bwd.

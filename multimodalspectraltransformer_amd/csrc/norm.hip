@@ -583,7 +583,7 @@ int mmst_layer_norm(const void* x, long ldx, const void* residual, long ldr, con
   if (!type_ok(dtype) || rows < 0 || cols < 1 || cols > MMST_LN_MAX_COLS || !drop_ok(p) || !(eps >= 0.f)) return MMST_ERR_ARG;
   if (rows == 0) return MMST_OK;
   if (!x || !y || !ld_ok(x, ldx, cols, rows) || !ld_ok(residual, ldr, cols, rows) || !ld_ok(y, ldy, cols, rows) ||
-      !ld_ok(z, ldz, cols, rows) || rows > 0x7FFFFFFFFFFFL / cols)
+      !ld_ok(z, ldz, cols, rows) || rows > 0x7FFFFFFFFFFFL / cols || y == z)
     return MMST_ERR_ARG;
   LnArgs a{x, residual, nullptr, gamma, beta, y, z, stats, nullptr, rows, cols, ldx, ldr, 0, ldy, ldz,
            eps, 1.0f / (float)cols, drop_key(p, seed, offset)};
@@ -610,11 +610,12 @@ int mmst_layer_norm_bwd(const void* dy, long lddy, const void* z, long ldz, cons
   const LnShape s = ln_bwd_shape(rows, cols, dtype);
   const bool sums = dgamma || dbeta;
   if (sums && ws_bytes < (size_t)s.grid * 2 * cols * sizeof(float)) return MMST_ERR_ARG;
+  if (dgamma && dbeta && dgamma < dbeta + cols && dbeta < dgamma + cols) return MMST_ERR_ARG;
   if (rows > 0) {
     const DropKey key = drop_key(p, seed, offset);
     if (!dy || !z || !stats || !dz || (key.thr && !dx) || (sums && (!ws || (uintptr_t)ws % 4)) || !ld_ok(dy, lddy, cols, rows) ||
         !ld_ok(z, ldz, cols, rows) || !ld_ok(dz_in, lddz_in, cols, rows) || !ld_ok(dz, lddz, cols, rows) ||
-        !ld_ok(key.thr ? dx : nullptr, lddx, cols, rows) || rows > 0x7FFFFFFFFFFFL / cols)
+        !ld_ok(key.thr ? dx : nullptr, lddx, cols, rows) || (key.thr && dx == dz) || rows > 0x7FFFFFFFFFFFL / cols)
       return MMST_ERR_ARG;
     LnArgs a{dy, dz_in, z, gamma, nullptr, dz, dx, const_cast<float*>(stats), sums ? (float*)ws : nullptr, rows, cols,
              lddy, lddz_in, ldz, lddz, lddx, 0.f, 1.0f / (float)cols, key};

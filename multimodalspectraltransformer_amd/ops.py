@@ -210,6 +210,15 @@ def _overlap(a, lda, b, ldb):
     return bool((((i > 0) & (before < cols * size)) | ((i < rows) & (behind < cols * size))).any())
 
 
+def _clear(out, ldo, t, ldt, name, same=True):
+    """Refuses an output that has some elements in common with another tensor of the call: a row could be written before
+    it is read.  `same`: the very same rows may be written over."""
+    if same and out.data_ptr() == t.data_ptr() and (ldo == ldt or t.numel() == t.shape[-1]):
+        return
+    if _overlap(out, ldo, t, ldt):
+        raise L.MMSTError(f"{name} shares some of its elements with another tensor of the call")
+
+
 def _vector(t, n, device, name):
     if t is None:
         return None
@@ -236,14 +245,15 @@ def _check_mask(p, seed, offset, what):
 def dropout(x, p, seed, offset=0, out=None):
     """x with each element set to 0 with probability p and scaled by 1 / (1 - p) otherwise (p rounded to a multiple of
     1 / 65536).  The mask is a function of (seed, offset, element of x read row by row) and never stored: the same call on
-    the gradient of the result is the backward pass.  `out` may be x; without it, x itself is returned where p rounds to 0.
-    fp32, bf16, fp16; any shape."""
+    the gradient of the result is the backward pass.  `out` may be x, but share no other elements with it; without `out`, x
+    itself is returned where p rounds to 0.  fp32, bf16, fp16; any shape of at least one dimension."""
     dt = _dtype_of(x, "dropout")
     _check_mask(p, seed, offset, "dropout")
+    y = None
     if out is None:
         if p * 65536.0 + 0.5 < 1.0:
             return x
-        y = out = _new_like(x)
+        out = _new_like(x)
         ldy = x.shape[-1]
     else:
         y, ldy = _rows(out, x, "dropout: out", out=True)
@@ -251,15 +261,18 @@ def dropout(x, p, seed, offset=0, out=None):
     if n == 0:
         return out
     x, ldx = _rows(x, x, "dropout: x")
+    if y is not None:
+        _clear(y, ldy, x, ldx, "dropout: out")
     cols = x.shape[-1]
-    _call("mmst_dropout", x.device, x.data_ptr(), ldx, y.data_ptr(), ldy, dt, n // cols, cols, p, seed, offset)
+    _call("mmst_dropout", x.device, x.data_ptr(), ldx, out.data_ptr(), ldy, dt, n // cols, cols, p, seed, offset)
     return out
 
 
 def layer_norm(x, gamma=None, beta=None, eps=1e-5, residual=None, p=0.0, seed=0, offset=0, out=None, z_out=None):
     """(y, z, stats): z = residual + dropout(x) and its layer norm over the last dimension, y = (z - mean) rstd gamma +
     beta; stats [..., 2] = (mean, rstd) in fp32.  z is x itself where there is neither residual nor dropout, and a copy of
-    it where `out` overwrites x.  gamma / beta fp32 or None; at most 16384 columns.  (p, seed, offset) as in dropout()."""
+    it where `out` overwrites x.  gamma / beta fp32 or None; at most 16384 columns.  (p, seed, offset) as in dropout().
+    `out` and `z_out` may each be x or the residual, but share no other elements with these and none with each other."""
     dt = _dtype_of(x, "layer_norm")
     _check_mask(p, seed, offset, "layer_norm")
     shape, device = x.shape, x.device
@@ -290,6 +303,13 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, residual=None, p=0.0, seed=0,
         elif _overlap(x, ldx, y, ldy):
             z = _new_like(x)
             zp = z.data_ptr()
+    for given, t, ld, name in ((out, y, ldy, "layer_norm: out"), (z_out, z, ldz, "layer_norm: z_out")):
+        if given is not None:
+            _clear(t, ld, x2, ldx, name)
+            if residual is not None:
+                _clear(t, ld, residual, ldr, name)
+    if out is not None and z_out is not None:
+        _clear(y, ldy, z, ldz, "layer_norm: out", same=False)
     stats = x.new_empty(shape[:-1] + (2,), dtype=torch.float32)
     _call("mmst_layer_norm", device, x2.data_ptr(), ldx, rp, ldr, gp, bp, y.data_ptr(), ldy, zp, ldz, stats.data_ptr(), dt,
           x.numel() // cols, cols, eps, p, seed, offset)
@@ -307,7 +327,8 @@ def _layer_norm_bwd_ws(dt, rows, cols):
 def layer_norm_bwd(dy, z, stats, gamma=None, dz_in=None, p=0.0, seed=0, offset=0, dgamma=None, dbeta=None):
     """(dz, dx, dgamma, dbeta) from the gradient at y and what layer_norm() returned: dz = gradient at z (the residual's
     too), plus dz_in where z is also used elsewhere; dx = dz through the dropout mask (dz itself where p is 0).  dgamma /
-    dbeta (fp32): given ones are added to, as the framework's parameter gradients are, None makes new ones."""
+    dbeta (fp32): given ones are added to, as the framework's parameter gradients are, and share no elements; None makes new
+    ones."""
     dt = _dtype_of(dy, "layer_norm_bwd")
     _check_mask(p, seed, offset, "layer_norm_bwd")
     shape, device = dy.shape, dy.device
@@ -336,6 +357,8 @@ def layer_norm_bwd(dy, z, stats, gamma=None, dz_in=None, p=0.0, seed=0, offset=0
         accumulate = 1
         dgp = _vector(dgamma, cols, device, "layer_norm_bwd: dgamma")
         dbp = _vector(dbeta, cols, device, "layer_norm_bwd: dbeta")
+        if abs(dgp - dbp) < 4 * cols:
+            raise L.MMSTError("layer_norm_bwd: dgamma and dbeta share elements")
     dz = _new_like(dy)
     dx = torch.empty_like(dz) if int(p * 65536.0 + 0.5) > 0 else dz
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)

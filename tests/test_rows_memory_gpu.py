@@ -6,6 +6,7 @@ import torch
 pytestmark = pytest.mark.gpu
 
 if torch.cuda.is_available():
+    from multimodalspectraltransformer_amd import _lib as L
     from multimodalspectraltransformer_amd import ops
 
 DEV = "cuda"
@@ -53,3 +54,26 @@ def test_layer_norm_over_a_transposed_input_that_is_copied():
     y, z, stats = ops.layer_norm(x, out=memory)
     want = ops.layer_norm(held)
     assert torch.equal(y, want[0]) and torch.equal(z, held) and torch.equal(stats, want[2])
+
+
+def test_outputs_that_share_some_elements_are_refused():
+    memory, w = torch.zeros(20, 40, device=DEV), torch.zeros(40, device=DEV)
+    x, below, right, left, wide = memory[:4, 8:16], memory[1:5, 8:16], memory[:4, 9:17], memory[:4, 1:9], memory[::2][:4, 8:16]
+    res = torch.zeros(4, 8, device=DEV)
+    for o in (below, right, left, wide):
+        for call in (lambda: ops.dropout(x, 0.5, 1, out=o), lambda: ops.layer_norm(x, out=o), lambda: ops.layer_norm(x, z_out=o),
+                     lambda: ops.layer_norm(res, residual=x, out=o), lambda: ops.layer_norm(res, residual=x, z_out=o),
+                     lambda: ops.layer_norm(res, out=x, z_out=o), lambda: ops.layer_norm(res, out=x, z_out=x)):
+            with pytest.raises(L.MMSTError):
+                call()
+    with pytest.raises(L.MMSTError):
+        ops.layer_norm_bwd(x, x, torch.zeros(4, 2, device=DEV), dgamma=w[:8], dbeta=w[7:15])
+    assert (memory == 0).all() and (w == 0).all()
+    # what shares none: rows in turn, and columns beside one another
+    x.copy_(rnd(4, 8, seed=1))
+    for o in (memory[4:8, 8:16], memory[:4, 16:24], memory[:4, :8]):
+        assert torch.equal(ops.dropout(x, 0.5, 1, out=o), ops.dropout(x, 0.5, 1))
+        assert torch.equal(ops.layer_norm(x, out=o)[0], ops.layer_norm(x)[0])
+    even, odd = memory[8::2][:4, :8], memory[9::2][:4, :8]
+    even.copy_(x)
+    assert torch.equal(ops.dropout(even, 0.5, 1, out=odd), ops.dropout(x, 0.5, 1)) and torch.equal(even, x)
