@@ -77,3 +77,15 @@ def test_outputs_that_share_some_elements_are_refused():
     even, odd = memory[8::2][:4, :8], memory[9::2][:4, :8]
     even.copy_(x)
     assert torch.equal(ops.dropout(even, 0.5, 1, out=odd), ops.dropout(x, 0.5, 1)) and torch.equal(even, x)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("p", [0.0, 2.0 ** -18, 2.0 ** -17, 0.5])
+def test_dropout_returns_one_layout_for_every_p(t, p):
+    """Rows one after another, whatever the input's strides and whether anything is dropped."""
+    base = rnd(12, 30, seed=5).to(t).to(DEV)
+    for x in (base[:, :17], base[:, 3:11], base.t(), base[::3], base[:1].expand(12, 30), base):
+        y = ops.dropout(x, p, 7)
+        assert y.is_contiguous() and (y.data_ptr() != x.data_ptr() or x is base)
+        if p < 2.0 ** -17:
+            assert torch.equal(y, x)
