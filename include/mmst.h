@@ -453,7 +453,10 @@ int mmst_layer_norm_bwd_ws(int dtype, long rows, int cols, size_t* bytes);
  *   - the gradient works through the rows in pieces; the workspace holds the logits' gradient of one piece in bf16
  *     (rows_per_piece x V, rounded up to multiples of 256; 0: as many rows as 4 GiB hold; never more than 64 GiB) and its
  *     gathered rows of h (never more than 16 GiB), with bf16 gradients of more than one piece also their fp32 sums, and the
- *     fp32 parts of products whose contraction is split.  The loss alone needs 8 bytes per row and 64 words, 1 GiB at most.
+ *     fp32 parts of products whose contraction is split.  The loss alone needs 8 bytes per row and 64 words (words rounded
+ *     up to a multiple of 256), or, where a layer of D <= 128 is streamed, 16 bytes per row (128 of more than 8064 words)
+ *     and 1 MiB; never more than 1 GiB of these, since more rows go in pieces.  Besides, 4 bytes per row of a piece and, of
+ *     layers with D >= 1024 and few tiles, 32 MiB at most; for D <= 128 and at most 128 words 256 bytes are all.
  *     mmst_linear_ce_ws says how many bytes (its pointers may be unset except dbias, which only has to say whether there is
  *     one); it has to be 256-byte aligned. */
 #define MMST_LINEAR_CE_MAX_ROWS (1 << 24)

@@ -731,6 +731,7 @@ template <bool JOIN> __global__ __launch_bounds__(256) void ce_scale_kernel(cons
 // single tiles, each beginning with an empty pipeline, the stats took 109 us).
 // A large vocabulary is cut into eight parts, one per XCD, so that the words that an XCD's workgroups read over and over stay
 // in its L2 (all of 32000 x 128 from everywhere: 48 us, at the rate of the memory behind the L2s).
+__host__ __device__ __forceinline__ int stream_parts(int qtiles) { return qtiles >= 64 ? 8 : 1; }
 struct CeStream {
   int ptiles, qtiles, parts, per_part;   // tiles of the rows that count and of the vocabulary; workgroups per part
   int q0, qn, G;                         // this part's first tile of the vocabulary, how many, workgroups that have any
@@ -738,7 +739,7 @@ struct CeStream {
   __device__ __forceinline__ CeStream(int rows, int V, int grid) {
     ptiles = (rows + 127) / 128;
     qtiles = (V + 127) / 128;
-    parts = qtiles >= 64 ? 8 : 1;
+    parts = stream_parts(qtiles);
     per_part = parts == 8 ? grid >> 3 : grid;
   }
   __device__ __forceinline__ void part(int x) {
@@ -1305,6 +1306,7 @@ struct CePlan {
   bool few;           // of these at most one per CU: four stages of LDS (loss of 200 x 4096 x 1000 uncut: 41 us, 46 with two)
   int split_logits;   // or in parts of the contraction, joined by ce_join_kernel
   bool big_dh, big_dw;
+  int parts, pairs;   // logits: parts of the vocabulary of the stream; (maximum, sum) per row otherwise: one per 64 words, or 160
   long Vp;
   size_t index, words, tlogit, lse, weight, part, hc, g, slab_logits, slab_dh, slab_dw, slab_bias, dwacc, dbacc, total;
 };
@@ -1314,6 +1316,7 @@ constexpr int JOIN_VOCAB = 8192, MERGE_ROWS = 16384;
 constexpr size_t PIECE_BYTES = (size_t)4 << 30;   // g of a piece, unless the caller says how many rows
 constexpr size_t PIECE_MAX = (size_t)64 << 30, HC_MAX = (size_t)16 << 30;   // g and the rows of h, in any case
 constexpr size_t PAIR_BYTES = (size_t)1 << 30;    // pairs of a piece, where only the loss is asked for
+constexpr size_t STREAM_PAIRS = (size_t)STREAM_GRID * 2 * 128 * 8;   // of the stream, where it has no rows
 
 bool sizes_ok(const mmst_linear_ce_args* a) {
   return a && a->N >= 0 && a->N <= MMST_LINEAR_CE_MAX_ROWS && a->V >= 1 && a->V <= MMST_LINEAR_CE_MAX_VOCAB && a->D >= 8 &&
@@ -1399,12 +1402,13 @@ bool streams(long n, const mmst_linear_ce_args* a) { return a->D <= 128 && tiles
 CePlan plan(const mmst_linear_ce_args* a, bool grad) {
   CePlan p = {};
   p.Vp = ((long)a->V + VT - 1) / VT * VT;
-  const long all = ((long)a->N + 255) / 256 * 256, pairs = (a->V + 255) / 256 * 4;
+  const long all = ((long)a->N + 255) / 256 * 256;
   auto limit = [&](size_t bytes, size_t row) {   // rows of a piece, so that `row` bytes of each are no more than `bytes`
     const long fit = (long)(bytes / row) / 256 * 256;
     p.rows = p.rows < fit ? p.rows : fit < 256 ? 256 : fit;
   };
   p.rows = all ? all : 256;
+  p.parts = stream_parts((a->V + 127) / 128);
   p.whole = !grad && a->D <= 128 && a->V <= 128;
   p.stream = p.whole || (!grad && streams(a->N, a));
   if (grad) {
@@ -1412,8 +1416,10 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
     else limit(PIECE_BYTES, p.Vp * 2);
     limit(PIECE_MAX, p.Vp * 2);
     limit(HC_MAX, (size_t)a->D * 2);
-  } else if (!p.stream) {
-    limit(PAIR_BYTES, pairs * 8);
+  } else if (p.stream && !p.whole) {   // what CeStream::slot counts: two pairs per row and part of the vocabulary
+    limit(PAIR_BYTES - STREAM_PAIRS, (size_t)p.parts * 16);
+  } else if (!p.whole) {
+    limit(PAIR_BYTES, (size_t)((a->V + 255) / 256 * 4) * 8);
   }
   p.pieces = all ? (int)((all + p.rows - 1) / p.rows) : 1;
   const long rows = a->N < p.rows ? a->N : p.rows;
@@ -1438,8 +1444,12 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
   size_t at = 256;   // count, unit
   auto take = [&](size_t n) { const size_t o = at; at += align(n); return o; };
   if (p.split_logits > 1) p.slab_logits = take((size_t)p.split_logits * p.rows * ((a->V + 7) & ~7) * 4);
-  p.tlogit = take(p.rows * 4);
-  p.part = take(p.stream ? (size_t)(STREAM_GRID + 8 * (p.rows / 128)) * 2 * 128 * 8 : (size_t)pairs * p.rows * 8);
+  p.pairs = p.split_logits > 1 ? (a->V + 63) / 64 : p.wide ? (a->V + 159) / 160 : p.big ? (a->V + 255) / 256 * 4
+                                                                                       : (a->V + 127) / 128 * 2;
+  if (!p.whole) {   // (which keeps both in LDS)
+    p.tlogit = take(p.rows * 4);
+    p.part = take(p.stream ? STREAM_PAIRS + (size_t)p.parts * 16 * p.rows : (size_t)p.pairs * p.rows * 8);
+  }
   if (grad) {
     p.index = take((size_t)(all + 256) * 4);
     p.words = take((size_t)(all + 256) * 4);
@@ -1542,9 +1552,7 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
   const bf16* w = (const bf16*)A.w;
   const int D = A.D, V = A.V, N = A.N, D8 = D / 8;
 
-  // per row: one per 64 words, or 160
-  const int pairs = p.split_logits > 1 ? (V + 63) / 64 : p.wide ? (V + 159) / 160 : p.big ? (V + 255) / 256 * 4
-                                                                                          : (V + 127) / 128 * 2;
+  const int pairs = p.pairs;
   CeGemm logit = {};
   logit.Q = w; logit.ldq = A.ldw; logit.Qn = V; logit.K = D; logit.ksplit = 1;
   logit.bias = A.bias; logit.target = A.target;
