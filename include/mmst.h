@@ -443,8 +443,10 @@ int mmst_layer_norm_bwd_ws(int dtype, long rows, int cols, size_t* bytes);
  * logits = h w^T + bias (bf16 operands, fp32 accumulation), loss[n] = logsumexp(logits[n]) - logits[n][target[n]]: what
  * the fc_out GEMM and mmst_ce_loss do for at most 64 words, for any vocabulary.  grad != 0 also computes, for
  * sum_n grad_scale dloss[n] loss[n], the gradients dh, dw and dbias.
- *   - rows whose target is ignore_index do not count: loss, lse and dh 0, nothing in dw, whatever h holds there, and no
- *     work in the products.  A target that is no word and not ignore_index gives loss and lse NaN and no gradient.
+ *   - rows whose target is ignore_index do not count: loss, lse and dh 0, nothing in dw, whatever h holds there.  They are
+ *     numbered out on the device and are no work in the products; those of the loss alone only where the products are so
+ *     long that the numbering is little beside them (from some 1e11 operations on), and below that cost what others do.
+ *     A target that is no word and not ignore_index gives loss and lse NaN and no gradient.
  *   - masked words: bias may be -infinity or any low number.  A row whose every logit is -infinity has lse -infinity, loss
  *     +infinity and no gradient.
  *   - h, w, dh, dw rows 16-byte aligned; D a multiple of 8.  dw [V][D] and dbias [V] (both without a stride) in bf16,
@@ -456,7 +458,8 @@ int mmst_layer_norm_bwd_ws(int dtype, long rows, int cols, size_t* bytes);
  *     fp32 parts of products whose contraction is split.  The loss alone needs 8 bytes per row and 64 words (words rounded
  *     up to a multiple of 256), or, where a layer of D <= 128 is streamed, 16 bytes per row (128 of more than 8064 words)
  *     and 1 MiB; never more than 1 GiB of these, since more rows go in pieces.  Besides, 4 bytes per row of a piece and, of
- *     layers with D >= 1024 and few tiles, 32 MiB at most; for D <= 128 and at most 128 words 256 bytes are all.
+ *     layers with D >= 1024 and few tiles, 32 MiB at most; where rows are numbered 8 bytes per row and 2 D bytes per row of a
+ *     piece, 1 GiB of those at most; for D <= 128 and at most 128 words 256 bytes are all.
  *     mmst_linear_ce_ws says how many bytes (its pointers may be unset except dbias, which only has to say whether there is
  *     one); it has to be 256-byte aligned. */
 #define MMST_LINEAR_CE_MAX_ROWS (1 << 24)

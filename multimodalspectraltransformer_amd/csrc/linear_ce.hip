@@ -14,7 +14,8 @@
 // those layers compute the logits twice (ce_stream_kernel).
 // The gradient goes in pieces of the ROWS: a piece's g [rows][V] is the only large buffer.  Rows that do not count
 // (ignore_index) are left out at the start: the others are numbered through on the device and gathered, so a padded batch
-// costs what its tokens cost, and what padding holds (NaN, infinities) reaches nothing.
+// costs what its tokens cost, and what padding holds (NaN, infinities) reaches nothing.  The loss alone does that where it
+// pays (numbers), and otherwise drops the results of such rows, which reach no other row.
 // g is made for weights relative to the largest one, which the products' results are multiplied with in fp32: weights that are
 // all the same (a mean's 1 / rows) are 1 then, and g of a target, near -1 in most rows, is near -1 in bf16 as well.  Rounded with
 // 1 / rows inside, all of them would be off by the same 2^-8 at worst, and so would their sum.
@@ -1104,7 +1105,7 @@ __global__ __launch_bounds__(1024) void ce_index_kernel(const int64_t* target, i
 }
 
 // A piece's rows, one after another (16 bytes per lane), and their weights; behind its `gather` workgroups those that clear dh
-// of the rows that do not count, 16 rows each.
+// of the rows that do not count, 16 rows each.  (The loss alone has neither weights nor dh, here and below.)
 __global__ __launch_bounds__(256) void ce_gather_kernel(const bf16* h, long ldh, int D8, const int* index, const int* count,
                                                         int row0, int rows_max, const float* dloss, float scale, bf16* out,
                                                         float* weight, const float* unit, unsigned gather,
@@ -1124,7 +1125,7 @@ __global__ __launch_bounds__(256) void ce_gather_kernel(const bf16* h, long ldh,
   rows = rows < rows_max ? rows : rows_max;
   if (r >= rows) return;
   const int n = index[row0 + r];
-  if (c == 0) weight[r] = scale * (dloss ? dloss[n] : 1.f) / *unit;
+  if (c == 0 && weight) weight[r] = scale * (dloss ? dloss[n] : 1.f) / *unit;
   reinterpret_cast<uint4*>(out)[(long)r * D8 + c] = reinterpret_cast<const uint4*>(h + (long)n * ldh)[c];
 }
 
@@ -1177,7 +1178,7 @@ __global__ __launch_bounds__(256) void ce_index_gather_kernel(const bf16* h, lon
     if ((tid & 15) == 0) {
       index[at] = n;
       words[at] = (int)t;
-      weight[at] = scale * (dloss ? dloss[n] : 1.f) / most;
+      if (weight) weight[at] = scale * (dloss ? dloss[n] : 1.f) / most;
     }
     for (int c = tid & 15; c < D8; c += 16)
       reinterpret_cast<uint4*>(out)[(long)at * D8 + c] = reinterpret_cast<const uint4*>(h + (long)n * ldh)[c];
@@ -1187,7 +1188,8 @@ __global__ __launch_bounds__(256) void ce_index_gather_kernel(const bf16* h, lon
       loss[n] = x;
       if (lse) lse[n] = x;
     }
-    for (int c = tid & 15; c < D8; c += 16) reinterpret_cast<uint4*>(dh + (long)n * lddh)[c] = make_uint4(0, 0, 0, 0);
+    if (dh)
+      for (int c = tid & 15; c < D8; c += 16) reinterpret_cast<uint4*>(dh + (long)n * lddh)[c] = make_uint4(0, 0, 0, 0);
   }
 }
 
@@ -1302,6 +1304,7 @@ struct CePlan {
   long rows;          // per piece, a multiple of 256
   int pieces, split_dh, split_dw;
   bool stream, whole; // logits: ce_stream_kernel; with the loss in it
+  bool number;        // the rows that count are numbered through and gathered
   bool big, wide;     // or tiles of 256 x 256, of 128 x 160 (loss); otherwise 128 x 128
   bool few;           // of these at most one per CU: four stages of LDS (loss of 200 x 4096 x 1000 uncut: 41 us, 46 with two)
   int split_logits;   // or in parts of the contraction, joined by ce_join_kernel
@@ -1312,6 +1315,7 @@ struct CePlan {
 };
 
 constexpr int STREAM_GRID = 512, TILE_GRID = 256;   // two workgroups per CU, one
+constexpr double NUMBER_PART = 1.0 / 16;
 constexpr int JOIN_VOCAB = 8192, MERGE_ROWS = 16384;
 constexpr size_t PIECE_BYTES = (size_t)4 << 30;   // g of a piece, unless the caller says how many rows
 constexpr size_t PIECE_MAX = (size_t)64 << 30, HC_MAX = (size_t)16 << 30;   // g and the rows of h, in any case
@@ -1399,6 +1403,16 @@ int logit_parts(long t, long steps) {
 // and 55 / 47.
 bool streams(long n, const mmst_linear_ce_args* a) { return a->D <= 128 && tiles(n, a->V, 128) > 2 * STREAM_GRID; }
 
+// The loss alone: rows that do not count are numbered out where that, estimated in nanoseconds and as if none could be left
+// out, takes at most NUMBER_PART of the products.  Measured, every row in the products / numbered through, of 0 and of half
+// the rows ignored: 4032 x 128 x 32000 47, 47 / 54, 37 us; 1000 x 1024 x 50001 110, 107 / 118, 64; 65536 x 128 x 32000 577, 574 /
+// 639, 356; 1000000 x 256 x 1000 944, 932 / 1993, 1526 (by the estimate not numbered); 2000 x 1024 x 50001 221, 206 / 226, 116;
+// 4032 x 1024 x 50001 377, 378 / 366, 206; 8192 x 2048 x 65536 1729, 1720 / 1735, 865; 4096 x 4096 x 32000 831, 827 / 843, 432.
+bool numbers(long n, long d, long v) {
+  const double products = (double)n * (double)v * (1e-4 + (double)d * 2 / 1.3e6), numbering = 6000 + n * (1 + (double)d / 5000);
+  return numbering <= products * NUMBER_PART;
+}
+
 CePlan plan(const mmst_linear_ce_args* a, bool grad) {
   CePlan p = {};
   p.Vp = ((long)a->V + VT - 1) / VT * VT;
@@ -1411,6 +1425,7 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
   p.parts = stream_parts((a->V + 127) / 128);
   p.whole = !grad && a->D <= 128 && a->V <= 128;
   p.stream = p.whole || (!grad && streams(a->N, a));
+  p.number = grad || (!p.whole && numbers(a->N, a->D, a->V));
   if (grad) {
     if (a->rows_per_piece) limit(((size_t)a->rows_per_piece + 255) / 256 * 256, 1);
     else limit(PIECE_BYTES, p.Vp * 2);
@@ -1421,6 +1436,7 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
   } else if (!p.whole) {
     limit(PAIR_BYTES, (size_t)((a->V + 255) / 256 * 4) * 8);
   }
+  if (!grad && p.number) limit(PAIR_BYTES, (size_t)a->D * 2);
   p.pieces = all ? (int)((all + p.rows - 1) / p.rows) : 1;
   const long rows = a->N < p.rows ? a->N : p.rows;
   if (grad) p.stream = streams(rows, a);
@@ -1450,12 +1466,14 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
     p.tlogit = take(p.rows * 4);
     p.part = take(p.stream ? STREAM_PAIRS + (size_t)p.parts * 16 * p.rows : (size_t)p.pairs * p.rows * 8);
   }
-  if (grad) {
+  if (p.number) {
     p.index = take((size_t)(all + 256) * 4);
     p.words = take((size_t)(all + 256) * 4);
+    p.hc = take((size_t)p.rows * a->D * 2);
+  }
+  if (grad) {
     p.lse = take(p.rows * 8);
     p.weight = take(p.rows * 4);
-    p.hc = take((size_t)p.rows * a->D * 2);
     p.g = take((size_t)p.rows * p.Vp * 2);
     const size_t dh = p.split_dh > 1 ? (size_t)p.split_dh * p.rows : 0, dw = p.split_dw > 1 ? (size_t)p.split_dw * a->V : 0;
     if (dh) p.slab_dh = take(dh * a->D * 4);
@@ -1558,7 +1576,7 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
   logit.bias = A.bias; logit.target = A.target;
   logit.part = (float2*)(ws + p.part); logit.tlogit = (float*)(ws + p.tlogit);
   logit.rows_max = (int)p.rows;
-  if (!grad) {
+  if (!p.number) {
     for (int i = 0; i < p.pieces; ++i) {
       const long row0 = i * p.rows;
       const int rows = (int)(N - row0 < p.rows ? N - row0 : p.rows);
@@ -1583,41 +1601,46 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
 
   bf16* hc = (bf16*)(ws + p.hc);
   bf16* gbuf = (bf16*)(ws + p.g);
-  float2* lse_c = (float2*)(ws + p.lse);
-  float* weight = (float*)(ws + p.weight);
+  float2* lse_c = grad ? (float2*)(ws + p.lse) : nullptr;
+  float* weight = grad ? (float*)(ws + p.weight) : nullptr;
+  bf16* clear = grad ? (bf16*)A.dh : nullptr;
+  const float* dloss = grad ? A.dloss : nullptr;
+  const float grad_scale = grad ? A.grad_scale : 1.f;
   const bool merged = p.pieces == 1 && N > 0 && N <= MERGE_ROWS;
   if (merged)
     hipLaunchKernelGGL(ce_index_gather_kernel, dim3((N + 15) / 16), dim3(256), 0, st, (const bf16*)A.h, A.ldh, D8, A.target,
-                       A.ignore_index, N, V, A.dloss, A.grad_scale, index, words, count, unit, weight, hc, A.loss, A.lse,
-                       (bf16*)A.dh, A.lddh);
+                       A.ignore_index, N, V, dloss, grad_scale, index, words, count, unit, weight, hc, A.loss, A.lse, clear,
+                       A.lddh);
   else
     hipLaunchKernelGGL(ce_index_kernel, dim3(1), dim3(1024), 0, st, A.target, A.ignore_index, N, V, index, words, count, A.loss,
-                       A.lse, A.dloss, A.grad_scale, unit);
+                       A.lse, dloss, grad_scale, unit);
   MMST_CHECK_LAUNCH();
   for (int i = 0; i < p.pieces; ++i) {
     const int row0 = (int)(i * p.rows);
     const int rows_max = (int)p.rows;
     const unsigned gather = (unsigned)((p.rows * D8 + 255) / 256);
     if (!merged) {
-      hipLaunchKernelGGL(ce_gather_kernel, dim3(gather + (i ? 0 : (N + 15) / 16)), dim3(256), 0, st, (const bf16*)A.h, A.ldh, D8,
-                         index, count, row0, rows_max, A.dloss, A.grad_scale, hc, weight, unit, gather, A.target, A.ignore_index,
-                         N, V, (bf16*)A.dh, A.lddh);
+      hipLaunchKernelGGL(ce_gather_kernel, dim3(gather + (i || !grad ? 0 : (N + 15) / 16)), dim3(256), 0, st, (const bf16*)A.h,
+                         A.ldh, D8, index, count, row0, rows_max, dloss, grad_scale, hc, weight, unit, gather, A.target,
+                         A.ignore_index, N, V, clear, A.lddh);
       MMST_CHECK_LAUNCH();
     }
     logit.P = hc; logit.ldp = D; logit.Pn = rows_max; logit.count = count; logit.row0 = row0; logit.index = index + row0;
     logit.word = words + row0;
     logit.g = gbuf; logit.ldg = p.Vp;
     if (p.stream) launch_stream<LOGIT_STATS>(logit, st);
-    else launch_logits<LOGIT_EXP>(logit, p, ws, st);
+    else if (grad) launch_logits<LOGIT_EXP>(logit, p, ws, st);
+    else launch_logits<LOGIT_STATS>(logit, p, ws, st);
     MMST_CHECK_LAUNCH();
     logit.lse = lse_c; logit.weight = weight;
     logit.loss_out = A.loss; logit.lse_out = A.lse;
     const dim3 scale((unsigned)((p.Vp + 2047) / 2048 * (p.rows / 4)));
-    if (p.stream || V > JOIN_VOCAB) {
+    if (!grad || p.stream || V > JOIN_VOCAB) {
       hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)(p.rows / 16)), dim3(256), 0, st, logit.part, pairs, rows_max,
                          p.stream ? STREAM_GRID : 0, count, row0, rows_max, index, A.target, A.ignore_index, V, logit.tlogit,
                          lse_c, A.loss, A.lse);
       MMST_CHECK_LAUNCH();
+      if (!grad) continue;
       if (p.stream) launch_stream<LOGIT_GRAD>(logit, st);
       else hipLaunchKernelGGL(ce_scale_kernel<false>, scale, dim3(256), 0, st, logit, pairs);
     } else {

@@ -1,4 +1,4 @@
-"""The loss alone at sizes where its rows go in pieces, against 64-bit arithmetic on picked rows."""
+"""The loss alone at sizes where its rows are numbered or go in pieces, against 64-bit arithmetic on picked rows."""
 import pytest
 import torch
 
@@ -30,3 +30,66 @@ def test_streamed_loss_whose_pairs_need_pieces():
     check_loss(oracle(h[pick].cpu(), w.cpu(), b.cpu(), t[pick].cpu(), None), loss[pick], lse[pick])
     assert int((loss == 0).sum()) == 2 and int(loss.isnan().sum()) == 1
     torch.cuda.empty_cache()
+
+
+# products long enough for the rows to be numbered: tiles of each size, a stream, more rows than one launch numbers, pieces
+NUMBERED = [(2100, 1024, 50001), (4100, 2048, 20000), (1100, 2056, 60001), (4000, 128, 200001), (17000, 64, 150001),
+            (20000, 520, 30000), (8500, 264, 1 << 20)]
+
+
+@pytest.mark.parametrize("n,d,v", NUMBERED)
+@pytest.mark.parametrize("part", [0.0, 0.5, 1.0])
+def test_loss_of_padded_batches(n, d, v, part):
+    """Rows that count, between rows that do not, by value; ignored rows 0 whatever they hold, targets that are no word NaN."""
+    h, w, b, t = big(n, d, v, seed=n)
+    b[v // 3] = float("-inf")
+    g = torch.Generator(device=DEV).manual_seed(n + 1)
+    t[torch.randperm(n, device=DEV, generator=g)[:int(n * part)]] = IGN
+    if part < 1:
+        t[3], t[n // 2], t[n - 2] = v, -1, 1 << 40
+    h[t == IGN] = float("nan")
+    loss, lse = ops.linear_ce(h, w, t, bias=b)
+    pad = t == IGN
+    assert (loss[pad] == 0).all() and (lse[pad] == 0).all()
+    assert int(loss.isnan().sum()) == int(lse.isnan().sum()) == (3 if part < 1 else 0)
+    pick = sorted({0, 1, 3, n // 2, n // 3, n - 2, n - 1} | set(range(min(n, 8300) - 24, min(n, 8300))))
+    check_loss(oracle(h[pick].cpu(), w.cpu(), b.cpu(), t[pick].cpu(), None), loss[pick], lse[pick])
+    again = ops.linear_ce(h, w, t, bias=b)
+    assert torch.equal(again[0].view(torch.int32), loss.view(torch.int32)) and torch.equal(again[1].view(torch.int32), lse.view(torch.int32))
+
+
+def test_ignored_rows_are_no_work_in_a_long_loss():
+    """Seven eighths of the rows ignored: an eighth of the products, which is less than half of the time whatever else it takes."""
+    h, w, _, t = big(8192, 1024, 32768, seed=1)
+    few = t.clone()
+    few[:7168] = IGN
+
+    def time(target):
+        best = float("inf")
+        for _ in range(5):
+            first, last = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            first.record()
+            for _ in range(4):
+                ops.linear_ce(h, w, target)
+            last.record()
+            last.synchronize()
+            best = min(best, first.elapsed_time(last))
+        return best
+    time(t)
+    assert time(few) < time(t) / 2
+
+
+def test_a_padded_loss_in_a_replayed_graph():
+    h, w, b, t = big(2100, 1024, 50001, seed=7)
+    targets = [t.clone() for _ in range(4)]
+    for k, x in enumerate(targets):
+        x[k::k + 1] = IGN   # all of them, then fewer
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = ops.linear_ce(h, w, t, bias=b)
+    for k, x in enumerate(targets + targets[:1]):
+        t.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = ops.linear_ce(h, w, t, bias=b)
+        assert all(torch.equal(p, q) for p, q in zip(captured, eager)), f"replay {k}"

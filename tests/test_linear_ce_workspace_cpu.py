@@ -30,4 +30,6 @@ def test_the_loss_alone_needs_what_the_header_says(d, v):
         if d <= 128:
             pairs = max(pairs, (1 << 20) + rows * (128 if v > 8064 else 16))
         most = min(pairs, 1 << 30) + 4 * rows + (32 << 20 if d >= 1024 else 0)
+        if 2 * n * d * v >= 1e10:   # rows that may be numbered
+            most += 8 * rows + min(2 * d * rows, 1 << 30) + 4096
         assert need(0, n, d, v) <= most + 4 * 256, (n, d, v)   # (every buffer begins at a multiple of 256 bytes)
