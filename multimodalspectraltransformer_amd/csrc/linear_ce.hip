@@ -314,8 +314,10 @@ struct CeTile {
     if constexpr (NW != 8) {
       int rd = 0, wr = NS - 1;
       for (int s = 0; s < nsteps; ++s) {
-        // this wave's share of step s has landed; behind the barrier everybody's has, and nobody reads the stage of step s - 1
+        // this wave's share of step s has landed and its reads of step s - 1 are done; behind the barrier everybody's have, and
+        // nobody reads the stage of step s - 1
         if (s) {
+          reads_done();
           dma_done();
           asm volatile("s_barrier" ::: "memory");
         }
@@ -325,6 +327,7 @@ struct CeTile {
         wr = rd;
         rd = rd + 1 == NS ? 0 : rd + 1;
       }
+      reads_done();
       if constexpr (NS > 2) all_done();
       barrier();
     } else {
@@ -982,7 +985,8 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
       }
     }
     // The next tile's words have landed (they had this tile's products and exponentials to do so, which is why those are made
-    // to be done here); waited for here and not at the barrier, which would wait for the following stores as well.
+    // to be done here); waited for here and not at the barrier, which would wait for the following stores as well.  So are this
+    // tile's LDS reads, behind which the next barrier lets its stage be written.
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       if constexpr (STATS) asm volatile("" : "+v"(sum[mt]), "+v"(m2[mt]));
@@ -990,7 +994,7 @@ __global__ __launch_bounds__(256, 2) void ce_stream_kernel(const CeGemm a) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) asm volatile("" : "+v"(acc[mt][nt]));
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     bias_arrived();
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
