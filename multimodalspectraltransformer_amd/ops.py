@@ -304,13 +304,14 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, residual=None, p=0.0, seed=0,
         elif _overlap(x, ldx, y, ldy):
             z = _new_like(x)
             zp = z.data_ptr()
-    for given, t, ld, name in ((out, y, ldy, "layer_norm: out"), (z_out, z, ldz, "layer_norm: z_out")):
-        if given is not None:
-            _clear(t, ld, x2, ldx, name)
-            if residual is not None:
-                _clear(t, ld, residual, ldr, name)
-    if out is not None and z_out is not None:
-        _clear(y, ldy, z, ldz, "layer_norm: out", same=False)
+    if out is not None or z_out is not None:
+        for given, t, ld, name in ((out, y, ldy, "layer_norm: out"), (z_out, z, ldz, "layer_norm: z_out")):
+            if given is not None:
+                _clear(t, ld, x2, ldx, name)
+                if residual is not None:
+                    _clear(t, ld, residual, ldr, name)
+        if out is not None and z_out is not None:
+            _clear(y, ldy, z, ldz, "layer_norm: out", same=False)
     stats = x.new_empty(shape[:-1] + (2,), dtype=torch.float32)
     _call("mmst_layer_norm", device, x2.data_ptr(), ldx, rp, ldr, gp, bp, y.data_ptr(), ldy, zp, ldz, stats.data_ptr(), dt,
           x.numel() // cols, cols, eps, p, seed, offset)
