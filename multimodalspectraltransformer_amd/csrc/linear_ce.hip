@@ -63,10 +63,10 @@ struct CeGemm {
   const float* unit; bf16* g; long ldg;
   float* loss_out; float* lse_out; int64_t ignore;   // LOGIT_LOSS; joining scale
   // products
-  void* out; long ldo; int out_f32; int accumulate;   // out_f32: fp32, else bf16; accumulate: added to
+  void* out; long ldo; int out_f32;                   // out_f32: fp32, else bf16
   const float* acc_in; float* slab; float* slab_bias;   // slabs: [ksplit][Pn][ldslab], [ksplit][Pn]
   int ldslab;
-  void* dbias; const float* dbias_in;                 // DW: sums of g over the rows, in out's type; added to dbias_in
+  void* dbias; const float* dbias_in; int dbias_f32;  // DW: sums of g over the rows; added to dbias_in
 };
 
 __device__ __forceinline__ int piece_rows(const CeGemm& a) {
@@ -415,7 +415,7 @@ __device__ __forceinline__ void ce_product(const CeGemm& a, int block, int n, ld
       if (lane < 16 && v < Pn) {
         const float x = sums.sum[MODE == DW ? mt : 0][0] * (a.slab ? 1.f : *a.unit) + (a.dbias_in && !a.slab ? a.dbias_in[v] : 0.f);
         if (a.slab) a.slab_bias[(size_t)ks_id * Pn + v] = x;
-        else if (a.out_f32) ((float*)a.dbias)[v] = x;
+        else if (a.dbias_f32) ((float*)a.dbias)[v] = x;
         else ((bf16*)a.dbias)[v] = (bf16)x;
       }
 #pragma unroll
@@ -1293,7 +1293,7 @@ template <int MODE> __device__ __forceinline__ void join_slabs(const CeGemm& a, 
     for (int k = 1; k < a.ksplit; ++k) s += a.slab_bias[(size_t)k * a.Pn + v];
     s *= unit;
     if (a.dbias_in) s += a.dbias_in[v];
-    if (a.out_f32) ((float*)a.dbias)[v] = s;
+    if (a.dbias_f32) ((float*)a.dbias)[v] = s;
     else ((bf16*)a.dbias)[v] = (bf16)s;
   }
 }
@@ -1325,6 +1325,8 @@ constexpr size_t PIECE_BYTES = (size_t)4 << 30;   // g of a piece, unless the ca
 constexpr size_t PIECE_MAX = (size_t)64 << 30, HC_MAX = (size_t)16 << 30;   // g and the rows of h, in any case
 constexpr size_t PAIR_BYTES = (size_t)1 << 30;    // pairs of a piece, where only the loss is asked for
 constexpr size_t STREAM_PAIRS = (size_t)STREAM_GRID * 2 * 128 * 8;   // of the stream, where it has no rows
+
+bool dw_f32(const mmst_linear_ce_args* a) { return a->grad_f32 && a->grad_f32 != 2; }
 
 bool sizes_ok(const mmst_linear_ce_args* a) {
   return a && a->N >= 0 && a->N <= MMST_LINEAR_CE_MAX_ROWS && a->V >= 1 && a->V <= MMST_LINEAR_CE_MAX_VOCAB && a->D >= 8 &&
@@ -1483,7 +1485,7 @@ CePlan plan(const mmst_linear_ce_args* a, bool grad) {
     if (dh) p.slab_dh = take(dh * a->D * 4);
     if (dw) p.slab_dw = take(dw * a->D * 4);
     if (dw) p.slab_bias = take(dw * 4);
-    if (p.pieces > 1 && !a->grad_f32) p.dwacc = take((size_t)a->V * a->D * 4);
+    if (p.pieces > 1 && !dw_f32(a)) p.dwacc = take((size_t)a->V * a->D * 4);
     if (p.pieces > 1 && !a->grad_f32 && a->dbias) p.dbacc = take((size_t)a->V * 4);
   }
   p.total = at;
@@ -1667,12 +1669,15 @@ int mmst_linear_ce(const mmst_linear_ce_args* args, int grad, void* stream) {
     float* acc = (float*)(ws + p.dwacc);
     dw.ldo = D;
     float* bacc = (float*)(ws + p.dbacc);
-    if (A.grad_f32) {
+    if (dw_f32(&A)) {
       dw.out = A.dw; dw.out_f32 = 1; dw.acc_in = (const float*)A.dw;
-      dw.dbias = A.dbias; dw.dbias_in = (const float*)A.dbias;
     } else {
       dw.out = last ? A.dw : (void*)acc; dw.out_f32 = last ? 0 : 1; dw.acc_in = i > 0 ? acc : nullptr;
-      if (A.dbias) { dw.dbias = last ? A.dbias : (void*)bacc; dw.dbias_in = i > 0 ? bacc : nullptr; }
+    }
+    if (A.grad_f32) {
+      dw.dbias = A.dbias; dw.dbias_f32 = 1; dw.dbias_in = (const float*)A.dbias;
+    } else if (A.dbias) {
+      dw.dbias = last ? A.dbias : (void*)bacc; dw.dbias_f32 = last ? 0 : 1; dw.dbias_in = i > 0 ? bacc : nullptr;
     }
     if (launch_products(dh, dw, p, st) != MMST_OK) return MMST_ERR_LAUNCH;
   }

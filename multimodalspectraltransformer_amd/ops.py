@@ -429,8 +429,8 @@ def linear_ce(h, w, target, bias=None, ignore_index=-100):
 def linear_ce_grad(h, w, target, bias=None, dloss=None, grad_scale=1.0, ignore_index=-100, dw=None, dbias=None,
                    rows_per_piece=0):
     """(loss, lse, dh, dw, dbias): linear_ce() and the gradients of sum(grad_scale * dloss * loss) (dloss fp32 [N], None:
-    ones).  dh is bf16; dw and dbias are bf16 as well, or, where fp32 tensors are given, added to those.  dbias is None
-    without a bias.  rows_per_piece bounds the workspace: that many rows' gradient of the logits, in bf16, at a time."""
+    ones).  dh is bf16; dw and dbias are bf16 as well, or, where fp32 tensors are given, added to those: dbias, or dw and
+    with a bias dbias.  dbias is None without a bias.  rows_per_piece bounds the workspace: that many rows' gradient of the logits, in bf16, at a time."""
     a, keep = _linear_ce_args(h, w, target, bias, ignore_index, "linear_ce_grad")
     device, n, d, v = h.device, a.N, a.D, a.V
     if not 0 <= rows_per_piece <= 1 << 24:
@@ -444,10 +444,14 @@ def linear_ce_grad(h, w, target, bias=None, dloss=None, grad_scale=1.0, ignore_i
     a.dloss = _vector(dloss, n, device, "linear_ce_grad: dloss")
     a.grad_scale, a.rows_per_piece = grad_scale, rows_per_piece
     if dw is None:
-        if dbias is not None:
-            raise L.MMSTError("linear_ce_grad: dbias to be added to comes with dw")
         dw = torch.empty((v, d), dtype=torch.bfloat16, device=device)
-        dbias = None if bias is None else torch.empty(v, dtype=torch.bfloat16, device=device)
+        if dbias is not None:
+            if bias is None:
+                raise L.MMSTError("linear_ce_grad: dbias comes with bias")
+            _vector(dbias, v, device, "linear_ce_grad: dbias")
+            a.grad_f32 = 2
+        elif bias is not None:
+            dbias = torch.empty(v, dtype=torch.bfloat16, device=device)
     else:
         if dw.dtype != torch.float32 or dw.device != device or dw.shape != (v, d) or not dw.is_contiguous() or dw.data_ptr() % 16:
             raise L.MMSTError(f"linear_ce_grad: dw as contiguous fp32 [{v}, {d}] on {device} expected")

@@ -1,0 +1,39 @@
+"""The gradient of an fp32 bias beside bf16 weights: dbias given without dw, in fp32, added to."""
+import pytest
+import torch
+
+from tests.test_linear_ce_gpu import DEV, U, check_grad, check_loss, dev, inside, make, oracle
+
+pytestmark = pytest.mark.gpu
+
+if torch.cuda.is_available():
+    from multimodalspectraltransformer_amd import _lib as L
+    from multimodalspectraltransformer_amd import ops
+
+
+# dw in one part, split over the rows, in large tiles, of the stream
+@pytest.mark.parametrize("n,d,v", [(300, 136, 1500), (3000, 264, 40), (300, 512, 32000), (1000, 128, 20001), (1, 8, 1)])
+@pytest.mark.parametrize("rows", [0, 256])
+def test_dbias_alone_in_fp32(n, d, v, rows):
+    """dw and dh are the bits that they are without it; dbias is that of fp32 gradients of both, bit by bit."""
+    h, w, b, t, dl = make(n, d, v, seed=n, ignored=n // 5)
+    base = torch.randn(v, generator=torch.Generator().manual_seed(2))
+    o = oracle(h, w, b, t, dl)
+    h, w, b, t, dl = dev(h, w, b, t, dl)
+    want = ops.linear_ce_grad(h, w, t, bias=b, dloss=dl, rows_per_piece=rows)
+    both = base.to(DEV)
+    ops.linear_ce_grad(h, w, t, bias=b, dloss=dl, rows_per_piece=rows, dw=torch.zeros(v, d, device=DEV), dbias=both)
+    alone = base.to(DEV)
+    got = ops.linear_ce_grad(h, w, t, bias=b, dloss=dl, rows_per_piece=rows, dbias=alone)
+    assert got[4] is alone and got[3].dtype == torch.bfloat16 and want[4].dtype == torch.bfloat16
+    assert all(torch.equal(x, y) for x, y in zip(got[:4], want[:4])) and torch.equal(alone, both)
+    check_loss(o, *got[:2])
+    check_grad(o, *got[2:4], None)
+    inside(alone, o["db"] + base.double(), o["ddb"] + 8 * U * (base.abs() + o["db"].abs()), "dbias")
+
+
+def test_dbias_without_a_bias_or_of_another_type_is_refused():
+    h, w, b, t, _ = dev(*make(20, 64, 100))
+    for kw in (dict(dbias=b.clone()), dict(bias=b, dbias=b.bfloat16()), dict(bias=b, dbias=b[:50].clone()), dict(bias=b, dbias=b.cpu())):
+        with pytest.raises(L.MMSTError):
+            ops.linear_ce_grad(h, w, t, **kw)

@@ -33,3 +33,9 @@ def test_the_loss_alone_needs_what_the_header_says(d, v):
         if 2 * n * d * v >= 1e10:   # rows that may be numbered
             most += 8 * rows + min(2 * d * rows, 1 << 30) + 4096
         assert need(0, n, d, v) <= most + 4 * 256, (n, d, v)   # (every buffer begins at a multiple of 256 bytes)
+
+
+def test_fp32_sums_of_pieces_only_for_bf16_gradients():
+    size = dict(n=4096, d=512, v=20000, rows_per_piece=256, dbias=1)
+    bf16, both, alone = (need(1, grad_f32=f, **size) for f in (0, 1, 2))
+    assert bf16 >= both + 20000 * 512 * 4 + 20000 * 4 and alone == both + 20000 * 512 * 4
