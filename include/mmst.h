@@ -451,8 +451,8 @@ int mmst_layer_norm_bwd_ws(int dtype, long rows, int cols, size_t* bytes);
  *     +infinity and no gradient.
  *   - h, w, dh, dw rows 16-byte aligned; D a multiple of 8.  dw [V][D] and dbias [V] (both without a stride) in bf16,
  *     overwritten, or with grad_f32 in fp32, added to (as the other parameter gradients of this library); with grad_f32 2
- *     that holds for dbias alone, the gradient of an fp32 bias beside bf16 weights.  All sums run in a fixed order: equal
- *     calls give equal bits.
+ *     that holds for dbias alone, the gradient of an fp32 bias beside bf16 weights.  They are written piece by piece, so no
+ *     input may lie under them.  All sums run in a fixed order: equal calls give equal bits.
  *   - the gradient works through the rows in pieces; the workspace holds the logits' gradient of one piece in bf16
  *     (rows_per_piece x V, rounded up to multiples of 256; 0: as many rows as 4 GiB hold; never more than 64 GiB) and its
  *     gathered rows of h (never more than 16 GiB), with bf16 gradients of more than one piece also their fp32 sums, and the

@@ -381,6 +381,12 @@ def _matrix(t, d, what):
     return t, ld
 
 
+def _share(a, b):
+    """Whether two tensors without strides share memory."""
+    p, q = a.data_ptr(), b.data_ptr()
+    return p < q + b.numel() * b.element_size() and q < p + a.numel() * a.element_size()
+
+
 def _linear_ce_args(h, w, target, bias, ignore_index, what):
     if not (isinstance(h, torch.Tensor) and isinstance(w, torch.Tensor) and h.is_cuda and h.dtype == w.dtype == torch.bfloat16
             and h.dim() == w.dim() == 2 and h.device == w.device and h.shape[1] == w.shape[1]):
@@ -430,7 +436,16 @@ def linear_ce_grad(h, w, target, bias=None, dloss=None, grad_scale=1.0, ignore_i
                    rows_per_piece=0):
     """(loss, lse, dh, dw, dbias): linear_ce() and the gradients of sum(grad_scale * dloss * loss) (dloss fp32 [N], None:
     ones).  dh is bf16; dw and dbias are bf16 as well, or, where fp32 tensors are given, added to those: dbias, or dw and
-    with a bias dbias.  dbias is None without a bias.  rows_per_piece bounds the workspace: that many rows' gradient of the logits, in bf16, at a time."""
+    with a bias dbias (which may be the bias itself: an update in place).  dbias is None without a bias.  rows_per_piece
+    bounds the workspace: that many rows' gradient of the logits, in bf16, at a time."""
+    given = [x for x in (dw, dbias) if x is not None]
+    if given:   # gradients are written while later rows are still to come: what lies under them is read from a copy
+        if len(given) == 2 and _share(dw, dbias):
+            raise L.MMSTError("linear_ce_grad: dw and dbias share memory")
+        if bias is not None and any(_share(x, bias) for x in given):
+            bias = bias.clone()
+        if dloss is not None and any(_share(x, dloss) for x in given):
+            dloss = dloss.clone()
     a, keep = _linear_ce_args(h, w, target, bias, ignore_index, "linear_ce_grad")
     device, n, d, v = h.device, a.N, a.D, a.V
     if not 0 <= rows_per_piece <= 1 << 24:

@@ -37,3 +37,25 @@ def test_dbias_without_a_bias_or_of_another_type_is_refused():
     for kw in (dict(dbias=b.clone()), dict(bias=b, dbias=b.bfloat16()), dict(bias=b, dbias=b[:50].clone()), dict(bias=b, dbias=b.cpu())):
         with pytest.raises(L.MMSTError):
             ops.linear_ce_grad(h, w, t, **kw)
+
+
+@pytest.mark.parametrize("rows", [0, 256])
+def test_gradients_over_the_bias_and_the_weights_of_the_losses(rows):
+    """dbias may be the bias, an update in place, and lie on dloss: every row's logits come from what they held before."""
+    n, d, v = 1100, 136, 1500
+    h, w, b, t, dl = dev(*make(n, d, v, seed=4, ignored=100))
+    want, base = b.clone(), b.clone()
+    out = ops.linear_ce_grad(h, w, t, bias=base, dloss=dl, grad_scale=-0.5, rows_per_piece=rows, dbias=want)
+    bias = b.clone()
+    got = ops.linear_ce_grad(h, w, t, bias=bias, dloss=dl, grad_scale=-0.5, rows_per_piece=rows, dbias=bias)
+    assert got[4] is bias and torch.equal(bias, want) and not torch.equal(bias, b)
+    assert all(torch.equal(x, y) for x, y in zip(got[:4], out[:4]))
+    memory = torch.zeros(v, device=DEV)
+    memory[:n] = dl
+    want = memory.clone()
+    out = ops.linear_ce_grad(h, w, t, bias=b, dloss=dl, rows_per_piece=rows, dbias=want)
+    got = ops.linear_ce_grad(h, w, t, bias=b, dloss=memory[:n], rows_per_piece=rows, dbias=memory)
+    assert torch.equal(memory, want) and all(torch.equal(x, y) for x, y in zip(got[:4], out[:4]))
+    with pytest.raises(L.MMSTError):
+        both = torch.zeros(v * d, device=DEV)
+        ops.linear_ce_grad(h, w, t, bias=b, dw=both.view(v, d), dbias=both[-v:])
