@@ -373,9 +373,10 @@ def layer_norm_bwd(dy, z, stats, gamma=None, dz_in=None, p=0.0, seed=0, offset=0
 # linear layer + softmax cross entropy over a large vocabulary (mmst_linear_ce)
 # ---------------------------------------------------------------------------------------------
 def _matrix(t, d, what):
-    """(tensor, row stride) of a bf16 matrix of d columns as the kernels read it: rows 16-byte aligned; copied otherwise."""
+    """(tensor, row stride) of a bf16 matrix of d columns as the kernels read it: rows 16-byte aligned and at most 2^20
+    elements apart; copied otherwise."""
     ld = t.stride(0) if t.shape[0] > 1 else d
-    if t.stride(1) != 1 or ld % 8 or ld < d or t.data_ptr() % 16:
+    if t.stride(1) != 1 or ld % 8 or not d <= ld <= 1 << 20 or t.data_ptr() % 16:
         t = torch.empty_like(t, memory_format=torch.contiguous_format).copy_(t)
         ld = d
     return t, ld
