@@ -462,7 +462,9 @@ int mmst_layer_norm_bwd_ws(int dtype, long rows, int cols, size_t* bytes);
  *     layers with D >= 1024 and few tiles, 32 MiB at most; where rows are numbered 8 bytes per row and 2 D bytes per row of a
  *     piece, 1 GiB of those at most; for D <= 128 and at most 128 words 256 bytes are all.
  *     mmst_linear_ce_ws says how many bytes (its pointers may be unset except dbias, which only has to say whether there is
- *     one); it has to be 256-byte aligned. */
+ *     one); it has to be 256-byte aligned.
+ * At most as many rows, words and columns and as long a stride as follows, and (N / 128) (V / 128), both rounded up, below
+ * 2^31 - 1. */
 #define MMST_LINEAR_CE_MAX_ROWS (1 << 24)
 #define MMST_LINEAR_CE_MAX_VOCAB (1 << 22)
 #define MMST_LINEAR_CE_MAX_DIM 32768

@@ -362,8 +362,9 @@ __device__ __forceinline__ void tile_of(int id, int ptiles, int qtiles, int& pt,
 }
 
 // ---------------------------------------------------------------------------------------------------- products with g
-// dh of a piece or dw, one tile per workgroup.  Bound by the matrix units at the clock that the card's power leaves them:
-// 8192 x 2048 x 65536 takes 1.81 ms for dh and 1.76 ms for dw, 1.21 and 1.25 PFLOP/s in 256 x 256 tiles (2.15 and 2.2 ms with
+// dh of a piece or dw, one tile per workgroup.  The matrix units work in 0.63 (dh) and 0.69 (dw) of the cycles, at the 1.6 to 1.8
+// GHz that the card's power leaves; 8192 x 2048 x 65536 takes 1.81 ms for dh and 1.76 ms for dw, 1.21 and 1.25 PFLOP/s in 256 x
+// 256 tiles (2.15 and 2.2 ms with
 // four waves of 128 x 128 each, that issue their DMA, read and multiply one after another).  In narrow layers by reading g: 3032
 // x 128 x 32000 takes 66 us for both, 388 MB at 5.9 TB/s.
 // block: the workgroup's number of n
@@ -482,9 +483,9 @@ __global__ __launch_bounds__(256, 1) void ce_products_kernel(const CeGemm dh, co
 // A workgroup walks over tiles of the logits (one workgroup per CU with large tiles, two with small ones); the first steps of
 // the next tile's contraction are requested before this tile's softmax, which a wave does for its 64 columns (or 160) alone.
 // LOGIT_STATS: (max, sum of exponentials) per row and 64 words (160).  LOGIT_EXP: these, and the exponentials themselves.  8192 x
-// 2048 x 65536: 2.02 ms with the exponentials, 1.09 PFLOP/s, bound by the matrix units and, for 1.1 GB of exponentials at
-// the ends of the tiles, by the softmax that nothing multiplies beside; 333 x 1024 x 50001: 45 us in two rounds of 128 x
-// 160, 50 in three of 128 x 128.
+// 2048 x 65536: 2.02 ms with the exponentials, 1.09 PFLOP/s; the matrix units work in 0.56 of the cycles, and nothing multiplies
+// beside the softmax at the ends of the tiles.  333 x 1024 x 50001: 45 us in two rounds of 128 x 160 (matrix units 0.42), 50 in
+// three of 128 x 128.
 template <int MODE, int BP, int BQ, int WP, int WQ, int STAGES = 2>
 __global__ __launch_bounds__(WP * WQ * 64, STAGES == 2 ? 2 : 1) void ce_logits_kernel(const CeGemm a) {
   using Tile = CeTile<MODE, BP, BQ, WP, WQ, STAGES>;
@@ -730,9 +731,12 @@ template <bool JOIN> __global__ __launch_bounds__(256) void ce_scale_kernel(cons
 // vocabulary; a wave keeps its 64 rows of h in registers for the run, and the words of the next tile arrive by LDS-DMA
 // while this one is multiplied and exponentiated: one barrier per tile.  A lane keeps the running maximum and sum of its
 // own columns of a row over the whole run; lanes, waves and workgroups are joined at its end.  Two workgroups per CU: one's
-// vector instructions (max, fused multiply-add, exponential and sum per logit, what bounds this kernel) run beside the
-// other's products.  Stats of 3032 x 128 x 32000: 42 us, g 61 us (as
-// single tiles, each beginning with an empty pipeline, the stats took 109 us).
+// vector instructions (max, fused multiply-add, exponential and sum per logit) run beside the other's products.  Stats of 3032
+// x 128 x 32000: 42 us, g 61 us (as single tiles, each beginning with an empty pipeline, the stats took 109 us).  By the
+// counters neither unit bounds it: of the stats' cycles the vector unit is given instructions in 0.51 and the matrix unit works
+// in 0.30, of which 0.28 lie beside vector work, so in a third neither does anything; of g's 0.38 and 0.21.  The waves spend 0.31
+// of their time waiting, for the tile that was requested one tile ago and at its barrier, and 0.30 and 0.39 ready but not
+// issued, behind the other wave of the SIMD.
 // A large vocabulary is cut into eight parts, one per XCD, so that the words that an XCD's workgroups read over and over stay
 // in its L2 (all of 32000 x 128 from everywhere: 48 us, at the rate of the memory behind the L2s).
 __host__ __device__ __forceinline__ int stream_parts(int qtiles) { return qtiles >= 64 ? 8 : 1; }
@@ -1366,9 +1370,11 @@ long cost_large(long n, long m) { return 26 * 5 * ((tiles(n, m, 256) + TILE_GRID
 long cost_small(long n, long m) { return 14 * fifths(tiles(n, m, 128)); }
 bool large_tiles(long n, long m) { return cost_large(n, m) <= cost_small(n, m); }
 
-// For the loss alone also 128 rows x 160 words, whose rounds take 17 / 26: measured, 160 words / 128: 333 x 1024 x 50001 (2 rounds)
-// 47 / 51 us, 1000 x 1024 x 50001 (5 against 6 and 56 tiles) 107 / 111; against 256 x 256 at 1400 x 1024 x 50001 (7 against 5) 147
-// / 159.
+// For the loss alone also 128 rows x 160 words, whose rounds take 17 / 26: measured, 160 words / what is taken without them: 333 x
+// 1024 x 50001 (2 rounds against 3 of 128) 50 / 54 us, 333 x 4096 x 50001 190 / 222, 128 x 2048 x 80000 83 / 104, 200 x 2048 x
+// 40000 49 / 62, 512 x 1024 x 20000 31 / 37, 1000 x 1024 x 10000 29 / 36, 512 x 2048 x 50001 111 / 124, 333 x 256 x 80000 32 / 38,
+// 1000 x 1024 x 40000 95 / 98, 2000 x 2048 x 20000 168 / 172, 3000 x 512 x 10000 44.6 / 45.0, 64 x 1024 x 100000 48 / 48, 512 x 512 x
+// 10000 15.9 / 15.6.
 bool wide_tiles(long n, long m) {
   const long wide = 17 * fifths((n + 127) / 128 * ((m + 159) / 160));
   return wide < cost_large(n, m) && wide < cost_small(n, m);

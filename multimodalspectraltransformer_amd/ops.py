@@ -116,7 +116,8 @@ def eptr(t, offset_elems):
 # row operators of any width: dropout, layer norm (mmst_dropout, mmst_layer_norm, mmst_layer_norm_bwd)
 #
 # A call on a few rows takes the GPU 2 us and the host several times that, so these wrappers look at a tensor once and
-# build their messages only where they raise.
+# build their messages only where they raise.  They record no graph: what they compute does not require gradients, also
+# where an input does, and the backward pass is the call that is named for it.
 # ---------------------------------------------------------------------------------------------
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # mmst_dtype
 _P, _I, _LONG, _SIZE, _F, _D, _U64 = C.c_void_p, C.c_int, C.c_long, C.c_size_t, C.c_float, C.c_double, C.c_uint64
