@@ -444,8 +444,9 @@ int mmst_layer_norm_bwd_ws(int dtype, long rows, int cols, size_t* bytes);
  * the fc_out GEMM and mmst_ce_loss do for at most 64 words, for any vocabulary.  grad != 0 also computes, for
  * sum_n grad_scale dloss[n] loss[n], the gradients dh, dw and dbias.
  *   - rows whose target is ignore_index do not count: loss, lse and dh 0, nothing in dw, whatever h holds there.  They are
- *     numbered out on the device and are no work in the products; those of the loss alone only where the products are so
- *     long that the numbering is little beside them (from some 1e11 operations on), and below that cost what others do.
+ *     numbered out on the device and are no work in the products; those of the loss alone only where the numbering is
+ *     little beside the products (2 N V D from some 1e11 on, with some 55000 words at D = 128, 12000 at 1024, 4500 at
+ *     4096), and cost what others do otherwise.
  *     A target that is no word and not ignore_index gives loss and lse NaN and no gradient.
  *   - masked words: bias may be -infinity or any low number.  A row whose every logit is -infinity has lse -infinity, loss
  *     +infinity and no gradient.

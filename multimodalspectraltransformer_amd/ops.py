@@ -247,8 +247,8 @@ def dropout(x, p, seed, offset=0, out=None):
     """x with each element set to 0 with probability p and scaled by 1 / (1 - p) otherwise (p rounded to a multiple of
     1 / 65536).  The mask is a function of (seed, offset, element of x read row by row) and never stored: the same call on
     the gradient of the result is the backward pass.  `out` may be x, but share no other elements with it.  Without
-    `out` the result is contiguous, and x itself where x is that and p rounds to 0: who changes it in place then gives an
-    `out`.  fp32, bf16, fp16; any shape of at least one dimension."""
+    `out` the result is contiguous, and x itself where x is that and p rounds to 0: with a p that may be 0, a result that is
+    changed in place needs an `out`.  fp32, bf16, fp16; any shape of at least one dimension."""
     dt = _dtype_of(x, "dropout")
     _check_mask(p, seed, offset, "dropout")
     y = None

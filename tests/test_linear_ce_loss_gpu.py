@@ -32,9 +32,10 @@ def test_streamed_loss_whose_pairs_need_pieces():
     torch.cuda.empty_cache()
 
 
-# products long enough for the rows to be numbered: tiles of each size, a stream, more rows than one launch numbers, pieces
+# products long enough for the rows to be numbered: tiles of each size, a stream, more rows than one launch numbers, pieces by
+# their pairs and by their rows of h
 NUMBERED = [(2100, 1024, 50001), (4100, 2048, 20000), (1100, 2056, 60001), (4000, 128, 200001), (17000, 64, 150001),
-            (20000, 520, 30000), (8500, 264, 1 << 20)]
+            (20000, 520, 30000), (8500, 264, 1 << 20), (16500, 32768, 3000)]
 
 
 @pytest.mark.parametrize("n,d,v", NUMBERED)
